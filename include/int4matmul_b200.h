@@ -228,6 +228,87 @@ int i4mm_check_mask(const void* mask, int64_t N, int64_t S, void* violations, vo
 int i4mm_row_norm(int mode, void* y, const void* a, const void* b, const void* c, int64_t rows, int64_t width,
                   int64_t stride_a, int64_t stride_b, int64_t stride_c, void* stream);
 
+/*
+ * ---- paged key-value cache in 8 bits ------------------------------------------------------------------------------
+ * What stands between the quantized linears of a decoder that generates text: the keys and values of all tokens so far, in
+ * pages of 16, 32, 64 or 128 tokens, 8 bits a value with one scale for each page and head, and the attention over them.  No
+ * counterpart in the reference, which has no model code.
+ *
+ *   k, v      (pages, heads, page_size, head_dim) int8 or e4m3 (1 byte a value), head_dim 64 or 128 and contiguous; the other strides
+ *             are free (multiples of 16 bytes)
+ *   scales    fp32 (pages, heads, 2) contiguous, 8-byte aligned: of the page's keys and of its values.  A byte q stands for q * scale.
+ *   slot      where a token lies: page * page_size + place in the page.  Slots outside of the cache (negative ones: padding) are
+ *             skipped by the writer and read as zeros.
+ *   block_table   int32 (requests, table_width): page j of a request holds its tokens j * page_size and on.  Entries outside of
+ *             [0, pages) are no pages: attention sees no tokens there.
+ * Lengths, slots and page numbers are int32; activations are fp16 (type 0) or bf16 (type 1).
+ */
+#define I4MM_CACHE_INT8 0
+#define I4MM_CACHE_E4M3 1
+#define I4MM_TYPE_FP16 0
+#define I4MM_TYPE_BF16 1
+typedef struct i4mm_cache {
+    void* k;
+    void* v;
+    void* scales;
+    int64_t pages, heads, page_size, head_dim;
+    int64_t k_page_stride, k_head_stride, k_token_stride;    /* bytes (= values) */
+    int64_t v_page_stride, v_head_stride, v_token_stride;
+    int32_t type;                                            /* I4MM_CACHE_INT8 or I4MM_CACHE_E4M3 */
+} i4mm_cache;
+
+/*
+ * The tables of one step, from the requests' lengths, in one launch.
+ *   seq_lens (requests)     tokens held before the step            new_lens (requests)   tokens that it adds; negative: the request ends,
+ *                                                                                        its pages are free again and its length is 0
+ *   block_table             entries of the pages that the step begins are written in place (row stride in entries)
+ *   free_pages (capacity)   a stack: entries [0, *free_count) are free.  The pages of the requests that end are pushed in request order,
+ *                           then new pages are taken off its top in request order; where none is left the entry becomes -1
+ *   outputs                 lens_after (requests); cu_lens (requests + 1): the packed place of each request's first new token;
+ *                           slots, positions, request_of (max_tokens): of every packed token, -1 beyond the last one and, for slots, where
+ *                           there is no page; counts (2): *free_count afterwards, and the number of pages that could not be had
+ *                           (the stack was empty, or the table's row full)
+ * seq_lens, new_lens and free_count are left alone, so that the same call again gives the same answers; free_count is not one of the
+ * outputs.  requests <= 16384; packed tokens beyond max_tokens get no entry.
+ */
+int i4mm_cache_plan(int64_t requests, const void* seq_lens, const void* new_lens, void* block_table, int64_t table_width,
+                    int64_t table_stride, void* free_pages, int64_t free_capacity, const void* free_count, int64_t page_size,
+                    int64_t max_tokens, void* lens_after, void* cu_lens, void* slots, void* positions, void* request_of, void* counts,
+                    void* stream);
+
+/*
+ * Quantises k and v (tokens, heads, head_dim; strides in elements) into the cache at `slots`.
+ * The tokens of one page that a call writes are neighbours in the call, with ascending slots (as i4mm_cache_plan lays them out); the
+ * places of the page before the first of them hold tokens already, or the first of them is the page's first and what the page held is void.
+ * With a = the largest finite |value| that a call adds to a page and head and `most` = 127 or 448, the scale becomes the larger of the old
+ * one and the least power of two s with a <= most * s, the new bytes are round(x / s), and if the scale grew the bytes already there
+ * become round(q * old / s).  Since scales grow by powers of two, a value is off by less than one step of its final scale however often
+ * that happens (1/2 + 1/4 + ...).  Infinities are stored as +-most, NaN as 0.
+ */
+int i4mm_cache_write(const i4mm_cache* cache, const void* k, const void* v, int type, int64_t tokens, int64_t k_token_stride,
+                     int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const void* slots, void* stream);
+
+/* The values at `slots`: k_out, v_out (tokens, heads, head_dim) contiguous.  Exact where the scales are powers of two. */
+int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type, int64_t tokens, const void* slots, void* stream);
+
+/*
+ * out[t, h, :] = sum_j w_j v_j,  w = softmax over the tokens j that row t sees of scale * q[t, h, :] . k_j
+ *   q (tokens, q_heads, head_dim), strides in elements; out the same, contiguous; q_heads a multiple of the cache's heads: query head h
+ *   reads head h / (q_heads / heads)
+ *   seq_lens (requests)       tokens in the cache, those of this step included
+ *   cu_lens (requests + 1)    rows of request b are cu_lens[b] .. cu_lens[b + 1] (NULL: one row for each request), its last ones: row i of
+ *                             n is at position p = seq_lens[b] - n + i and sees the tokens j <= p, with window > 0 those with
+ *                             j > p - window.  Rows that see no token, and rows of no request, are 0.
+ *   max_len                   the most rows of a request, for the choice of a kernel (a wrong one costs time, nothing else)
+ * Sums and softmax statistics are fp32.  `workspace`: i4mm_cache_attention_workspace_bytes() bytes, zero-filled before the first use,
+ * shared by calls of one stream only.
+ */
+size_t i4mm_cache_attention_workspace_bytes(void);
+int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,
+                         int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
+                         int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
+                         int64_t window, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

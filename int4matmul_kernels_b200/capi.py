@@ -20,6 +20,17 @@ PATH_STATIC_WEIGHTS = 0x100000      # I4MM_PATH_STATIC_WEIGHTS: or-ed into a pat
 # i4mm_last_launch_schedule
 WHOLE_TILES, K_PARTS, STREAM_EQUAL_RANGES, STREAM_WHOLE_TILES, STREAM_CTAS_PER_TILE = 1, 2, 3, 4, 1000
 
+
+class Cache(ctypes.Structure):
+    """i4mm_cache"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "scales")] + [(n, ctypes.c_int64) for n in (
+        "pages", "heads", "page_size", "head_dim", "k_page_stride", "k_head_stride", "k_token_stride",
+        "v_page_stride", "v_head_stride", "v_token_stride")] + [("type", ctypes.c_int32)]
+
+
+CACHE_INT8, CACHE_E4M3 = 0, 1
+TYPE_FP16, TYPE_BF16 = 0, 1
+
 # every symbol the header declares, with its ctypes signature
 _SIGNATURES = {
     "i4mm_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -59,6 +70,19 @@ _SIGNATURES = {
                                      ctypes.c_void_p]),
     "i4mm_sparse_pack": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                         ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    "i4mm_cache_plan": (ctypes.c_int, [ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                       ctypes.c_void_p]),
+    "i4mm_cache_write": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    "i4mm_cache_read": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                       ctypes.c_void_p, ctypes.c_void_p]),
+    "i4mm_cache_attention_workspace_bytes": (ctypes.c_size_t, []),
+    "i4mm_cache_attention": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                            ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                            ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                            ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "i4mm_check_mask": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
 }
 

@@ -1,0 +1,162 @@
+// extern "C" entry points of the paged 8-bit key-value cache: argument validation and launches.
+#include "../../include/int4matmul_b200.h"
+
+#include "cache.cuh"
+#include "common.cuh"
+
+namespace {
+
+inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+constexpr int64_t kMost = 0x7FFFFFFF;                 // lengths, slots and page numbers are int32
+
+int finish(cudaError_t e) {
+    if (e == cudaSuccess) return I4MM_OK;
+    i4mm::record_cuda_error((int)e);
+    return I4MM_ERR_LAUNCH;
+}
+
+// log2 of a page's tokens, -1 for a size that there is not
+int shift_of(int64_t page_size) {
+    switch (page_size) {
+        case 16: return 4;
+        case 32: return 5;
+        case 64: return 6;
+        case 128: return 7;
+        default: return -1;
+    }
+}
+
+int view_of(const i4mm_cache* c, i4mm::CacheView& w) {
+    if (!c) return I4MM_ERR_NULL;
+    if (c->type != I4MM_CACHE_INT8 && c->type != I4MM_CACHE_E4M3) return I4MM_ERR_UNSUPPORTED;
+    if (c->head_dim != 64 && c->head_dim != 128) return I4MM_ERR_UNSUPPORTED;
+    if (shift_of(c->page_size) < 0) return I4MM_ERR_UNSUPPORTED;
+    if (c->pages <= 0 || c->heads <= 0 || c->heads > 65535 || c->pages > kMost / c->page_size) return I4MM_ERR_SHAPE;
+    if (!c->k || !c->v || !c->scales) return I4MM_ERR_NULL;
+    const int64_t strides = c->k_page_stride | c->k_head_stride | c->k_token_stride | c->v_page_stride | c->v_head_stride | c->v_token_stride;
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 8) || (strides & 15)) return I4MM_ERR_ALIGN;
+    w.k = (uint8_t*)c->k;
+    w.v = (uint8_t*)c->v;
+    w.scales = (float2*)c->scales;
+    w.k_page = c->k_page_stride;
+    w.k_head = c->k_head_stride;
+    w.k_token = c->k_token_stride;
+    w.v_page = c->v_page_stride;
+    w.v_head = c->v_head_stride;
+    w.v_token = c->v_token_stride;
+    w.pages = (int)c->pages;
+    w.heads = (int)c->heads;
+    w.page_shift = shift_of(c->page_size);
+    w.dim = (int)c->head_dim;
+    return I4MM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int i4mm_cache_plan(int64_t requests, const void* seq_lens, const void* new_lens, void* block_table, int64_t table_width,
+                    int64_t table_stride, void* free_pages, int64_t free_capacity, const void* free_count, int64_t page_size,
+                    int64_t max_tokens, void* lens_after, void* cu_lens, void* slots, void* positions, void* request_of, void* counts,
+                    void* stream) {
+    if (shift_of(page_size) < 0) return I4MM_ERR_UNSUPPORTED;
+    if (requests < 0 || requests > 16384 || table_width < 0 || table_width > kMost || table_stride < table_width || free_capacity < 0 ||
+        free_capacity > kMost || max_tokens < 0 || max_tokens > kMost - 4096)
+        return I4MM_ERR_SHAPE;
+    if (!cu_lens || !counts || !free_count) return I4MM_ERR_NULL;
+    if (requests > 0 && (!seq_lens || !new_lens || !lens_after || (table_width > 0 && !block_table))) return I4MM_ERR_NULL;
+    if ((max_tokens > 0 && (!slots || !positions || !request_of)) || (free_capacity > 0 && !free_pages)) return I4MM_ERR_NULL;
+    for (const void* p : {seq_lens, new_lens, (const void*)block_table, (const void*)free_pages, free_count, (const void*)lens_after,
+                          (const void*)cu_lens, (const void*)slots, (const void*)positions, (const void*)request_of, (const void*)counts})
+        if (!aligned(p, 4)) return I4MM_ERR_ALIGN;
+    i4mm::PlanParams p{};
+    p.seq_lens = (const int*)seq_lens;
+    p.new_lens = (const int*)new_lens;
+    p.table = (int*)block_table;
+    p.free_pages = (int*)free_pages;
+    p.free_count = (const int*)free_count;
+    p.lens_after = (int*)lens_after;
+    p.cu_lens = (int*)cu_lens;
+    p.slots = (int*)slots;
+    p.positions = (int*)positions;
+    p.request_of = (int*)request_of;
+    p.counts = (int*)counts;
+    p.table_stride = table_stride;
+    p.requests = (int)requests;
+    p.table_width = (int)table_width;
+    p.free_capacity = (int)free_capacity;
+    p.page_shift = shift_of(page_size);
+    p.max_tokens = (int)max_tokens;
+    return finish(i4mm::cache_plan_launch(p, (cudaStream_t)stream));
+}
+
+int i4mm_cache_write(const i4mm_cache* cache, const void* k, const void* v, int type, int64_t tokens, int64_t k_token_stride,
+                     int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride, const void* slots, void* stream) {
+    i4mm::CacheView c{};
+    const int status = view_of(cache, c);
+    if (status != I4MM_OK) return status;
+    if (type != I4MM_TYPE_FP16 && type != I4MM_TYPE_BF16) return I4MM_ERR_UNSUPPORTED;
+    if (tokens < 0 || tokens > kMost) return I4MM_ERR_SHAPE;
+    if (tokens == 0) return I4MM_OK;
+    if (!k || !v || !slots) return I4MM_ERR_NULL;
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 4) || ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7))
+        return I4MM_ERR_ALIGN;
+    return finish(i4mm::cache_write_launch(c, cache->type == I4MM_CACHE_E4M3, {k, k_token_stride, k_head_stride},
+                                           {v, v_token_stride, v_head_stride}, type == I4MM_TYPE_BF16, (int)tokens, (const int*)slots,
+                                           (cudaStream_t)stream));
+}
+
+int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type, int64_t tokens, const void* slots, void* stream) {
+    i4mm::CacheView c{};
+    const int status = view_of(cache, c);
+    if (status != I4MM_OK) return status;
+    if (type != I4MM_TYPE_FP16 && type != I4MM_TYPE_BF16) return I4MM_ERR_UNSUPPORTED;
+    if (tokens < 0 || tokens > kMost) return I4MM_ERR_SHAPE;
+    if (tokens == 0) return I4MM_OK;
+    if (!k_out || !v_out || !slots) return I4MM_ERR_NULL;
+    if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(slots, 4)) return I4MM_ERR_ALIGN;
+    return finish(i4mm::cache_read_launch(c, cache->type == I4MM_CACHE_E4M3, k_out, v_out, type == I4MM_TYPE_BF16, (int)tokens,
+                                          (const int*)slots, (cudaStream_t)stream));
+}
+
+size_t i4mm_cache_attention_workspace_bytes(void) { return i4mm::cache_attention_workspace(); }
+
+int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,
+                         int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
+                         int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
+                         int64_t window, void* workspace, size_t workspace_bytes, void* stream) {
+    i4mm::AttentionParams p{};
+    const int status = view_of(cache, p.cache);
+    if (status != I4MM_OK) return status;
+    if (type != I4MM_TYPE_FP16 && type != I4MM_TYPE_BF16) return I4MM_ERR_UNSUPPORTED;
+    if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->heads) return I4MM_ERR_SHAPE;
+    if (tokens < 0 || tokens > kMost / q_heads || requests < 0 || requests > 16384 || table_width < 0 || table_width > kMost / cache->page_size ||
+        table_stride < table_width || max_len < 0 || max_len > kMost || window < 0 || window > kMost)
+        return I4MM_ERR_SHAPE;
+    if (!cu_lens && tokens < requests) return I4MM_ERR_SHAPE;
+    if (tokens == 0) return I4MM_OK;
+    if (!out || !q || (requests > 0 && (!seq_lens || (table_width > 0 && !block_table)))) return I4MM_ERR_NULL;
+    if (!aligned(out, 16) || !aligned(q, 16) || !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(cu_lens, 4) ||
+        ((q_token_stride | q_head_stride) & 7))
+        return I4MM_ERR_ALIGN;
+    if (!workspace || workspace_bytes < i4mm::cache_attention_workspace()) return I4MM_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return I4MM_ERR_ALIGN;
+    p.q = {q, q_token_stride, q_head_stride};
+    p.out = out;
+    p.table = (const int*)block_table;
+    p.seq_lens = (const int*)seq_lens;
+    p.cu_lens = (const int*)cu_lens;
+    p.workspace = workspace;
+    p.table_stride = table_stride;
+    p.table_width = (int)table_width;
+    p.requests = (int)requests;
+    p.tokens = (int)tokens;
+    p.q_heads = (int)q_heads;
+    p.group = (int)(q_heads / cache->heads);
+    p.window = (int)window;
+    p.scale = scale;
+    return finish(i4mm::cache_attention_launch(p, cache->type == I4MM_CACHE_E4M3, type == I4MM_TYPE_BF16, (int)max_len, (cudaStream_t)stream));
+}
+
+}  // extern "C"
