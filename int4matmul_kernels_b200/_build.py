@@ -20,7 +20,7 @@ INCLUDE_DIR = os.path.join(ROOT_DIR, "include")
 
 CAPI_LIB = os.path.join(LIB_DIR, "libint4matmul_b200.so")
 CUDA_SOURCES = ["capi.cu", "stream_kernel.cu", "umma_kernel.cu", "rows_kernel.cu", "pack_kernel.cu", "noalloc.cu", "rownorm_kernel.cu", "gather.cu",
-                "cache_capi.cu", "cache_plan_kernel.cu", "cache_write_kernel.cu", "cache_attention_kernel.cu"]
+                "cache_capi.cu", "cache_plan_kernel.cu", "cache_write_kernel.cu", "cache_rows_kernel.cu", "cache_prompt_kernel.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

@@ -48,6 +48,7 @@ struct AttentionParams {
     const int* seq_lens;
     const int* cu_lens;                               // or nullptr: one row for each request
     void* workspace;
+    size_t prompt_parts;                              // where in it the prompt kernel's parts lie
     long long table_stride;
     int table_width, requests, tokens, q_heads, group; // group = q_heads / cache.heads
     int window;                                       // 0: none
@@ -59,7 +60,5 @@ cudaError_t cache_write_launch(const CacheView& c, bool e4m3, const RowsView& k,
                                cudaStream_t stream);
 cudaError_t cache_read_launch(const CacheView& c, bool e4m3, void* k_out, void* v_out, bool bf16, int tokens, const int* slots,
                               cudaStream_t stream);
-cudaError_t cache_attention_launch(const AttentionParams& p, bool e4m3, bool bf16, int max_len, cudaStream_t stream);
-size_t cache_attention_workspace();
 
 }  // namespace i4mm

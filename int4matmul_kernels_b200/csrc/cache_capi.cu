@@ -1,7 +1,9 @@
 // extern "C" entry points of the paged 8-bit key-value cache: argument validation and launches.
 #include "../../include/int4matmul_b200.h"
 
-#include "cache.cuh"
+#include <algorithm>
+
+#include "cache_attention.cuh"
 #include "common.cuh"
 
 namespace {
@@ -50,6 +52,18 @@ int view_of(const i4mm_cache* c, i4mm::CacheView& w) {
     w.page_shift = shift_of(c->page_size);
     w.dim = (int)c->head_dim;
     return I4MM_OK;
+}
+
+size_t attention_workspace() { return i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace() + i4mm::cache_prompt_workspace(); }
+
+// Which kernel.  A request's rows are its new tokens times the query heads of a key head.  Up to 16 of them, the few-row kernel reads the
+// cache once and is bound by that; more of them are the prompt kernel's.  Where a batch may have both, both run, each on its own requests.
+cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t max_len, cudaStream_t stream) {
+    const int64_t rows = (p.cu_lens ? std::max<int64_t>(max_len, 1) : 1) * p.group;
+    if (rows <= i4mm::kFewRows) return i4mm::cache_rows_launch(p, e4m3, bf16, 0x7FFFFFFF, rows <= 8, stream);
+    if (p.group > i4mm::kFewRows) return i4mm::cache_prompt_launch(p, e4m3, bf16, 1, true, stream);
+    const cudaError_t e = i4mm::cache_rows_launch(p, e4m3, bf16, i4mm::kFewRows, p.group <= 8, stream);
+    return e != cudaSuccess ? e : i4mm::cache_prompt_launch(p, e4m3, bf16, i4mm::kFewRows + 1, false, stream);
 }
 
 }  // namespace
@@ -120,7 +134,7 @@ int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type,
                                           (const int*)slots, (cudaStream_t)stream));
 }
 
-size_t i4mm_cache_attention_workspace_bytes(void) { return i4mm::cache_attention_workspace(); }
+size_t i4mm_cache_attention_workspace_bytes(void) { return attention_workspace(); }
 
 int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,
                          int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
@@ -140,7 +154,7 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
     if (!aligned(out, 16) || !aligned(q, 16) || !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(cu_lens, 4) ||
         ((q_token_stride | q_head_stride) & 7))
         return I4MM_ERR_ALIGN;
-    if (!workspace || workspace_bytes < i4mm::cache_attention_workspace()) return I4MM_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < attention_workspace()) return I4MM_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return I4MM_ERR_ALIGN;
     p.q = {q, q_token_stride, q_head_stride};
     p.out = out;
@@ -148,6 +162,7 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
     p.seq_lens = (const int*)seq_lens;
     p.cu_lens = (const int*)cu_lens;
     p.workspace = workspace;
+    p.prompt_parts = i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace();
     p.table_stride = table_stride;
     p.table_width = (int)table_width;
     p.requests = (int)requests;
@@ -156,7 +171,7 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
     p.group = (int)(q_heads / cache->heads);
     p.window = (int)window;
     p.scale = scale;
-    return finish(i4mm::cache_attention_launch(p, cache->type == I4MM_CACHE_E4M3, type == I4MM_TYPE_BF16, (int)max_len, (cudaStream_t)stream));
+    return finish(attend(p, cache->type == I4MM_CACHE_E4M3, type == I4MM_TYPE_BF16, max_len, (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -23,17 +23,12 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "cache.cuh"
-#include "common.cuh"
-#include "ptx.cuh"
+#include "cache_attention.cuh"
 
 namespace i4mm {
 namespace {
 
-constexpr uint32_t kAll = 0xFFFFFFFFu;
 constexpr int kTile = 16;                             // tokens; divides every page size
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxBlocks = 148;
 constexpr int kMinBlockTiles = 8, kMinWarpTiles = 2;  // fewer tiles than this are not cut further
 constexpr uint32_t kNoPage = 0x7FC0DEADu;             // in the place of a scale: there is no such page
 
@@ -49,37 +44,19 @@ struct Shape {
     static_assert(kPartFloats * 4 <= kWarpBytes, "a warp leaves its last part in its ring");
 };
 
-// ---- the workspace: [a counter per block][a part per warp][two parts per block] --------------------------------------------------
-constexpr size_t kCountersBytes = 1024;
+// ---- behind the workspace's header: [a part per warp][two parts per block] ----
 constexpr size_t kWarpPartsBytes = (size_t)kMaxBlocks * 12 * Shape<128, 2>::kPartFloats * 4;
 static_assert(16 * Shape<128, 1>::kPartFloats <= 12 * Shape<128, 2>::kPartFloats, "room for either shape");
 constexpr size_t kBlockPartsBytes = (size_t)kMaxBlocks * 2 * Shape<128, 2>::kPartFloats * 4;
 
-// ---- a request as the kernel sees it ---------------------------------------------------------------------------------------------
-struct Request {
-    int row0, rows;                                   // its packed rows
-    int position;                                     // of the first of them
-    int lo, limit;                                    // tokens lo .. limit - 1 may be seen
-    int tiles;                                        // from lo / 16 on; at least one if there are rows (rows that see nothing are written too)
+// a request and its tiles of tokens: at least one if there are rows (rows that see nothing are written too)
+struct Few : Request {
+    int tiles;
 };
-
-__device__ __forceinline__ Request load_request(const AttentionParams& p, int b) {
-    Request r;
-    const int seq = p.seq_lens[b];
-    int n = 1;
-    if (p.cu_lens) {
-        const int from = p.cu_lens[b], to = p.cu_lens[b + 1];
-        n = to - from;
-        r.row0 = min(max(from, 0), p.tokens);
-        r.rows = max(min(to, p.tokens) - r.row0, 0);
-    } else {
-        r.row0 = b;
-        r.rows = 1;
-    }
-    r.position = seq - n;
-    r.limit = max(min(min(seq, r.position + r.rows), p.table_width << p.cache.page_shift), 0);
-    r.lo = p.window && r.position >= p.window ? r.position - p.window + 1 : 0;
-    if (r.lo > r.limit) r.lo = r.limit;
+__device__ __forceinline__ Few load_few(const AttentionParams& p, int most_rows, int b) {
+    Few r;
+    static_cast<Request&>(r) = load_request(p, b);
+    if ((long long)r.rows * p.group > most_rows) r.rows = 0;    // the other kernel's
     r.tiles = max((r.limit + kTile - 1) / kTile - r.lo / kTile, 1);
     return r;
 }
@@ -91,8 +68,8 @@ __device__ __forceinline__ int row_tiles(const AttentionParams& p, const Request
 }
 
 template <int ROWS>
-__device__ __forceinline__ long long units_of(const AttentionParams& p, int b) {
-    const Request r = load_request(p, b);
+__device__ __forceinline__ long long units_of(const AttentionParams& p, int most_rows, int b) {
+    const Few r = load_few(p, most_rows, b);
     if (r.rows == 0) return 0;
     return (long long)r.tiles * p.cache.heads * row_tiles<ROWS>(p, r);
 }
@@ -100,20 +77,20 @@ __device__ __forceinline__ long long units_of(const AttentionParams& p, int b) {
 // A place in the row of all tiles.
 struct Cursor {
     long long left;                                   // tiles of the range from here on
-    Request r;
+    Few r;
     int b, segment, segments, tile;                   // the segment within the request, the tile within the segment
 };
 
 template <int ROWS>
-__device__ __forceinline__ void enter_request(const AttentionParams& p, Cursor& c) {
-    c.r = load_request(p, c.b);
+__device__ __forceinline__ void enter_request(const AttentionParams& p, int most_rows, Cursor& c) {
+    c.r = load_few(p, most_rows, c.b);
     c.segments = p.cache.heads * row_tiles<ROWS>(p, c.r);
     c.segment = 0;
     c.tile = 0;
 }
 
 template <int ROWS>
-__device__ __forceinline__ void advance(const AttentionParams& p, Cursor& c) {
+__device__ __forceinline__ void advance(const AttentionParams& p, int most_rows, Cursor& c) {
     if (--c.left == 0) return;
     if (++c.tile < c.r.tiles) return;
     c.tile = 0;
@@ -123,7 +100,7 @@ __device__ __forceinline__ void advance(const AttentionParams& p, Cursor& c) {
             c.left = 0;
             return;
         }
-        enter_request<ROWS>(p, c);
+        enter_request<ROWS>(p, most_rows, c);
     } while (c.r.rows == 0);
 }
 
@@ -137,43 +114,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// two e4m3 bytes (low and high) -> two fp16
-__device__ __forceinline__ uint32_t e4m3_to_h2(uint32_t two) {
-    uint32_t d;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(two));
-    return d;
-}
-__device__ __forceinline__ uint32_t int8_to_h2(uint32_t masked) { return hsub2_u(masked ^ 0x64806480u, 0x64806480u); }   // bytes 0 and 2: 1152 + q
-// 4 bytes -> 2 x 2 fp16.  int8: bytes (0, 2) and (1, 3); e4m3: (0, 1) and (2, 3)
-template <bool E4M3>
-__device__ __forceinline__ void decode4(uint32_t w, uint32_t& x, uint32_t& y) {
-    if (E4M3) {
-        x = e4m3_to_h2(w);
-        y = e4m3_to_h2(w >> 16);
-    } else {
-        x = int8_to_h2(w & 0x00FF00FFu);
-        y = int8_to_h2((w >> 8) & 0x00FF00FFu);
-    }
-}
-// bytes 2 * half, 2 * half + 1 of two rows a, b -> fp16 pairs (a, b) of the one place and of the next
-template <bool E4M3>
-__device__ __forceinline__ void decode_pair(uint32_t a, uint32_t b, int half, uint32_t& x, uint32_t& y) {
-    if (E4M3) {
-        const uint32_t w = prmt(a, b, half ? 0x7362 : 0x5140);
-        x = e4m3_to_h2(w);
-        y = e4m3_to_h2(w >> 16);
-    } else {
-        const uint32_t w = prmt(a, b, half ? 0x7632 : 0x5410);
-        x = int8_to_h2(w & 0x00FF00FFu);
-        y = int8_to_h2((w >> 8) & 0x00FF00FFu);
-    }
-}
-
 __device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src, uint32_t src_bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
@@ -183,12 +123,7 @@ __device__ __forceinline__ void sts64(uint32_t addr, uint32_t a, uint32_t b) {
 
 template <bool BF16>
 __device__ __forceinline__ void store4(void* out, long long at, float a, float b, float c, float d) {
-    if (BF16) {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-    } else {
-        *reinterpret_cast<uint2*>(static_cast<__half*>(out) + at) = make_uint2(h2_as_u32(__floats2half2_rn(a, b)), h2_as_u32(__floats2half2_rn(c, d)));
-    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) = make_uint2(pack_out<BF16>(a, b), pack_out<BF16>(c, d));
 }
 
 // a part of a segment that a range has cut: where the segment lies among all tiles, and which one it is
@@ -198,7 +133,7 @@ struct Piece {
 };
 
 template <bool E4M3, bool BF16, int D, int NT>
-__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(const AttentionParams p, int most_rows) {
     using S = Shape<D, NT>;
     constexpr int kSteps = D / 16, kWords = D / 32;   // k steps of 16; words of 4 bytes that a thread has of a value row
     extern __shared__ __align__(16) uint8_t ring[];
@@ -219,7 +154,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
 
     // all tiles; the block's range and the warp's
     long long total = 0;
-    for (int b = lane; b < p.requests; b += 32) total += units_of<S::kRows>(p, b);
+    for (int b = lane; b < p.requests; b += 32) total += units_of<S::kRows>(p, most_rows, b);
 #pragma unroll
     for (int d = 16; d; d /= 2) total += __shfl_xor_sync(kAll, total, d);
     const long long blocks = min((long long)gridDim.x, (total + kMinBlockTiles - 1) / kMinBlockTiles);
@@ -232,7 +167,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         s_tail[warp].from = -1;
     }
 
-    float* const warp_part = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + kCountersBytes) + ((size_t)blockIdx.x * S::kWarps + warp) * S::kPartFloats;
+    float* const warp_part = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + kCacheHeaderBytes) + ((size_t)blockIdx.x * S::kWarps + warp) * S::kPartFloats;
     const uint32_t my_ring = ptx::smem_u32(ring) + warp * S::kWarpBytes;
 
     if (u0 < u1) {
@@ -242,7 +177,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
             long long before = 0;
             int base = 0;
             for (;; base += 32) {
-                const long long own = base + lane < p.requests ? units_of<S::kRows>(p, base + lane) : 0;
+                const long long own = base + lane < p.requests ? units_of<S::kRows>(p, most_rows, base + lane) : 0;
                 long long sum = own;
 #pragma unroll
                 for (int d = 1; d < 32; d *= 2) {
@@ -260,7 +195,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                 if (base + 32 >= p.requests) break;   // (as above)
             }
             cur.b = min(base, p.requests - 1);
-            enter_request<S::kRows>(p, cur);
+            enter_request<S::kRows>(p, most_rows, cur);
             const long long in = u0 - before;
             cur.segment = (int)(in / cur.r.tiles);
             cur.tile = (int)(in - (long long)cur.segment * cur.r.tiles);
@@ -301,7 +236,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                 if (there) cp_async_8(fill + 32 * D + lane * 8, cache.scales + page * cache.heads + head, 8);
                 else sts64(fill + 32 * D + lane * 8, kNoPage, kNoPage);
                 const int b = ahead.b;
-                advance<S::kRows>(p, ahead);
+                advance<S::kRows>(p, most_rows, ahead);
                 if (ahead.left > 0) {
                     if (ahead.b != b) rt = row_tiles<S::kRows>(p, ahead.r);
                     id = page_of(ahead);
@@ -316,12 +251,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         uint32_t stage = my_ring;
         long long at = u0;
         while (at < u1) {
-            const Request r = cur.r;
+            const Few r = cur.r;
             const int tiles_here = (int)min((long long)(r.tiles - cur.tile), u1 - at), first_tile = cur.tile;
             const int row_tile_count = row_tiles<S::kRows>(p, r), head = cur.segment / row_tile_count, base = (cur.segment - head * row_tile_count) * S::kRows;
             const int b = cur.b, segment = cur.segment, all_rows = r.rows * p.group;
-            // q as the second operand of the score products: the lane's row is base + 8 * n + g.  bf16 is brought into fp16's range by a power
-            // of two for each row.
+            // q as the second operand of the score products: the lane's row is base + 8 * n + g
             uint32_t q[NT][2 * kSteps];
             float factor[NT][2], m[NT][2], sum[NT][2], o[NT][2 * kWords][4];
             int position[NT][2];                      // of the lane's rows of the products' results, base + 8 * n + 2 * t and the next: -1 if there is none
@@ -336,28 +270,21 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
 #pragma unroll
                     for (int s = 0; s < kSteps; ++s) w[s] = *reinterpret_cast<const uint2*>(from + 64 * (s >> 2) + 4 * (s & 3));
                     if (BF16) {
-                        float most = 0.f;
+                        float most = 0.f, down;
 #pragma unroll
-                        for (int s = 0; s < kSteps; ++s)
-                            most = fmaxf(most, fmaxf(fmaxf(fabsf(__uint_as_float(w[s].x << 16)), fabsf(__uint_as_float(w[s].x & 0xFFFF0000u))),
-                                                     fmaxf(fabsf(__uint_as_float(w[s].y << 16)), fabsf(__uint_as_float(w[s].y & 0xFFFF0000u)))));
+                        for (int s = 0; s < kSteps; ++s) most = fmaxf(most, bf16_most(w[s]));
                         const uint32_t peers = 0xFu << (lane & 28);
                         most = fmaxf(most, __shfl_xor_sync(peers, most, 1));
                         most = fmaxf(most, __shfl_xor_sync(peers, most, 2));
-                        // 2^e <= most < 2^(e + 1): q * 2^-e is below 2
-                        const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
-                        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                        mine = __uint_as_float((uint32_t)(127 + e) << 23);
+                        bf16_powers(most, mine, down);
 #pragma unroll
-                        for (int s = 0; s < kSteps; ++s) {
-                            w[s].x = h2_as_u32(__floats2half2_rn(__uint_as_float(w[s].x << 16) * down, __uint_as_float(w[s].x & 0xFFFF0000u) * down));
-                            w[s].y = h2_as_u32(__floats2half2_rn(__uint_as_float(w[s].y << 16) * down, __uint_as_float(w[s].y & 0xFFFF0000u) * down));
-                        }
+                        for (int s = 0; s < kSteps; ++s) w[s] = bf16_scaled(w[s], down);
                     }
 #pragma unroll
                     for (int s = 0; s < kSteps; ++s) {
-                        q[n][2 * s] = E4M3 ? w[s].x : prmt(w[s].x, w[s].y, 0x5410);       // the order that decode4 gives
-                        q[n][2 * s + 1] = E4M3 ? w[s].y : prmt(w[s].x, w[s].y, 0x7632);
+                        const uint2 x = key_order<E4M3>(w[s]);
+                        q[n][2 * s] = x.x;
+                        q[n][2 * s + 1] = x.y;
                     }
                 } else {
 #pragma unroll
@@ -482,7 +409,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                     }
                 }
                 stage = stage + S::kStageBytes == my_ring + S::kWarpBytes ? my_ring : stage + S::kStageBytes;
-                advance<S::kRows>(p, cur);
+                advance<S::kRows>(p, most_rows, cur);
             }
             at += tiles_here;
 #pragma unroll
@@ -561,14 +488,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         if constexpr (kMine == 4) {
             store4<BF16>(p.out, to, a.o[0] * f, a.o[1] * f, a.o[2] * f, a.o[3] * f);
         } else {
-            if (BF16) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + to) = __floats2bfloat162_rn(a.o[0] * f, a.o[1] * f);
-            else *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + to) = __floats2half2_rn(a.o[0] * f, a.o[1] * f);
+            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + to) = pack_out<BF16>(a.o[0] * f, a.o[1] * f);
         }
     };
-    float* const block_parts = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + kCountersBytes + kWarpPartsBytes);
+    float* const block_parts = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + kCacheHeaderBytes + kWarpPartsBytes);
     const auto ring_part = [&](int w) { return reinterpret_cast<const float*>(ring + w * S::kWarpBytes); };
     const auto workspace_part = [&](int w) {
-        return reinterpret_cast<const float*>(static_cast<const uint8_t*>(p.workspace) + kCountersBytes) + ((size_t)blockIdx.x * S::kWarps + w) * S::kPartFloats;
+        return reinterpret_cast<const float*>(static_cast<const uint8_t*>(p.workspace) + kCacheHeaderBytes) + ((size_t)blockIdx.x * S::kWarps + w) * S::kPartFloats;
     };
     int item = 0;
     for (int l = -1; l < S::kWarps; ++l) {
@@ -618,7 +544,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         const Piece& piece = cut[threadIdx.x];
         if (piece.from >= 0) {
             const int a = range_owner(total, blocks, piece.from), z = range_owner(total, blocks, piece.to - 1);
-            unsigned int* const counter = static_cast<unsigned int*>(p.workspace) + a;
+            unsigned int* const counter = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(p.workspace) + kRowsCounters) + a;
             __threadfence();
             if (atomicAdd(counter, 1u) == (unsigned int)(z - a)) {
                 last = 1;
@@ -641,7 +567,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
 }
 
 template <bool E4M3, bool BF16, int D, int NT>
-cudaError_t launch_rows(const AttentionParams& p, cudaStream_t stream) {
+cudaError_t launch_rows(const AttentionParams& p, int most_rows, cudaStream_t stream) {
     using S = Shape<D, NT>;
     const auto kernel = cache_rows_kernel<E4M3, BF16, D, NT>;
     constexpr int kSmem = S::kWarps * S::kWarpBytes;
@@ -657,20 +583,21 @@ cudaError_t launch_rows(const AttentionParams& p, cudaStream_t stream) {
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    e = cudaLaunchKernelEx(&cfg, kernel, p, most_rows);
     if (e == cudaSuccess) count_launch();
     return e;
 }
 
 }  // namespace
 
-size_t cache_attention_workspace() { return kCountersBytes + kWarpPartsBytes + kBlockPartsBytes; }
+size_t cache_rows_workspace() { return kWarpPartsBytes + kBlockPartsBytes; }
 
-cudaError_t cache_attention_launch(const AttentionParams& p, bool e4m3, bool bf16, int max_len, cudaStream_t stream) {
+// Two column tiles (16 rows) where a request may have more than 8 rows: its bytes are decoded once for both.
+cudaError_t cache_rows_launch(const AttentionParams& p, bool e4m3, bool bf16, int most_rows, bool few, cudaStream_t stream) {
     const auto by_rows = [&](auto e, auto h, auto d) {
         constexpr bool E = decltype(e)::value, H = decltype(h)::value;
         constexpr int D = decltype(d)::value;
-        return (long long)std::max(max_len, 1) * p.group <= 8 ? launch_rows<E, H, D, 1>(p, stream) : launch_rows<E, H, D, 2>(p, stream);
+        return few ? launch_rows<E, H, D, 1>(p, most_rows, stream) : launch_rows<E, H, D, 2>(p, most_rows, stream);
     };
     const auto by_dim = [&](auto e, auto h) {
         return p.cache.dim == 128 ? by_rows(e, h, std::integral_constant<int, 128>{}) : by_rows(e, h, std::integral_constant<int, 64>{});
