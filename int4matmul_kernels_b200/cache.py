@@ -22,7 +22,6 @@ from . import capi, ops
 
 _HELD = {torch.int8: capi.CACHE_INT8, torch.float8_e4m3fn: capi.CACHE_E4M3}
 _INPUT = {torch.float16: capi.TYPE_FP16, torch.bfloat16: capi.TYPE_BF16}
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
 
 
 class Plan(NamedTuple):
@@ -38,10 +37,10 @@ class Plan(NamedTuple):
 
 def _workspace(device: torch.device, stream: torch.cuda.Stream) -> torch.Tensor:
     key = (device.index if device.index is not None else torch.cuda.current_device(), stream.cuda_stream)
-    ws = _workspaces.get(key)
+    ws = ops._cache_workspaces.get(key)
     if ws is None:
         ws = torch.zeros(capi.load().i4mm_cache_attention_workspace_bytes(), dtype=torch.uint8, device=device)
-        _workspaces[key] = ws
+        ops._cache_workspaces[key] = ws
     return ws
 
 
@@ -112,6 +111,12 @@ def plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tens
     entries free: the pages of requests that end are pushed, then new ones popped, in request order.  seq_lens, new_lens and
     free_count are left alone: the next step takes the Plan's.  Where no page is left the table's entry and the slots become -1 and
     Plan.missing counts it."""
+    mod = ops.native()
+    if mod:
+        out = mod._try_cache_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens)
+        if not isinstance(out, int):
+            return Plan._make(out)
+        _check(max(out, 0), "cache plan")
     if not seq_lens.is_cuda:
         raise ValueError("seq_lens must be a CUDA tensor")
     dev, n = seq_lens.device, seq_lens.shape[0] if seq_lens.dim() == 1 else -1
@@ -144,6 +149,12 @@ def write(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, k:
     The tokens of a page that one call writes are neighbours with ascending slots, as `plan` lays them out.  A page's scale is
     the least power of two that holds its values; where new tokens raise it, the bytes that the page holds already are requantised.  A page
     whose first place is written begins anew."""
+    mod = ops.native()
+    if mod:
+        status = mod._try_cache_write(k_cache, v_cache, scales, k, v, slots)
+        if status == capi.OK:
+            return
+        _check(max(status, 0), "cache write")
     c = _cache(k_cache, v_cache, scales)
     dev = k_cache.device
     kind = _rows(k, "k", dev, c.heads, c.head_dim)
@@ -162,6 +173,12 @@ def write(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, k:
 def read(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, slots: torch.Tensor,
          dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
     """k, v (len(slots), heads, head_dim): the values that the cache holds at `slots` (zeros for slots outside of it)."""
+    mod = ops.native() if dtype in _INPUT else False
+    if mod:
+        out = mod._try_cache_read(k_cache, v_cache, scales, slots, dtype == torch.bfloat16)
+        if not isinstance(out, int):
+            return out
+        _check(max(out, 0), "cache read")
     c = _cache(k_cache, v_cache, scales)
     dev = k_cache.device
     if dtype not in _INPUT:
@@ -186,6 +203,12 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sca
     cu_lens[b] .. cu_lens[b + 1] (without cu_lens: row b) are the last tokens of request b, which has seq_lens[b] tokens in the cache, their
     own included; each sees the tokens up to its own, with window > 0 the last `window` of them.  A row that sees none is 0.
     `max_len`: the most rows of a request.  `scale`: 1 / sqrt(head_dim) unless given."""
+    mod = ops.native()
+    if mod:
+        out = mod._try_cache_attention(q, k_cache, v_cache, scales, block_table, seq_lens, cu_lens, max_len, scale, window, ops._cache_workspaces)
+        if not isinstance(out, int):
+            return out
+        _check(max(out, 0), "cache attention")
     c = _cache(k_cache, v_cache, scales)
     dev = k_cache.device
     kind = _rows(q, "q", dev, None, c.head_dim)

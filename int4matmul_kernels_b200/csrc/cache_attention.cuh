@@ -1,6 +1,8 @@
 // What the two attention kernels of the paged 8-bit cache share: a request as they see it, the decoding of bytes, the workspace.
 #pragma once
 
+#include <cuda.h>
+
 #include "cache.cuh"
 #include "common.cuh"
 #include "ptx.cuh"
@@ -52,13 +54,24 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float log2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLeastScale = 7.888609e-31f;          // 2^-100 in the place of a value scale of 0: its bytes are 0, its tokens still have weight
 // two e4m3 bytes (low and high) -> two fp16
 __device__ __forceinline__ uint32_t e4m3_to_h2(uint32_t two) {
     uint32_t d;
     asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(two));
     return d;
 }
-__device__ __forceinline__ uint32_t int8_to_h2(uint32_t masked) { return hsub2_u(masked ^ 0x64806480u, 0x64806480u); }   // bytes 0 and 2: 1152 + q
+// bytes 0 and 2 of w -> two fp16: in the mantissa of 1024, with the sign bit turned over, q is 1152 + q
+__device__ __forceinline__ uint32_t int8_to_h2(uint32_t w) {
+    uint32_t x;
+    asm("lop3.b32 %0, %1, 0x00FF00FF, %2, 0x6A;" : "=r"(x) : "r"(w), "r"(0x64806480u));    // (w & 0x00FF00FF) ^ 0x64806480
+    return hsub2_u(x, 0x64806480u);
+}
 // 4 bytes -> 2 x 2 fp16.  int8: bytes (0, 2) and (1, 3); e4m3: (0, 1) and (2, 3)
 template <bool E4M3>
 __device__ __forceinline__ void decode4(uint32_t w, uint32_t& x, uint32_t& y) {
@@ -66,8 +79,8 @@ __device__ __forceinline__ void decode4(uint32_t w, uint32_t& x, uint32_t& y) {
         x = e4m3_to_h2(w);
         y = e4m3_to_h2(w >> 16);
     } else {
-        x = int8_to_h2(w & 0x00FF00FFu);
-        y = int8_to_h2((w >> 8) & 0x00FF00FFu);
+        x = int8_to_h2(w);
+        y = int8_to_h2(w >> 8);
     }
 }
 // four fp16 of a query in the order that decode4 gives the keys
@@ -84,8 +97,8 @@ __device__ __forceinline__ void decode_pair(uint32_t a, uint32_t b, int half, ui
         y = e4m3_to_h2(w >> 16);
     } else {
         const uint32_t w = prmt(a, b, half ? 0x7632 : 0x5410);
-        x = int8_to_h2(w & 0x00FF00FFu);
-        y = int8_to_h2((w >> 8) & 0x00FF00FFu);
+        x = int8_to_h2(w);
+        y = int8_to_h2(w >> 8);
     }
 }
 
@@ -117,6 +130,8 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
 // Prompts: requests of fewer than least_rows rows are left to the other one; `alone`: it is not launched.
 cudaError_t cache_rows_launch(const AttentionParams& p, bool e4m3, bool bf16, int most_rows, bool few, cudaStream_t stream);
 cudaError_t cache_prompt_launch(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, bool alone, cudaStream_t stream);
+bool encode_bytes(CUtensorMap* out, int rank, const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+                  CUtensorMapSwizzle swizzle);        // umma_kernel.cu
 size_t cache_rows_workspace();                        // bytes behind the header
 size_t cache_prompt_workspace();                      // bytes behind those
 

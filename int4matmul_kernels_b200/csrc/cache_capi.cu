@@ -36,16 +36,24 @@ int view_of(const i4mm_cache* c, i4mm::CacheView& w) {
     if (shift_of(c->page_size) < 0) return I4MM_ERR_UNSUPPORTED;
     if (c->pages <= 0 || c->heads <= 0 || c->heads > 65535 || c->pages > kMost / c->page_size) return I4MM_ERR_SHAPE;
     if (!c->k || !c->v || !c->scales) return I4MM_ERR_NULL;
+    for (const int64_t stride : {c->k_page_stride, c->k_head_stride, c->k_token_stride, c->v_page_stride, c->v_head_stride, c->v_token_stride})
+        if (stride < 0 || stride > kMost) return I4MM_ERR_SHAPE;
     const int64_t strides = c->k_page_stride | c->k_head_stride | c->k_token_stride | c->v_page_stride | c->v_head_stride | c->v_token_stride;
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 8) || (strides & 15)) return I4MM_ERR_ALIGN;
+    // (the stride of a single page, head or token says nothing)
+    const int64_t one = c->head_dim;
+    const auto stride = [&](int64_t n, int64_t s) { return n > 1 ? s : std::max(s, one); };
+    for (const int64_t s : {stride(c->pages, c->k_page_stride), stride(c->heads, c->k_head_stride), stride(c->pages, c->v_page_stride),
+                            stride(c->heads, c->v_head_stride), c->k_token_stride, c->v_token_stride})
+        if (s < one) return I4MM_ERR_SHAPE;
     w.k = (uint8_t*)c->k;
     w.v = (uint8_t*)c->v;
     w.scales = (float2*)c->scales;
-    w.k_page = c->k_page_stride;
-    w.k_head = c->k_head_stride;
+    w.k_page = stride(c->pages, c->k_page_stride);
+    w.k_head = stride(c->heads, c->k_head_stride);
     w.k_token = c->k_token_stride;
-    w.v_page = c->v_page_stride;
-    w.v_head = c->v_head_stride;
+    w.v_page = stride(c->pages, c->v_page_stride);
+    w.v_head = stride(c->heads, c->v_head_stride);
     w.v_token = c->v_token_stride;
     w.pages = (int)c->pages;
     w.heads = (int)c->heads;

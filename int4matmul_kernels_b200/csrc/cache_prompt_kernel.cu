@@ -35,7 +35,6 @@ constexpr int kThreads = 32 * (kSchedule + 1);
 constexpr int kScaleSlots = 4;
 constexpr int kMinTiles = 4;                          // a part of a segment has at least so many tiles
 constexpr float kGrowth = 8.f;                        // log2 of what a weight may exceed its reference by
-constexpr float kLeastScale = 7.888609e-31f;          // 2^-100 in the place of a value scale of 0: its bytes are 0, its tokens still have weight
 
 template <int D>
 struct Layout {

@@ -9,8 +9,8 @@
 //   equal contiguous ranges, to the blocks (one to an SM) and within them to the warps, whatever the lengths are.  What a
 //   range cuts is joined: warps of a block through shared memory, blocks through the workspace, where the block that comes last adds up
 //   all parts in their order (so results do not depend on which one it is).  Nobody waits for anybody.
-// * Bytes.  A thread copies (cp.async) exactly the bytes that it will decode itself into a ring of its own, several tiles
-//   ahead: no barrier anywhere in the loop, and no registers are held by loads in flight.
+// * Bytes.  Each warp fetches its own tiles, two ahead, into a ring of its own (a TMA copy for each 16 keys and 16 values, swizzled, one
+//   barrier for a tile): warps do not wait for one another, and no registers are held by loads in flight.
 // * Products.  S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16: the cache is the 16-row operand, the head's rows are the 8 columns, so a
 //   tile costs 16 instructions for 8 rows.  The order of the 16 k of an instruction is free as long as both operands agree, so a thread
 //   takes 16 consecutive bytes of a key row (and the same places of q), and 16 consecutive bytes of each of its four value rows; two
@@ -28,25 +28,25 @@
 namespace i4mm {
 namespace {
 
-constexpr int kTile = 16;                             // tokens; divides every page size
-constexpr int kMinBlockTiles = 8, kMinWarpTiles = 2;  // fewer tiles than this are not cut further
+constexpr int kTile = 32;                             // tokens: two halves of 16, each within one page
+constexpr int kMinBlockTiles = 4, kMinWarpTiles = 1;  // fewer tiles than this are not cut further
 constexpr uint32_t kNoPage = 0x7FC0DEADu;             // in the place of a scale: there is no such page
 
 template <int D, int NT>
 struct Shape {
-    static constexpr int kWarps = NT == 1 ? 16 : 12;
+    static constexpr int kWarps = 8;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kRows = 8 * NT;
-    static constexpr int kStageBytes = 32 * D + 256;                          // a tile's keys, values, and 8 bytes of scales for each lane
-    static constexpr int kStages = D == 128 ? (NT == 1 ? 3 : 4) : (NT == 1 ? 5 : 6);
+    static constexpr int kHalfBytes = 32 * D;                                 // 16 tokens: keys, then values
+    static constexpr int kStageBytes = 2 * kHalfBytes;
+    static constexpr int kStages = D == 128 ? 3 : 6;
     static constexpr int kWarpBytes = kStages * kStageBytes;
     static constexpr int kPartFloats = kRows * D + 2 * kRows;                 // sums, maxima, totals of a part of a segment
     static_assert(kPartFloats * 4 <= kWarpBytes, "a warp leaves its last part in its ring");
 };
 
 // ---- behind the workspace's header: [a part per warp][two parts per block] ----
-constexpr size_t kWarpPartsBytes = (size_t)kMaxBlocks * 12 * Shape<128, 2>::kPartFloats * 4;
-static_assert(16 * Shape<128, 1>::kPartFloats <= 12 * Shape<128, 2>::kPartFloats, "room for either shape");
+constexpr size_t kWarpPartsBytes = (size_t)kMaxBlocks * Shape<128, 2>::kWarps * Shape<128, 2>::kPartFloats * 4;
 constexpr size_t kBlockPartsBytes = (size_t)kMaxBlocks * 2 * Shape<128, 2>::kPartFloats * 4;
 
 // a request and its tiles of tokens: at least one if there are rows (rows that see nothing are written too)
@@ -74,51 +74,26 @@ __device__ __forceinline__ long long units_of(const AttentionParams& p, int most
     return (long long)r.tiles * p.cache.heads * row_tiles<ROWS>(p, r);
 }
 
-// A place in the row of all tiles.
-struct Cursor {
-    long long left;                                   // tiles of the range from here on
-    Few r;
-    int b, segment, segments, tile;                   // the segment within the request, the tile within the segment
-};
-
-template <int ROWS>
-__device__ __forceinline__ void enter_request(const AttentionParams& p, int most_rows, Cursor& c) {
-    c.r = load_few(p, most_rows, c.b);
-    c.segments = p.cache.heads * row_tiles<ROWS>(p, c.r);
-    c.segment = 0;
-    c.tile = 0;
-}
-
-template <int ROWS>
-__device__ __forceinline__ void advance(const AttentionParams& p, int most_rows, Cursor& c) {
-    if (--c.left == 0) return;
-    if (++c.tile < c.r.tiles) return;
-    c.tile = 0;
-    if (++c.segment < c.segments) return;
-    do {
-        if (++c.b >= p.requests) {                    // (not unless the lengths change under the kernel)
-            c.left = 0;
-            return;
-        }
-        enter_request<ROWS>(p, most_rows, c);
-    } while (c.r.rows == 0);
-}
-
 // ---- decoding and products -----------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {   // onto zeros
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-__device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src, uint32_t src_bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
-}
-__device__ __forceinline__ void sts64(uint32_t addr, uint32_t a, uint32_t b) {
-    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+// The token of a half that the products' row (and k) index i stands for.  Any order is right as long as keys, values and masks agree;
+// in this one the lanes of a quarter warp, which read the swizzled rows of i = 2 j, 2 j + 1 (keys) and of i = 0, 2, 4, 6 (values), meet
+// in no bank (head_dim 128).
+__device__ __forceinline__ int token_of(int i) {
+    const int pair = (i & 7) >> 1;
+    return (i & 8) + ((2 * pair + (pair >> 1)) ^ ((i & 1) << 2));
 }
 
 template <bool BF16>
@@ -133,14 +108,25 @@ struct Piece {
 };
 
 template <bool E4M3, bool BF16, int D, int NT>
-__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(const AttentionParams p, int most_rows) {
+__global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(const AttentionParams p, int most_rows,
+                                                                              const __grid_constant__ CUtensorMap k_map,
+                                                                              const __grid_constant__ CUtensorMap v_map) {
     using S = Shape<D, NT>;
     constexpr int kSteps = D / 16, kWords = D / 32;   // k steps of 16; words of 4 bytes that a thread has of a value row
-    extern __shared__ __align__(16) uint8_t ring[];
+    extern __shared__ uint8_t dynamic[];
+    uint8_t* const ring = dynamic + (1024 - (ptx::smem_u32(dynamic) & 1023)) % 1024;
+    __shared__ unsigned long long s_full[S::kWarps][S::kStages];
+    __shared__ float2 s_scales[S::kWarps][S::kStages][2];
     __shared__ Piece s_head[S::kWarps], s_tail[S::kWarps];
     __shared__ int s_last[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const CacheView& cache = p.cache;
+    if (lane == 0) {
+        // two lanes fetch a half each: each of them arrives with the bytes that it expects, and once its scales are there
+        for (int i = 0; i < S::kStages; ++i) ptx::mbar_init(ptx::smem_u32(&s_full[warp][i]), 4);
+        ptx::fence_mbar_init();
+    }
+    __syncwarp();
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
 
@@ -171,13 +157,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
     const uint32_t my_ring = ptx::smem_u32(ring) + warp * S::kWarpBytes;
 
     if (u0 < u1) {
-        // the request that the range begins in
-        Cursor cur;
+        // the request that the range begins in, the segment within it and the tile within that
+        int b = 0, segment, tile;
+        Few r;
         {
             long long before = 0;
-            int base = 0;
-            for (;; base += 32) {
-                const long long own = base + lane < p.requests ? units_of<S::kRows>(p, most_rows, base + lane) : 0;
+            for (;; b += 32) {
+                const long long own = b + lane < p.requests ? units_of<S::kRows>(p, most_rows, b + lane) : 0;
                 long long sum = own;
 #pragma unroll
                 for (int d = 1; d < 32; d *= 2) {
@@ -188,73 +174,107 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                 if (here) {
                     const int l = __ffs(here) - 1;
                     before += __shfl_sync(kAll, sum - own, l);
-                    base += l;
+                    b += l;
                     break;
                 }
                 before += __shfl_sync(kAll, sum, 31);
-                if (base + 32 >= p.requests) break;   // (as above)
+                if (b + 32 >= p.requests) break;      // (not unless the lengths change under the kernel)
             }
-            cur.b = min(base, p.requests - 1);
-            enter_request<S::kRows>(p, most_rows, cur);
-            const long long in = u0 - before;
-            cur.segment = (int)(in / cur.r.tiles);
-            cur.tile = (int)(in - (long long)cur.segment * cur.r.tiles);
-            cur.left = u1 - u0;
+            b = min(b, p.requests - 1);
+            r = load_few(p, most_rows, b);
+            segment = (int)((u0 - before) / r.tiles);
+            tile = (int)(u0 - before - (long long)segment * r.tiles);
         }
 
-        // ---- copies ----
-        Cursor ahead = cur;
-        int rt = row_tiles<S::kRows>(p, ahead.r);
-        const auto page_of = [&](const Cursor& c) {
-            const int j = (c.r.lo / kTile + c.tile) >> (cache.page_shift - 4);
-            return j < p.table_width && c.r.limit > c.r.lo ? p.table[c.b * p.table_stride + j] : -1;
+        // ---- copies: the same tiles, kStages - 1 of them ahead.  Lanes 0 and 1 take a half each. ----
+        struct {
+            int left;                                 // tiles to be copied
+            int b, segment, segments, row_tiles, head;
+            int tile, end, lo, limit;                 // the tile (from the request's token 0), the segment's end, its tokens
+            const int* table;
+            int id;                                   // the page of the lane's half of the tile
+            int stage;
+        } c = {};
+        const int page_mask = (1 << cache.page_shift) - 1;
+        const auto enter_request = [&](const Few& r) {
+            c.row_tiles = row_tiles<S::kRows>(p, r);
+            c.segments = cache.heads * c.row_tiles;
+            c.tile = r.lo / kTile;
+            c.end = c.tile + r.tiles;
+            c.lo = r.lo;
+            c.limit = r.limit;
+            c.table = p.table + c.b * p.table_stride;
         };
-        int id = page_of(ahead);
-        uint32_t fill = my_ring;
+        const auto find_page = [&]() {                // (nothing is done with what is loaded before the next copy)
+            const int first = c.tile * kTile + 16 * (lane & 1), j = first >> cache.page_shift;
+            c.id = -1;
+            if (lane < 2 && first < c.limit && first + 16 > c.lo && c.limit > c.lo && j < p.table_width) c.id = c.table[j];
+        };
+        c.left = (int)(u1 - u0);
+        c.b = b;
+        c.segment = segment;
+        enter_request(r);
+        c.tile += tile;
+        c.head = segment / c.row_tiles;
+        find_page();
         const auto copy = [&]() {
-            if (ahead.left > 0) {
-                const int first = (ahead.r.lo / kTile + ahead.tile) * kTile, place = first & ((1 << cache.page_shift) - 1);
-                const int head = ahead.segment / rt;
-                const bool there = id >= 0 && id < cache.pages;
-                const long long page = there ? id : 0;
-                const uint8_t* const k = cache.k + page * cache.k_page + head * cache.k_head + (place + g) * cache.k_token + 16 * t;
-                const uint8_t* const v = cache.v + page * cache.v_page + head * cache.v_head + (place + 2 * t) * cache.v_token + (D / 8) * g;
-                // bytes of tokens that nobody sees are not brought in: they may be anything, and 0 * NaN is NaN
-                const auto seen = [&](int i) { return there && first + i >= ahead.r.lo && first + i < ahead.r.limit; };
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int j = 0; j < D / 64; ++j)
-                        ptx::cp_async_16(fill + (h * (D / 64) + j) * 512 + lane * 16, k + 8 * h * cache.k_token + 64 * j, there ? 16 : 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int token = (i & 1) + 8 * (i >> 1);
-                    const uint8_t* const from = v + token * cache.v_token;
-                    if (D == 128) ptx::cp_async_16(fill + 2048 + i * 512 + lane * 16, from, seen(2 * t + token) ? 16 : 0);
-                    else cp_async_8(fill + 1024 + i * 256 + lane * 8, from, seen(2 * t + token) ? 8 : 0);
-                }
-                if (there) cp_async_8(fill + 32 * D + lane * 8, cache.scales + page * cache.heads + head, 8);
-                else sts64(fill + 32 * D + lane * 8, kNoPage, kNoPage);
-                const int b = ahead.b;
-                advance<S::kRows>(p, most_rows, ahead);
-                if (ahead.left > 0) {
-                    if (ahead.b != b) rt = row_tiles<S::kRows>(p, ahead.r);
-                    id = page_of(ahead);
+            if (c.left <= 0) return;
+            if (lane < 2) {
+                const uint32_t bar = ptx::smem_u32(&s_full[warp][c.stage]), to = my_ring + c.stage * S::kStageBytes + lane * S::kHalfBytes;
+                if ((unsigned int)c.id < (unsigned int)cache.pages) {
+                    const int place = (c.tile * kTile + 16 * lane) & page_mask;
+                    ptx::mbar_arrive_expect_tx(bar, S::kHalfBytes);
+                    ptx::tma_load_4d(to, &k_map, 0, place, c.head, c.id, bar);
+                    ptx::tma_load_4d(to + 16 * D, &v_map, 0, place, c.head, c.id, bar);
+                    ptx::cp_async_8(ptx::smem_u32(&s_scales[warp][c.stage][lane]), cache.scales + (long long)c.id * cache.heads + c.head);
+                    ptx::cp_async_arrive(bar);
+                } else {
+                    s_scales[warp][c.stage][lane] = make_float2(__uint_as_float(kNoPage), 0.f);
+                    ptx::mbar_arrive(bar);
+                    ptx::mbar_arrive(bar);
                 }
             }
-            ptx::cp_async_commit();
-            fill = fill + S::kStageBytes == my_ring + S::kWarpBytes ? my_ring : fill + S::kStageBytes;
+            c.stage = c.stage + 1 == S::kStages ? 0 : c.stage + 1;
+            if (--c.left == 0) return;
+            if (++c.tile == c.end) {
+                if (++c.segment < c.segments) {
+                    c.tile = c.lo / kTile;
+                } else {
+                    c.segment = 0;
+                    Few next;
+                    do {
+                        ++c.b;
+                        if (c.b < p.requests) next = load_few(p, most_rows, c.b);
+                    } while (c.b < p.requests && next.rows == 0);
+                    if (c.b < p.requests) enter_request(next);
+                    else c.left = 0;                  // (as above)
+                }
+                c.head = c.segment / c.row_tiles;
+            }
+            find_page();
         };
         for (int i = 0; i < S::kStages - 1; ++i) copy();
 
+        // where the lane's bytes lie in a half
+        const int k_row = token_of(g), v_row0 = token_of(2 * t), v_row1 = token_of(2 * t + 1);
+        const auto keys_at = [&](int j) {             // chunk 4 * j + t of 16 bytes
+            return D == 128 ? k_row * 128 + (((4 * j + t) ^ (k_row & 7)) << 4) : k_row * 64 + ((t ^ ((k_row >> 1) & 3)) << 4);
+        };
+        const auto values_at = [&](int row) {         // D / 8 bytes from place D / 8 * g on
+            return 16 * D + (D == 128 ? row * 128 + ((g ^ (row & 7)) << 4) : row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + 8 * (g & 1));
+        };
+        const uint32_t keys_lane[2] = {(uint32_t)keys_at(0), (uint32_t)keys_at(D / 64 - 1)};
+        const uint32_t values_lane[2] = {(uint32_t)values_at(v_row0), (uint32_t)values_at(v_row1)};
+
         // ---- the segments of the range ----
-        uint32_t stage = my_ring;
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
         long long at = u0;
-        while (at < u1) {
-            const Few r = cur.r;
-            const int tiles_here = (int)min((long long)(r.tiles - cur.tile), u1 - at), first_tile = cur.tile;
-            const int row_tile_count = row_tiles<S::kRows>(p, r), head = cur.segment / row_tile_count, base = (cur.segment - head * row_tile_count) * S::kRows;
-            const int b = cur.b, segment = cur.segment, all_rows = r.rows * p.group;
+        while (at < u1 && ok) {
+            const int tiles_here = (int)min((long long)(r.tiles - tile), u1 - at);
+            const int row_tile_count = row_tiles<S::kRows>(p, r), head = segment / row_tile_count, base = (segment - head * row_tile_count) * S::kRows;
+            const int all_rows = r.rows * p.group;
             // q as the second operand of the score products: the lane's row is base + 8 * n + g
             uint32_t q[NT][2 * kSteps];
             float factor[NT][2], m[NT][2], sum[NT][2], o[NT][2 * kWords][4];
@@ -304,48 +324,75 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                     for (int i = 0; i < 4; ++i) o[n][j][i] = 0.f;
             }
 
-            for (int i = 0; i < tiles_here; ++i) {
+            // tiles that begin in [whole_from, whole_to] are seen whole by all rows of the tile of rows
+            const int whole_from = p.window ? max(r.position + r.rows - p.window, r.lo) : r.lo;
+            const int whole_to = base + S::kRows <= all_rows ? min(r.position + 1, r.limit) - kTile : -1;
+            int first = (r.lo / kTile + tile) * kTile;
+            for (int i = 0; i < tiles_here; ++i, first += kTile) {
+                __syncwarp();                         // (the stage that the copy goes to has been read)
                 copy();
-                ptx::cp_async_wait_group<S::kStages - 1>();
-                const int first = (r.lo / kTile + first_tile + i) * kTile;
-                // scores
-                float s[NT][4] = {};
-#pragma unroll
-                for (int j = 0; j < D / 64; ++j) {
-                    const uint4 ka = ptx::lds128(stage + j * 512 + lane * 16), kb = ptx::lds128(stage + (D / 64 + j) * 512 + lane * 16);
-                    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t a0, a1, a2, a3;
-                        decode4<E4M3>(wa[w], a0, a2);
-                        decode4<E4M3>(wb[w], a1, a3);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma(s[n], a0, a1, a2, a3, q[n][2 * (4 * j + w)], q[n][2 * (4 * j + w) + 1]);
-                    }
+                ok = __all_sync(kAll, ptx::mbar_wait(ptx::smem_u32(&s_full[warp][stage]), phase));
+                if (!ok) {
+                    if (lane == 0) atomicExch(reinterpret_cast<int*>(static_cast<uint8_t*>(p.workspace) + kStatusOffset), 62);
+                    break;
                 }
-                const uint2 both = ptx::lds64(stage + 32 * D + lane * 8);
-                const bool there = both.x != kNoPage;
-                const float k_scale = there ? __uint_as_float(both.x) : 0.f, v_scale = there ? __uint_as_float(both.y) : 0.f;
-                const bool whole = there && first >= r.lo && first + kTile - 1 <= r.position && first + kTile <= r.limit &&
-                                   (!p.window || first > r.position + r.rows - 1 - p.window) && base + S::kRows <= all_rows;
-                uint32_t high[NT][2], low[NT][2];
+                const uint32_t half0 = my_ring + stage * S::kStageBytes;
+                // scores
+                float s[NT][2][4];
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) {
+                        const uint32_t keys = half0 + half * S::kHalfBytes + keys_lane[j];
+                        const uint4 ka = ptx::lds128(keys), kb = ptx::lds128(keys + 8 * D);
+                        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            uint32_t a0, a1, a2, a3;
+                            decode4<E4M3>(wa[w], a0, a2);
+                            decode4<E4M3>(wb[w], a1, a3);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const uint32_t b0 = q[n][2 * (4 * j + w)], b1 = q[n][2 * (4 * j + w) + 1];
+                                if (j == 0 && w == 0) mma_first(s[n][half], a0, a1, a2, a3, b0, b1);
+                                else mma(s[n][half], a0, a1, a2, a3, b0, b1);
+                            }
+                        }
+                    }
+                bool there[2];
+                float k_scale[2], v_log2[2], v_inverse[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float2 both = s_scales[warp][stage][half];
+                    there[half] = __float_as_uint(both.x) != kNoPage;
+                    const float v_scale = there[half] ? fmaxf(both.y, kLeastScale) : 1.f;
+                    k_scale[half] = there[half] ? both.x : 0.f;
+                    v_log2[half] = log2_approx(v_scale);
+                    v_inverse[half] = exp2_approx(-v_log2[half]);
+                }
+                const bool whole = there[0] && there[1] && first >= whole_from && first <= whole_to;
+                uint32_t high[NT][2][2], low[NT][2][2];
                 float weight[NT][2];                  // of the tile's sums in the segment's
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float most[2];
 #pragma unroll
-                    for (int i2 = 0; i2 < 4; ++i2) s[n][i2] *= factor[n][i2 & 1] * k_scale;
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int i2 = 0; i2 < 4; ++i2) s[n][half][i2] = fmaf(s[n][half][i2], factor[n][i2 & 1] * k_scale[half], v_log2[half]);
                     if (!whole) {
 #pragma unroll
-                        for (int i2 = 0; i2 < 4; ++i2) {
-                            const int token = first + g + 8 * (i2 >> 1), at_row = position[n][i2 & 1];
-                            const bool sees = there && token <= at_row && token < r.limit && token >= r.lo && (!p.window || token > at_row - p.window);
-                            if (!sees) s[n][i2] = -INFINITY;
-                        }
+                        for (int half = 0; half < 2; ++half)
+#pragma unroll
+                            for (int i2 = 0; i2 < 4; ++i2) {
+                                const int token = first + 16 * half + k_row + 8 * (i2 >> 1), at_row = position[n][i2 & 1];
+                                const bool sees = there[half] && token <= at_row && token < r.limit && token >= r.lo && (!p.window || token > at_row - p.window);
+                                if (!sees) s[n][half][i2] = -INFINITY;
+                            }
                     }
 #pragma unroll
                     for (int i2 = 0; i2 < 2; ++i2) {
-                        float x = fmaxf(s[n][i2], s[n][2 + i2]);
+                        float x = fmaxf(fmaxf(s[n][0][i2], s[n][0][2 + i2]), fmaxf(s[n][1][i2], s[n][1][2 + i2]));
                         x = fmaxf(x, __shfl_xor_sync(kAll, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(kAll, x, 8));
                         most[i2] = fmaxf(x, __shfl_xor_sync(kAll, x, 16));
@@ -364,53 +411,84 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                             }
                         }
                     }
-                    float e[4];
+                    float e[2][4];
 #pragma unroll
                     for (int i2 = 0; i2 < 2; ++i2) {
                         const bool any = most[i2] != -INFINITY;
-                        const float from = any ? most[i2] : 0.f, up = any ? exp2_approx(most[i2] - m[n][i2]) : 0.f;
-                        e[i2] = exp2_approx(s[n][i2] - from);
-                        e[2 + i2] = exp2_approx(s[n][2 + i2] - from);
-                        sum[n][i2] += up * (e[i2] + e[2 + i2]);
-                        weight[n][i2] = up * v_scale;
+                        const float from = any ? most[i2] : 0.f;
+                        weight[n][i2] = any ? exp2_approx(most[i2] - m[n][i2]) : 0.f;
+                        float all = 0.f;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            e[half][i2] = exp2_approx(s[n][half][i2] - from);
+                            e[half][2 + i2] = exp2_approx(s[n][half][2 + i2] - from);
+                            all = fmaf(e[half][i2] + e[half][2 + i2], v_inverse[half], all);
+                        }
+                        sum[n][i2] = fmaf(weight[n][i2], all, sum[n][i2]);
                     }
 #pragma unroll
-                    for (int i2 = 0; i2 < 2; ++i2) {
-                        const __half2 h = __floats2half2_rn(e[2 * i2], e[2 * i2 + 1]);
-                        const float2 back = __half22float2(h);
-                        high[n][i2] = transpose8x8(h2_as_u32(h));
-                        low[n][i2] = transpose8x8(h2_as_u32(__floats2half2_rn(e[2 * i2] - back.x, e[2 * i2 + 1] - back.y)));
-                    }
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int i2 = 0; i2 < 2; ++i2) {
+                            const __half2 h = __floats2half2_rn(e[half][2 * i2], e[half][2 * i2 + 1]);
+                            const float2 back = __half22float2(h);
+                            high[n][half][i2] = transpose8x8(h2_as_u32(h));
+                            low[n][half][i2] = transpose8x8(h2_as_u32(__floats2half2_rn(e[half][2 * i2] - back.x, e[half][2 * i2 + 1] - back.y)));
+                        }
                 }
                 // values
-                uint32_t v[4][kWords];
+                uint32_t v[2][4][kWords];
 #pragma unroll
-                for (int i2 = 0; i2 < 4; ++i2) {
-                    if constexpr (D == 128) {
-                        const uint4 w = ptx::lds128(stage + 2048 + i2 * 512 + lane * 16);
-                        v[i2][0] = w.x; v[i2][1] = w.y; v[i2][2] = w.z; v[i2][3] = w.w;
-                    } else {
-                        const uint2 w = ptx::lds64(stage + 1024 + i2 * 256 + lane * 8);
-                        v[i2][0] = w.x; v[i2][1] = w.y;
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int i2 = 0; i2 < 4; ++i2) {
+                        const uint32_t values = half0 + half * S::kHalfBytes + values_lane[i2 & 1] + (i2 >> 1) * 8 * D;
+                        if constexpr (D == 128) {
+                            const uint4 w = ptx::lds128(values);
+                            v[half][i2][0] = w.x; v[half][i2][1] = w.y; v[half][i2][2] = w.z; v[half][i2][3] = w.w;
+                        } else {
+                            const uint2 w = ptx::lds64(values);
+                            v[half][i2][0] = w.x; v[half][i2][1] = w.y;
+                        }
                     }
+                if (!(there[0] && there[1] && first >= r.lo && first + kTile <= r.limit)) {
+                    // bytes of tokens that nobody sees may be anything, and 0 * NaN is NaN
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int i2 = 0; i2 < 4; ++i2) {
+                            const int token = first + 16 * half + (i2 & 1 ? v_row1 : v_row0) + 8 * (i2 >> 1);
+                            if (!(there[half] && token >= r.lo && token < r.limit))
+#pragma unroll
+                                for (int w = 0; w < kWords; ++w) v[half][i2][w] = 0;
+                        }
                 }
 #pragma unroll
                 for (int j = 0; j < 2 * kWords; ++j) {
-                    uint32_t a0, a1, a2, a3;
-                    decode_pair<E4M3>(v[0][j >> 1], v[1][j >> 1], j & 1, a0, a1);
-                    decode_pair<E4M3>(v[2][j >> 1], v[3][j >> 1], j & 1, a2, a3);
+                    float d[NT][4];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float d[4] = {};
-                        mma(d, a0, a1, a2, a3, low[n][0], low[n][1]);
-                        mma(d, a0, a1, a2, a3, high[n][0], high[n][1]);
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t a0, a1, a2, a3;
+                        decode_pair<E4M3>(v[half][0][j >> 1], v[half][1][j >> 1], j & 1, a0, a1);
+                        decode_pair<E4M3>(v[half][2][j >> 1], v[half][3][j >> 1], j & 1, a2, a3);
 #pragma unroll
-                        for (int i2 = 0; i2 < 4; ++i2) o[n][j][i2] += weight[n][i2 & 1] * d[i2];
+                        for (int n = 0; n < NT; ++n) {
+                            if (half == 0) mma_first(d[n], a0, a1, a2, a3, low[n][half][0], low[n][half][1]);
+                            else mma(d[n], a0, a1, a2, a3, low[n][half][0], low[n][half][1]);
+                            mma(d[n], a0, a1, a2, a3, high[n][half][0], high[n][half][1]);
+                        }
                     }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i2 = 0; i2 < 4; ++i2) o[n][j][i2] = fmaf(weight[n][i2 & 1], d[n][i2], o[n][j][i2]);
                 }
-                stage = stage + S::kStageBytes == my_ring + S::kWarpBytes ? my_ring : stage + S::kStageBytes;
-                advance<S::kRows>(p, most_rows, cur);
+                if (++stage == S::kStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
             }
+            if (!ok) break;
             at += tiles_here;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -436,7 +514,6 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
             } else {
                 // a part: the range's last one stays in the ring (nothing is on its way there any more), its first goes to the workspace
                 const bool last = at == u1;
-                if (last) ptx::cp_async_wait_group<0>();
                 __syncwarp();
                 float* const part = last ? reinterpret_cast<float*>(ring + warp * S::kWarpBytes) : warp_part;
 #pragma unroll
@@ -455,9 +532,19 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                         }
                     }
                 if (lane == 0) {
-                    const long long from = at - tiles_here - first_tile;
+                    const long long from = at - tiles_here - tile;
                     (last ? s_tail : s_head)[warp] = Piece{from, from + r.tiles, b, segment, min(S::kRows, all_rows - base)};
                 }
+            }
+            // the next segment
+            tile = 0;
+            if (++segment == cache.heads * row_tile_count && at < u1) {
+                segment = 0;
+                do {
+                    ++b;
+                    if (b < p.requests) r = load_few(p, most_rows, b);
+                } while (b < p.requests && r.rows == 0);
+                if (b >= p.requests) break;           // (as above)
             }
         }
     }
@@ -566,11 +653,21 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
     }
 }
 
+// the cache's keys or values as (dim, token, head, page), read 16 tokens at a time in rows whose 16-byte chunks are swizzled
+bool cache_map(CUtensorMap* out, const CacheView& c, bool keys) {
+    const uint64_t dims[4] = {(uint64_t)c.dim, 1ull << c.page_shift, (uint64_t)c.heads, (uint64_t)c.pages};
+    const uint64_t strides[3] = {(uint64_t)(keys ? c.k_token : c.v_token), (uint64_t)(keys ? c.k_head : c.v_head), (uint64_t)(keys ? c.k_page : c.v_page)};
+    const uint32_t box[4] = {(uint32_t)c.dim, 16, 1, 1};
+    return encode_bytes(out, 4, keys ? c.k : c.v, dims, strides, box, c.dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 template <bool E4M3, bool BF16, int D, int NT>
 cudaError_t launch_rows(const AttentionParams& p, int most_rows, cudaStream_t stream) {
     using S = Shape<D, NT>;
     const auto kernel = cache_rows_kernel<E4M3, BF16, D, NT>;
-    constexpr int kSmem = S::kWarps * S::kWarpBytes;
+    constexpr int kSmem = S::kWarps * S::kWarpBytes + 1024;
+    CUtensorMap k_map, v_map;
+    if (!cache_map(&k_map, p.cache, true) || !cache_map(&v_map, p.cache, false)) return cudaErrorNotSupported;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -583,7 +680,7 @@ cudaError_t launch_rows(const AttentionParams& p, int most_rows, cudaStream_t st
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, p, most_rows);
+    e = cudaLaunchKernelEx(&cfg, kernel, p, most_rows, k_map, v_map);
     if (e == cudaSuccess) count_launch();
     return e;
 }

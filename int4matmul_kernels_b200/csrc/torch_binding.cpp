@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <atomic>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <stdexcept>
@@ -393,6 +394,173 @@ py::object try_layer(const py::object& mats, const py::object& h_, const py::obj
     }
 }
 
+// ---- the paged cache's calls (cache.py), in the same manner ----------------------------------------------------------------
+// int32 on dev; contiguous unless `table`, which may have a row stride
+bool ints(const Tensor& t, const c10::Device& dev, int64_t dims) {
+    return t.is_cuda() && t.device() == dev && t.scalar_type() == torch::kInt && t.dim() == dims;
+}
+bool ints1(const Tensor& t, const c10::Device& dev) { return ints(t, dev, 1) && t.is_contiguous(); }
+bool block_table(const Tensor& t, const c10::Device& dev, int64_t& stride) {
+    if (!ints(t, dev, 2) || (t.size(1) > 1 && t.stride(1) != 1)) return false;
+    stride = t.size(0) > 1 ? t.stride(0) : t.size(1);
+    return true;
+}
+
+bool cache_view(const Tensor& k, const Tensor& v, const Tensor& scales, i4mm_cache& c) {
+    if (!k.is_cuda() || v.device() != k.device() || scales.device() != k.device() || k.dim() != 4 || v.sizes() != k.sizes() ||
+        v.scalar_type() != k.scalar_type() || k.stride(3) != 1 || v.stride(3) != 1)
+        return false;
+    if (k.scalar_type() == torch::kChar) c.type = I4MM_CACHE_INT8;
+    else if (k.scalar_type() == torch::kFloat8_e4m3fn) c.type = I4MM_CACHE_E4M3;
+    else return false;
+    if (scales.scalar_type() != torch::kFloat || scales.dim() != 3 || scales.size(0) != k.size(0) || scales.size(1) != k.size(1) || scales.size(2) != 2 ||
+        !scales.is_contiguous())
+        return false;
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.scales = scales.data_ptr();
+    c.pages = k.size(0);
+    c.heads = k.size(1);
+    c.page_size = k.size(2);
+    c.head_dim = k.size(3);
+    c.k_page_stride = k.stride(0);
+    c.k_head_stride = k.stride(1);
+    c.k_token_stride = k.stride(2);
+    c.v_page_stride = v.stride(0);
+    c.v_head_stride = v.stride(1);
+    c.v_token_stride = v.stride(2);
+    return true;
+}
+
+// (tokens, heads, dim) activations; the C ABI's type, -1: not such
+int rows_type(const Tensor& t, const c10::Device& dev, int64_t dim) {
+    if (!t.is_cuda() || t.device() != dev || t.dim() != 3 || t.size(2) != dim || t.stride(2) != 1) return -1;
+    return t.scalar_type() == torch::kHalf ? I4MM_TYPE_FP16 : t.scalar_type() == torch::kBFloat16 ? I4MM_TYPE_BF16 : -1;
+}
+
+cudaStream_t current_stream(const c10::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+
+// cache.plan: the seven outputs, or a status / -1
+py::object try_cache_plan(const py::object& seq_, const py::object& new_, const py::object& table_, const py::object& free_, const py::object& count_,
+                          const py::object& page_, const py::object& tokens_) {
+    Tensor seq, add, table, free_pages, count;
+    int64_t page = 0, tokens = 0, stride = 0;
+    if (!as_tensor(seq_, seq) || !as_tensor(new_, add) || !as_tensor(table_, table) || !as_tensor(free_, free_pages) || !as_tensor(count_, count) ||
+        !as_int(page_, page) || !as_int(tokens_, tokens))
+        return py::int_(-1);
+    try {
+        if (!seq.is_cuda()) return py::int_(-1);
+        const auto dev = seq.device();
+        if (c10::cuda::current_device() != dev.index() || !ints1(seq, dev) || !ints1(add, dev) || !block_table(table, dev, stride) || !ints1(free_pages, dev) ||
+            !ints1(count, dev) || tokens < 0 || tokens > (1 << 30))
+            return py::int_(-1);
+        const int64_t n = seq.size(0);
+        if (add.size(0) != n || table.size(0) != n || count.size(0) != 1) return py::int_(-1);
+        const Tensor flat = at::empty({n + n + 1 + 3 * tokens + 2}, at::TensorOptions().dtype(torch::kInt).device(dev));
+        int* const base = flat.data_ptr<int>();
+        const int64_t sizes[7] = {n, n + 1, tokens, tokens, tokens, 1, 1};
+        int64_t at[7], next = 0;
+        for (int i = 0; i < 7; ++i) {
+            at[i] = next;
+            next += sizes[i];
+        }
+        const cudaStream_t stream = current_stream(dev);
+        int status;
+        {
+            py::gil_scoped_release release;
+            status = i4mm_cache_plan(n, seq.data_ptr(), add.data_ptr(), table.data_ptr(), table.size(1), stride, free_pages.data_ptr(), free_pages.size(0),
+                                     count.data_ptr(), page, tokens, base + at[0], base + at[1], base + at[2], base + at[3], base + at[4], base + at[5], (void*)stream);
+        }
+        if (status != I4MM_OK) return py::int_(status);
+        py::tuple out(7);
+        for (int i = 0; i < 7; ++i) out[i] = py::cast(flat.narrow(0, at[i], sizes[i]));
+        return out;
+    } catch (const c10::Error&) {
+        return py::int_(-1);
+    }
+}
+
+// cache.write: a status, or -1
+int try_cache_write(const py::object& kc_, const py::object& vc_, const py::object& scales_, const py::object& k_, const py::object& v_, const py::object& slots_) {
+    Tensor kc, vc, scales, k, v, slots;
+    i4mm_cache c{};
+    if (!as_tensor(kc_, kc) || !as_tensor(vc_, vc) || !as_tensor(scales_, scales) || !as_tensor(k_, k) || !as_tensor(v_, v) || !as_tensor(slots_, slots)) return -1;
+    try {
+        if (!cache_view(kc, vc, scales, c)) return -1;
+        const auto dev = kc.device();
+        const int type = rows_type(k, dev, c.head_dim);
+        if (type < 0 || rows_type(v, dev, c.head_dim) != type || v.sizes() != k.sizes() || k.size(1) != c.heads || !ints1(slots, dev) || slots.size(0) < k.size(0) ||
+            c10::cuda::current_device() != dev.index())
+            return -1;
+        const cudaStream_t stream = current_stream(dev);
+        py::gil_scoped_release release;
+        return i4mm_cache_write(&c, k.data_ptr(), v.data_ptr(), type, k.size(0), k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), (void*)stream);
+    } catch (const c10::Error&) {
+        return -1;
+    }
+}
+
+// cache.read, `bf16`: the type of the result: (k, v), or a status / -1
+py::object try_cache_read(const py::object& kc_, const py::object& vc_, const py::object& scales_, const py::object& slots_, bool bf16) {
+    Tensor kc, vc, scales, slots;
+    i4mm_cache c{};
+    if (!as_tensor(kc_, kc) || !as_tensor(vc_, vc) || !as_tensor(scales_, scales) || !as_tensor(slots_, slots)) return py::int_(-1);
+    try {
+        if (!cache_view(kc, vc, scales, c)) return py::int_(-1);
+        const auto dev = kc.device();
+        if (!ints1(slots, dev) || c10::cuda::current_device() != dev.index()) return py::int_(-1);
+        const auto options = at::TensorOptions().dtype(bf16 ? torch::kBFloat16 : torch::kHalf).device(dev);
+        Tensor k = at::empty({slots.size(0), c.heads, c.head_dim}, options), v = at::empty({slots.size(0), c.heads, c.head_dim}, options);
+        const cudaStream_t stream = current_stream(dev);
+        int status;
+        {
+            py::gil_scoped_release release;
+            status = i4mm_cache_read(&c, k.data_ptr(), v.data_ptr(), bf16 ? I4MM_TYPE_BF16 : I4MM_TYPE_FP16, slots.size(0), slots.data_ptr(), (void*)stream);
+        }
+        if (status != I4MM_OK) return py::int_(status);
+        return py::make_tuple(k, v);
+    } catch (const c10::Error&) {
+        return py::int_(-1);
+    }
+}
+
+// cache.attention (`scale` None: 1 / sqrt(head_dim)): the output, or a status / -1
+py::object try_cache_attention(const py::object& q_, const py::object& kc_, const py::object& vc_, const py::object& scales_, const py::object& table_,
+                               const py::object& seq_, const py::object& cu_, const py::object& longest_, const py::object& scale_, const py::object& window_,
+                               const py::dict& workspaces) {
+    Tensor q, kc, vc, scales, table, seq, cu;
+    int64_t longest = 0, window = 0, stride = 0;
+    i4mm_cache c{};
+    if (!as_tensor(q_, q) || !as_tensor(kc_, kc) || !as_tensor(vc_, vc) || !as_tensor(scales_, scales) || !as_tensor(table_, table) || !as_tensor(seq_, seq) ||
+        !as_optional_tensor(cu_, cu) || !as_int(longest_, longest) || !as_int(window_, window) || !(scale_.is_none() || PyFloat_Check(scale_.ptr())))
+        return py::int_(-1);
+    try {
+        if (!cache_view(kc, vc, scales, c)) return py::int_(-1);
+        const auto dev = kc.device();
+        const int type = rows_type(q, dev, c.head_dim);
+        if (type < 0 || c.heads == 0 || q.size(1) % c.heads || !block_table(table, dev, stride) || !ints1(seq, dev) || seq.size(0) != table.size(0) || longest < 0 ||
+            window < 0 || c10::cuda::current_device() != dev.index())
+            return py::int_(-1);
+        if (cu.defined() ? !ints1(cu, dev) || cu.size(0) != seq.size(0) + 1 : q.size(0) < seq.size(0)) return py::int_(-1);
+        const cudaStream_t stream = current_stream(dev);
+        const Tensor ws = scratch(workspaces, dev, stream);
+        if (!ws.defined()) return py::int_(-1);
+        const float scale = scale_.is_none() ? (float)(1.0 / std::sqrt((double)c.head_dim)) : (float)PyFloat_AS_DOUBLE(scale_.ptr());
+        Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+        int status;
+        {
+            py::gil_scoped_release release;
+            status = i4mm_cache_attention(&c, out.data_ptr(), q.data_ptr(), type, q.size(0), q.size(1), q.stride(0), q.stride(1), table.data_ptr(), table.size(1), stride,
+                                          seq.data_ptr(), cu.defined() ? cu.data_ptr() : nullptr, seq.size(0), longest, scale, window, ws.data_ptr(),
+                                          (size_t)ws.numel(), (void*)stream);
+        }
+        if (status != I4MM_OK) return py::int_(status);
+        return py::cast(out);
+    } catch (const c10::Error&) {
+        return py::int_(-1);
+    }
+}
+
 // Not in the reference (its kernels have no waits): waits for every stream this module has launched on, on the
 // current device, and raises if a kernel gave up on one of its bounded device-side waits since the last check.
 // The multiply entries do not call it themselves, because it synchronises.
@@ -429,6 +597,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("_try_linear", &try_linear, "QuantLinear.forward for arguments that pass its checks: output, status or -1");
     m.def("_try_layer", &try_layer, "one layer of sharding.DecoderStack on one GPU: h, or (h, x), a status or -1");
     m.def("_try_row_norm", &try_row_norm, "ops.row_norm for arguments that pass its checks: output, status or -1");
+
+    m.def("_try_cache_plan", &try_cache_plan, "cache.plan for arguments that pass its checks: outputs, a status or -1");
+    m.def("_try_cache_write", &try_cache_write, "cache.write for arguments that pass its checks: a status or -1");
+    m.def("_try_cache_read", &try_cache_read, "cache.read for arguments that pass its checks: (k, v), a status or -1");
+    m.def("_try_cache_attention", &try_cache_attention, "cache.attention for arguments that pass its checks: output, a status or -1");
 
     m.def("weight_matrix_packing", &weight_matrix_packing, "int4_sparse_pack");
 

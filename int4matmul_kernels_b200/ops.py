@@ -18,6 +18,7 @@ import torch
 from . import capi
 
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_cache_workspaces: dict[tuple[int, int], torch.Tensor] = {}        # of cache.attention
 _static_weights = False
 
 
@@ -77,14 +78,14 @@ def workspace(device: torch.device, stream: torch.cuda.Stream) -> torch.Tensor:
 
 
 def check_device_status(device: torch.device | None = None) -> None:
-    """Waits for every stream `workspace()` has served on `device` and raises Int4MatmulError(ERR_TIMEOUT) if a
+    """Waits for every stream that the multiplies or `cache.attention` have used on `device` and raises Int4MatmulError(ERR_TIMEOUT) if a
     kernel gave up on one of its bounded device-side waits since the last check (the results of that launch are
     void).  Not called by the multiply entries themselves, because it synchronises; no reference counterpart."""
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     lib = capi.load()
     worst = capi.OK
     with torch.cuda.device(index):
-        for (dev, stream), ws in list(_workspaces.items()):
+        for (dev, stream), ws in [*_workspaces.items(), *_cache_workspaces.items()]:
             if dev != index:
                 continue
             status = lib.i4mm_device_status(ws.data_ptr(), stream)
