@@ -185,6 +185,24 @@ __device__ __forceinline__ void find_item(const AttentionParams& p, int least_ro
     __syncwarp();
 }
 
+// ---- two fp32 at a time ----
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // address of 16 bytes (8 values) `unit` of `row` in an operand tile of `rows` rows: sub-tiles of 64 values, 128-byte rows, swizzled
 __device__ __forceinline__ uint32_t swizzled(uint32_t tile, int rows, int row, int unit) {
     return tile + (unit >> 3) * (rows * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
@@ -520,25 +538,35 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                                    (!p.window || first > last_position - p.window);
                 // tokens below `from` and at `to` and beyond are hidden from this row (relative to the tile)
                 const int from = max(p.window ? position - p.window + 1 : 0, t.lo) - first, to = min(position + 1, t.limit) - first;
+                // the largest x of the tile
                 float high = -INFINITY;
+                const auto largest = [&](auto masked) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32];
+                        ptx::tmem_ld32(s_at + 32 * c, x);
+                        ptx::tc_wait_ld();
+                        if constexpr (decltype(masked)::value) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32];
-                    ptx::tmem_ld32(s_at + 32 * c, x);
-                    ptx::tc_wait_ld();
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float4 sc = scales[slot][2 * c + g];
-                        float m = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float s = __uint_as_float(x[16 * g + i]);
-                            const int at = 32 * c + 16 * g + i;
-                            m = fmaxf(m, whole || (at >= from && at < to) ? s : -INFINITY);
+                            for (int i = 0; i < 32; ++i)
+                                if (32 * c + i < from || 32 * c + i >= to) x[i] = 0xFF800000u;
                         }
-                        if (m != -INFINITY) high = fmaxf(high, fmaf(m, factor * sc.x, sc.y));
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const float4 sc = scales[slot][2 * c + g];
+                            float m = __uint_as_float(x[16 * g]), m2 = __uint_as_float(x[16 * g + 1]);
+#pragma unroll
+                            for (int i = 2; i < 14; i += 4) {
+                                m = max3(m, __uint_as_float(x[16 * g + i]), __uint_as_float(x[16 * g + i + 1]));
+                                m2 = max3(m2, __uint_as_float(x[16 * g + i + 2]), __uint_as_float(x[16 * g + i + 3]));
+                            }
+                            m = max3(max3(m, m2, __uint_as_float(x[16 * g + 14])), __uint_as_float(x[16 * g + 15]), -INFINITY);
+                            if (m != -INFINITY) high = fmaxf(high, fmaf(m, factor * sc.x, sc.y));
+                        }
                     }
-                }
+                };
+                if (whole) largest(std::false_type{});
+                else largest(std::true_type{});
                 const bool grown = high > top + kGrowth;
                 if (__any_sync(kAll, grown)) {
                     const float next = grown ? high : top;
@@ -562,31 +590,36 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                     top = next;
                 }
                 const float base = top == -INFINITY ? 0.f : top;
+                const auto weights = [&](auto masked) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32], w[16];
+                        ptx::tmem_ld32(s_at + 32 * c, x);
+                        ptx::tc_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32], w[16];
-                    ptx::tmem_ld32(s_at + 32 * c, x);
-                    ptx::tc_wait_ld();
+                        for (int g = 0; g < 2; ++g) {
+                            const float4 sc = scales[slot][2 * c + g];
+                            const float a = factor * sc.x, b = sc.y - base;
+                            float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float4 sc = scales[slot][2 * c + g];
-                        const float a = factor * sc.x, b = sc.y - base;
-                        float part = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const int at = 32 * c + 16 * g + i;
-                            float e0 = exp2_approx(fmaf(__uint_as_float(x[16 * g + i]), a, b)), e1 = exp2_approx(fmaf(__uint_as_float(x[16 * g + i + 1]), a, b));
-                            if (!whole) {
-                                if (at < from || at >= to) e0 = 0.f;
-                                if (at + 1 < from || at + 1 >= to) e1 = 0.f;
+                            for (int i = 0; i < 16; i += 2) {
+                                const int at = 32 * c + 16 * g + i;
+                                const float2 y = fma2(make_float2(__uint_as_float(x[16 * g + i]), __uint_as_float(x[16 * g + i + 1])), make_float2(a, a), make_float2(b, b));
+                                float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                                if constexpr (decltype(masked)::value) {
+                                    if (at < from || at >= to) e.x = 0.f;
+                                    if (at + 1 < from || at + 1 >= to) e.y = 0.f;
+                                }
+                                part = add2(part, e);
+                                w[8 * g + i / 2] = h2_as_u32(__floats2half2_rn(e.x, e.y));
                             }
-                            part += e0 + e1;
-                            w[8 * g + i / 2] = h2_as_u32(__floats2half2_rn(e0, e1));
+                            sum = fmaf(part.x + part.y, sc.z, sum);
                         }
-                        sum = fmaf(part, sc.z, sum);
+                        ptx::tmem_st16(s_at + 16 * c, w);
                     }
-                    ptx::tmem_st16(s_at + 16 * c, w);
-                }
+                };
+                if (whole) weights(std::false_type{});
+                else weights(std::true_type{});
                 ptx::tc_wait_st();
                 ptx::tc_fence_before_sync();
                 __syncwarp();
