@@ -1,6 +1,7 @@
 // Attention over the paged 8-bit cache (i4mm_cache_attention), many rows per request: prompts and chunks of them.
 //
-//   x_j = log2(e) * scale * s_key * (q . k_j) + log2(s_value),  M = running max of x_j,  P_j = 2^(x_j - M)   (fp16)
+//   x_j = log2(e) * scale * s_key * (q . k_j) + log2(s_value),  P_j = 2^(x_j - M)   (fp16)
+//   with a reference M, an x_j of the row,
 //   o = sum_j P_j v_j / sum_j (P_j / s_value),  k_j and v_j the cache's bytes, s_key and s_value their page's scales
 // so the value scale is in the weight that is rounded anyway, and the bytes go into the tensor cores as they are.
 //
@@ -16,8 +17,8 @@
 //   warp 13            takes the next item (request, key head, 256 rows, a range of tokens) off a common counter, one ahead
 //
 // The rows of all query heads of a key head are packed into one tile: row r is token r / group, head r % group.  Sums stay in
-// tensor memory in fp32 and are rescaled only when a row's maximum has grown by more than 2^8 since (P <= 256 has the same relative
-// precision).  Long contexts under few rows are cut along the tokens into items of their own; the block that finishes a
+// tensor memory in fp32 and are rescaled only when a row's weights would outgrow fp16 (below that their relative precision is the
+// same), which costs no maximum on the way: the weights' sum, which is needed anyhow, tells.  Long contexts under few rows are cut along the tokens into items of their own; the block that finishes a
 // segment's last part joins them in order.  Every wait is bounded; a block that gives up records it in the status word.
 #include <algorithm>
 #include <type_traits>
@@ -34,7 +35,8 @@ constexpr int kDecode0 = kSoftmaxWarps, kMma = kDecode0 + kDecodeWarps, kSchedul
 constexpr int kThreads = 32 * (kSchedule + 1);
 constexpr int kScaleSlots = 4;
 constexpr int kMinTiles = 4;                          // a part of a segment has at least so many tiles
-constexpr float kGrowth = 8.f;                        // log2 of what a weight may exceed its reference by
+constexpr float kLeastFactor = 1e-30f;                // in the place of a key scale of 0: scores are 0 either way
+constexpr float kMostWeight = 16384.f;                // fp16 holds 65504
 
 template <int D>
 struct Layout {
@@ -55,7 +57,7 @@ struct Item {
 
 struct Barriers {
     unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], scale_full[kScaleSlots], item_full[2], item_empty[2];
-    unsigned long long q_full[2], s_full[2], p_full[2], pv_done[2], group[2], drained;
+    unsigned long long q_full[2], s_full[2], p_full[2][2], pv_half[2], pv_done[2], group[2], drained;
 };
 
 // A whole warp waits; false (in all of its lanes) once the block gives up.
@@ -236,7 +238,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
             init(bars.item_empty[i], kSoftmaxWarps + kDecodeWarps + 1);
             init(bars.q_full[i], 4);
             init(bars.s_full[i], 1);
-            init(bars.p_full[i], 4);
+            init(bars.p_full[i][0], 4);
+            init(bars.p_full[i][1], 4);
+            init(bars.pv_half[i], 1);
             init(bars.pv_done[i], 1);
             init(bars.group[i], 4);
         }
@@ -333,19 +337,23 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
             for (int j = 0; j < most && ok; ++j) {
                 for (int h = 0; h < 2; ++h) {
                     if (j >= tiles[h]) continue;
-                    ok = ok && wait_on(&bars.p_full[h], p_phase[h], &s_abort);
-                    p_phase[h] ^= 1;
+                    // O_h += P_h V_j, as far as the weights are there
                     ok = ok && wait_on(&bars.v_full[v_stage & 1], (v_stage >> 1) & 1, &s_abort);
-                    if (!ok) break;
-                    ptx::tc_fence_after_sync();
-                    if (ptx::elect_one()) {           // O_h += P_h V_j
-                        const uint64_t b = ptx::smem_desc_sw128(v_tile + (v_stage & 1) * L::kV);
+                    for (int part = 0; part < 2 && ok; ++part) {
+                        ok = wait_on(&bars.p_full[h][part], p_phase[h], &s_abort);
+                        if (!ok) break;
+                        ptx::tc_fence_after_sync();
+                        if (ptx::elect_one()) {
+                            const uint64_t b = ptx::smem_desc_sw128(v_tile + (v_stage & 1) * L::kV) + (uint64_t)part * (D * 128 >> 4);
+                            const uint32_t a = s_col(h) + 32 * part;
 #pragma unroll
-                        for (int k = 0; k < kTokens / 16; ++k)
-                            ptx::umma_f16_ts(o_col(h), s_col(h) + 8 * k, b + (uint64_t)((k >> 2) * (D * 128 >> 4) + (k & 3) * 2), idesc_o, j > 0 || k > 0);
-                        ptx::tc_commit(ptx::smem_u32(&bars.pv_done[h]));
+                            for (int k = 0; k < kTokens / 32; ++k) ptx::umma_f16_ts(o_col(h), a + 8 * k, b + k * 2, idesc_o, j > 0 || part > 0 || k > 0);
+                            ptx::tc_commit(ptx::smem_u32(part == 0 ? &bars.pv_half[h] : &bars.pv_done[h]));
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    p_phase[h] ^= 1;
+                    if (!ok) break;
                     if (j + 1 < tiles[h]) score(h, j + 1);
                 }
                 if (!ok) break;
@@ -377,13 +385,20 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
             const int* const table = p.table + t.b * p.table_stride;
             uint4 k[kKeyRows];
             VBytes v[8];
-            int ids = 0;                              // lane l < 8: the page of tokens 16 * l of the tile
-            float2 both = {};
+            int ids = -1, later = -1;                 // lane l: the page of tokens 16 * (l & 7) of the tile that is fetched next, and of the one after
+            float2 both = {}, later_both = {}, now = {};                      // their scales, and those of the tile that is decoded
             const auto load_pages = [&](int j) {
                 const int token = (t.tile0 + j) * kTokens + 16 * (lane & 7), at = token >> cache.page_shift;
-                ids = at < p.table_width && token + 16 > t.lo && token < t.limit ? table[at] : -1;
-                if (ids < 0 || ids >= cache.pages) ids = -1;
-                if (ids >= 0) both = cache.scales[(long long)ids * cache.heads + t.head];
+                later = -1;
+                if (j < most && at < p.table_width && token + 16 > t.lo && token < t.limit) later = table[at];
+            };
+            const auto load_scales = [&]() {          // of `later`
+                if ((unsigned int)later >= (unsigned int)cache.pages) later = -1;
+                if (later >= 0) later_both = cache.scales[(long long)later * cache.heads + t.head];
+            };
+            const auto next_pages = [&]() {
+                ids = later;
+                both = later_both;
             };
             const auto load_keys = [&](int j) {
                 const int first = (t.tile0 + j) * kTokens;
@@ -410,15 +425,23 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
             };
             if (most > 0) {
                 load_pages(0);
+                load_scales();
+                next_pages();
                 load_keys(0);
                 load_values(0);
+                load_pages(1);
             }
             for (int j = 0; j < most && ok; ++j, ++stage) {
+                const bool there = ids >= 0;
+                now = both;
+                load_scales();                        // of tile j + 1, whose pages were asked for a tile ago
+                next_pages();
+                load_pages(j + 2);
                 const int s = stage & 1;
                 const uint32_t phase = ((stage >> 1) & 1) ^ 1;
                 if (w == 0 && lane < 8) {
-                    const float value = ids < 0 ? 0.f : fmaxf(both.y, kLeastScale);
-                    scales[stage % kScaleSlots][lane] = ids < 0 ? make_float4(0.f, -INFINITY, 0.f, 0.f) : make_float4(both.x, log2f(value), 1.f / value, 0.f);
+                    const float value = fmaxf(now.y, kLeastScale);
+                    scales[stage % kScaleSlots][lane] = there ? make_float4(now.x, log2f(value), 1.f / value, 0.f) : make_float4(0.f, -INFINITY, 0.f, 0.f);
                 }
                 ok = wait_on(&bars.k_empty[s], phase, &s_abort);
                 if (!ok) break;
@@ -440,10 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                     arrive(&bars.k_full[s]);
                     if (w == 0) arrive(&bars.scale_full[stage % kScaleSlots]);
                 }
-                if (j + 1 < most) {
-                    load_pages(j + 1);
-                    load_keys(j + 1);
-                }
+                if (j + 1 < most) load_keys(j + 1);
                 ok = wait_on(&bars.v_empty[s], phase, &s_abort);
                 if (!ok) break;
                 const auto word = [&](int i, int c) {
@@ -484,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
             group_phase ^= 1;
         };
         for (uint32_t n = 0; ok && next_item(n); ++n) {
-            const Item t = items[n & 1];
+            const Item& t = items[n & 1];
             const int tiles = t.tiles[h], most = max(t.tiles[0], t.tiles[1]);
             const int mine = t.base + h * kHalf + row;                        // the row
             const bool real = row < t.rows[h];
@@ -523,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                 __syncwarp();
                 if (lane == 0) arrive(&bars.q_full[h]);
             }
-            float top = -INFINITY, sum = 0.f;         // the reference that weights are taken relative to; their total
+            float top = real ? -INFINITY : 0.f, sum = 0.f;                    // the reference that weights are taken relative to; their total
             // the warp's rows see a tile whole if the first of them does and, with a window, the last
             const int first_position = __shfl_sync(kAll, position, 0), last_position = __reduce_max_sync(kAll, position);
             for (int j = 0; j < tiles; ++j) {
@@ -538,92 +558,111 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                                    (!p.window || first > last_position - p.window);
                 // tokens below `from` and at `to` and beyond are hidden from this row (relative to the tile)
                 const int from = max(p.window ? position - p.window + 1 : 0, t.lo) - first, to = min(position + 1, t.limit) - first;
-                // the largest x of the tile
-                float high = -INFINITY;
-                const auto largest = [&](auto masked) {
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t x[32];
-                        ptx::tmem_ld32(s_at + 32 * c, x);
-                        ptx::tc_wait_ld();
-                        if constexpr (decltype(masked)::value) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (32 * c + i < from || 32 * c + i >= to) x[i] = 0xFF800000u;
-                        }
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const float4 sc = scales[slot][2 * c + g];
-                            float m = __uint_as_float(x[16 * g]), m2 = __uint_as_float(x[16 * g + 1]);
-#pragma unroll
-                            for (int i = 2; i < 14; i += 4) {
-                                m = max3(m, __uint_as_float(x[16 * g + i]), __uint_as_float(x[16 * g + i + 1]));
-                                m2 = max3(m2, __uint_as_float(x[16 * g + i + 2]), __uint_as_float(x[16 * g + i + 3]));
-                            }
-                            m = max3(max3(m, m2, __uint_as_float(x[16 * g + 14])), __uint_as_float(x[16 * g + 15]), -INFINITY);
-                            if (m != -INFINITY) high = fmaxf(high, fmaf(m, factor * sc.x, sc.y));
-                        }
-                    }
+                // Half a tile of tokens at a time: x = a * score + b of each 16 (a is not 0: hidden scores are -infinity), weights 2^x.  They are
+                // taken relative to a reference that is no maximum any more once scores exceed it, which does no harm until the half's
+                // weights add up to more than kMostWeight; then the reference moves, sums follow it, and the half is taken again.
+                uint32_t x[2][32];
+                const auto load = [&](int half) {
+                    ptx::tmem_ld32(s_at + 64 * half, x[0]);
+                    ptx::tmem_ld32(s_at + 64 * half + 32, x[1]);
                 };
-                if (whole) largest(std::false_type{});
-                else largest(std::true_type{});
-                const bool grown = high > top + kGrowth;
-                if (__any_sync(kAll, grown)) {
-                    const float next = grown ? high : top;
-                    const float keep = top == -INFINITY ? 0.f : exp2_approx(top - next);
-                    if (j > 0) {
-                        ok = wait_on(&bars.pv_done[h], (pv_count - 1) & 1, &s_abort);
-                        if (!ok) break;
-                        ptx::tc_fence_after_sync();
-                        const float scale = next == top ? 1.f : keep;
+                const auto hide = [&](int half) {
+                    if (whole) return;
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            uint32_t x[32];
-                            ptx::tmem_ld32(o_at + 32 * c, x);
-                            ptx::tc_wait_ld();
+                    for (int c = 0; c < 2; ++c)
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * scale);
-                            ptx::tmem_st32(o_at + 32 * c, x);
-                        }
-                    }
-                    if (next != top) sum *= keep;
-                    top = next;
-                }
-                const float base = top == -INFINITY ? 0.f : top;
-                const auto weights = [&](auto masked) {
+                        for (int i = 0; i < 32; ++i)
+                            if (64 * half + 32 * c + i < from || 64 * half + 32 * c + i >= to) x[c][i] = 0xFF800000u;
+                };
+                load(0);
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t x[32], w[16];
-                        ptx::tmem_ld32(s_at + 32 * c, x);
+                for (int half = 0; half < 2; ++half) {
+                    float total;
+                    bool again = false;
+#pragma unroll 1
+                    for (;;) {
                         ptx::tc_wait_ld();
+                        hide(half);
+                        if (again || __any_sync(kAll, top == -INFINITY)) {
+                            float high = -INFINITY;
 #pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const float4 sc = scales[slot][2 * c + g];
-                            const float a = factor * sc.x, b = sc.y - base;
-                            float2 part = make_float2(0.f, 0.f);
+                            for (int g = 0; g < 4; ++g) {
+                                float m = -INFINITY;
+#pragma unroll
+                                for (int i = 0; i < 16; i += 2) m = max3(m, __uint_as_float(x[g >> 1][16 * (g & 1) + i]), __uint_as_float(x[g >> 1][16 * (g & 1) + i + 1]));
+                                const float4 sc = scales[slot][4 * half + g];
+                                high = fmaxf(high, fmaf(m, fmaxf(factor * sc.x, kLeastFactor), sc.y));
+                            }
+                            const float next = fmaxf(top, high), keep = next == top ? 1.f : exp2_approx(top - next);     // (0 from -infinity on)
+                            if ((j > 0 || half > 0) && __any_sync(kAll, keep != 1.f)) {
+                                // (the scores of a tile come after the sums of the one before it)
+                                if (half > 0) ok = wait_on(&bars.pv_half[h], pv_count & 1, &s_abort);
+                                if (!ok) break;
+                                ptx::tc_fence_after_sync();
+#pragma unroll 1
+                                for (int c = 0; c < D / 16; ++c) {
+                                    uint32_t y[16];
+                                    ptx::tmem_ld16(o_at + 16 * c, y);
+                                    ptx::tc_wait_ld();
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
+                                    ptx::tmem_st16(o_at + 16 * c, y);
+                                }
+                            }
+                            sum *= keep;
+                            top = next;
+                        }
+                        // all exponents, then all exponentials, then sums and packing: the exponential pipe is fed without a pause
+                        const float base = top == -INFINITY ? 0.f : top;
+                        float2 part[4];
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const float4 sc = scales[slot][4 * half + g];
+                            const float a = fmaxf(factor * sc.x, kLeastFactor), b = sc.y - base;
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) {
-                                const int at = 32 * c + 16 * g + i;
-                                const float2 y = fma2(make_float2(__uint_as_float(x[16 * g + i]), __uint_as_float(x[16 * g + i + 1])), make_float2(a, a), make_float2(b, b));
-                                float2 e = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-                                if constexpr (decltype(masked)::value) {
-                                    if (at < from || at >= to) e.x = 0.f;
-                                    if (at + 1 < from || at + 1 >= to) e.y = 0.f;
-                                }
-                                part = add2(part, e);
-                                w[8 * g + i / 2] = h2_as_u32(__floats2half2_rn(e.x, e.y));
+                                uint32_t* const s2 = &x[g >> 1][16 * (g & 1) + i];
+                                const float2 y = fma2(make_float2(__uint_as_float(s2[0]), __uint_as_float(s2[1])), make_float2(a, a), make_float2(b, b));
+                                s2[0] = __float_as_uint(y.x);
+                                s2[1] = __float_as_uint(y.y);
                             }
-                            sum = fmaf(part.x + part.y, sc.z, sum);
                         }
-                        ptx::tmem_st16(s_at + 16 * c, w);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) x[c][i] = __float_as_uint(exp2_approx(__uint_as_float(x[c][i])));
+                        total = 0.f;
+                        float largest = 0.f;
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            part[g] = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2)
+                                part[g] = add2(part[g], make_float2(__uint_as_float(x[g >> 1][16 * (g & 1) + i]), __uint_as_float(x[g >> 1][16 * (g & 1) + i + 1])));
+                            const float all = part[g].x + part[g].y;
+                            largest = fmaxf(largest, all);
+                            total = fmaf(all, scales[slot][4 * half + g].z, total);
+                        }
+                        if (again || !__any_sync(kAll, largest > kMostWeight)) break;
+                        again = true;
+                        load(half);
                     }
-                };
-                if (whole) weights(std::false_type{});
-                else weights(std::true_type{});
-                ptx::tc_wait_st();
-                ptx::tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) arrive(&bars.p_full[h]);
+                    if (!ok) break;
+                    sum += total;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) w[i] = h2_as_u32(__floats2half2_rn(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])));
+                        ptx::tmem_st16(s_at + 32 * half + 16 * c, w);
+                        if (half == 0) ptx::tmem_ld32(s_at + 64 + 32 * c, x[c]);
+                    }
+                    ptx::tc_wait_st();
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) arrive(&bars.p_full[h][half]);
+                }
+                if (!ok) break;
                 ++pv_count;
             }
             tile_count += most;
