@@ -724,22 +724,23 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                     if (!ok) break;
                     if (s_last[h] && real) {
                         __threadfence();
+                        // (every pass over the parts has independent loads only: what it costs is their latency)
                         float m = -INFINITY, total = 0.f;
+#pragma unroll 4
                         for (int i = 0; i < t.parts; ++i) m = fmaxf(m, __ldcg(part_at(i) + kHalf * D + row));
-                        const auto weight = [&](int i) {
-                            const float x = __ldcg(part_at(i) + kHalf * D + row);
-                            return x == -INFINITY ? 0.f : exp2_approx(x - m);
-                        };
-                        for (int i = 0; i < t.parts; ++i) total += weight(i) * __ldcg(part_at(i) + kHalf * D + kHalf + row);
+                        const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+                        for (int i = 0; i < t.parts; ++i)
+                            total += exp2_approx(__ldcg(part_at(i) + kHalf * D + row) - from) * __ldcg(part_at(i) + kHalf * D + kHalf + row);
                         const float f = total > 0.f ? 1.f / total : total;
-                        constexpr int kChunk = 8;                             // columns at a time
-                        for (int c = 0; c < D; c += kChunk) {
-                            float y[kChunk] = {};
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            float y[32] = {};
+#pragma unroll 2
                             for (int i = 0; i < t.parts; ++i) {
-                                const float take = weight(i);
-                                if (take == 0.f) continue;                    // (nothing was summed there)
+                                const float take = exp2_approx(__ldcg(part_at(i) + kHalf * D + row) - from) * f;
 #pragma unroll
-                                for (int k = 0; k < kChunk / 4; ++k) {
+                                for (int k = 0; k < 8; ++k) {
                                     const float4 x = __ldcg(reinterpret_cast<const float4*>(part_at(i) + ((c / 4 + k) * kHalf + row) * 4));
                                     y[4 * k] += take * x.x;
                                     y[4 * k + 1] += take * x.y;
@@ -747,8 +748,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                                     y[4 * k + 3] += take * x.w;
                                 }
                             }
-                            *reinterpret_cast<uint4*>(out + c) = make_uint4(pack_out<BF16>(y[0] * f, y[1] * f), pack_out<BF16>(y[2] * f, y[3] * f),
-                                                                            pack_out<BF16>(y[4] * f, y[5] * f), pack_out<BF16>(y[6] * f, y[7] * f));
+#pragma unroll
+                            for (int k = 0; k < 32; k += 8)
+                                *reinterpret_cast<uint4*>(out + c + k) = make_uint4(pack_out<BF16>(y[k], y[k + 1]), pack_out<BF16>(y[k + 2], y[k + 3]),
+                                                                                    pack_out<BF16>(y[k + 4], y[k + 5]), pack_out<BF16>(y[k + 6], y[k + 7]));
                         }
                     }
                     meet();                                                   // (s_last is free again)

@@ -473,7 +473,13 @@ py::object try_cache_plan(const py::object& seq_, const py::object& new_, const 
         }
         if (status != I4MM_OK) return py::int_(status);
         py::tuple out(7);
-        for (int i = 0; i < 7; ++i) out[i] = py::cast(flat.narrow(0, at[i], sizes[i]));
+        for (int i = 0; i < 7; ++i) {
+            // a view of `flat`, made without a trip through the dispatcher (seven of those take longer than the kernel)
+            auto impl = c10::make_intrusive<at::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
+            impl->set_storage_offset(at[i]);
+            impl->set_sizes_contiguous({sizes[i]});
+            out[i] = py::cast(Tensor(std::move(impl)));
+        }
         return out;
     } catch (const c10::Error&) {
         return py::int_(-1);
