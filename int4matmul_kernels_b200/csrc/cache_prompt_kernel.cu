@@ -73,17 +73,40 @@ __device__ __forceinline__ bool wait_on(unsigned long long* bar, uint32_t parity
 __device__ __forceinline__ void arrive(unsigned long long* bar) { ptx::mbar_arrive(ptx::smem_u32(bar)); }
 
 // ---- items ---------------------------------------------------------------------------------------------------------------------
-// How a request is cut: its segments (key heads x tiles of 256 rows), and the parts of each.
+// A segment is a key head and a tile of 256 rows of a request.  Segments are items of their own, or cut along the tokens into parts:
+//   * long ones, so that none has more than its share of the GPU's work;
+//   * those that are left over when all blocks have had the same number of whole ones (of 512 equal segments 444 make three rounds of 148
+//     blocks; the other 68, cut in two, make half a round instead of a whole one), unless they are short.
+// A part costs about two tiles' time for writing its sums and joining them.
+struct Split {
+    int part_tiles;                                   // of the first kind
+    long long whole;                                  // segments (in their order) before those that are left over
+    int spread;                                       // parts of one that is left over
+};
 struct Cut {
-    int row_tiles, parts;
+    int row_tiles, segments, parts, last, last_parts; // the last `last` segments are cut into last_parts, the others into `parts`
 };
 __device__ __forceinline__ int row_tiles_of(const AttentionParams& p, const Request& r, int least_rows) {
     const long long rows = (long long)r.rows * p.group;
     return rows < least_rows ? 0 : (int)((rows + 2 * kHalf - 1) / (2 * kHalf));
 }
 __device__ __forceinline__ int tiles_of(const Request& r) { return r.limit > r.lo ? (r.limit + kTokens - 1) / kTokens - r.lo / kTokens : 0; }
-__device__ __forceinline__ Cut cut_of(const AttentionParams& p, const Request& r, int least_rows, int part_tiles) {
-    return {row_tiles_of(p, r, least_rows), max(1, (tiles_of(r) + part_tiles - 1) / part_tiles)};
+// `before`: segments of the requests before this one
+__device__ __forceinline__ Cut cut_of(const AttentionParams& p, const Request& r, int least_rows, const Split& s, long long before) {
+    Cut c;
+    const int tiles = tiles_of(r);
+    c.row_tiles = row_tiles_of(p, r, least_rows);
+    c.segments = c.row_tiles * p.cache.heads;
+    c.parts = max(1, (tiles + s.part_tiles - 1) / s.part_tiles);
+    // the segments at the end of a request are those of its first rows: what they see
+    const int few = min(tiles, max(0, (r.position + (2 * kHalf + p.group - 1) / p.group + kTokens - 1) / kTokens - r.lo / kTokens));
+    c.last_parts = max(c.parts, min(s.spread, few / (2 * kMinTiles)));
+    c.last = c.last_parts > c.parts ? (int)max(0ll, min((long long)c.segments, before + c.segments - s.whole)) : 0;
+    return c;
+}
+__device__ __forceinline__ long long items_of(const Cut& c) { return (long long)(c.segments - c.last) * c.parts + (long long)c.last * c.last_parts; }
+__device__ __forceinline__ long long parts_of(const Cut& c) {             // of segments that are cut
+    return (c.parts > 1 ? (long long)(c.segments - c.last) * c.parts : 0) + (c.last_parts > 1 ? (long long)c.last * c.last_parts : 0);
 }
 
 __device__ __forceinline__ long long warp_sum(long long v) {
@@ -91,56 +114,69 @@ __device__ __forceinline__ long long warp_sum(long long v) {
     for (int d = 16; d; d /= 2) v += __shfl_xor_sync(kAll, v, d);
     return v;
 }
-
-// Tiles of a part: segments are cut only as far as it takes for all blocks to have work; parts must find room in the workspace.
-__device__ __forceinline__ int choose_part(const AttentionParams& p, int least_rows, int blocks, long long* items) {
+__device__ __forceinline__ long long warp_prefix(long long v) {             // sum over this lane and those before it
     const int lane = threadIdx.x & 31;
-    long long tiles = 0;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const long long o = __shfl_up_sync(kAll, v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+// How all segments are cut, and the number of items.  Parts must find room in the workspace.
+__device__ __forceinline__ Split choose_split(const AttentionParams& p, int least_rows, int blocks, long long* items) {
+    const int lane = threadIdx.x & 31;
+    long long tiles = 0, segments = 0;
     for (int b = lane; b < p.requests; b += 32) {
         const Request r = load_request(p, b);
-        tiles += (long long)row_tiles_of(p, r, least_rows) * p.cache.heads * tiles_of(r);
+        const long long n = (long long)row_tiles_of(p, r, least_rows) * p.cache.heads;
+        segments += n;
+        tiles += n * tiles_of(r);
     }
     tiles = warp_sum(tiles);
+    segments = warp_sum(segments);
+    Split s;
+    s.whole = segments / blocks * blocks;
+    s.spread = segments > s.whole ? (int)(blocks / (segments - s.whole)) : 1;
     long long part = max((long long)kMinTiles, (tiles * 9 / 8 + blocks - 1) / blocks);
     for (;; part *= 2) {
-        long long all = 0, cut = 0;
-        for (int b = lane; b < p.requests; b += 32) {
-            const Request r = load_request(p, b);
-            const Cut c = cut_of(p, r, least_rows, (int)min(part, (long long)0x7FFFFFFF));
-            const long long n = (long long)c.row_tiles * p.cache.heads * c.parts;
-            all += n;
-            if (c.parts > 1) cut += n;
+        s.part_tiles = (int)min(part, (long long)0x3FFFFFFF);
+        long long all = 0, cut = 0, before = 0;
+        for (int base = 0; base < p.requests; base += 32) {
+            Cut c{};
+            c.parts = c.last_parts = 1;
+            Request r{};
+            if (base + lane < p.requests) r = load_request(p, base + lane);
+            const long long own = base + lane < p.requests ? (long long)row_tiles_of(p, r, least_rows) * p.cache.heads : 0, upto = warp_prefix(own);
+            if (base + lane < p.requests) c = cut_of(p, r, least_rows, s, before + upto - own);
+            before += __shfl_sync(kAll, upto, 31);
+            all += items_of(c);
+            cut += parts_of(c);
         }
         all = warp_sum(all);
         cut = warp_sum(cut);
         if (cut <= kPromptParts || part > 0x3FFFFFFF) {
             *items = all;
-            return (int)min(part, (long long)0x7FFFFFFF);
+            return s;
         }
+        if (part > tiles) s.spread = 1;
     }
 }
 
 // Item `index` in the order of requests, from each one's last rows to its first (they see the most).  The whole warp calls.
-__device__ __forceinline__ void find_item(const AttentionParams& p, int least_rows, int part_tiles, long long index, Item* out) {
+__device__ __forceinline__ void find_item(const AttentionParams& p, int least_rows, const Split& split, long long index, Item* out) {
     const int lane = threadIdx.x & 31;
-    long long before = 0, parts_before = 0;
+    long long before = 0, parts_before = 0, segments_before = 0;
     for (int base = 0; base < p.requests; base += 32) {
         Request r{};
-        Cut c{0, 1};
-        if (base + lane < p.requests) {
-            r = load_request(p, base + lane);
-            c = cut_of(p, r, least_rows, part_tiles);
-        }
-        const long long own = (long long)c.row_tiles * p.cache.heads * c.parts, own_parts = c.parts > 1 ? own : 0;
-        long long sum = own, parts = own_parts;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const long long o = __shfl_up_sync(kAll, sum, d), q = __shfl_up_sync(kAll, parts, d);
-            if (lane >= d) {
-                sum += o;
-                parts += q;
-            }
-        }
+        Cut c{};
+        c.parts = c.last_parts = 1;
+        if (base + lane < p.requests) r = load_request(p, base + lane);
+        const long long segments = base + lane < p.requests ? (long long)row_tiles_of(p, r, least_rows) * p.cache.heads : 0, upto = warp_prefix(segments);
+        if (base + lane < p.requests) c = cut_of(p, r, least_rows, split, segments_before + upto - segments);
+        segments_before += __shfl_sync(kAll, upto, 31);
+        const long long own = items_of(c), own_parts = parts_of(c), sum = warp_prefix(own), parts = warp_prefix(own_parts);
         const uint32_t here = __ballot_sync(kAll, before + sum > index);
         if (here == 0) {
             before += __shfl_sync(kAll, sum, 31);
@@ -148,9 +184,18 @@ __device__ __forceinline__ void find_item(const AttentionParams& p, int least_ro
             continue;
         }
         if (lane == __ffs(here) - 1) {
-            const long long in = index - (before + sum - own);
-            const int which = (int)(in % c.parts);
-            const long long segment = in / c.parts;
+            long long in = index - (before + sum - own), first_part = parts_before + parts - own_parts;
+            const long long plain = (long long)(c.segments - c.last) * c.parts;
+            int n_parts = c.parts;
+            long long segment = 0;
+            if (in >= plain) {
+                in -= plain;
+                segment = c.segments - c.last;
+                if (c.parts > 1) first_part += plain;
+                n_parts = c.last_parts;
+            }
+            const int which = (int)(in % n_parts);
+            segment += in / n_parts;
             const int head = (int)(segment % p.cache.heads), tile = c.row_tiles - 1 - (int)(segment / p.cache.heads);
             Item t;
             t.valid = 1;
@@ -160,9 +205,9 @@ __device__ __forceinline__ void find_item(const AttentionParams& p, int least_ro
             t.all_rows = r.rows * p.group;
             t.head = head;
             t.base = tile * 2 * kHalf;
-            t.parts = c.parts;
+            t.parts = n_parts;
             t.which = which;
-            t.part = c.parts > 1 ? (int)(parts_before + parts - own_parts + in - which) : -1;
+            t.part = n_parts > 1 ? (int)(first_part + in - which) : -1;
             // the tokens that the rows of A and of B see, in tiles
             const int first = t.base / p.group;
             t.lo = p.window && r.position + first >= p.window ? min(r.position + first - p.window + 1, r.limit) : r.lo;
@@ -175,8 +220,8 @@ __device__ __forceinline__ void find_item(const AttentionParams& p, int least_ro
                 t.limit = limit;
             }
             const int begin = t.lo / kTokens, n = max(max(end[0], end[1]) - begin, 0);
-            t.tile0 = begin + (int)((long long)n * which / c.parts);
-            const int stop = begin + (int)((long long)n * (which + 1) / c.parts);
+            t.tile0 = begin + (int)((long long)n * which / n_parts);
+            const int stop = begin + (int)((long long)n * (which + 1) / n_parts);
             for (int h = 0; h < 2; ++h) t.tiles[h] = max(min(end[h], stop) - t.tile0, 0);
             *out = t;
         }
@@ -278,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
 
     if (warp == kSchedule) {
         long long count = 0;
-        const int part_tiles = choose_part(p, least_rows, gridDim.x, &count);
+        const Split split = choose_split(p, least_rows, gridDim.x, &count);
         unsigned int* const next = reinterpret_cast<unsigned int*>(header + kPromptNext);
         for (uint32_t n = 0;; ++n) {
             if (!wait_on(&bars.item_empty[n & 1], ((n >> 1) & 1) ^ 1, &s_abort)) break;
@@ -286,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
             if (lane == 0) i = atomicAdd(next, 1u);
             i = __shfl_sync(kAll, i, 0);
             const bool more = i < count;
-            if (more) find_item(p, least_rows, part_tiles, i, &items[n & 1]);
+            if (more) find_item(p, least_rows, split, i, &items[n & 1]);
             else if (lane == 0) items[n & 1].valid = 0;
             __syncwarp();
             if (lane == 0) {
