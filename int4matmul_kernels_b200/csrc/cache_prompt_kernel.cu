@@ -327,17 +327,22 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
         unsigned int* const next = reinterpret_cast<unsigned int*>(header + kPromptNext);
         for (uint32_t n = 0;; ++n) {
             if (!wait_on(&bars.item_empty[n & 1], ((n >> 1) & 1) ^ 1, &s_abort)) break;
-            unsigned int i = 0;
-            if (lane == 0) i = atomicAdd(next, 1u);
-            i = __shfl_sync(kAll, i, 0);
+            // the first item is the block's own number, the others come off the counter
+            long long i = blockIdx.x;
+            if (n > 0) {
+                unsigned int taken = 0;
+                if (lane == 0) taken = atomicAdd(next, 1u);
+                i = (long long)gridDim.x + __shfl_sync(kAll, taken, 0);
+            }
             const bool more = i < count;
             if (more) find_item(p, least_rows, split, i, &items[n & 1]);
             else if (lane == 0) items[n & 1].valid = 0;
             __syncwarp();
             if (lane == 0) {
                 arrive(&bars.item_full[n & 1]);
-                // each block takes one number too many; the last of those leaves the counter as the next launch expects it
-                if (!more && i == count + gridDim.x - 1) atomicExch(next, 0u);
+                // every block that had an item takes one number too many, `count` numbers in all; the last one leaves the counter as the next
+                // launch expects it
+                if (!more && n > 0 && i == count + gridDim.x - 1) atomicExch(next, 0u);
             }
             if (!more) break;
         }
@@ -560,22 +565,23 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                 // q -> shared memory; a negative scale goes into q, so that larger scores are larger weights
                 const uint16_t* const from = static_cast<const uint16_t*>(p.q.p) + (t.row0 + token) * p.q.token + head * p.q.head;
                 float down = 1.f, up = 1.f;
-                if (BF16 && real) {
+                uint4 x[D / 8];
+#pragma unroll
+                for (int u = 0; u < D / 8; ++u) {
+                    x[u] = make_uint4(0, 0, 0, 0);
+                    if (real) x[u] = *reinterpret_cast<const uint4*>(from + 8 * u);
+                }
+                if (BF16) {
                     float top = 0.f;
-#pragma unroll 4
-                    for (int u = 0; u < D / 8; ++u) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(from + 8 * u);
-                        top = fmaxf(top, fmaxf(bf16_most(make_uint2(x.x, x.y)), bf16_most(make_uint2(x.z, x.w))));
-                    }
+#pragma unroll
+                    for (int u = 0; u < D / 8; ++u) top = fmaxf(top, fmaxf(bf16_most(make_uint2(x[u].x, x[u].y)), bf16_most(make_uint2(x[u].z, x[u].w))));
                     bf16_powers(top, up, down);
                 }
                 const uint32_t flip = factor < 0.f ? 0x80008000u : 0u;
                 factor = fabsf(factor) * up;
-#pragma unroll 4
+#pragma unroll
                 for (int u = 0; u < D / 8; ++u) {
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (real) x = *reinterpret_cast<const uint4*>(from + 8 * u);
-                    uint2 a = make_uint2(x.x ^ flip, x.y ^ flip), b = make_uint2(x.z ^ flip, x.w ^ flip);
+                    uint2 a = make_uint2(x[u].x ^ flip, x[u].y ^ flip), b = make_uint2(x[u].z ^ flip, x[u].w ^ flip);
                     if (BF16) {
                         a = bf16_scaled(a, down);
                         b = bf16_scaled(b, down);
