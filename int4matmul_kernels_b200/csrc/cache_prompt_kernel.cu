@@ -450,27 +450,36 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                 ids = later;
                 both = later_both;
             };
+            // (32-bit strides: 64-bit products for each row would take longer than the decoding)
+            const uint8_t* const k_base = cache.k + t.head * cache.k_head + (lane & 7) * cache.k_token + 16 * k_unit;
+            const uint8_t* const v_base = cache.v + t.head * cache.v_head + (D / 8) * v_unit;
+            const int page_mask = (1 << cache.page_shift) - 1;
+            const int k_page = (int)cache.k_page, v_page = (int)cache.v_page, k_token = (int)cache.k_token, v_token = (int)cache.v_token;
             const auto load_keys = [&](int j) {
                 const int first = (t.tile0 + j) * kTokens;
+                const bool all = first >= t.lo && first + kTokens <= t.limit;
 #pragma unroll
                 for (int i = 0; i < kKeyRows; ++i) {
-                    const int row = 8 * (k_block + i) + (lane & 7), token = first + row;
+                    const int token = first + 8 * (k_block + i);              // and lane & 7
                     const int id = __shfl_sync(kAll, ids, (k_block + i) >> 1);
                     k[i] = make_uint4(0, 0, 0, 0);
-                    if (id >= 0 && token >= t.lo && token < t.limit)
-                        k[i] = *reinterpret_cast<const uint4*>(cache.k + (long long)id * cache.k_page + t.head * cache.k_head +
-                                                               (token & ((1 << cache.page_shift) - 1)) * cache.k_token + 16 * k_unit);
+                    if (id >= 0 && (all || (token + (lane & 7) >= t.lo && token + (lane & 7) < t.limit)))
+                        k[i] = *reinterpret_cast<const uint4*>(k_base + (long long)id * k_page + (long long)(token & page_mask) * k_token);
                 }
             };
             const auto load_values = [&](int j) {
                 const int first = (t.tile0 + j) * kTokens + 8 * v_group;
                 const int id = __shfl_sync(kAll, ids, v_group >> 1);
-                const uint8_t* const from = cache.v + (long long)max(id, 0) * cache.v_page + t.head * cache.v_head +
-                                            (first & ((1 << cache.page_shift) - 1)) * cache.v_token + (D / 8) * v_unit;
+                const uint8_t* const from = v_base + (long long)max(id, 0) * v_page + (long long)(first & page_mask) * v_token;
+                if (id >= 0 && first >= t.lo && first + 8 <= t.limit) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    v[i] = VBytes{};
-                    if (id >= 0 && first + i >= t.lo && first + i < t.limit) v[i] = *reinterpret_cast<const VBytes*>(from + i * cache.v_token);
+                    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const VBytes*>(from + (long long)i * v_token);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        v[i] = VBytes{};
+                        if (id >= 0 && first + i >= t.lo && first + i < t.limit) v[i] = *reinterpret_cast<const VBytes*>(from + (long long)i * v_token);
+                    }
                 }
             };
             if (most > 0) {
