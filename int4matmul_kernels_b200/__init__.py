@@ -5,12 +5,13 @@
   packing   producers of the packed weight formats (dense int4/int3/int2, 16:32 sparse int4)
   sharding  column-sharded execution over several GPUs with an all-gather of the outputs
   cache     a paged key-value cache in 8 bits: its tables, its writer, and the attention over it
+  serving   the layer stack with that cache: prompts and single tokens of many requests
   int4matmul (compiled, in lib/)  the torch extension module with the reference's module name
 
 The CUDA library must be built first (`python -m int4matmul_kernels_b200._build`); nothing here computes
 on the CPU and nothing falls back to PyTorch ops.
 """
-__all__ = ["capi", "ops", "packing", "sharding", "cache", "load_extension"]
+__all__ = ["capi", "ops", "packing", "sharding", "cache", "serving", "load_extension"]
 
 
 def load_extension():

@@ -234,3 +234,46 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sca
             stream.cuda_stream)
     _check(status, "cache attention")
     return out
+
+
+class PageTable:
+    """The requests' lengths, their block table and the free pages, all on the GPU; `step` moves them on.
+
+    A place of the batch (a row of the table) that holds no request has length 0; a request begins there with its first step and ends
+    with a step of -1 tokens."""
+
+    def __init__(self, requests: int, pages: int, page_size: int, max_seq: int, device="cuda"):
+        dev = torch.device(device)
+        self.page_size = int(page_size)
+        self.seq_lens = torch.zeros(requests, dtype=torch.int32, device=dev)
+        self.block_table = torch.full((requests, -(-max_seq // self.page_size)), -1, dtype=torch.int32, device=dev)
+        self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.free_count = torch.full((1,), pages, dtype=torch.int32, device=dev)
+
+    def step(self, new_lens: torch.Tensor, max_tokens: int) -> Plan:
+        """Request b adds new_lens[b] tokens (int32 on the GPU; -1: it ends).  max_tokens: their sum, or more."""
+        p = plan(self.seq_lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size, max_tokens)
+        self.seq_lens, self.free_count = p.seq_lens, p.free_count
+        return p
+
+
+class PagedCache:
+    """One layer's keys and values: `pages` pages of `page_size` tokens, `heads` heads of `head_dim`, in int8 or float8_e4m3fn."""
+
+    def __init__(self, pages: int, heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.int8, device="cuda"):
+        if dtype not in _HELD:
+            raise TypeError("dtype must be int8 or float8_e4m3fn")
+        # (bytes of places that nothing was written to are read by no result, but they should be numbers)
+        self.k, self.v = (torch.zeros((pages, heads, page_size, head_dim), dtype=torch.int8, device=device).view(dtype) for _ in range(2))
+        self.scales = torch.zeros((pages, heads, 2), dtype=torch.float32, device=device)
+
+    def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        write(self.k, self.v, self.scales, k, v, slots)
+
+    def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
+        return read(self.k, self.v, self.scales, slots, dtype)
+
+    def attention(self, q: torch.Tensor, table: PageTable, cu_lens: Optional[torch.Tensor] = None, max_len: int = 1, *,
+                  scale: Optional[float] = None, window: int = 0) -> torch.Tensor:
+        """Of the step that `table` has just made: its lengths include the step's tokens."""
+        return attention(q, self.k, self.v, self.scales, table.block_table, table.seq_lens, cu_lens, max_len, scale=scale, window=window)
