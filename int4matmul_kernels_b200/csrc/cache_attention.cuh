@@ -48,6 +48,22 @@ __device__ __forceinline__ Request load_request(const AttentionParams& p, int b)
     return r;
 }
 
+// ---- sums over a warp
+__device__ __forceinline__ long long warp_sum(long long v) {
+#pragma unroll
+    for (int d = 16; d; d /= 2) v += __shfl_xor_sync(kAll, v, d);
+    return v;
+}
+__device__ __forceinline__ long long warp_prefix(long long v) {             // sum over this lane and those before it
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const long long o = __shfl_up_sync(kAll, v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
 // ---- decoding --------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;

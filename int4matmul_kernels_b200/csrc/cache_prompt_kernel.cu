@@ -109,21 +109,6 @@ __device__ __forceinline__ long long parts_of(const Cut& c) {             // of 
     return (c.parts > 1 ? (long long)(c.segments - c.last) * c.parts : 0) + (c.last_parts > 1 ? (long long)c.last * c.last_parts : 0);
 }
 
-__device__ __forceinline__ long long warp_sum(long long v) {
-#pragma unroll
-    for (int d = 16; d; d /= 2) v += __shfl_xor_sync(kAll, v, d);
-    return v;
-}
-__device__ __forceinline__ long long warp_prefix(long long v) {             // sum over this lane and those before it
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const long long o = __shfl_up_sync(kAll, v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-
 // How all segments are cut, and the number of items.  Parts must find room in the workspace.
 __device__ __forceinline__ Split choose_split(const AttentionParams& p, int least_rows, int blocks, long long* items) {
     const int lane = threadIdx.x & 31;

@@ -68,8 +68,7 @@ __device__ __forceinline__ int row_tiles(const AttentionParams& p, const Request
 }
 
 template <int ROWS>
-__device__ __forceinline__ long long units_of(const AttentionParams& p, int most_rows, int b) {
-    const Few r = load_few(p, most_rows, b);
+__device__ __forceinline__ long long units_of(const AttentionParams& p, const Few& r) {
     if (r.rows == 0) return 0;
     return (long long)r.tiles * p.cache.heads * row_tiles<ROWS>(p, r);
 }
@@ -138,11 +137,17 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + i) = make_uint4(0, 0, 0, 0);
     }
 
-    // all tiles; the block's range and the warp's
-    long long total = 0;
-    for (int b = lane; b < p.requests; b += 32) total += units_of<S::kRows>(p, most_rows, b);
-#pragma unroll
-    for (int d = 16; d; d /= 2) total += __shfl_xor_sync(kAll, total, d);
+    // all tiles; the block's range and the warp's.  The first 32 requests stay in the lanes' registers.
+    Few mine{};
+    long long own = 0;
+    if (lane < p.requests) {
+        mine = load_few(p, most_rows, lane);
+        own = units_of<S::kRows>(p, mine);
+    }
+    long long total = own;
+    for (int b = lane + 32; b < p.requests; b += 32) total += units_of<S::kRows>(p, load_few(p, most_rows, b));
+    const long long own_upto = warp_prefix(own);
+    total = warp_sum(total);
     const long long blocks = min((long long)gridDim.x, (total + kMinBlockTiles - 1) / kMinBlockTiles);
     if (blockIdx.x >= blocks) return;
     const long long c0 = range_lo(total, blocks, blockIdx.x), c1 = range_lo(total, blocks, blockIdx.x + 1);
@@ -161,27 +166,32 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         int b = 0, segment, tile;
         Few r;
         {
-            long long before = 0;
-            for (;; b += 32) {
-                const long long own = b + lane < p.requests ? units_of<S::kRows>(p, most_rows, b + lane) : 0;
-                long long sum = own;
-#pragma unroll
-                for (int d = 1; d < 32; d *= 2) {
-                    const long long o = __shfl_up_sync(kAll, sum, d);
-                    if (lane >= d) sum += o;
-                }
-                const uint32_t here = __ballot_sync(kAll, before + sum > u0);
+            long long before = 0, here_own = own, upto = own_upto;
+            for (;;) {
+                const uint32_t here = __ballot_sync(kAll, before + upto > u0);
                 if (here) {
                     const int l = __ffs(here) - 1;
-                    before += __shfl_sync(kAll, sum - own, l);
+                    before += __shfl_sync(kAll, upto - here_own, l);
                     b += l;
                     break;
                 }
-                before += __shfl_sync(kAll, sum, 31);
-                if (b + 32 >= p.requests) break;      // (not unless the lengths change under the kernel)
+                before += __shfl_sync(kAll, upto, 31);
+                b += 32;
+                if (b >= p.requests) break;           // (not unless the lengths change under the kernel)
+                here_own = b + lane < p.requests ? units_of<S::kRows>(p, load_few(p, most_rows, b + lane)) : 0;
+                upto = warp_prefix(here_own);
             }
             b = min(b, p.requests - 1);
-            r = load_few(p, most_rows, b);
+            if (b < 32) {
+                r.row0 = __shfl_sync(kAll, mine.row0, b);
+                r.rows = __shfl_sync(kAll, mine.rows, b);
+                r.position = __shfl_sync(kAll, mine.position, b);
+                r.lo = __shfl_sync(kAll, mine.lo, b);
+                r.limit = __shfl_sync(kAll, mine.limit, b);
+                r.tiles = __shfl_sync(kAll, mine.tiles, b);
+            } else {
+                r = load_few(p, most_rows, b);
+            }
             segment = (int)((u0 - before) / r.tiles);
             tile = (int)(u0 - before - (long long)segment * r.tiles);
         }
