@@ -5,21 +5,30 @@
 //   o = sum_j P_j v_j / sum_j (P_j / s_value),  k_j and v_j the cache's bytes, s_key and s_value their page's scales
 // so the value scale is in the weight that is rounded anyway, and the bytes go into the tensor cores as they are.
 //
-// With hundreds of rows for each byte the tensor cores and the exponentials bound it: per tile of 256 rows and 128 tokens at
-// head_dim 128, 4 products of 128 x 128 x 128 (510 cycles each at the measured rate of the tensor cores) and 32768 exponentials (16 a
-// cycle and SM: 2048 cycles).  Both have to run all the time, so they belong to different warps:
+// With hundreds of rows for each byte the tensor cores and the exponentials bound it: per tile of 256 rows and 128 tokens at head_dim 128,
+// 16 score instructions of 128 x 128 x 16 with both operands in shared memory (106 cycles each, measured alone), 16 of the second product
+// with the weights in tensor memory (76), 2900 cycles together, and 32768 exponentials (16 a cycle and SM: 2048 cycles).  They have to run
+// at the same time, so they belong to different warps:
 //
 //   warps 0..3, 4..7   softmax of 128 rows each (A and B): a thread owns a row; scores come from tensor memory, weights go back there,
 //                      where they are the A operand of the second product
 //   warps 8..11        read the pages, turn bytes into fp16 (exact) and lay out K and V^T for the tensor cores (128-byte swizzle);
 //                      K and V tiles are decoded once for 256 rows
 //   warp 12            issues the products: while the softmax of A runs, the tensor cores work for B
-//   warp 13            takes the next item (request, key head, 256 rows, a range of tokens) off a common counter, one ahead
+//   warp 13            takes the next item (request, key head, 256 rows, a range of tokens), one ahead
 //
 // The rows of all query heads of a key head are packed into one tile: row r is token r / group, head r % group.  Sums stay in
 // tensor memory in fp32 and are rescaled only when a row's weights would outgrow fp16 (below that their relative precision is the
-// same), which costs no maximum on the way: the weights' sum, which is needed anyhow, tells.  Long contexts under few rows are cut along the tokens into items of their own; the block that finishes a
-// segment's last part joins them in order.  Every wait is bounded; a block that gives up records it in the status word.
+// same), which costs no maximum on the way: the weights' sum, which is needed anyhow, tells.  Long contexts under few rows are cut along the
+// tokens into items of their own; the block that finishes a segment's last part joins them in order.  Every wait is bounded; a block that
+// gives up records it in the status word.
+//
+// Measured: 2 x 1024 new tokens after 8000, 64 heads in groups of 8: 735 us, 730 TFLOP/s; a prompt of 2048 tokens, 40 heads: 103 us.  A tile
+// takes about 5000 cycles: the chain of one half (scores 850 and more, 400 until they are in registers, 2 x 1000 for weights, 2 x 250 to pack and
+// publish them, the second product) against the other half's, and the decoding warps' chain, which is as long.  Without exponentials it is
+// 2 % faster, without decoding 17 %, with neither softmax nor decoding 40 %.  Slower: scores of 64 tokens at a time in two halves of their
+// columns (1000 us: 75 cycles an instruction, and loads from tensor memory wait for products), one thread waiting and issuing instead of
+// an elected lane of a whole warp (900).
 #include <algorithm>
 #include <type_traits>
 

@@ -5,21 +5,27 @@
 // rows, so DRAM bounds it: 24 bytes a cycle and SM.  What the rest is made for is to keep that many bytes in flight and to decode them
 // in less than that time:
 //
-// * Work.  The tokens of a request and head (a segment) are cut into tiles of 16.  All tiles of all segments in a row are dealt out in
+// * Work.  The tokens of a request and head (a segment) are cut into tiles of 32.  All tiles of all segments in a row are dealt out in
 //   equal contiguous ranges, to the blocks (one to an SM) and within them to the warps, whatever the lengths are.  What a
 //   range cuts is joined: warps of a block through shared memory, blocks through the workspace, where the block that comes last adds up
 //   all parts in their order (so results do not depend on which one it is).  Nobody waits for anybody.
 // * Bytes.  Each warp fetches its own tiles, two ahead, into a ring of its own (a TMA copy for each 16 keys and 16 values, swizzled, one
-//   barrier for a tile): warps do not wait for one another, and no registers are held by loads in flight.
-// * Products.  S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16: the cache is the 16-row operand, the head's rows are the 8 columns, so a
-//   tile costs 16 instructions for 8 rows.  The order of the 16 k of an instruction is free as long as both operands agree, so a thread
-//   takes 16 consecutive bytes of a key row (and the same places of q), and 16 consecutive bytes of each of its four value rows; two
-//   value rows become operand words by byte permutes.  int8 becomes fp16 by placing the byte in the mantissa of 1024 (exact), e4m3 by
-//   the conversion instruction (exact).  The weights go from the accumulator layout to the operand layout by a transpose of 8 x 8 matrices.
-// * Scales.  The page's key scale multiplies the scores.  Weights are rounded to fp16 relative to the largest of their tile, and each
-//   tile's product joins the fp32 sums with the factor 2^(m_tile - m) * value scale: pages of any scales, none of it lost to fp16's
-//   range.  A second product with the weights' rounding errors (their low halves) brings the output to fp32's exactness for 8 more
-//   tensor instructions a tile, which the tensor pipe has spare.
+//   barrier for a tile): warps do not wait for one another, and no registers are held by loads in flight.  Copies alone, with nothing
+//   done to what they bring, take 207 us for 1.32 GB (64 requests of up to 4000 tokens, 40 heads of 128); the same bytes by 16-byte
+//   copies of each thread took 314.
+// * Products.  S^T = K Q^T and O^T = V^T P^T with mma.m16n8k16: the cache is the 16-row operand, the head's rows are the 8 columns.  The
+//   order of the 16 k of an instruction is free as long as both operands agree, so a thread takes 16 consecutive bytes of a key row (and
+//   the same places of q), and 16 consecutive bytes of each of its value rows; two value rows become operand words by byte
+//   permutes.  int8 becomes fp16 by placing the byte in the mantissa of 1024 (exact), e4m3 by the conversion instruction (exact).  The
+//   weights go from the accumulator layout to the operand layout by a transpose of 8 x 8 matrices.
+// * Scales.  x = s + log2(value scale) of the page: weights are 2^(x - the tile's largest x), rounded to fp16, and a tile's product joins the
+//   fp32 sums with the factor 2^(largest x - reference): pages of any scales, none of it lost to fp16's range; the totals take each weight
+//   divided by its page's value scale again.  A second product with the weights' rounding errors (their low halves) brings the output to
+//   fp32's exactness for 16 more tensor instructions a tile, which the tensor pipe (20 % busy) has spare.
+//
+// Measured: the requests above 284 us (4.7 TB/s; some 830 instructions a tile of 32 tokens, half of them for the bytes' decoding, are what is left
+// to hide); 12 requests of 20000 to 34000 tokens, 8 heads, e4m3, 8 rows: 118 us (5.7 TB/s); one request of 1011 tokens: 14 us, of which
+// 5 find and fetch the first tile, 3.6 join parts over blocks.  (Whole segments to blocks, without that join: 14.8.)
 #include <algorithm>
 #include <type_traits>
 
@@ -34,12 +40,15 @@ constexpr uint32_t kNoPage = 0x7FC0DEADu;             // in the place of a scale
 
 template <int D, int NT>
 struct Shape {
-    static constexpr int kWarps = 8;
+    // Registers (about 180 to 245 where nothing is spilled) allow 8 warps; with half the bytes to a token, 12 warps of 168 hide more of a tile's
+    // dependent steps than they lose (33 drafts, head_dim 64: 63.5 us with 8, 61.6 with 12; 64 single tokens, head_dim 128: 284 and 279
+    // with a ring of two stages, 118 and 122 on long contexts).
+    static constexpr int kWarps = D == 64 ? 12 : 8;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kRows = 8 * NT;
     static constexpr int kHalfBytes = 32 * D;                                 // 16 tokens: keys, then values
     static constexpr int kStageBytes = 2 * kHalfBytes;
-    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kStages = D == 128 ? 3 : 4;
     static constexpr int kWarpBytes = kStages * kStageBytes;
     static constexpr int kPartFloats = kRows * D + 2 * kRows;                 // sums, maxima, totals of a part of a segment
     static_assert(kPartFloats * 4 <= kWarpBytes, "a warp leaves its last part in its ring");
@@ -47,6 +56,7 @@ struct Shape {
 
 // ---- behind the workspace's header: [a part per warp][two parts per block] ----
 constexpr size_t kWarpPartsBytes = (size_t)kMaxBlocks * Shape<128, 2>::kWarps * Shape<128, 2>::kPartFloats * 4;
+static_assert(Shape<64, 2>::kWarps * Shape<64, 2>::kPartFloats <= Shape<128, 2>::kWarps * Shape<128, 2>::kPartFloats, "room for any shape");
 constexpr size_t kBlockPartsBytes = (size_t)kMaxBlocks * 2 * Shape<128, 2>::kPartFloats * 4;
 
 // a request and its tiles of tokens: at least one if there are rows (rows that see nothing are written too)
