@@ -13,7 +13,7 @@ constexpr uint32_t kAll = 0xFFFFFFFFu;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxBlocks = 148;                       // one block to an SM
 // Requests of at most this many rows (new tokens times query heads of a key head) are the few-row kernel's, wherever both run
-constexpr int kFewRows = 16;
+constexpr int kFewRows = 64;
 
 // ---- the workspace: [counters, with the status word where i4mm_device_status looks for it][parts of the few-row kernel][of the other] ----
 constexpr size_t kCacheHeaderBytes = kCounterBytes;

@@ -64,10 +64,10 @@ int view_of(const i4mm_cache* c, i4mm::CacheView& w) {
 
 size_t attention_workspace() { return i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace() + i4mm::cache_prompt_workspace(); }
 
-// Which kernel.  A request's rows are its new tokens times the query heads of a key head.  Up to 16 of them, the few-row kernel reads the
-// cache once and is bound by that; more of them are the prompt kernel's.  Where a batch may have both, both run, each on its own requests.
-// (16 requests of one token beside a chunk of 256 after 2200, groups of 4: 31 us and 53 us; a tile of 256 rows for each of the 16 would take
-// the prompt kernel twice the few-row kernel's time.)
+// Which kernel.  A request's rows are its new tokens times the query heads of a key head.  The few-row kernel takes 8 or 16 of them at a time
+// and reads the cache again (from the second-level cache) for the next ones, the prompt kernel works on 256 whatever they are: 16 requests of one
+// token with contexts around 2250, 8 key heads of 128, 8 / 16 / 32 / 64 rows: 27 / 41 / 61 / 101 us and always 118; 2 requests 16 / 23 / 27 / 29
+// and 35; 64 requests around 2000 65 / 99 / 168 / 295 and 259.  Where a batch may have both kinds, both run, each on its own requests.
 cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t max_len, cudaStream_t stream) {
     const int64_t rows = (p.cu_lens ? std::max<int64_t>(max_len, 1) : 1) * p.group;
     if (rows <= i4mm::kFewRows) return i4mm::cache_rows_launch(p, e4m3, bf16, 0x7FFFFFFF, rows <= 8, stream);
