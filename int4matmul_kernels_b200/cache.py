@@ -109,8 +109,9 @@ def plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tens
 
     `block_table` (requests, width) gets the pages that the step begins, in place; `free_pages` is a stack with its first free_count[0]
     entries free: the pages of requests that end are pushed, then new ones popped, in request order.  seq_lens, new_lens and
-    free_count are left alone: the next step takes the Plan's.  Where no page is left the table's entry and the slots become -1 and
-    Plan.missing counts it."""
+    free_count are left alone: the next step takes the Plan's.  Where no page is left the table's entry and the slots become -1, so that
+    nothing is written or seen there, and Plan.missing counts it: drop such a Plan and make a smaller step from the same lengths and count
+    (a request that goes on without its pages must not end: it would give -1 back as pages)."""
     mod = ops.native()
     if mod:
         out = mod._try_cache_plan(seq_lens, new_lens, block_table, free_pages, free_count, page_size, max_tokens)
@@ -249,12 +250,20 @@ class PageTable:
         self.block_table = torch.full((requests, -(-max_seq // self.page_size)), -1, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)
         self.free_count = torch.full((1,), pages, dtype=torch.int32, device=dev)
+        self._before = None
 
     def step(self, new_lens: torch.Tensor, max_tokens: int) -> Plan:
         """Request b adds new_lens[b] tokens (int32 on the GPU; -1: it ends).  max_tokens: their sum, or more."""
         p = plan(self.seq_lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size, max_tokens)
+        self._before = (self.seq_lens, self.free_count)
         self.seq_lens, self.free_count = p.seq_lens, p.free_count
         return p
+
+    def undo(self) -> None:
+        """Takes the last step back (its Plan.missing was not 0, say); what it wrote into caches is overwritten by the next."""
+        if self._before is None:
+            raise ValueError("there is no step to take back")
+        (self.seq_lens, self.free_count), self._before = self._before, None
 
 
 class PagedCache:

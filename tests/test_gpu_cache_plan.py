@@ -69,6 +69,20 @@ def test_pages_that_run_out():
         assert p.missing.item() > 0 and p.free_count.item() == 0
 
 
+def test_a_step_that_finds_no_pages_is_taken_back():
+    t = cache.PageTable(3, 5, 16, 200)
+    with pytest.raises(ValueError):
+        t.undo()
+    assert t.step(ints([30, 16, 0]), 46).missing.item() == 0
+    assert t.step(ints([40, 1, 20]), 61).missing.item() == 4
+    t.undo()
+    assert t.seq_lens.tolist() == [30, 16, 0] and t.free_count.item() == 2
+    p = t.step(ints([-1, 1, 40]), 41)
+    assert p.missing.item() == 0 and p.free_count.item() == 0
+    table = t.block_table.tolist()
+    assert sorted(table[1][:2] + table[2][:3]) == [0, 1, 2, 3, 4] and p.slots.min().item() >= 0
+
+
 def test_table_rows_that_are_full():
     for seed in range(4):
         check(*problem(9, 16, 100, 200, 0.1, 100, seed, width=4), 16, 2000)
