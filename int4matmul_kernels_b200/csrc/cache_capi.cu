@@ -68,9 +68,19 @@ size_t attention_workspace() { return i4mm::kCacheHeaderBytes + i4mm::cache_rows
 // and reads the cache again (from the second-level cache) for the next ones, the prompt kernel works on 256 whatever they are: 16 requests of one
 // token with contexts around 2250, 8 key heads of 128, 8 / 16 / 32 / 64 rows: 27 / 41 / 61 / 101 us and always 118; 2 requests 16 / 23 / 27 / 29
 // and 35; 64 requests around 2000 65 / 99 / 168 / 295 and 259.  Where a batch may have both kinds, both run, each on its own requests.
+// Little work is the few-row kernel's alone, more rows or not: it begins 5 to 10 us earlier, and a second launch costs 10.  `tiles` bounds its tiles
+// of 32 tokens and 16 rows by what the host knows (lengths are on the GPU).  Single tokens beside a chunk: up to 12000 (bound 2250: 20 us and
+// 34 for both, 5780: 34 and 45, 10192: 43 and 65, 12480: 40 and 44, 17680: 60 and 51).  Prompts alone: up to 8000 (1360: 25 and 33, 4160: 31 and
+// 34, 10640: 44 and 36), but not those whose rows are more than twice their tokens, which fill the prompt kernel's tiles (1764: 26 and
+// 25, 2576: 31 and 22, 4644: 31 and 19).
 cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t max_len, cudaStream_t stream) {
-    const int64_t rows = (p.cu_lens ? std::max<int64_t>(max_len, 1) : 1) * p.group;
-    if (rows <= i4mm::kFewRows) return i4mm::cache_rows_launch(p, e4m3, bf16, 0x7FFFFFFF, rows <= 8, stream);
+    const int64_t len = p.cu_lens ? std::max<int64_t>(max_len, 1) : 1, rows = len * p.group;
+    int64_t span = (int64_t)p.table_width << p.cache.page_shift;
+    if (p.window) span = std::min(span, (int64_t)p.window + len);
+    const int64_t tiles = ((int64_t)p.tokens * p.group / 16 + p.requests) * p.cache.heads * (span / 32 + 1);
+    const bool mixed = (int64_t)p.tokens * 2 < p.requests * len;
+    const bool little = mixed ? tiles <= 12000 : tiles <= 8000 && (rows < 2 * span || tiles <= 1000);
+    if (rows <= i4mm::kFewRows || little) return i4mm::cache_rows_launch(p, e4m3, bf16, 0x7FFFFFFF, rows <= 8, stream);
     if (p.group > i4mm::kFewRows) return i4mm::cache_prompt_launch(p, e4m3, bf16, 1, true, stream);
     const cudaError_t e = i4mm::cache_rows_launch(p, e4m3, bf16, i4mm::kFewRows, p.group <= 8, stream);
     return e != cudaSuccess ? e : i4mm::cache_prompt_launch(p, e4m3, bf16, i4mm::kFewRows + 1, false, stream);

@@ -45,12 +45,18 @@ def make(seqs, heads, page, dim, held, seed, order="heads", spread=0.7, spare=3)
 def check(q, k, v, scales, table, seq, cu=None, max_len=1, scale=None, window=0):
     got = cache.attention(q, k, v, scales, table, seq, cu, max_len, scale=scale, window=window)
     assert got.shape == q.shape and got.dtype == q.dtype and got.is_contiguous()
+    # The kernel is chosen by how much work a call may be, which the table's width bounds: one with many places for pages that are not there is
+    # more, and takes the prompt kernel for requests of more than 64 rows.
+    wide = torch.full((table.shape[0], table.shape[1] + 200000 // k.shape[2]), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    other = cache.attention(q, k, v, scales, wide, seq, cu, max_len, scale=scale, window=window)
     s = 1 / math.sqrt(q.shape[2]) if scale is None else scale
     out, size, reach, tail = reference(q, values(k, scales[..., 0]), values(v, scales[..., 1]), table, seq, cu, s, window)
     limit = attention_bound(out, size, reach, tail, q.dtype)
-    off = (got.double() - out).abs()
-    assert (off <= limit).all(), ((off / limit).max().item(), (off > limit).nonzero()[:3].tolist())
-    assert (got[(size == 0).all(-1)] == 0).all()
+    for result in (got, other):
+        off = (result.double() - out).abs()
+        assert (off <= limit).all(), ((off / limit).max().item(), (off > limit).nonzero()[:3].tolist())
+        assert (result[(size == 0).all(-1)] == 0).all()
     return got
 
 
@@ -162,11 +168,13 @@ def test_a_wrong_max_len_changes_nothing_but_time(max_len):
     check(queries(gen, sum(lens), 6, 128, FP16), k, v, scales, table, ints(seqs), cu, max_len)
 
 
+@pytest.mark.parametrize("places", [0, 10000])
 @pytest.mark.parametrize("lens", [[1, 1, 1], [3, 2, 1], [60, 1, 200]])
-def test_bytes_and_scales_of_places_that_no_row_sees(lens):
+def test_bytes_and_scales_of_places_that_no_row_sees(lens, places):
     """The rest of a last page, and whole pages beyond it: NaN bytes, scales that are infinite or NaN."""
     seqs = [77, 201, 203]
     k, v, scales, table, gen = make(seqs, 2, 16, 128, E4M3, 62)
+    table = torch.cat([table, torch.full((3, places), -1, dtype=torch.int32, device="cuda")], dim=1)
     cu = ints([0] + torch.tensor(lens).cumsum(0).tolist())
     q = queries(gen, sum(lens), 4, 128, BF16)
     want = check(q, k, v, scales, table, ints(seqs), cu, max(lens))
@@ -246,11 +254,13 @@ def test_a_cache_whose_offsets_pass_32_bits():
     assert (r[0] - x[:, :heads]).abs().max() < 0.05 and r[0].abs().max() > 1
 
 
+@pytest.mark.parametrize("places", [0, 10000])
 @pytest.mark.parametrize("lens", [[1] * 30, [2] * 30, [90] + [1] * 28 + [200]])
-def test_repeated_calls_give_the_same_bits(lens):
+def test_repeated_calls_give_the_same_bits(lens, places):
     """Beside other work on another stream too: nothing depends on which block comes first."""
     seqs = [max(n, 37 * (i + 3) % 4000) for i, n in enumerate(lens)]
     k, v, scales, table, gen = make(seqs, 4, 16, 128, INT8, 67)
+    table = torch.cat([table, torch.full((len(seqs), places), -1, dtype=torch.int32, device="cuda")], dim=1)
     cu = ints([0] + torch.tensor(lens).cumsum(0).tolist())
     q = queries(gen, sum(lens), 8, 128, FP16)
     first = cache.attention(q, k, v, scales, table, ints(seqs), cu, max(lens))
