@@ -578,13 +578,20 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
     // (parts of other blocks are read past the first-level cache)
     const auto add = [&](Joined& a, const float* part, int row, bool mine) {
         const auto load = [&](int i) { return mine ? part[i] : __ldcg(part + i); };
+        using Columns = std::conditional_t<kMine == 4, float4, float2>;
+        const Columns* const at = reinterpret_cast<const Columns*>(part + row * D) + lane;
+        const Columns x = mine ? *at : __ldcg(at);
         const float pm = load(S::kRows * D + row), ps = load(S::kRows * D + S::kRows + row);
         const float next = fmaxf(a.m, pm);
         const float keep = a.m == -INFINITY ? 0.f : exp2_approx(a.m - next), take = pm == -INFINITY ? 0.f : exp2_approx(pm - next);
         a.m = next;
         a.sum = a.sum * keep + ps * take;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) a.o[i] = a.o[i] * keep + load(row * D + kMine * lane + i) * take;
+        a.o[0] = a.o[0] * keep + x.x * take;
+        a.o[1] = a.o[1] * keep + x.y * take;
+        if constexpr (kMine == 4) {
+            a.o[2] = a.o[2] * keep + x.z * take;
+            a.o[3] = a.o[3] * keep + x.w * take;
+        }
     };
     const auto finish = [&](const Joined& a, const Piece& piece, int row) {
         const Request r = load_request(p, piece.b);
