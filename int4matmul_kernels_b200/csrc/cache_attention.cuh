@@ -12,6 +12,30 @@ namespace i4mm {
 constexpr uint32_t kAll = 0xFFFFFFFFu;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxBlocks = 148;                       // one block to an SM
+// ---- PTX that only these kernels use ---------------------------------------------------------------------------------------------------------
+namespace ptx {
+// 8 bytes; cp_async_arrive: this thread arrives on the barrier (which counts it) once its copies so far are done
+__device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// 4-D tiled tensor-map copy, coordinates (x = innermost, y, z, w)
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
+}
+// D[tmem] (+)= A[smem descriptor] * B[smem descriptor]; kind::f16; one thread issues
+__device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+}  // namespace ptx
+
 // Requests of at most this many rows (new tokens times query heads of a key head) are the few-row kernel's, wherever both run
 constexpr int kFewRows = 64;
 
@@ -146,8 +170,6 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
 // Prompts: requests of fewer than least_rows rows are left to the other one; `alone`: it is not launched.
 cudaError_t cache_rows_launch(const AttentionParams& p, bool e4m3, bool bf16, int most_rows, bool few, cudaStream_t stream);
 cudaError_t cache_prompt_launch(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, bool alone, cudaStream_t stream);
-bool encode_bytes(CUtensorMap* out, int rank, const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
-                  CUtensorMapSwizzle swizzle);        // umma_kernel.cu
 size_t cache_rows_workspace();                        // bytes behind the header
 size_t cache_prompt_workspace();                      // bytes behind those
 

@@ -1961,23 +1961,4 @@ int umma_launch(int bits, bool sparse, const StreamParams& sp, int total_rows, i
     return launch_fmt<2, false>(p, sp.x, n_groups, cta_pairs, force_nt, stream, cuda_err);
 }
 
-// A tensor map of `rank` dimensions of bytes, innermost first (strides from the second on), for the other kernels of the library.
-bool encode_bytes(CUtensorMap* out, int rank, const void* base, const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
-                  CUtensorMapSwizzle swizzle) {
-    EncodeTiledFn enc = encode_tiled_fn();
-    if (!enc || rank > 5) return false;
-    cuuint64_t d[5], s[5];
-    cuuint32_t b[5];
-    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
-    for (int i = 0; i < rank; ++i) {
-        d[i] = dims[i];
-        b[i] = box[i];
-        if (i + 1 < rank) s[i] = strides[i];
-    }
-    return encode_with_context([&] {
-        return enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    });
-}
-
 }  // namespace i4mm
