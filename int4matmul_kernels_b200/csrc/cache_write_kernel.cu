@@ -188,8 +188,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) cache_write_kernel(const Cache
         const float s = fmaxf(old, scale_for<E4M3>(a));
         uint8_t* const held = (which ? c.v : c.k) + id * (which ? c.v_page : c.k_page) + head * (which ? c.v_head : c.k_head);
         const long long held_token = which ? c.v_token : c.k_token;
-        if (s > old && old > 0.f) {
-            const float ratio = old / s;
+        if (s > old && place > 0) {
+            const float ratio = old / s;              // (0 where the scale was: bytes of infinities beside zeros go on standing for 0)
             for (int i = row; i < place; i += rows_per_step) {
                 uint2* const at = reinterpret_cast<uint2*>(held + i * held_token + col);
                 uint2 w = *at;
