@@ -241,29 +241,36 @@ class PageTable:
     """The requests' lengths, their block table and the free pages, all on the GPU; `step` moves them on.
 
     A place of the batch (a row of the table) that holds no request has length 0; a request begins there with its first step and ends
-    with a step of -1 tokens."""
+    with a step of -1 tokens.  The arrays stay where they are, so that a step captured in a CUDA graph is the next step whenever the graph
+    is replayed."""
 
     def __init__(self, requests: int, pages: int, page_size: int, max_seq: int, device="cuda"):
         dev = torch.device(device)
         self.page_size = int(page_size)
-        self.seq_lens = torch.zeros(requests, dtype=torch.int32, device=dev)
+        # lengths and the count of free pages lie together: what `undo` keeps of them is one copy
+        self._state = torch.zeros(requests + 1, dtype=torch.int32, device=dev)
+        self._saved = torch.empty_like(self._state)
+        self.seq_lens, self.free_count = self._state[:requests], self._state[requests:]
+        self.free_count.fill_(pages)
         self.block_table = torch.full((requests, -(-max_seq // self.page_size)), -1, dtype=torch.int32, device=dev)
         self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)
-        self.free_count = torch.full((1,), pages, dtype=torch.int32, device=dev)
-        self._before = None
+        self._can_undo = False
 
     def step(self, new_lens: torch.Tensor, max_tokens: int) -> Plan:
         """Request b adds new_lens[b] tokens (int32 on the GPU; -1: it ends).  max_tokens: their sum, or more."""
         p = plan(self.seq_lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size, max_tokens)
-        self._before = (self.seq_lens, self.free_count)
-        self.seq_lens, self.free_count = p.seq_lens, p.free_count
+        self._saved.copy_(self._state)
+        self.seq_lens.copy_(p.seq_lens)
+        self.free_count.copy_(p.free_count)
+        self._can_undo = self._can_undo or not torch.cuda.is_current_stream_capturing()
         return p
 
     def undo(self) -> None:
         """Takes the last step back (its Plan.missing was not 0, say); what it wrote into caches is overwritten by the next."""
-        if self._before is None:
+        if not self._can_undo:
             raise ValueError("there is no step to take back")
-        (self.seq_lens, self.free_count), self._before = self._before, None
+        self._state.copy_(self._saved)
+        self._can_undo = False
 
 
 class PagedCache:
