@@ -241,7 +241,7 @@ class PageTable:
     """The requests' lengths, their block table and the free pages, all on the GPU; `step` moves them on.
 
     A place of the batch (a row of the table) that holds no request has length 0; a request begins there with its first step and ends
-    with a step of -1 tokens.  The arrays stay where they are, so that a step captured in a CUDA graph is the next step whenever the graph
+    with a step of -1 tokens.  A step that cannot have all of its pages is not made: see `step`.  The arrays stay where they are, so that a step captured in a CUDA graph is the next step whenever the graph
     is replayed."""
 
     def __init__(self, requests: int, pages: int, page_size: int, max_seq: int, device="cuda"):
@@ -257,16 +257,23 @@ class PageTable:
         self._can_undo = False
 
     def step(self, new_lens: torch.Tensor, max_tokens: int) -> Plan:
-        """Request b adds new_lens[b] tokens (int32 on the GPU; -1: it ends).  max_tokens: their sum, or more."""
+        """Request b adds new_lens[b] tokens (int32 on the GPU; -1: it ends).  max_tokens: their sum, or more.
+
+        Where Plan.missing is not 0 there were too few pages, and the step is not made: all of Plan.slots are -1, so that its tokens
+        are written nowhere, no request ends, and lengths and free pages stay.  (They are kept on the GPU: nothing waits.  What is
+        computed with such a Plan is void; Plan.seq_lens and free_count are what would have come.)  The next step may be any other one."""
         p = plan(self.seq_lens, new_lens, self.block_table, self.free_pages, self.free_count, self.page_size, max_tokens)
+        short = p.missing != 0
+        p.slots.masked_fill_(short, -1)
         self._saved.copy_(self._state)
-        self.seq_lens.copy_(p.seq_lens)
-        self.free_count.copy_(p.free_count)
+        torch.where(short, self.seq_lens, p.seq_lens, out=self.seq_lens)
+        torch.where(short, self.free_count, p.free_count, out=self.free_count)
         self._can_undo = self._can_undo or not torch.cuda.is_current_stream_capturing()
         return p
 
     def undo(self) -> None:
-        """Takes the last step back (its Plan.missing was not 0, say); what it wrote into caches is overwritten by the next."""
+        """Takes the last step back, before any of its tokens has been written into a cache: what a write does to a page (pages of requests
+        that end are given out again in the same step; a scale that grows rounds the bytes beside the new ones again) is not undone."""
         if not self._can_undo:
             raise ValueError("there is no step to take back")
         self._state.copy_(self._saved)
