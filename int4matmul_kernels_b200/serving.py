@@ -5,6 +5,7 @@ paged 8-bit cache between the quantized linears.
     server = CachedStack(stack, heads=40, pages=4096, page_size=16, requests=64, max_seq=4096)
     h = server.step(prompts, new_lens, max_len)         # packed rows of the step's new tokens, request by request
     h = server.step(tokens, ones, 1)                    # one token of every request
+    server.plan.missing                                 # of the last step, on the GPU: not 0 where there were too few pages
 """
 from __future__ import annotations
 
@@ -33,12 +34,16 @@ class CachedStack:
         self.stack, self.heads, self.head_dim, self.window = stack, heads, hidden // heads, window
         device = stack.layers[0]["qkv"].matrix.device
         self.table = cache.PageTable(requests, pages, page_size, max_seq, device)
+        self.plan = None                               # the last step's
         self.caches = [cache.PagedCache(pages, heads, page_size, self.head_dim, dtype, device) for _ in stack.layers]
 
     def step(self, h: torch.Tensor, new_lens: torch.Tensor, max_len: int) -> torch.Tensor:
         """h (tokens, hidden) fp16: the new tokens' rows, request by request; new_lens (requests) int32 on the GPU, -1 where a request
-        ends; max_len: the most new tokens of a request.  Returns the last layer's rows.  Nothing here waits for the GPU."""
-        plan = self.table.step(new_lens, h.shape[0])
+        ends; max_len: the most new tokens of a request.  Returns the last layer's rows.  Nothing here waits for the GPU.
+
+        Where self.plan.missing (on the GPU) is not 0, there were too few pages: the rows are void, tables and caches are as before the
+        step, and a smaller one, or one in which requests end, can be made instead."""
+        plan = self.plan = self.table.step(new_lens, h.shape[0])
         hidden, shape = self.stack.cfg.hidden, (h.shape[0], self.heads, self.head_dim)
         comb = self.stack.combine
         x = comb(0, h)
