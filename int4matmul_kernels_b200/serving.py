@@ -43,8 +43,16 @@ class CachedStack:
 
         Where self.plan.missing (on the GPU) is not 0, there were too few pages: the rows are void, tables and caches are as before the
         step, and a smaller one, or one in which requests end, can be made instead."""
+        hidden = self.stack.cfg.hidden
+        # (refused before the table moves)
+        if h.device != self.table.seq_lens.device or h.dim() != 2 or h.shape[1] != hidden or h.stride(1) != 1:
+            raise ValueError(f"h must be (tokens, {hidden}) on {self.table.seq_lens.device}, contiguous in its last dimension")
+        if h.dtype != torch.float16:
+            raise TypeError("h must be float16")
+        if int(max_len) < 0:
+            raise ValueError("max_len must not be negative")
         plan = self.plan = self.table.step(new_lens, h.shape[0])
-        hidden, shape = self.stack.cfg.hidden, (h.shape[0], self.heads, self.head_dim)
+        shape = (h.shape[0], self.heads, self.head_dim)
         comb = self.stack.combine
         x = comb(0, h)
         for i, (mats, held) in enumerate(zip(self.stack.layers, self.caches)):

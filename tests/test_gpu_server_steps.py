@@ -45,3 +45,16 @@ def test_a_server_that_runs_out_of_pages():
             table, seq = s.table.block_table.tolist(), s.table.seq_lens.tolist()
             used = [p for row, n in zip(table, seq) for p in row[:-(-n // 16)]]
             assert sorted(used + s.table.free_pages[:s.table.free_count.item()].tolist()) == list(range(7)), i
+
+
+def test_rows_that_are_refused_leave_the_table_as_it_was():
+    s = server()
+    s.step(rows(6, 1), ints([3, 3, 0, 0, 0]), 3)
+    seq, count = s.table.seq_lens.tolist(), s.table.free_count.item()
+    for h, error in ((rows(5, 2).float(), TypeError), (rows(5, 2)[:, :128], ValueError), (rows(5, 2)[None], ValueError), (rows(5, 2).cpu(), ValueError)):
+        with pytest.raises(error):
+            s.step(h, ints([1, 1, 3, 0, 0]), 3)
+        assert s.table.seq_lens.tolist() == seq and s.table.free_count.item() == count
+    with pytest.raises(ValueError):
+        s.step(rows(5, 2), ints([1, 1, 3, 0, 0]), -1)
+    assert s.table.seq_lens.tolist() == seq
