@@ -284,12 +284,11 @@ class DecoderStack:
         if getattr(self, "peer", None) is not None:
             return self.peer.multiply(name, w, x, parts)
         local = self.multiply(w, x)                                   # (rows, parts * S_part / P)
-        rows = local.shape[0]
         if self.world == 1:
-            return list(local.view(rows, parts, -1).unbind(1))
+            return list(local.unflatten(1, (parts, local.shape[1] // parts)).unbind(1))
         gathered = gather_columns(local, self.world, self.group)      # (rows, P * parts * S_part / P), rank-major
-        g = gathered.view(rows, self.world, parts, -1)                 # [row, rank, part, cols of that rank]
-        return [g[:, :, i, :].reshape(rows, -1) for i in range(parts)]
+        g = gathered.unflatten(1, (self.world, parts, local.shape[1] // parts))      # [row, rank, part, cols of that rank]
+        return [g[:, :, i, :].flatten(1) for i in range(parts)]
 
     @staticmethod
     def combine(mode: int, a: torch.Tensor, b: Optional[torch.Tensor] = None, c: Optional[torch.Tensor] = None) -> torch.Tensor:

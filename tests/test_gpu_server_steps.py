@@ -58,3 +58,15 @@ def test_rows_that_are_refused_leave_the_table_as_it_was():
     with pytest.raises(ValueError):
         s.step(rows(5, 2), ints([1, 1, 3, 0, 0]), -1)
     assert s.table.seq_lens.tolist() == seq
+
+
+def test_a_step_in_which_requests_only_end():
+    s, plain = server(), server()
+    for x in (s, plain):
+        x.step(rows(40, 3), ints([30, 3, 7, 0, 0]), 30)
+    out = s.step(rows(0, 4), ints([-1, 0, -1, 0, 0]), 0)
+    assert out.shape == (0, 256) and s.table.seq_lens.tolist() == [0, 3, 0, 0, 0] and s.table.free_count.item() == 39
+    h = rows(3, 5)
+    got, want = s.step(h, ints([0, 1, 0, 2, 0]), 2), plain.step(h, ints([-1, 1, -1, 2, 0]), 2)
+    assert torch.equal(got, want)
+    assert s.stack.forward(rows(0, 4)).shape == (0, 256)
