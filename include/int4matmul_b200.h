@@ -195,6 +195,13 @@ int i4mm_device_status(void* workspace, void* stream);
 /* The same check for i4mm_quant_matvec_static, whose status word lives in the library's fixed scratch on the
  * current device: waits for the stream, returns I4MM_OK or (after clearing the word) I4MM_ERR_TIMEOUT. */
 int i4mm_static_device_status(void* stream);
+/*
+ * Scratch whose first use comes while a stream is being captured into a CUDA graph has to be allocated, zero-filled and waited for outside
+ * of the graph: as nodes of it, the zero-filling would be repeated at every replay, and missing where another graph that shares the
+ * scratch is replayed first.  A thread may do that during a capture if its capture mode is relaxed.  Sets the calling thread's mode to *mode
+ * (0 global, 1 thread-local, 2 relaxed) and leaves the former one there, as cudaThreadExchangeStreamCaptureMode does.
+ */
+int i4mm_exchange_capture_mode(int* mode);
 
 /*
  * 16:32 packer.  Replaces sparse_int4_pack / PackMatrix (utils_kernel.cu:67-119, 19-64).

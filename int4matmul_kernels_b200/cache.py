@@ -39,7 +39,7 @@ def _workspace(device: torch.device, stream: torch.cuda.Stream) -> torch.Tensor:
     key = (device.index if device.index is not None else torch.cuda.current_device(), stream.cuda_stream)
     ws = ops._cache_workspaces.get(key)
     if ws is None:
-        ws = torch.zeros(capi.load().i4mm_cache_attention_workspace_bytes(), dtype=torch.uint8, device=device)
+        ws = ops.zeroed_scratch(capi.load().i4mm_cache_attention_workspace_bytes(), device)
         ops._cache_workspaces[key] = ws
     return ws
 

@@ -63,6 +63,7 @@ _SIGNATURES = {
                                                 ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                                 ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                                 ctypes.c_void_p]),
+    "i4mm_exchange_capture_mode": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
     "i4mm_device_status": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "i4mm_static_device_status": (ctypes.c_int, [ctypes.c_void_p]),
     "i4mm_row_norm": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,

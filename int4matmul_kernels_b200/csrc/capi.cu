@@ -263,6 +263,16 @@ int i4mm_device_status(void* workspace, void* stream) {
     return I4MM_ERR_TIMEOUT;
 }
 
+int i4mm_exchange_capture_mode(int* mode) {
+    if (!mode) return I4MM_ERR_NULL;
+    if (*mode < 0 || *mode > 2) return I4MM_ERR_SHAPE;
+    cudaStreamCaptureMode m = *mode == 0 ? cudaStreamCaptureModeGlobal : *mode == 1 ? cudaStreamCaptureModeThreadLocal : cudaStreamCaptureModeRelaxed;
+    const cudaError_t e = cudaThreadExchangeStreamCaptureMode(&m);
+    if (e != cudaSuccess) return fail_cuda(e);
+    *mode = m == cudaStreamCaptureModeGlobal ? 0 : m == cudaStreamCaptureModeThreadLocal ? 1 : 2;
+    return I4MM_OK;
+}
+
 int i4mm_row_norm(int mode, void* y, const void* a, const void* b, const void* c, int64_t rows, int64_t width,
                   int64_t stride_a, int64_t stride_b, int64_t stride_c, void* stream) {
     const int early = mode > 0 && (mode & I4MM_PATH_STATIC_WEIGHTS) ? 1 : 0;

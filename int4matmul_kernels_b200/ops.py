@@ -13,6 +13,8 @@ Every other violated precondition raises (the reference asserts, or traps the de
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import capi
@@ -65,6 +67,29 @@ def _require_cuda(t: torch.Tensor, name: str, device: torch.device) -> None:
         raise ValueError(f"{name} must be a CUDA tensor on {device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def zeroed_scratch(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Zero-filled bytes for the current stream of `device` (the current device).  While that stream is being captured they are made on
+    another one and waited for: they belong to no graph, and no replay clears them."""
+    if not torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    lib, mode = capi.load(), ctypes.c_int(2)
+    status = lib.i4mm_exchange_capture_mode(ctypes.byref(mode))
+    if status != capi.OK:
+        raise Int4MatmulError(status, "capture mode")
+    try:
+        for _ in range(64):                   # (streams come from a pool of 32, of which the captured one is one)
+            side = torch.cuda.Stream(device)
+            with torch.cuda.stream(side):
+                if torch.cuda.is_current_stream_capturing():
+                    continue
+                ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            side.synchronize()
+            return ws
+        raise RuntimeError("every stream is being captured: call once before the capture")
+    finally:
+        lib.i4mm_exchange_capture_mode(ctypes.byref(mode))
 
 
 def workspace(device: torch.device, stream: torch.cuda.Stream) -> torch.Tensor:
