@@ -44,22 +44,49 @@ struct Workspace {
 std::mutex g_ws_mutex;
 std::map<std::pair<int, int64_t>, Workspace> g_workspaces;
 
-Tensor workspace_for(const c10::Device& dev, const c10::cuda::CUDAStream& stream) {
-    std::lock_guard<std::mutex> lock(g_ws_mutex);
-    const auto key = std::make_pair((int)dev.index(), (int64_t)stream.id());
-    auto it = g_workspaces.find(key);
-    if (it != g_workspaces.end()) return it->second.buffer;
-    Tensor ws = torch::zeros({(int64_t)i4mm_workspace_bytes()}, torch::dtype(torch::kUInt8).device(dev));
-    g_workspaces.emplace(key, Workspace{ws, stream.stream()});
-    return ws;
-}
-
 void check_status(int status, const char* what) {
     if (status == I4MM_OK) return;
     std::string msg = std::string(what) + ": " + i4mm_status_string(status);
     if (status == I4MM_ERR_LAUNCH) msg += " (cudaError " + std::to_string(i4mm_last_cuda_error()) + ")";
     if (status == I4MM_ERR_BITS) throw std::invalid_argument(msg);
     TORCH_CHECK(false, msg);
+}
+
+bool capturing(const c10::cuda::CUDAStream& stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    TORCH_CHECK(cudaStreamIsCapturing(stream.stream(), &status) == cudaSuccess, "the stream's capture status");
+    return status != cudaStreamCaptureStatusNone;
+}
+
+// Zero-filled bytes for `stream`, the current one.  While it is being captured they are made on another stream and waited for: they belong to no
+// graph, and no replay clears them.
+Tensor zeroed_scratch(int64_t bytes, const c10::Device& dev, const c10::cuda::CUDAStream& stream) {
+    const auto options = torch::dtype(torch::kUInt8).device(dev);
+    if (!capturing(stream)) return torch::zeros({bytes}, options);
+    struct Relaxed {
+        int mode = 2;
+        Relaxed() { check_status(i4mm_exchange_capture_mode(&mode), "capture mode"); }
+        ~Relaxed() { (void)i4mm_exchange_capture_mode(&mode); }
+    } relaxed;
+    for (int i = 0; i < 64; ++i) {                        // (streams come from a pool of 32, of which the captured one is one)
+        const auto side = c10::cuda::getStreamFromPool(false, dev.index());
+        if (capturing(side)) continue;
+        c10::cuda::CUDAStreamGuard guard(side);
+        Tensor ws = torch::zeros({bytes}, options);
+        side.synchronize();
+        return ws;
+    }
+    TORCH_CHECK(false, "every stream is being captured: call once before the capture");
+}
+
+Tensor workspace_for(const c10::Device& dev, const c10::cuda::CUDAStream& stream) {
+    std::lock_guard<std::mutex> lock(g_ws_mutex);
+    const auto key = std::make_pair((int)dev.index(), (int64_t)stream.id());
+    auto it = g_workspaces.find(key);
+    if (it != g_workspaces.end()) return it->second.buffer;
+    Tensor ws = zeroed_scratch((int64_t)i4mm_workspace_bytes(), dev, stream);
+    g_workspaces.emplace(key, Workspace{ws, stream.stream()});
+    return ws;
 }
 
 enum class Route { AUTO, MATMUL, MATVEC };

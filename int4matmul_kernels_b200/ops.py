@@ -97,7 +97,7 @@ def workspace(device: torch.device, stream: torch.cuda.Stream) -> torch.Tensor:
     key = (device.index if device.index is not None else torch.cuda.current_device(), stream.cuda_stream)
     ws = _workspaces.get(key)
     if ws is None:
-        ws = torch.zeros(capi.load().i4mm_workspace_bytes(), dtype=torch.uint8, device=device)
+        ws = zeroed_scratch(capi.load().i4mm_workspace_bytes(), device)
         _workspaces[key] = ws
     return ws
 

@@ -3,6 +3,7 @@ it, and what a kernel has recorded in it stays until it is read."""
 import pytest
 import torch
 
+import int4matmul_kernels_b200 as package
 from int4matmul_kernels_b200 import cache, capi, ops
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +68,32 @@ def test_attention(compiled, monkeypatch):
     many = lambda: c.attention(x, table, p.cu_lens, 3000)                          # noqa: E731
     stream, made = check([few, many, few], capi.load().i4mm_cache_attention_workspace_bytes())
     status_stays(ops._cache_workspaces, stream, made)
+
+
+def problem(rows):
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    matrix = torch.randint(-2 ** 31, 2 ** 31 - 1, (128, 512), dtype=torch.int32, device="cuda", generator=gen)
+    scales = (torch.rand((8, 512), device="cuda", generator=gen) * 0.01).half()
+    zeros = torch.randint(0, 16, (8, 512), device="cuda", generator=gen).half()
+    x = torch.randn((1, rows, 1024), device="cuda", generator=gen).half()
+    out = torch.empty((1, rows, 512), dtype=torch.float16, device="cuda")
+    return out, matrix, x, scales, zeros
+
+
+@pytest.mark.parametrize("route", ["ops", "ops without the compiled module", "module"])
+def test_multiplies(route, monkeypatch):
+    monkeypatch.setattr(ops, "_workspaces", {})
+    if "without" in route:
+        monkeypatch.setattr(ops, "_native", False)
+    entry = package.load_extension() if route == "module" else ops
+
+    def multiply(rows):
+        out, matrix, x, scales, zeros = problem(rows)
+
+        def call():
+            entry.quant_matmul(4, out, matrix, x, scales, zeros, 128, None)
+            return out
+        return call
+    stream, made = check([multiply(r) for r in (48, 300, 12)], capi.load().i4mm_workspace_bytes())
+    if route != "module":
+        status_stays(ops._workspaces, stream, made)
