@@ -317,6 +317,11 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
                          int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
                          int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
                          int64_t window, void* workspace, size_t workspace_bytes, void* stream);
+/* The kernels that the last i4mm_cache_attention call of this host thread launched, or-ed; 0: none (an empty or a refused call).  For tests
+ * that must know which kernel they exercised. */
+#define I4MM_ATTENTION_FEW_ROWS 1
+#define I4MM_ATTENTION_PROMPT 2
+int i4mm_last_attention_kernels(void);
 
 #ifdef __cplusplus
 }

@@ -30,6 +30,7 @@ class Cache(ctypes.Structure):
 
 CACHE_INT8, CACHE_E4M3 = 0, 1
 TYPE_FP16, TYPE_BF16 = 0, 1
+ATTENTION_FEW_ROWS, ATTENTION_PROMPT = 1, 2    # i4mm_last_attention_kernels
 
 # every symbol the header declares, with its ctypes signature
 _SIGNATURES = {
@@ -84,6 +85,7 @@ _SIGNATURES = {
                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
                                             ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                             ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "i4mm_last_attention_kernels": (ctypes.c_int, []),
     "i4mm_check_mask": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
 }
 

@@ -62,6 +62,8 @@ int view_of(const i4mm_cache* c, i4mm::CacheView& w) {
     return I4MM_OK;
 }
 
+thread_local int g_attention_kernels = 0;             // i4mm_last_attention_kernels
+
 size_t attention_workspace() { return i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace() + i4mm::cache_prompt_workspace(); }
 
 // Which kernel.  A request's rows are its new tokens times the query heads of a key head.  The few-row kernel takes 8 or 16 of them at a time
@@ -80,10 +82,18 @@ cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t
     const int64_t tiles = ((int64_t)p.tokens * p.group / 16 + p.requests) * p.cache.heads * (span / 32 + 1);
     const bool mixed = (int64_t)p.tokens * 2 < p.requests * len;
     const bool little = mixed ? tiles <= 12000 : tiles <= 8000 && (rows < 2 * span || tiles <= 1000);
-    if (rows <= i4mm::kFewRows || little) return i4mm::cache_rows_launch(p, e4m3, bf16, 0x7FFFFFFF, rows <= 8, stream);
-    if (p.group > i4mm::kFewRows) return i4mm::cache_prompt_launch(p, e4m3, bf16, 1, true, stream);
-    const cudaError_t e = i4mm::cache_rows_launch(p, e4m3, bf16, i4mm::kFewRows, p.group <= 8, stream);
-    return e != cudaSuccess ? e : i4mm::cache_prompt_launch(p, e4m3, bf16, i4mm::kFewRows + 1, false, stream);
+    const auto few = [&](int most_rows, bool to_8) {
+        g_attention_kernels |= I4MM_ATTENTION_FEW_ROWS;
+        return i4mm::cache_rows_launch(p, e4m3, bf16, most_rows, to_8, stream);
+    };
+    const auto prompt = [&](int least_rows, bool alone) {
+        g_attention_kernels |= I4MM_ATTENTION_PROMPT;
+        return i4mm::cache_prompt_launch(p, e4m3, bf16, least_rows, alone, stream);
+    };
+    if (rows <= i4mm::kFewRows || little) return few(0x7FFFFFFF, rows <= 8);
+    if (p.group > i4mm::kFewRows) return prompt(1, true);
+    const cudaError_t e = few(i4mm::kFewRows, p.group <= 8);
+    return e != cudaSuccess ? e : prompt(i4mm::kFewRows + 1, false);
 }
 
 }  // namespace
@@ -154,12 +164,15 @@ int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type,
                                           (const int*)slots, (cudaStream_t)stream));
 }
 
+int i4mm_last_attention_kernels(void) { return g_attention_kernels; }
+
 size_t i4mm_cache_attention_workspace_bytes(void) { return attention_workspace(); }
 
 int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,
                          int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
                          int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
                          int64_t window, void* workspace, size_t workspace_bytes, void* stream) {
+    g_attention_kernels = 0;
     i4mm::AttentionParams p{};
     const int status = view_of(cache, p.cache);
     if (status != I4MM_OK) return status;
