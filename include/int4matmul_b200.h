@@ -277,7 +277,8 @@ typedef struct i4mm_cache {
  *                           (the stack was empty, or the table's row full)
  * seq_lens, new_lens and free_count are left alone, so that the same call again gives the same answers; free_count is not one of the
  * outputs.  Where counts[1] is not 0 the step had better be dropped, and a smaller one made from the same lengths and count: a request
- * that went on without its pages would give -1 back as pages when it ends.  requests <= 16384; packed tokens beyond max_tokens get no entry.
+ * that went on without its pages would give -1 back as pages when it ends.  requests <= 16384, requests * table_width and max_tokens
+ * <= 2^30; packed tokens beyond max_tokens get no entry.
  */
 int i4mm_cache_plan(int64_t requests, const void* seq_lens, const void* new_lens, void* block_table, int64_t table_width,
                     int64_t table_stride, void* free_pages, int64_t free_capacity, const void* free_count, int64_t page_size,

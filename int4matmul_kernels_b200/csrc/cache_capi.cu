@@ -105,8 +105,10 @@ int i4mm_cache_plan(int64_t requests, const void* seq_lens, const void* new_lens
                     int64_t max_tokens, void* lens_after, void* cu_lens, void* slots, void* positions, void* request_of, void* counts,
                     void* stream) {
     if (shift_of(page_size) < 0) return I4MM_ERR_UNSUPPORTED;
-    if (requests < 0 || requests > 16384 || table_width < 0 || table_width > kMost || table_stride < table_width || free_capacity < 0 ||
-        free_capacity > kMost || max_tokens < 0 || max_tokens > kMost - 4096)
+    // the kernel's loops over tokens and table entries step by up to 296 * 512 in 32 bits
+    constexpr int64_t kMostSteps = int64_t(1) << 30;
+    if (requests < 0 || requests > 16384 || table_width < 0 || table_width > kMost || requests * table_width > kMostSteps ||
+        table_stride < table_width || free_capacity < 0 || free_capacity > kMost || max_tokens < 0 || max_tokens > kMostSteps)
         return I4MM_ERR_SHAPE;
     if (!cu_lens || !counts || !free_count) return I4MM_ERR_NULL;
     if (requests > 0 && (!seq_lens || !new_lens || !lens_after || (table_width > 0 && !block_table))) return I4MM_ERR_NULL;
