@@ -242,7 +242,7 @@ int i4mm_row_norm(int mode, void* y, const void* a, const void* b, const void* c
  * counterpart in the reference, which has no model code.
  *
  *   k, v      (pages, heads, page_size, head_dim) int8 or e4m3 (1 byte a value), head_dim 64 or 128 and contiguous; the other strides
- *             are free (multiples of 16 bytes, below 2^31)
+ *             are free (multiples of 16 bytes, below 2^31).  Here and for activations, the stride of a dimension of size 1 may be anything
  *   scales    fp32 (pages, heads, 2) contiguous, 8-byte aligned: of the page's keys and of its values.  A byte q stands for q * scale.
  *   slot      where a token lies: page * page_size + place in the page.  Slots outside of the cache (negative ones: padding) are
  *             skipped by the writer and read as zeros.

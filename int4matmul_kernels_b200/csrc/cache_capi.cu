@@ -29,6 +29,12 @@ int shift_of(int64_t page_size) {
     }
 }
 
+// rows of activations (tokens, heads, dim); the stride of a single token or head says nothing
+i4mm::RowsView rows_of(const void* p, int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride) {
+    return {p, tokens > 1 ? token_stride : 0, heads > 1 ? head_stride : 0};
+}
+bool aligned(const i4mm::RowsView& r) { return aligned(r.p, 16) && ((r.token | r.head) & 7) == 0; }
+
 int view_of(const i4mm_cache* c, i4mm::CacheView& w) {
     if (!c) return I4MM_ERR_NULL;
     if (c->type != I4MM_CACHE_INT8 && c->type != I4MM_CACHE_E4M3) return I4MM_ERR_UNSUPPORTED;
@@ -36,24 +42,26 @@ int view_of(const i4mm_cache* c, i4mm::CacheView& w) {
     if (shift_of(c->page_size) < 0) return I4MM_ERR_UNSUPPORTED;
     if (c->pages <= 0 || c->heads <= 0 || c->heads > 65535 || c->pages > kMost / c->page_size) return I4MM_ERR_SHAPE;
     if (!c->k || !c->v || !c->scales) return I4MM_ERR_NULL;
-    for (const int64_t stride : {c->k_page_stride, c->k_head_stride, c->k_token_stride, c->v_page_stride, c->v_head_stride, c->v_token_stride})
-        if (stride < 0 || stride > kMost) return I4MM_ERR_SHAPE;
-    const int64_t strides = c->k_page_stride | c->k_head_stride | c->k_token_stride | c->v_page_stride | c->v_head_stride | c->v_token_stride;
-    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 8) || (strides & 15)) return I4MM_ERR_ALIGN;
-    // (the stride of a single page, head or token says nothing)
+    // (the stride of a single page or head says nothing)
     const int64_t one = c->head_dim;
-    const auto stride = [&](int64_t n, int64_t s) { return n > 1 ? s : std::max(s, one); };
-    for (const int64_t s : {stride(c->pages, c->k_page_stride), stride(c->heads, c->k_head_stride), stride(c->pages, c->v_page_stride),
-                            stride(c->heads, c->v_head_stride), c->k_token_stride, c->v_token_stride})
+    const auto stride = [&](int64_t n, int64_t s) { return n > 1 ? s : one; };
+    const int64_t k_page = stride(c->pages, c->k_page_stride), k_head = stride(c->heads, c->k_head_stride);
+    const int64_t v_page = stride(c->pages, c->v_page_stride), v_head = stride(c->heads, c->v_head_stride);
+    for (const int64_t s : {k_page, k_head, c->k_token_stride, v_page, v_head, c->v_token_stride})
+        if (s < 0 || s > kMost) return I4MM_ERR_SHAPE;
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 8) ||
+        ((k_page | k_head | c->k_token_stride | v_page | v_head | c->v_token_stride) & 15))
+        return I4MM_ERR_ALIGN;
+    for (const int64_t s : {k_page, k_head, c->k_token_stride, v_page, v_head, c->v_token_stride})
         if (s < one) return I4MM_ERR_SHAPE;
     w.k = (uint8_t*)c->k;
     w.v = (uint8_t*)c->v;
     w.scales = (float2*)c->scales;
-    w.k_page = stride(c->pages, c->k_page_stride);
-    w.k_head = stride(c->heads, c->k_head_stride);
+    w.k_page = k_page;
+    w.k_head = k_head;
     w.k_token = c->k_token_stride;
-    w.v_page = stride(c->pages, c->v_page_stride);
-    w.v_head = stride(c->heads, c->v_head_stride);
+    w.v_page = v_page;
+    w.v_head = v_head;
     w.v_token = c->v_token_stride;
     w.pages = (int)c->pages;
     w.heads = (int)c->heads;
@@ -146,11 +154,11 @@ int i4mm_cache_write(const i4mm_cache* cache, const void* k, const void* v, int 
     if (tokens < 0 || tokens > kMost) return I4MM_ERR_SHAPE;
     if (tokens == 0) return I4MM_OK;
     if (!k || !v || !slots) return I4MM_ERR_NULL;
-    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 4) || ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7))
-        return I4MM_ERR_ALIGN;
-    return finish(i4mm::cache_write_launch(c, cache->type == I4MM_CACHE_E4M3, {k, k_token_stride, k_head_stride},
-                                           {v, v_token_stride, v_head_stride}, type == I4MM_TYPE_BF16, (int)tokens, (const int*)slots,
-                                           (cudaStream_t)stream));
+    const i4mm::RowsView k_rows = rows_of(k, tokens, k_token_stride, c.heads, k_head_stride);
+    const i4mm::RowsView v_rows = rows_of(v, tokens, v_token_stride, c.heads, v_head_stride);
+    if (!aligned(k_rows) || !aligned(v_rows) || !aligned(slots, 4)) return I4MM_ERR_ALIGN;
+    return finish(i4mm::cache_write_launch(c, cache->type == I4MM_CACHE_E4M3, k_rows, v_rows, type == I4MM_TYPE_BF16, (int)tokens,
+                                           (const int*)slots, (cudaStream_t)stream));
 }
 
 int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type, int64_t tokens, const void* slots, void* stream) {
@@ -186,12 +194,10 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
     if (!cu_lens && tokens < requests) return I4MM_ERR_SHAPE;
     if (tokens == 0) return I4MM_OK;
     if (!out || !q || (requests > 0 && (!seq_lens || (table_width > 0 && !block_table)))) return I4MM_ERR_NULL;
-    if (!aligned(out, 16) || !aligned(q, 16) || !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(cu_lens, 4) ||
-        ((q_token_stride | q_head_stride) & 7))
-        return I4MM_ERR_ALIGN;
+    p.q = rows_of(q, tokens, q_token_stride, q_heads, q_head_stride);
+    if (!aligned(out, 16) || !aligned(p.q) || !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(cu_lens, 4)) return I4MM_ERR_ALIGN;
     if (!workspace || workspace_bytes < attention_workspace()) return I4MM_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return I4MM_ERR_ALIGN;
-    p.q = {q, q_token_stride, q_head_stride};
     p.out = out;
     p.table = (const int*)block_table;
     p.seq_lens = (const int*)seq_lens;
