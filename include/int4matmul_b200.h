@@ -310,8 +310,8 @@ int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type,
  *                             j > p - window.  Rows that see no token, and rows of no request, are 0.
  *   max_len                   the most rows of a request, for the choice of a kernel (a wrong one costs time, nothing else)
  * Sums and softmax statistics are fp32.  Which kernel runs goes by sizes that the host has (rows, max_len, the table's width, window); results of
- * the two differ by rounding.  The same call gives the same bits.  `workspace` (about 55 MB): i4mm_cache_attention_workspace_bytes() bytes, zero-filled before the first use,
- * shared by calls of one stream only.
+ * the two differ by rounding.  The same call gives the same bits.  `workspace` (about 55 MB): i4mm_cache_attention_workspace_bytes() bytes, zero-filled before the first use
+ * and after i4mm_device_status has reported I4MM_ERR_TIMEOUT for it, shared by calls of one stream only.
  */
 size_t i4mm_cache_attention_workspace_bytes(void);
 int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,

@@ -567,6 +567,16 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                 if (b >= p.requests) break;           // (as above)
             }
         }
+        // A warp that stops early waits, bounded again, for what is on its way to its ring: the shared memory is someone else's once the block
+        // has ended.  (All kStages are where it gave up on the tile that lies as many behind the next copy.)
+        int in_flight = c.stage - stage + (c.stage < stage || (c.stage == stage && !ok) ? S::kStages : 0);
+        for (; in_flight > 0; --in_flight) {
+            (void)ptx::mbar_wait(ptx::smem_u32(&s_full[warp][stage]), phase);
+            if (++stage == S::kStages) {
+                stage = 0;
+                phase ^= 1;
+            }
+        }
     }
     __syncthreads();
 
