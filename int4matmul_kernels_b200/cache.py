@@ -247,13 +247,14 @@ class PageTable:
     def __init__(self, requests: int, pages: int, page_size: int, max_seq: int, device="cuda"):
         dev = torch.device(device)
         self.page_size = int(page_size)
-        # lengths and the count of free pages lie together: what `undo` keeps of them is one copy
-        self._state = torch.zeros(requests + 1, dtype=torch.int32, device=dev)
-        self._saved = torch.empty_like(self._state)
-        self.seq_lens, self.free_count = self._state[:requests], self._state[requests:]
-        self.free_count.fill_(pages)
-        self.block_table = torch.full((requests, -(-max_seq // self.page_size)), -1, dtype=torch.int32, device=dev)
-        self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)
+        with torch.inference_mode(False):             # (`step` writes to them, in that mode or not)
+            # lengths and the count of free pages lie together: what `undo` keeps of them is one copy
+            self._state = torch.zeros(requests + 1, dtype=torch.int32, device=dev)
+            self._saved = torch.empty_like(self._state)
+            self.seq_lens, self.free_count = self._state[:requests], self._state[requests:]
+            self.free_count.fill_(pages)
+            self.block_table = torch.full((requests, -(-max_seq // self.page_size)), -1, dtype=torch.int32, device=dev)
+            self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)
         self._can_undo = False
 
     def step(self, new_lens: torch.Tensor, max_tokens: int) -> Plan:

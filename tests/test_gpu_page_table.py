@@ -89,3 +89,14 @@ def test_undo_before_a_step_is_written():
     kept = t.seq_lens
     t.step(ints([1, 0, 0]), 1)
     assert kept.tolist() == [31, 17, 0]
+
+
+def test_tables_made_and_used_in_and_out_of_inference_mode():
+    with torch.inference_mode():
+        t = cache.PageTable(2, 8, 16, 64)
+        t.step(ints([3, 0]), 3)
+    t.step(ints([1, 20]), 21)
+    with torch.inference_mode():
+        assert t.step(ints([1, 1]), 2).slots.tolist() == [t.block_table[0, 0].item() * 16 + 4, t.block_table[1, 1].item() * 16 + 4]
+        t.undo()
+    assert t.seq_lens.tolist() == [4, 20] and t.free_count.item() == 5
