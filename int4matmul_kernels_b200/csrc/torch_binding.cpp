@@ -62,6 +62,7 @@ bool capturing(const c10::cuda::CUDAStream& stream) {
 // graph, and no replay clears them.
 Tensor zeroed_scratch(int64_t bytes, const c10::Device& dev, const c10::cuda::CUDAStream& stream) {
     const auto options = torch::dtype(torch::kUInt8).device(dev);
+    c10::InferenceMode plain(false);                      // (check_device_status may have to clear them outside of that mode)
     if (!capturing(stream)) return torch::zeros({bytes}, options);
     struct Relaxed {
         int mode = 2;

@@ -73,7 +73,8 @@ def zeroed_scratch(nbytes: int, device: torch.device) -> torch.Tensor:
     """Zero-filled bytes for the current stream of `device` (the current device).  While that stream is being captured they are made on
     another one and waited for: they belong to no graph, and no replay clears them."""
     if not torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        with torch.inference_mode(False):     # (`check_device_status` may have to clear them outside of it)
+            return torch.zeros(nbytes, dtype=torch.uint8, device=device)
     lib, mode = capi.load(), ctypes.c_int(2)
     status = lib.i4mm_exchange_capture_mode(ctypes.byref(mode))
     if status != capi.OK:
@@ -81,7 +82,7 @@ def zeroed_scratch(nbytes: int, device: torch.device) -> torch.Tensor:
     try:
         for _ in range(64):                   # (streams come from a pool of 32, of which the captured one is one)
             side = torch.cuda.Stream(device)
-            with torch.cuda.stream(side):
+            with torch.cuda.stream(side), torch.inference_mode(False):
                 if torch.cuda.is_current_stream_capturing():
                     continue
                 ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
