@@ -30,6 +30,7 @@
 #include <type_traits>
 
 #include "cache_attention.cuh"
+#include "tensor_map.cuh"
 
 namespace i4mm {
 namespace {
@@ -690,42 +691,18 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
     }
 }
 
-// The driver's tensor-map encoder, found at run time so that the library does not link against libcuda; nullptr if there is none.
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encoder() {
-    static const EncodeTiled fn = [] {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
-            (void)cudaGetLastError();
-            return (EncodeTiled) nullptr;
-        }
-        return (EncodeTiled)ptr;
-    }();
-    return fn;
-}
-
 // the cache's keys or values as (dim, token, head, page), read 16 tokens at a time in rows whose 16-byte chunks are swizzled
 bool cache_map(CUtensorMap* out, const CacheView& c, bool keys) {
-    const EncodeTiled encode = encoder();
+    const EncodeTiledFn encode = encode_tiled_fn();
     if (!encode) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)c.dim, 1ull << c.page_shift, (cuuint64_t)c.heads, (cuuint64_t)c.pages};
     const cuuint64_t strides[3] = {(cuuint64_t)(keys ? c.k_token : c.v_token), (cuuint64_t)(keys ? c.k_head : c.v_head), (cuuint64_t)(keys ? c.k_page : c.v_page)};
     const cuuint32_t box[4] = {(cuuint32_t)c.dim, 16, 1, 1}, steps[4] = {1, 1, 1, 1};
-    const auto made = [&] {
+    return encode_with_context([&] {
         return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, keys ? c.k : c.v, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       c.dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-    };
-    if (made()) return true;
-    // it needs a context that is current in the calling thread, which the first CUDA call of a new thread may find missing
-    int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return false;
-    }
-    return made();
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 template <bool E4M3, bool BF16, int D, int NT>

@@ -29,7 +29,6 @@
 #include "../../include/int4matmul_b200.h"
 
 #include <cuda.h>
-#include <dlfcn.h>
 
 #include <atomic>
 #include <mutex>
@@ -38,6 +37,7 @@
 #include "common.cuh"
 #include "dequant.cuh"
 #include "ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace i4mm {
 
@@ -1474,42 +1474,6 @@ __global__ void kparts_reduce_kernel(float* parts, const OutMap om, int rows, in
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver's tensor-map encoder, found at run time so that the library does not link against libcuda.
-EncodeTiledFn encode_tiled_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess && ptr)
-            fn = (EncodeTiledFn)ptr;
-        if (!fn) {
-            (void)cudaGetLastError();
-            void* h = dlopen("libcuda.so.1", RTLD_NOW | RTLD_GLOBAL);
-            if (h) fn = (EncodeTiledFn)dlsym(h, "cuTensorMapEncodeTiled");
-        }
-    }
-    return fn;
-}
-
-// The encoder needs a context that is current in the calling thread, which the first CUDA call of a new thread may find missing.
-template <class Encode>
-bool encode_with_context(Encode encode) {
-    if (encode() == CUDA_SUCCESS) return true;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return false;
-    }
-    return encode() == CUDA_SUCCESS;
-}
-
 // 2-D row-major tensor (rows, cols) of `elem_bytes` elements, box (box_rows, box_cols)
 bool encode_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dt, int elem_bytes, uint64_t rows, uint64_t cols,
                uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swz) {
