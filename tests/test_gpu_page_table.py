@@ -100,3 +100,22 @@ def test_tables_made_and_used_in_and_out_of_inference_mode():
         assert t.step(ints([1, 1]), 2).slots.tolist() == [t.block_table[0, 0].item() * 16 + 4, t.block_table[1, 1].item() * 16 + 4]
         t.undo()
     assert t.seq_lens.tolist() == [4, 20] and t.free_count.item() == 5
+
+
+def test_a_captured_step_that_runs_out_of_pages_stops():
+    t = cache.PageTable(2, 5, 16, 160)
+    t.step(ints([16, 30]), 46)
+    new = ints([4, 4])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        p = t.step(new, 8)
+    for want in ([20, 34], [24, 38], [28, 42], [32, 46], [32, 46], [32, 46]):        # (the next would be 36 and 50: 3 and 4 pages of 5)
+        graph.replay()
+        assert t.seq_lens.tolist() == want
+        assert (p.missing.item() > 0) == (p.slots.max().item() < 0)
+    assert p.missing.item() == 2 and t.free_count.item() == 0
+    new.copy_(ints([-1, 4]))
+    graph.replay()
+    assert t.seq_lens.tolist() == [0, 50] and p.missing.item() == 0 and t.free_count.item() == 1
