@@ -290,7 +290,7 @@ int i4mm_cache_plan(int64_t requests, const void* seq_lens, const void* new_lens
  * The tokens of one page that a call writes are neighbours in the call, with ascending slots (as i4mm_cache_plan lays them out); the
  * places of the page before the first of them hold tokens already, or the first of them is the page's first and what the page held is void.
  * With a = the largest finite |value| that a call adds to a page and head and `most` = 127 or 448, the scale becomes the larger of the old
- * one and the least power of two s with a <= most * s, the new bytes are round(x / s), and if the scale grew the bytes already there
+ * one and the least power of two s (2^-100 at least) with a <= most * s, 0 for a = 0, the new bytes are round(x / s), and if the scale grew the bytes already there
  * become round(q * old / s).  Since scales grow by powers of two, a value is off by less than one step of its final scale however often
  * that happens (1/2 + 1/4 + ...).  Infinities are stored as +-most, NaN as 0.
  */
@@ -309,8 +309,9 @@ int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type,
  *                             n is at position p = seq_lens[b] - n + i and sees the tokens j <= p, with window > 0 those with
  *                             j > p - window.  Rows that see no token, and rows of no request, are 0.
  *   max_len                   the most rows of a request, for the choice of a kernel (a wrong one costs time, nothing else)
- * Sums and softmax statistics are fp32.  Which kernel runs goes by sizes that the host has (rows, max_len, the table's width, window); results of
- * the two differ by rounding.  The same call gives the same bits.  `workspace` (about 55 MB): i4mm_cache_attention_workspace_bytes() bytes, zero-filled before the first use
+ * Sums and softmax statistics are fp32.  Which kernel runs goes by sizes that the host has (rows, max_len, the table's width, window), and the two
+ * round differently: the one for few rows multiplies the values by weights of about 22 bits, the one for prompts by weights rounded to fp16
+ * (2^-11 of each; against 64 bits 2.6e-4 to 2.8e-4 of an fp16 output's norm, where rounding the output alone makes 2.1e-4).  The same call gives the same bits.  `workspace` (about 55 MB): i4mm_cache_attention_workspace_bytes() bytes, zero-filled before the first use
  * and after i4mm_device_status has reported I4MM_ERR_TIMEOUT for it, shared by calls of one stream only.
  */
 size_t i4mm_cache_attention_workspace_bytes(void);

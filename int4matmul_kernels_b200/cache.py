@@ -8,7 +8,8 @@
 
 The cache is (pages, heads, page_size, head_dim) int8 or float8_e4m3fn for keys and values, with fp32 scales (pages, heads, 2): a
 byte q stands for q * scale.  page_size is 16, 32, 64 or 128 and head_dim 64 or 128.  Activations are fp16 or bf16.  Everything runs on
-torch's current stream and nothing waits for the GPU.
+torch's current stream and nothing waits for the GPU, but for the first `attention` of a stream if it is made inside a graph capture: that
+waits until its scratch has been cleared.
 """
 from __future__ import annotations
 
@@ -203,7 +204,10 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sca
     q (tokens, q_heads, head_dim), q_heads a multiple of the cache's heads (query head h reads head h * heads // q_heads).  Rows
     cu_lens[b] .. cu_lens[b + 1] (without cu_lens: row b) are the last tokens of request b, which has seq_lens[b] tokens in the cache, their
     own included; each sees the tokens up to its own, with window > 0 the last `window` of them.  A row that sees none is 0.
-    `max_len`: the most rows of a request.  `scale`: 1 / sqrt(head_dim) unless given."""
+    `max_len`: the most rows of a request; a wrong one costs time, nothing else.  `scale`: 1 / sqrt(head_dim) unless given.
+
+    Two kernels serve it, chosen by sizes.  Both keep sums in fp32; the one for prompts rounds weights to fp16 before they multiply the values.
+    There is no backward pass: the output carries no gradient."""
     mod = ops.native()
     if mod:
         out = mod._try_cache_attention(q, k_cache, v_cache, scales, block_table, seq_lens, cu_lens, max_len, scale, window, ops._cache_workspaces)

@@ -23,7 +23,8 @@
 // tokens into items of their own; the block that finishes a segment's last part joins them in order.  Every wait is bounded; a block that
 // gives up records it in the status word.
 //
-// Measured: 2 x 1024 new tokens after 8000, 64 heads in groups of 8: 735 us, 730 TFLOP/s; a prompt of 2048 tokens, 40 heads: 103 us.  A tile
+// Measured: 2 x 1024 new tokens after 8000, 64 heads in groups of 8: 750 us, 720 TFLOP/s; a prompt of 2048 tokens, 40 heads: 102 us, the few-row
+// kernel's empty launch before it included.  A tile
 // takes about 5000 cycles: the chain of one half (scores 850 and more, 400 until they are in registers, 2 x 1000 for weights, 2 x 250 to pack and
 // publish them, the second product) against the other half's, and the decoding warps' chain, which is as long.  Without exponentials it is
 // 2 % faster, without decoding 17 %, with neither softmax nor decoding 40 %.  Slower: scores of 64 tokens at a time in two halves of their

@@ -23,8 +23,8 @@
 //   divided by its page's value scale again.  A second product with the weights' rounding errors (their low halves) brings the output to
 //   fp32's exactness for 16 more tensor instructions a tile, which the tensor pipe (20 % busy) has spare.
 //
-// Measured: the requests above 284 us (4.7 TB/s; some 830 instructions a tile of 32 tokens, half of them for the bytes' decoding, are what is left
-// to hide); 12 requests of 20000 to 34000 tokens, 8 heads, e4m3, 8 rows: 118 us (5.7 TB/s); one request of 1011 tokens: 14 us, of which
+// Measured: the requests above 285 us (4.6 TB/s; some 830 instructions a tile of 32 tokens, half of them for the bytes' decoding, are what is left
+// to hide); 12 requests of 20000 to 34000 tokens, 8 heads, e4m3, 8 rows: 120 us (5.6 TB/s); one request of 1011 tokens: 13.5 us, of which
 // 5 find and fetch the first tile, 3.6 join parts over blocks.  (Whole segments to blocks, without that join: 14.8.)
 #include <algorithm>
 #include <type_traits>
@@ -41,8 +41,10 @@ constexpr uint32_t kNoPage = 0x7FC0DEADu;             // in the place of a scale
 
 template <int D, int NT>
 struct Shape {
-    // Registers (about 180 to 245 where nothing is spilled) allow 8 warps; with half the bytes to a token, 12 warps of 168 hide more of a tile's
-    // dependent steps than they lose (33 drafts, head_dim 64: 63.5 us with 8, 61.6 with 12; 64 single tokens, head_dim 128: 284 and 279
+    // Registers (234 to 243 for one column tile at head_dim 128, nothing spilled; two column tiles take all 255 and spill 100 to 128 bytes,
+    // which 360 to 456 bytes of loads bring back) allow 8 warps; with half the bytes to a token, 12 warps of 168 hide more of a tile's
+    // dependent steps than they lose, though two column tiles spill 124 bytes there (524 of loads) and one, of 155 to 158 registers, nothing
+    // (33 drafts, head_dim 64: 63.5 us with 8, 61.6 with 12; 64 single tokens, head_dim 128: 284 and 279
     // with a ring of two stages, 118 and 122 on long contexts).
     static constexpr int kWarps = D == 64 ? 12 : 8;
     static constexpr int kThreads = 32 * kWarps;
