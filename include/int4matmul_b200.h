@@ -308,6 +308,7 @@ int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type,
  *   cu_lens (requests + 1)    rows of request b are cu_lens[b] .. cu_lens[b + 1] (NULL: one row for each request), its last ones: row i of
  *                             n is at position p = seq_lens[b] - n + i and sees the tokens j <= p, with window > 0 those with
  *                             j > p - window.  Rows that see no token, and rows of no request, are 0.
+ *   table_width               a row of the block table stands for table_width * page_size tokens, at most 2^31 - 128
  *   max_len                   the most rows of a request, for the choice of a kernel (a wrong one costs time, nothing else)
  * Sums and softmax statistics are fp32.  Which kernel runs goes by sizes that the host has (rows, max_len, the table's width, window), and the two
  * round differently: the one for few rows multiplies the values by weights of about 22 bits, the one for prompts by weights rounded to fp16

@@ -188,7 +188,8 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
     if (status != I4MM_OK) return status;
     if (type != I4MM_TYPE_FP16 && type != I4MM_TYPE_BF16) return I4MM_ERR_UNSUPPORTED;
     if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->heads) return I4MM_ERR_SHAPE;
-    if (tokens < 0 || tokens > kMost / q_heads || requests < 0 || requests > 16384 || table_width < 0 || table_width > kMost / cache->page_size ||
+    // (tokens of a table's row: a tile of 128 that begins among them ends below 2^31)
+    if (tokens < 0 || tokens > kMost / q_heads || requests < 0 || requests > 16384 || table_width < 0 || table_width > (kMost - 127) / cache->page_size ||
         table_stride < table_width || max_len < 0 || max_len > kMost || window < 0 || window > kMost)
         return I4MM_ERR_SHAPE;
     if (!cu_lens && tokens < requests) return I4MM_ERR_SHAPE;

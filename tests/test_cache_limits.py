@@ -42,3 +42,13 @@ def test_strides_of_a_single_page_head_or_token(built_library):
     assert write == attend == capi.ERR_ALIGN
     write, _, attend = calls(cache(heads=1), 1, token=4, tokens=2)
     assert write == attend == capi.ERR_ALIGN
+
+
+def test_the_widest_block_table(built_library):
+    """Tiles of up to 128 tokens are counted in 32 bits: their last one has to end below 2^31."""
+    def attend(page, width):
+        c = capi.Cache(16, 16, 16, 4, 1, page, 128, page * 128, 128, 128, page * 128, 128, 128, 0)
+        return built_library.i4mm_cache_attention(ctypes.byref(c), 16, 16, 0, 1, 1, 128, 128, 16, width, width, 16, None, 1, 1, 1.0, 0, 16, 0, None)
+    for page in (16, 32, 64, 128):
+        assert attend(page, (2 ** 31 - 128) // page) == capi.ERR_WORKSPACE             # (accepted: the next check is the scratch's)
+        assert attend(page, (2 ** 31 - 128) // page + 1) == capi.ERR_SHAPE
