@@ -324,7 +324,56 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
  * that must know which kernel they exercised. */
 #define I4MM_ATTENTION_FEW_ROWS 1
 #define I4MM_ATTENTION_PROMPT 2
+#define I4MM_ATTENTION_PREFIX 4
 int i4mm_last_attention_kernels(void);
+
+/*
+ * angles[t, i] = (cos, sin) of positions[t] * freqs[i], fp32 (tokens, pairs, 2) contiguous; (1, 0) where the position is negative (padding).
+ *   positions int32 (tokens), freqs fp32 (pairs), pairs a multiple of 8 up to 128; angles 16-byte, freqs 8-byte aligned.
+ * The products and their reduction by whole turns are fp64, so that far positions are as exact as near ones.
+ */
+int i4mm_cache_angles(void* angles, const void* positions, const void* freqs, int64_t tokens, int64_t pairs, void* stream);
+
+/*
+ * i4mm_cache_write for a model whose queries and keys are normed and rotated, in the same launch.  For each row x (head_dim values) of a head of q or k:
+ *   y = x / sqrt(mean(x^2) + eps) * weight     (q_weight, k_weight: (head_dim) in the activations' type, 16-byte aligned; NULL: y = x)
+ *   (a, b) -> (a cos - b sin, b cos + a sin)   of the first 2 * pairs values, a and b being values i and i + pairs, or with pairs_beside 2 i and 2 i + 1;
+ *                                              cos, sin = angles[t, i] (fp32 (tokens, pairs, 2), 16-byte aligned); pairs a multiple of 8, 0: no rotation
+ * in fp32, rounded once to the activations' type.  q_out (tokens, q_heads, head_dim) contiguous gets the queries of all tokens; the keys, and
+ * the values as they are, go into the cache as i4mm_cache_write's do, to the byte.  q_out is none of the inputs; q_heads is free here.
+ */
+int i4mm_cache_append(const i4mm_cache* cache, void* q_out, const void* q, const void* k, const void* v, int type, int64_t tokens, int64_t q_heads,
+                      int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                      int64_t v_head_stride, const void* slots, const void* angles, int64_t pairs, int pairs_beside, const void* q_weight,
+                      const void* k_weight, float eps, void* stream);
+
+/*
+ * Shared prefixes: requests that begin alike hold what they share once.  A prefix is a place of the batch like any request (its tokens are
+ * written, and its pages given back, as theirs are); a request names it and holds only what comes after it.
+ *   prefix_of (requests)      the place whose tokens come before the request's own.  None: negative, no place of the batch, the request itself, a
+ *                             place without tokens; a prefix's own prefix is not looked at.
+ *   seq_lens, cu_lens         as for i4mm_cache_attention, after the step
+ * Outputs: effective (requests): prefix_of, -1 for none; starts (requests + 1), rows (max_tokens): the packed rows that read place p are
+ * rows[starts[p]] .. rows[starts[p + 1] - 1], ascending, -1 behind the last of all; positions (max_tokens): of the packed rows, the prefix counted
+ * (for i4mm_cache_angles), -1 for padding.  requests <= 16384, max_tokens <= 2^30.
+ */
+int i4mm_cache_share(int64_t requests, const void* prefix_of, const void* seq_lens, const void* cu_lens, int64_t max_tokens, void* effective,
+                     void* starts, void* rows, void* positions, void* stream);
+
+/*
+ * i4mm_cache_attention of rows that see their request's prefix before its own tokens: with L tokens in the prefix, a row at position p of its request
+ * (p >= 0) sees tokens j of the prefix and j' <= p of its own; with window > 0 those with j > L + p - window and j' > p - window.  The prefix's pages
+ * are read once for all rows that share it, not once for each.
+ *   prefix_of, prefix_starts, prefix_rows (listed >= tokens entries)   i4mm_cache_share's effective, starts and rows of the same step
+ *   scratch   i4mm_cache_shared_scratch_bytes(tokens, q_heads, head_dim) bytes, 16-byte aligned, of any contents, this call's alone
+ * The prefix's sums are fp32 too, its weights rounded to fp16; everything else is as above.
+ */
+size_t i4mm_cache_shared_scratch_bytes(int64_t tokens, int64_t q_heads, int64_t head_dim);
+int i4mm_cache_attention_shared(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,
+                                int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
+                                int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
+                                int64_t window, const void* prefix_of, const void* prefix_starts, const void* prefix_rows, int64_t listed,
+                                void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

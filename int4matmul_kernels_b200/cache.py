@@ -1,9 +1,12 @@
 """The paged key-value cache in 8 bits, and attention over it: what a decoder needs between its quantized linears.
 
     plan       the step's block tables and slot maps, on the GPU, from the requests' lengths
+    share      which of the step's rows read which shared prefix, and their positions
+    angles     cosines and sines of positions
     write      quantise the step's keys and values into their pages
+    append     norm the step's queries and keys, rotate them, and write keys and values, in one launch
     read       tokens of the cache as the values that they stand for
-    attention  softmax attention of the step's queries over the cached tokens
+    attention  softmax attention of the step's queries over the cached tokens, those of a shared prefix among them
     PagedCache one layer's arrays;  PageTable  the requests' lengths, block table and free pages
 
 The cache is (pages, heads, page_size, head_dim) int8 or float8_e4m3fn for keys and values, with fp32 scales (pages, heads, 2): a
@@ -34,6 +37,14 @@ class Plan(NamedTuple):
     requests: torch.Tensor      # (max_tokens) its request; -1: padding
     free_count: torch.Tensor    # (1) pages left on the stack
     missing: torch.Tensor       # (1) pages that the step asked for and did not get
+
+
+class Shared(NamedTuple):
+    """A step's shared prefixes; int32 on the GPU."""
+    prefix_of: torch.Tensor     # (requests) the place of the batch whose tokens come before the request's own; -1: none
+    starts: torch.Tensor        # (requests + 1) where the list of each place's readers begins in `rows`
+    rows: torch.Tensor          # (max_tokens) packed tokens that read a prefix, by place and then in order; -1 behind the last
+    positions: torch.Tensor     # (max_tokens) position of each packed token, its prefix counted; -1: padding
 
 
 def _workspace(device: torch.device, stream: torch.cuda.Stream) -> torch.Tensor:
@@ -145,6 +156,67 @@ def plan(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tens
     return out
 
 
+def share(prefix_of: torch.Tensor, seq_lens: torch.Tensor, cu_lens: torch.Tensor, max_tokens: int) -> Shared:
+    """Which rows of a step read which shared prefix, for `attention`, and the rows' positions, for `angles`; once a step, for all layers.
+
+    A prefix (a system prompt, a document) is a place of the batch like any request: its tokens are written and its pages given back as theirs
+    are.  prefix_of[b] is the place whose tokens come before those of request b, which holds only what comes after; a negative number, no place
+    of the batch, the request itself or a place without tokens: none.  One level: a prefix's own prefix is not looked at.  `seq_lens`
+    and `cu_lens` are the Plan's, after the step; `max_tokens` as for `plan`.  A place must go on holding its tokens while requests name it."""
+    mod = ops.native()
+    if mod:
+        out = mod._try_cache_share(prefix_of, seq_lens, cu_lens, max_tokens)
+        if not isinstance(out, int):
+            return Shared._make(out)
+        _check(max(out, 0), "cache share")
+    if not seq_lens.is_cuda:
+        raise ValueError("seq_lens must be a CUDA tensor")
+    dev, n = seq_lens.device, seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    _int32(seq_lens, "seq_lens", dev, (n,))
+    _int32(prefix_of, "prefix_of", dev, (n,))
+    _int32(cu_lens, "cu_lens", dev, (n + 1,))
+    max_tokens = int(max_tokens)
+    if max_tokens < 0:
+        raise ValueError("max_tokens must not be negative")
+    sizes = (n, n + 1, max_tokens, max_tokens)
+    with torch.cuda.device(dev):
+        out = Shared(*torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes))
+        status = capi.load().i4mm_cache_share(n, prefix_of.data_ptr(), seq_lens.data_ptr(), cu_lens.data_ptr(), max_tokens, *(t.data_ptr() for t in out),
+                                              torch.cuda.current_stream(dev).cuda_stream)
+    _check(status, "cache share")
+    return out
+
+
+def angles(positions: torch.Tensor, freqs: torch.Tensor) -> torch.Tensor:
+    """(tokens, pairs, 2) fp32: cos and sin of positions[t] * freqs[i], as exact for far positions as for near ones; (1, 0) for negative positions.
+
+    positions (tokens) int32, freqs (pairs) fp32, their number a multiple of 8 up to 128.  Once a step, for all layers."""
+    mod = ops.native()
+    if mod:
+        out = mod._try_cache_angles(positions, freqs)
+        if not isinstance(out, int):
+            return out
+        _check(max(out, 0), "cache angles")
+    if not positions.is_cuda:
+        raise ValueError("positions must be a CUDA tensor")
+    dev = positions.device
+    _int32(positions, "positions", dev)
+    if positions.dim() != 1:
+        raise ValueError("positions must be (tokens)")
+    if freqs.device != dev:
+        raise ValueError(f"freqs must be a CUDA tensor on {dev}")
+    if freqs.dtype != torch.float32:
+        raise TypeError("freqs must be float32")
+    if freqs.dim() != 1 or not freqs.is_contiguous():
+        raise ValueError("freqs must be contiguous (pairs)")
+    with torch.cuda.device(dev):
+        out = torch.empty((positions.shape[0], freqs.shape[0], 2), dtype=torch.float32, device=dev)
+        status = capi.load().i4mm_cache_angles(out.data_ptr(), positions.data_ptr(), freqs.data_ptr(), positions.shape[0], freqs.shape[0],
+                                               torch.cuda.current_stream(dev).cuda_stream)
+    _check(status, "cache angles")
+    return out
+
+
 def write(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantises k and v (tokens, heads, head_dim) into the cache, in place, at `slots` (tokens or more; those below 0 are skipped).
 
@@ -170,6 +242,55 @@ def write(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, k:
             ctypes.byref(c), k.data_ptr(), v.data_ptr(), kind, k.shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
             slots.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
     _check(status, "cache write")
+
+
+def append(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+           slots: torch.Tensor, angles: Optional[torch.Tensor] = None, *, q_weight: Optional[torch.Tensor] = None,
+           k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
+    """`write` of a model whose queries and keys are normed and rotated: returns the queries (tokens, q_heads, head_dim), and quantises the keys so
+    treated, and the values as they are, into the cache.
+
+    Each head of q (k) is divided by the root of its mean square (+ eps) and multiplied by q_weight (k_weight), (head_dim) in q's type; None: no
+    norm.  Then its first 2 * pairs values are rotated by `angles` (tokens or more, pairs, 2), as `angles` makes them: value i with value i + pairs,
+    or, `interleaved`, value 2 i with value 2 i + 1; None: no rotation.  All in fp32, rounded once to q's type, so that the cache
+    holds what a `write` of such keys would put there.  q, k and v may be columns of one projection's output; padding (slots below 0) is not written."""
+    mod = ops.native()
+    if mod:
+        out = mod._try_cache_append(k_cache, v_cache, scales, q, k, v, slots, angles, q_weight, k_weight, eps, interleaved)
+        if not isinstance(out, int):
+            return out
+        _check(max(out, 0), "cache append")
+    c = _cache(k_cache, v_cache, scales)
+    dev = k_cache.device
+    kind = _rows(k, "k", dev, c.heads, c.head_dim)
+    if _rows(v, "v", dev, c.heads, c.head_dim) != kind or v.shape != k.shape:
+        raise ValueError("k and v must have one type and shape")
+    if _rows(q, "q", dev, None, c.head_dim) != kind or q.shape[0] != k.shape[0]:
+        raise ValueError("q must have the type and tokens of k")
+    _int32(slots, "slots", dev)
+    if slots.dim() != 1 or slots.shape[0] < k.shape[0]:
+        raise ValueError("slots must be (tokens)")
+    if angles is None and q_weight is None and k_weight is None:
+        raise ValueError("without angles and weights there is nothing to append that write does not")
+    pairs = 0
+    if angles is not None:
+        if angles.device != dev or angles.dtype != torch.float32:
+            raise TypeError(f"angles must be float32 on {dev}")
+        if angles.dim() != 3 or angles.shape[0] < k.shape[0] or angles.shape[2] != 2 or not angles.is_contiguous():
+            raise ValueError("angles must be contiguous (tokens, pairs, 2)")
+        pairs = angles.shape[1]
+    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if t is not None and (t.device != dev or t.dtype != k.dtype or tuple(t.shape) != (c.head_dim,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be ({c.head_dim}) in the type of k on {dev}")
+    with torch.cuda.device(dev):
+        out = torch.empty((q.shape[0], q.shape[1], c.head_dim), dtype=q.dtype, device=dev)
+        status = capi.load().i4mm_cache_append(
+            ctypes.byref(c), out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), kind, k.shape[0], q.shape[1], q.stride(0), q.stride(1),
+            k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), angles.data_ptr() if angles is not None else None, pairs,
+            int(interleaved), q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
+            float(eps), torch.cuda.current_stream(dev).cuda_stream)
+    _check(status, "cache append")
+    return out
 
 
 def read(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, slots: torch.Tensor,
@@ -198,7 +319,7 @@ def read(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, slo
 
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
               seq_lens: torch.Tensor, cu_lens: Optional[torch.Tensor] = None, max_len: int = 1, *, scale: Optional[float] = None,
-              window: int = 0) -> torch.Tensor:
+              window: int = 0, shared: Optional[Shared] = None) -> torch.Tensor:
     """softmax(scale * q k^T) v over the cached tokens that each row sees; (tokens, q_heads, head_dim) in q's type.
 
     q (tokens, q_heads, head_dim), q_heads a multiple of the cache's heads (query head h reads head h * heads // q_heads).  Rows
@@ -206,11 +327,14 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sca
     own included; each sees the tokens up to its own, with window > 0 the last `window` of them.  A row that sees none is 0.
     `max_len`: the most rows of a request; a wrong one costs time, nothing else.  `scale`: 1 / sqrt(head_dim) unless given.
 
-    Two kernels serve it, chosen by sizes.  Both keep sums in fp32; the one for prompts rounds weights to fp16 before they multiply the values.
+    `shared`, of the same step: rows of a request that has a prefix see all of the prefix's tokens and then their own, as if the request held both
+    (a window counts over both); the prefix is read once for all rows that share it.
+
+    Two kernels serve it, chosen by sizes, and a third one shared prefixes.  All keep sums in fp32; those for prompts and prefixes round weights to fp16 before they multiply the values.
     There is no backward pass: the output carries no gradient."""
     mod = ops.native()
     if mod:
-        out = mod._try_cache_attention(q, k_cache, v_cache, scales, block_table, seq_lens, cu_lens, max_len, scale, window, ops._cache_workspaces)
+        out = mod._try_cache_attention(q, k_cache, v_cache, scales, block_table, seq_lens, cu_lens, max_len, scale, window, shared, ops._cache_workspaces)
         if not isinstance(out, int):
             return out
         _check(max(out, 0), "cache attention")
@@ -228,15 +352,26 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sca
         raise ValueError("without cu_lens, q must have a row for each request")
     if int(window) < 0 or int(max_len) < 0:
         raise ValueError("window and max_len must not be negative")
+    if shared is not None:
+        _int32(shared.prefix_of, "shared.prefix_of", dev, (n,))
+        _int32(shared.starts, "shared.starts", dev, (n + 1,))
+        _int32(shared.rows, "shared.rows", dev)
+        if shared.rows.dim() != 1 or shared.rows.shape[0] < q.shape[0]:
+            raise ValueError("shared.rows must have an entry for each row of q")
     with torch.cuda.device(dev):
         stream = torch.cuda.current_stream(dev)
         ws = _workspace(dev, stream)
         out = torch.empty((q.shape[0], q.shape[1], c.head_dim), dtype=q.dtype, device=dev)
-        status = capi.load().i4mm_cache_attention(
-            ctypes.byref(c), out.data_ptr(), q.data_ptr(), kind, q.shape[0], q.shape[1], q.stride(0), q.stride(1), block_table.data_ptr(),
-            width, row_stride, seq_lens.data_ptr(), cu_lens.data_ptr() if cu_lens is not None else None, n,
-            int(max_len), 1.0 / math.sqrt(c.head_dim) if scale is None else float(scale), int(window), ws.data_ptr(), ws.numel(),
-            stream.cuda_stream)
+        lib = capi.load()
+        args = (ctypes.byref(c), out.data_ptr(), q.data_ptr(), kind, q.shape[0], q.shape[1], q.stride(0), q.stride(1), block_table.data_ptr(),
+                width, row_stride, seq_lens.data_ptr(), cu_lens.data_ptr() if cu_lens is not None else None, n,
+                int(max_len), 1.0 / math.sqrt(c.head_dim) if scale is None else float(scale), int(window))
+        if shared is None:
+            status = lib.i4mm_cache_attention(*args, ws.data_ptr(), ws.numel(), stream.cuda_stream)
+        else:
+            room = torch.empty(lib.i4mm_cache_shared_scratch_bytes(q.shape[0], q.shape[1], c.head_dim), dtype=torch.uint8, device=dev)
+            status = lib.i4mm_cache_attention_shared(*args, shared.prefix_of.data_ptr(), shared.starts.data_ptr(), shared.rows.data_ptr(),
+                                                     shared.rows.shape[0], room.data_ptr(), room.numel(), ws.data_ptr(), ws.numel(), stream.cuda_stream)
     _check(status, "cache attention")
     return out
 
@@ -276,6 +411,10 @@ class PageTable:
         self._can_undo = self._can_undo or not torch.cuda.is_current_stream_capturing()
         return p
 
+    def share(self, prefix_of: torch.Tensor, plan: Plan) -> Shared:
+        """`share` of the step that this table has just made, which was `plan`: prefix_of (requests) int32 on the GPU, places of this table."""
+        return share(prefix_of, self.seq_lens, plan.cu_lens, plan.slots.shape[0])
+
     def undo(self) -> None:
         """Takes the last step back, before any of its tokens has been written into a cache: what a write does to a page (pages of requests
         that end are given out again in the same step; a scale that grows rounds the bytes beside the new ones again) is not undone."""
@@ -298,10 +437,16 @@ class PagedCache:
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         write(self.k, self.v, self.scales, k, v, slots)
 
+    def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, angles: Optional[torch.Tensor] = None, *,
+               q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               interleaved: bool = False) -> torch.Tensor:
+        return append(self.k, self.v, self.scales, q, k, v, slots, angles, q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved)
+
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
         return read(self.k, self.v, self.scales, slots, dtype)
 
     def attention(self, q: torch.Tensor, table: PageTable, cu_lens: Optional[torch.Tensor] = None, max_len: int = 1, *,
-                  scale: Optional[float] = None, window: int = 0) -> torch.Tensor:
+                  scale: Optional[float] = None, window: int = 0, shared: Optional[Shared] = None) -> torch.Tensor:
         """Of the step that `table` has just made: its lengths include the step's tokens."""
-        return attention(q, self.k, self.v, self.scales, table.block_table, table.seq_lens, cu_lens, max_len, scale=scale, window=window)
+        more = {} if shared is None else {"shared": shared}
+        return attention(q, self.k, self.v, self.scales, table.block_table, table.seq_lens, cu_lens, max_len, scale=scale, window=window, **more)

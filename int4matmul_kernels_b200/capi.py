@@ -30,7 +30,7 @@ class Cache(ctypes.Structure):
 
 CACHE_INT8, CACHE_E4M3 = 0, 1
 TYPE_FP16, TYPE_BF16 = 0, 1
-ATTENTION_FEW_ROWS, ATTENTION_PROMPT = 1, 2    # i4mm_last_attention_kernels
+ATTENTION_FEW_ROWS, ATTENTION_PROMPT, ATTENTION_PREFIX = 1, 2, 4    # i4mm_last_attention_kernels
 
 # every symbol the header declares, with its ctypes signature
 _SIGNATURES = {
@@ -85,6 +85,17 @@ _SIGNATURES = {
                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
                                             ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
                                             ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "i4mm_cache_angles": (ctypes.c_int, [ctypes.c_void_p] * 3 + [ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p]),
+    "i4mm_cache_share": (ctypes.c_int, [ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 5),
+    "i4mm_cache_append": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+                                         *[ctypes.c_int64] * 8, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                         ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p]),
+    "i4mm_cache_shared_scratch_bytes": (ctypes.c_size_t, [ctypes.c_int64] * 3),
+    "i4mm_cache_attention_shared": (ctypes.c_int, [ctypes.POINTER(Cache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64,
+                                                   ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                                   ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64,
+                                                   ctypes.c_float, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                   ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "i4mm_last_attention_kernels": (ctypes.c_int, []),
     "i4mm_check_mask": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
 }

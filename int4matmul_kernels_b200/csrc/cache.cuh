@@ -53,11 +53,40 @@ struct AttentionParams {
     int table_width, requests, tokens, q_heads, group; // group = q_heads / cache.heads
     int window;                                       // 0: none
     float scale;
+    // shared prefixes (`shared` below): of request b, the place of the batch whose tokens come before its own, or -1; the list of the
+    // rows that read place p is rows[starts[p]] .. rows[starts[p + 1] - 1]
+    const int* prefix_of;
+    const int* prefix_starts;
+    const int* prefix_rows;
+    int prefix_listed;                                // entries of the list
+    // what the rows' prefixes come to, by packed row and head: (m, sum of 2^(s - m)) and the sums of 2^(s - m) v
+    float2* prefix_total;
+    float* prefix_sums;
+};
+
+struct AppendParams {
+    CacheView cache;
+    RowsView q, k, v;
+    void* q_out;                                      // (tokens, q_heads, dim) contiguous
+    const int* slots;
+    const float2* angles;                             // (tokens, pairs): cos, sin
+    const void *q_weight, *k_weight;                  // (dim) in the activations' type, or nullptr: no norm
+    int tokens, q_heads, pairs;                       // pairs 0: no rotation
+    float eps;
+};
+
+struct ShareParams {
+    const int *prefix_of, *seq_lens, *cu_lens;
+    int *effective, *starts, *rows, *positions;
+    int requests, max_tokens;
 };
 
 cudaError_t cache_plan_launch(const PlanParams& p, cudaStream_t stream);
 cudaError_t cache_write_launch(const CacheView& c, bool e4m3, const RowsView& k, const RowsView& v, bool bf16, int tokens, const int* slots,
                                cudaStream_t stream);
+cudaError_t cache_append_launch(const AppendParams& p, bool e4m3, bool bf16, bool pairs_beside, cudaStream_t stream);
+cudaError_t cache_angles_launch(void* out, const int* positions, const float* freqs, int tokens, int pairs, cudaStream_t stream);
+cudaError_t cache_share_launch(const ShareParams& p, cudaStream_t stream);
 cudaError_t cache_read_launch(const CacheView& c, bool e4m3, void* k_out, void* v_out, bool bf16, int tokens, const int* slots,
                               cudaStream_t stream);
 

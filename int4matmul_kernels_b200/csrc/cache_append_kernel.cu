@@ -1,0 +1,263 @@
+// A step's queries and keys on their way from the projection to the attention (i4mm_cache_append): norm of each head, rotation, and keys and values
+// quantised into their pages, in one launch.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w      (without weights: y = x)
+//   (a, b) -> (a cos - b sin, b cos + a sin)      for the pairs (i, i + F) or (2 i, 2 i + 1) of the first 2 F values, cos and sin from the step's table
+// in fp32, rounded once to the activations' type; queries are stored so, keys go on to the cache as cache_write_kernel.cu says, and so do values,
+// which are not changed.  So the bytes are those of a write of the rotated keys.
+// What bounds it: 16-bit rows in and out, bytes out, and issue slots.
+#include <algorithm>
+
+#include "cache_bytes.cuh"
+#include "ptx.cuh"
+
+namespace i4mm {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kHeld = 8;                              // rows (two at head_dim 128, four at 64) that a warp holds at once
+constexpr uint32_t kAll = 0xFFFFFFFFu;
+
+enum Turn { kStraight, kHalves, kPairs };             // no rotation; pairs (i, i + F); pairs (2 i, 2 i + 1)
+
+// What a lane does to its 8 values of a row; the lanes of a row call together.
+template <bool BF16, int TURN>
+struct Turned {
+    float weight[8];
+    bool norm, turns, second;                         // second: the lane has the b of its pairs (kHalves)
+    int partner, lanes;                               // the lane with the other halves; lanes of a row
+    float eps, per;                                   // 1 / head_dim
+    const float2* angles;                             // the lane's first pair of token 0
+    long long stride;                                 // pairs of a token
+
+    __device__ __forceinline__ Turned(const AppendParams& p, const void* w, int lane) {
+        lanes = p.cache.dim >> 3;
+        const int at = lane % lanes, col = 8 * at, pairs = p.pairs;
+        norm = w != nullptr;
+        eps = p.eps;
+        per = 1.f / (float)p.cache.dim;
+        turns = TURN != kStraight && col < 2 * pairs;
+        second = TURN == kHalves && col >= pairs;
+        partner = !turns ? lane : second ? lane - (pairs >> 3) : lane + (pairs >> 3);
+        stride = pairs;
+        angles = p.angles + (!turns ? 0 : TURN == kPairs ? col / 2 : second ? col - pairs : col);
+        if (norm) {
+            unpack8<BF16>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + col), weight);
+        }
+    }
+
+    __device__ __forceinline__ uint4 operator()(uint4 w, long long token) const {
+        float4 table[4];
+        if (turns) {
+            const float4* const from = reinterpret_cast<const float4*>(angles + token * stride);
+#pragma unroll
+            for (int i = 0; i < (TURN == kPairs ? 2 : 4); ++i) table[i] = __ldg(from + i);
+        }
+        float f[8];
+        unpack8<BF16>(w, f);
+        if (norm) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+            for (int d = lanes >> 1; d; d >>= 1) sum += __shfl_xor_sync(kAll, sum, d);
+            const float r = rsqrtf(fmaf(sum, per, eps));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] *= r * weight[i];
+        }
+        if (TURN == kHalves) {
+            float other[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(kAll, f[i], partner);
+            if (turns) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float c = i & 1 ? table[i / 2].z : table[i / 2].x, s = i & 1 ? table[i / 2].w : table[i / 2].y;
+                    f[i] = fmaf(f[i], c, other[i] * (second ? s : -s));
+                }
+            }
+        } else if (TURN == kPairs && turns) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float c = i & 1 ? table[i / 2].z : table[i / 2].x, s = i & 1 ? table[i / 2].w : table[i / 2].y, a = f[2 * i], b = f[2 * i + 1];
+                f[2 * i] = fmaf(a, c, -b * s);
+                f[2 * i + 1] = fmaf(b, c, a * s);
+            }
+        }
+        return make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
+    }
+};
+
+// Units of the tokens of a window (at most 16): the heads' keys, then their values, then the queries' heads.  A block takes a window and every
+// `groups`-th eight units, a warp one at a time.  Keys and values go by runs: neighbouring tokens with ascending slots of one page, of which those
+// that begin in the window are the window's, every gridDim.y-th of them to a block; queries are cut into gridDim.y parts.
+template <bool E4M3, bool BF16, int TURN>
+__global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const AppendParams p, int window, int groups) {
+    const int lane = threadIdx.x & 31;
+    const int block = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - block * groups), units = 2 * p.cache.heads + p.q_heads;
+    const CacheView& c = p.cache;
+    const int page = 1 << c.page_shift, lanes_per_row = c.dim >> 3, rows_per_step = 32 / lanes_per_row;
+    const int row = lane / lanes_per_row, col = (lane % lanes_per_row) * 8, chunk = kHeld * rows_per_step;
+    const int t0 = block * window, tokens = p.tokens;
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    // lane i: the slot of token t0 - 1 + i, and whether it goes on with the run of the one before
+    const int t = t0 - 1 + lane;
+    const int slot = t >= 0 && t < tokens ? p.slots[t] : -1;
+    const int before = __shfl_up_sync(kAll, slot, 1);
+    const bool goes_on = lane > 0 && before >= 0 && slot == before + 1 && (slot & (page - 1)) != 0;
+    const bool begins = lane > 0 && lane <= window && slot >= 0 && (slot >> c.page_shift) < c.pages && !goes_on;
+    const uint32_t on = __ballot_sync(kAll, goes_on), all_starts = __ballot_sync(kAll, begins);
+
+    for (int unit = group * kWarps + (threadIdx.x >> 5); unit < units; unit += groups * kWarps) {
+        uint4 w[kHeld];
+        if (unit >= 2 * c.heads) {
+            // ---- queries ----
+            const int head = unit - 2 * c.heads, n = min(window, tokens - t0), part = (n + (int)gridDim.y - 1) / (int)gridDim.y;
+            const Turned<BF16, TURN> turned(p, p.q_weight, lane);
+            const uint16_t* const from = static_cast<const uint16_t*>(p.q.p) + head * p.q.head + col;
+            uint16_t* const to = static_cast<uint16_t*>(p.q_out) + head * c.dim + col;
+            const int end = min(n, part * ((int)blockIdx.y + 1));
+            for (int i0 = part * (int)blockIdx.y; i0 < end; i0 += chunk) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    const int r = i0 + i * rows_per_step + row;
+                    w[i] = make_uint4(0, 0, 0, 0);
+                    if (r < end) w[i] = *reinterpret_cast<const uint4*>(from + (long long)(t0 + r) * p.q.token);
+                }
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    if (i0 + i * rows_per_step >= end) break;
+                    const int r = i0 + i * rows_per_step + row;
+                    const uint4 y = turned(w[i], t0 + min(r, end - 1));
+                    if (r < end) *reinterpret_cast<uint4*>(to + (long long)(t0 + r) * p.q_heads * c.dim) = y;
+                }
+            }
+            continue;
+        }
+        // ---- keys and values ----
+        const int which = unit >= c.heads, head = which ? unit - c.heads : unit;
+        const Turned<BF16, TURN> turned(p, which ? nullptr : p.k_weight, lane);
+        const uint16_t* const x = (const uint16_t*)(which ? p.v.p : p.k.p) + head * (which ? p.v.head : p.k.head) + col;
+        const long long x_token = which ? p.v.token : p.k.token;
+        int turn = 0;
+        for (uint32_t starts = all_starts; starts; starts &= starts - 1) {
+            if (turn++ % (int)gridDim.y != (int)blockIdx.y) continue;
+            const int from = __ffs(starts) - 1, run = t0 - 1 + from;
+            const int first_slot = __shfl_sync(kAll, slot, from);
+            const int id = first_slot >> c.page_shift, place = first_slot & (page - 1);
+            // its length: up to the first lane that does not go on; beyond the 32 lanes it is looked for
+            const uint32_t stop = ~on & (from == 31 ? 0u : ~0u << (from + 1));
+            int n = stop ? __ffs(stop) - 1 - from : 32 - from;
+            while (!stop && n < page - place) {
+                const int i = n + lane;
+                const bool more = i < page - place && run + i < tokens && p.slots[run + i] == first_slot + i;
+                const uint32_t end = __ballot_sync(kAll, !more);
+                if (end) {
+                    n += __ffs(end) - 1;
+                    break;
+                }
+                n += 32;
+            }
+            // the lane's part of kHeld rows at a time; a run that fits (a page of 16 tokens does) is read once
+            const uint16_t* const rows = x + (long long)run * x_token;
+            const auto fetch = [&](int i0) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    const int r = i0 + i * rows_per_step + row;
+                    w[i] = make_uint4(0, 0, 0, 0);
+                    if (r < n) w[i] = *reinterpret_cast<const uint4*>(rows + r * x_token);
+                }
+                if (which == 0 && (TURN != kStraight || turned.norm)) {
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i) {
+                        if (i0 + i * rows_per_step >= n) break;
+                        w[i] = turned(w[i], run + min(i0 + i * rows_per_step + row, n - 1));       // (rows beyond the run are 0 and stay so)
+                    }
+                }
+            };
+            // magnitudes of either 16-bit type are ordered as their bits are, infinities and NaN on top
+            uint32_t most = 0;
+            for (int i0 = 0; i0 < n; i0 += chunk) {
+                fetch(i0);
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i)
+                    most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu)));
+            }
+            most = __reduce_max_sync(kAll, max(most & 0xFFFFu, most >> 16));
+            const bool finite = most < (BF16 ? 0x7F80u : 0x7C00u);
+            float a = BF16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half((unsigned short)most));
+            if (!finite) {                                                   // the largest of the others
+                a = 0.f;
+                for (int i0 = 0; i0 < n; i0 += chunk) {
+                    if (n > chunk) fetch(i0);
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i) {
+                        float f[8];
+                        unpack8<BF16>(w[i], f);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) a = fabsf(f[j]) <= 3.4e38f ? fmaxf(a, fabsf(f[j])) : a;
+                    }
+                }
+#pragma unroll
+                for (int d = 16; d; d /= 2) a = fmaxf(a, __shfl_xor_sync(kAll, a, d));
+            }
+            float* const scale = reinterpret_cast<float*>(c.scales + (long long)id * c.heads + head) + which;
+            const float old = place ? *scale : 0.f;
+            const float s = fmaxf(old, scale_for<E4M3>(a));
+            uint8_t* const held = (which ? c.v : c.k) + id * (which ? c.v_page : c.k_page) + head * (which ? c.v_head : c.k_head);
+            const long long held_token = which ? c.v_token : c.k_token;
+            if (s > old && place > 0) {
+                const float ratio = old / s;          // (0 where the scale was: bytes of infinities beside zeros go on standing for 0)
+                for (int i = row; i < place; i += rows_per_step) {
+                    uint2* const at = reinterpret_cast<uint2*>(held + i * held_token + col);
+                    const uint2 b = *at;
+                    uint32_t u[2] = {b.x, b.y}, r[2] = {0, 0};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) r[j >> 2] |= to_byte<E4M3>(from_byte<E4M3>(u[j >> 2] >> (8 * (j & 3)) & 0xFFu) * ratio) << (8 * (j & 3));
+                    *at = make_uint2(r[0], r[1]);
+                }
+            }
+            const float inverse = s > 0.f ? 1.f / s : 1.f;
+            for (int i0 = 0; i0 < n; i0 += chunk) {
+                if (n > chunk) fetch(i0);
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) {
+                    if (i0 + i * rows_per_step >= n) break;
+                    const int r = i0 + i * rows_per_step + row;
+                    uint2 q;
+                    if (finite) {
+                        float f[8];
+                        unpack8<BF16>(w[i], f);
+                        q = to_bytes<E4M3>(f, inverse);
+                    } else {
+                        q = to_bytes_any<E4M3, BF16>(w[i], inverse);
+                    }
+                    if (r < n) *reinterpret_cast<uint2*>(held + (place + r) * held_token + col) = q;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) *scale = s;
+        }
+    }
+}
+
+}  // namespace
+
+cudaError_t cache_append_launch(const AppendParams& p, bool e4m3, bool bf16, bool pairs_beside, cudaStream_t stream) {
+    const int window = p.tokens > 1024 ? 16 : 1, units = 2 * p.cache.heads + p.q_heads;
+    const int groups = (units + kWarps - 1) / kWarps;
+    const long long blocks = (long long)((p.tokens + window - 1) / window) * groups;
+    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)blocks, window > 1 ? 2 : 1, 1);
+    const auto go = [&](auto e, auto h, auto t) {
+        return launch_overlapping(cache_append_kernel<decltype(e)::value, decltype(h)::value, decltype(t)::value>, grid, kWarps * 32, stream, p, window, groups);
+    };
+    const auto by_turn = [&](auto e, auto h) {
+        if (p.pairs == 0) return go(e, h, std::integral_constant<int, kStraight>{});
+        return pairs_beside ? go(e, h, std::integral_constant<int, kPairs>{}) : go(e, h, std::integral_constant<int, kHalves>{});
+    };
+    const auto by_type = [&](auto e) { return bf16 ? by_turn(e, std::true_type{}) : by_turn(e, std::false_type{}); };
+    return e4m3 ? by_type(std::true_type{}) : by_type(std::false_type{});
+}
+
+}  // namespace i4mm

@@ -166,10 +166,27 @@ __device__ __forceinline__ uint32_t pack_out(float a, float b) {
     return h2_as_u32(__floats2half2_rn(a, b));
 }
 
+// ---- a row's own sums and those of its shared prefix -------------------------------------------------------------------------------
+// (m, sum, o) of disjoint sets of tokens add up as in (max m; factors 2^(m - max) on sum and o): `own` and `prefix` are those factors over the whole sum
+struct Joint {
+    float own, prefix;
+};
+__device__ __forceinline__ Joint join_prefix(float m, float sum, float2 prefix) {
+    const float top = fmaxf(m, prefix.x);
+    const float a = m == -INFINITY ? 0.f : exp2_approx(m - top), b = prefix.x == -INFINITY ? 0.f : exp2_approx(prefix.x - top);
+    const float total = fmaf(sum, a, prefix.y * b), f = total > 0.f ? 1.f / total : total;      // (a NaN stays one)
+    return {a * f, b * f};
+}
+// whether a row of request b at this position sees a prefix
+__device__ __forceinline__ bool sees_prefix(const AttentionParams& p, int b, int position) { return position >= 0 && p.prefix_of[b] >= 0; }
+
 // The two kernels.  Few rows: requests of more than most_rows rows are left to the other one; `few`: no request has more than 8.
 // Prompts: requests of fewer than least_rows rows are left to the other one; `alone`: it is not launched.
+// With p.prefix_of set, both add what p.prefix_total and p.prefix_sums say to each row that has a prefix.
 cudaError_t cache_rows_launch(const AttentionParams& p, bool e4m3, bool bf16, int most_rows, bool few, cudaStream_t stream);
 cudaError_t cache_prompt_launch(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, bool alone, cudaStream_t stream);
+// Rows of all requests that share a prefix over that prefix, into p.prefix_total and p.prefix_sums.
+cudaError_t cache_prefix_launch(const AttentionParams& p, bool e4m3, bool bf16, cudaStream_t stream);
 size_t cache_rows_workspace();                        // bytes behind the header
 size_t cache_prompt_workspace();                      // bytes behind those
 

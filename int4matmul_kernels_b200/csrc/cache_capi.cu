@@ -104,6 +104,74 @@ cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t
     return e != cudaSuccess ? e : prompt(i4mm::kFewRows + 1, false);
 }
 
+// A step's shared prefixes, as i4mm_cache_share lays them out; prefix_of nullptr: none
+struct Prefixes {
+    const void *prefix_of, *starts, *rows;
+    int64_t listed;
+    void* scratch;
+    size_t scratch_bytes;
+};
+
+size_t shared_scratch(int64_t tokens, int64_t q_heads, int64_t head_dim) {
+    return (size_t)(tokens * q_heads + 1) / 2 * 16 + (size_t)tokens * q_heads * head_dim * 4;
+}
+
+int attention(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,
+                         int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
+                         int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
+                         int64_t window, void* workspace, size_t workspace_bytes, const Prefixes& shared, void* stream) {
+    g_attention_kernels = 0;
+    i4mm::AttentionParams p{};
+    const int status = view_of(cache, p.cache);
+    if (status != I4MM_OK) return status;
+    if (type != I4MM_TYPE_FP16 && type != I4MM_TYPE_BF16) return I4MM_ERR_UNSUPPORTED;
+    if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->heads) return I4MM_ERR_SHAPE;
+    // (tokens of a table's row: a tile of 128 that begins among them ends below 2^31)
+    if (tokens < 0 || tokens > kMost / q_heads || requests < 0 || requests > 16384 || table_width < 0 || table_width > (kMost - 127) / cache->page_size ||
+        table_stride < table_width || max_len < 0 || max_len > kMost || window < 0 || window > kMost)
+        return I4MM_ERR_SHAPE;
+    if (!cu_lens && tokens < requests) return I4MM_ERR_SHAPE;
+    if (tokens == 0) return I4MM_OK;
+    if (!out || !q || (requests > 0 && (!seq_lens || (table_width > 0 && !block_table)))) return I4MM_ERR_NULL;
+    p.q = rows_of(q, tokens, q_token_stride, q_heads, q_head_stride);
+    if (!aligned(out, 16) || !aligned(p.q) || !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(cu_lens, 4)) return I4MM_ERR_ALIGN;
+    if (!workspace || workspace_bytes < attention_workspace()) return I4MM_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return I4MM_ERR_ALIGN;
+    if (shared.prefix_of) {
+        if (shared.listed < tokens || shared.listed > kMost) return I4MM_ERR_SHAPE;
+        if (!shared.starts || !shared.rows || !shared.scratch) return I4MM_ERR_NULL;
+        if (!aligned(shared.prefix_of, 4) || !aligned(shared.starts, 4) || !aligned(shared.rows, 4) || !aligned(shared.scratch, 16)) return I4MM_ERR_ALIGN;
+        if (shared.scratch_bytes < shared_scratch(tokens, q_heads, cache->head_dim)) return I4MM_ERR_WORKSPACE;
+        p.prefix_of = (const int*)shared.prefix_of;
+        p.prefix_starts = (const int*)shared.starts;
+        p.prefix_rows = (const int*)shared.rows;
+        p.prefix_listed = (int)shared.listed;
+        p.prefix_total = (float2*)shared.scratch;
+        p.prefix_sums = (float*)((char*)shared.scratch + (size_t)(tokens * q_heads + 1) / 2 * 16);
+    }
+    p.out = out;
+    p.table = (const int*)block_table;
+    p.seq_lens = (const int*)seq_lens;
+    p.cu_lens = (const int*)cu_lens;
+    p.workspace = workspace;
+    p.prompt_parts = i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace();
+    p.table_stride = table_stride;
+    p.table_width = (int)table_width;
+    p.requests = (int)requests;
+    p.tokens = (int)tokens;
+    p.q_heads = (int)q_heads;
+    p.group = (int)(q_heads / cache->heads);
+    p.window = (int)window;
+    p.scale = scale;
+    const bool e4m3 = cache->type == I4MM_CACHE_E4M3, bf16 = type == I4MM_TYPE_BF16;
+    if (p.prefix_of && requests > 0) {
+        const cudaError_t e = i4mm::cache_prefix_launch(p, e4m3, bf16, (cudaStream_t)stream);
+        if (e != cudaSuccess) return finish(e);
+        g_attention_kernels |= I4MM_ATTENTION_PREFIX;
+    }
+    return finish(attend(p, e4m3, bf16, max_len, (cudaStream_t)stream));
+}
+
 }  // namespace
 
 extern "C" {
@@ -182,38 +250,83 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
                          int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
                          int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
                          int64_t window, void* workspace, size_t workspace_bytes, void* stream) {
-    g_attention_kernels = 0;
-    i4mm::AttentionParams p{};
-    const int status = view_of(cache, p.cache);
-    if (status != I4MM_OK) return status;
-    if (type != I4MM_TYPE_FP16 && type != I4MM_TYPE_BF16) return I4MM_ERR_UNSUPPORTED;
-    if (q_heads <= 0 || q_heads > 65535 || q_heads % cache->heads) return I4MM_ERR_SHAPE;
-    // (tokens of a table's row: a tile of 128 that begins among them ends below 2^31)
-    if (tokens < 0 || tokens > kMost / q_heads || requests < 0 || requests > 16384 || table_width < 0 || table_width > (kMost - 127) / cache->page_size ||
-        table_stride < table_width || max_len < 0 || max_len > kMost || window < 0 || window > kMost)
-        return I4MM_ERR_SHAPE;
-    if (!cu_lens && tokens < requests) return I4MM_ERR_SHAPE;
-    if (tokens == 0) return I4MM_OK;
-    if (!out || !q || (requests > 0 && (!seq_lens || (table_width > 0 && !block_table)))) return I4MM_ERR_NULL;
-    p.q = rows_of(q, tokens, q_token_stride, q_heads, q_head_stride);
-    if (!aligned(out, 16) || !aligned(p.q) || !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(cu_lens, 4)) return I4MM_ERR_ALIGN;
-    if (!workspace || workspace_bytes < attention_workspace()) return I4MM_ERR_WORKSPACE;
-    if (!aligned(workspace, 16)) return I4MM_ERR_ALIGN;
-    p.out = out;
-    p.table = (const int*)block_table;
+    return attention(cache, out, q, type, tokens, q_heads, q_token_stride, q_head_stride, block_table, table_width, table_stride, seq_lens, cu_lens,
+                     requests, max_len, scale, window, workspace, workspace_bytes, Prefixes{}, stream);
+}
+
+size_t i4mm_cache_shared_scratch_bytes(int64_t tokens, int64_t q_heads, int64_t head_dim) {
+    return tokens < 0 || q_heads < 0 || head_dim < 0 ? 0 : shared_scratch(tokens, q_heads, head_dim);
+}
+
+int i4mm_cache_attention_shared(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,
+                                int64_t q_token_stride, int64_t q_head_stride, const void* block_table, int64_t table_width,
+                                int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
+                                int64_t window, const void* prefix_of, const void* prefix_starts, const void* prefix_rows, int64_t listed,
+                                void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+    if (tokens > 0 && !prefix_of) {
+        g_attention_kernels = 0;
+        return I4MM_ERR_NULL;
+    }
+    return attention(cache, out, q, type, tokens, q_heads, q_token_stride, q_head_stride, block_table, table_width, table_stride, seq_lens, cu_lens,
+                     requests, max_len, scale, window, workspace, workspace_bytes,
+                     Prefixes{prefix_of, prefix_starts, prefix_rows, listed, scratch, scratch_bytes}, stream);
+}
+
+int i4mm_cache_angles(void* angles, const void* positions, const void* freqs, int64_t tokens, int64_t pairs, void* stream) {
+    if (tokens < 0 || tokens > kMost || pairs < 0 || pairs > 128) return I4MM_ERR_SHAPE;
+    if (pairs % 8) return I4MM_ERR_UNSUPPORTED;
+    if (tokens == 0 || pairs == 0) return I4MM_OK;
+    if (!angles || !positions || !freqs) return I4MM_ERR_NULL;
+    if (!aligned(angles, 16) || !aligned(positions, 4) || !aligned(freqs, 8)) return I4MM_ERR_ALIGN;
+    return finish(i4mm::cache_angles_launch(angles, (const int*)positions, (const float*)freqs, (int)tokens, (int)pairs, (cudaStream_t)stream));
+}
+
+int i4mm_cache_share(int64_t requests, const void* prefix_of, const void* seq_lens, const void* cu_lens, int64_t max_tokens, void* effective,
+                     void* starts, void* rows, void* positions, void* stream) {
+    if (requests < 0 || requests > 16384 || max_tokens < 0 || max_tokens > (int64_t(1) << 30)) return I4MM_ERR_SHAPE;
+    if (!starts || !cu_lens || (requests > 0 && (!prefix_of || !seq_lens || !effective)) || (max_tokens > 0 && (!rows || !positions))) return I4MM_ERR_NULL;
+    for (const void* q : {prefix_of, seq_lens, cu_lens, (const void*)effective, (const void*)starts, (const void*)rows, (const void*)positions})
+        if (!aligned(q, 4)) return I4MM_ERR_ALIGN;
+    i4mm::ShareParams p{};
+    p.prefix_of = (const int*)prefix_of;
     p.seq_lens = (const int*)seq_lens;
     p.cu_lens = (const int*)cu_lens;
-    p.workspace = workspace;
-    p.prompt_parts = i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace();
-    p.table_stride = table_stride;
-    p.table_width = (int)table_width;
+    p.effective = (int*)effective;
+    p.starts = (int*)starts;
+    p.rows = (int*)rows;
+    p.positions = (int*)positions;
     p.requests = (int)requests;
+    p.max_tokens = (int)max_tokens;
+    return finish(i4mm::cache_share_launch(p, (cudaStream_t)stream));
+}
+
+int i4mm_cache_append(const i4mm_cache* cache, void* q_out, const void* q, const void* k, const void* v, int type, int64_t tokens, int64_t q_heads,
+                      int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                      int64_t v_head_stride, const void* slots, const void* angles, int64_t pairs, int pairs_beside, const void* q_weight,
+                      const void* k_weight, float eps, void* stream) {
+    i4mm::AppendParams p{};
+    const int status = view_of(cache, p.cache);
+    if (status != I4MM_OK) return status;
+    if ((type != I4MM_TYPE_FP16 && type != I4MM_TYPE_BF16) || pairs % 8) return I4MM_ERR_UNSUPPORTED;
+    if (q_heads <= 0 || q_heads > 65535 || tokens < 0 || tokens > kMost / q_heads || pairs < 0 || 2 * pairs > cache->head_dim) return I4MM_ERR_SHAPE;
+    if (tokens == 0) return I4MM_OK;
+    if (!q_out || !q || !k || !v || !slots || (pairs > 0 && !angles)) return I4MM_ERR_NULL;
+    p.q = rows_of(q, tokens, q_token_stride, q_heads, q_head_stride);
+    p.k = rows_of(k, tokens, k_token_stride, p.cache.heads, k_head_stride);
+    p.v = rows_of(v, tokens, v_token_stride, p.cache.heads, v_head_stride);
+    if (!aligned(p.q) || !aligned(p.k) || !aligned(p.v) || !aligned(q_out, 16) || !aligned(slots, 4) || !aligned(angles, 16) || !aligned(q_weight, 16) ||
+        !aligned(k_weight, 16))
+        return I4MM_ERR_ALIGN;
+    p.q_out = q_out;
+    p.slots = (const int*)slots;
+    p.angles = (const float2*)angles;
+    p.q_weight = q_weight;
+    p.k_weight = k_weight;
     p.tokens = (int)tokens;
     p.q_heads = (int)q_heads;
-    p.group = (int)(q_heads / cache->heads);
-    p.window = (int)window;
-    p.scale = scale;
-    return finish(attend(p, cache->type == I4MM_CACHE_E4M3, type == I4MM_TYPE_BF16, max_len, (cudaStream_t)stream));
+    p.pairs = (int)pairs;
+    p.eps = eps;
+    return finish(i4mm::cache_append_launch(p, cache->type == I4MM_CACHE_E4M3, type == I4MM_TYPE_BF16, pairs_beside != 0, (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -250,7 +250,8 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t tile, int rows, int row, i
     return tile + (unit >> 3) * (rows * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
 }
 
-template <bool E4M3, bool BF16, int D>
+// PREFIX: a request's rows may have seen a shared prefix before its own tokens; what that came to is added at the end.
+template <bool E4M3, bool BF16, int D, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const AttentionParams p, int least_rows, int alone) {
     using L = Layout<D>;
     extern __shared__ uint8_t dynamic[];
@@ -730,8 +731,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
             if (t.rows[h] > 0) {
                 const long long to = ((long long)(t.row0 + token) * p.q_heads + head) * D;
                 uint16_t* const out = static_cast<uint16_t*>(p.out) + to;
+                // what the sums are multiplied with, once there are all of the row's own; the same of its prefix's
+                const auto joint = [&](float m, float sum) {
+                    if constexpr (PREFIX) {
+                        if (real && sees_prefix(p, t.b, position)) return join_prefix(m, sum, __ldcg(p.prefix_total + (long long)(t.row0 + token) * p.q_heads + head));
+                    }
+                    return Joint{sum > 0.f ? 1.f / sum : sum, 0.f};                           // (a NaN stays one)
+                };
+                const auto prefix4 = [&](int at) { return __ldcg(reinterpret_cast<const float4*>(p.prefix_sums + to + at)); };
                 if (t.part < 0) {
-                    const float f = sum > 0.f ? 1.f / sum : sum;                              // (a NaN stays one)
+                    const Joint both = joint(top, sum);
+                    const float f = both.own;
 #pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         uint32_t x[32] = {};
@@ -739,7 +749,19 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                             ptx::tmem_ld32(o_at + 32 * c, x);
                             ptx::tc_wait_ld();
                         }
-                        if (real)
+                        if (PREFIX && both.prefix != 0.f) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                const float4 a = prefix4(32 * c + i), b = prefix4(32 * c + i + 4);
+                                const float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                                uint32_t y[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    y[k] = pack_out<BF16>(fmaf(__uint_as_float(x[i + 2 * k]), f, z[2 * k] * both.prefix),
+                                                          fmaf(__uint_as_float(x[i + 2 * k + 1]), f, z[2 * k + 1] * both.prefix));
+                                *reinterpret_cast<uint4*>(out + 32 * c + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                            }
+                        } else if (real) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 8) {
                                 uint32_t y[4];
@@ -747,6 +769,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                                 for (int k = 0; k < 4; ++k) y[k] = pack_out<BF16>(__uint_as_float(x[i + 2 * k]) * f, __uint_as_float(x[i + 2 * k + 1]) * f);
                                 *reinterpret_cast<uint4*>(out + 32 * c + i) = make_uint4(y[0], y[1], y[2], y[3]);
                             }
+                        }
+                        if (PREFIX) __syncwarp();
                     }
                 } else {
                     float* const parts = reinterpret_cast<float*>(header + p.prompt_parts) + (size_t)h * L::kPartFloats;
@@ -787,10 +811,22 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
 #pragma unroll 4
                         for (int i = 0; i < t.parts; ++i)
                             total += exp2_approx(__ldcg(part_at(i) + kHalf * D + row) - from) * __ldcg(part_at(i) + kHalf * D + kHalf + row);
-                        const float f = total > 0.f ? 1.f / total : total;
+                        const Joint both = joint(m, total);
+                        const float f = both.own;
 #pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
                             float y[32] = {};
+                            if constexpr (PREFIX) {
+                                if (both.prefix != 0.f)
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) {
+                                        const float4 x = prefix4(c + 4 * k);
+                                        y[4 * k] = x.x * both.prefix;
+                                        y[4 * k + 1] = x.y * both.prefix;
+                                        y[4 * k + 2] = x.z * both.prefix;
+                                        y[4 * k + 3] = x.w * both.prefix;
+                                    }
+                            }
 #pragma unroll 2
                             for (int i = 0; i < t.parts; ++i) {
                                 const float take = exp2_approx(__ldcg(part_at(i) + kHalf * D + row) - from) * f;
@@ -826,9 +862,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
     if (warp == kMma) ptx::tmem_dealloc(tmem, 512);
 }
 
-template <bool E4M3, bool BF16, int D>
+template <bool E4M3, bool BF16, int D, bool PREFIX>
 cudaError_t launch_prompt(const AttentionParams& p, int least_rows, bool alone, cudaStream_t stream) {
-    const auto kernel = cache_prompt_kernel<E4M3, BF16, D>;
+    const auto kernel = cache_prompt_kernel<E4M3, BF16, D, PREFIX>;
     constexpr int kSmem = Layout<D>::kBytes;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
@@ -854,7 +890,8 @@ size_t cache_prompt_workspace() { return (size_t)kPromptParts * 2 * Layout<128>:
 cudaError_t cache_prompt_launch(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, bool alone, cudaStream_t stream) {
     const auto by_dim = [&](auto e, auto h) {
         constexpr bool E = decltype(e)::value, H = decltype(h)::value;
-        return p.cache.dim == 128 ? launch_prompt<E, H, 128>(p, least_rows, alone, stream) : launch_prompt<E, H, 64>(p, least_rows, alone, stream);
+        if (p.prefix_of) return p.cache.dim == 128 ? launch_prompt<E, H, 128, true>(p, least_rows, alone, stream) : launch_prompt<E, H, 64, true>(p, least_rows, alone, stream);
+        return p.cache.dim == 128 ? launch_prompt<E, H, 128, false>(p, least_rows, alone, stream) : launch_prompt<E, H, 64, false>(p, least_rows, alone, stream);
     };
     const auto by_type = [&](auto e) { return bf16 ? by_dim(e, std::true_type{}) : by_dim(e, std::false_type{}); };
     return e4m3 ? by_type(std::true_type{}) : by_type(std::false_type{});

@@ -119,7 +119,8 @@ struct Piece {
     int b, segment, rows;                             // rows of its row tile
 };
 
-template <bool E4M3, bool BF16, int D, int NT>
+// PREFIX: a request's rows may have seen a shared prefix before its own tokens; what that came to is added at the end.
+template <bool E4M3, bool BF16, int D, int NT, bool PREFIX>
 __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(const AttentionParams p, int most_rows,
                                                                               const __grid_constant__ CUtensorMap k_map,
                                                                               const __grid_constant__ CUtensorMap v_map) {
@@ -529,6 +530,18 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                         if (row >= all_rows) continue;
                         const int token = row / p.group, h = head * p.group + row - token * p.group;
                         const long long to = ((long long)(r.row0 + token) * p.q_heads + h) * D + (D / 8) * g;
+                        if constexpr (PREFIX) {
+                            if (sees_prefix(p, b, r.position + token)) {
+                                const Joint f = join_prefix(m[n][i], sum[n][i], __ldcg(p.prefix_total + (long long)(r.row0 + token) * p.q_heads + h));
+#pragma unroll
+                                for (int j = 0; j < kWords; ++j) {
+                                    const float4 x = __ldcg(reinterpret_cast<const float4*>(p.prefix_sums + to + 4 * j));
+                                    store4<BF16>(p.out, to + 4 * j, fmaf(o[n][2 * j][i], f.own, x.x * f.prefix), fmaf(o[n][2 * j][2 + i], f.own, x.y * f.prefix),
+                                                 fmaf(o[n][2 * j + 1][i], f.own, x.z * f.prefix), fmaf(o[n][2 * j + 1][2 + i], f.own, x.w * f.prefix));
+                                }
+                                continue;
+                            }
+                        }
                         const float f = sum[n][i] > 0.f ? 1.f / sum[n][i] : sum[n][i];       // (a NaN stays one)
 #pragma unroll
                         for (int j = 0; j < kWords; ++j)
@@ -611,6 +624,18 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         const int count = row_tiles<S::kRows>(p, r), head = piece.segment / count, in = (piece.segment - head * count) * S::kRows + row;
         const int token = in / p.group, h = head * p.group + in - token * p.group;
         const long long to = ((long long)(r.row0 + token) * p.q_heads + h) * D + kMine * lane;
+        if constexpr (PREFIX) {
+            if (sees_prefix(p, piece.b, r.position + token)) {
+                const Joint f = join_prefix(a.m, a.sum, __ldcg(p.prefix_total + (long long)(r.row0 + token) * p.q_heads + h));
+                const float* const x = p.prefix_sums + to;
+                float y[kMine];
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) y[i] = fmaf(a.o[i], f.own, __ldcg(x + i) * f.prefix);
+                if constexpr (kMine == 4) store4<BF16>(p.out, to, y[0], y[1], y[2], y[3]);
+                else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + to) = pack_out<BF16>(y[0], y[1]);
+                return;
+            }
+        }
         const float f = a.sum > 0.f ? 1.f / a.sum : a.sum;
         if constexpr (kMine == 4) {
             store4<BF16>(p.out, to, a.o[0] * f, a.o[1] * f, a.o[2] * f, a.o[3] * f);
@@ -707,10 +732,10 @@ bool cache_map(CUtensorMap* out, const CacheView& c, bool keys) {
     });
 }
 
-template <bool E4M3, bool BF16, int D, int NT>
+template <bool E4M3, bool BF16, int D, int NT, bool PREFIX>
 cudaError_t launch_rows(const AttentionParams& p, int most_rows, cudaStream_t stream) {
     using S = Shape<D, NT>;
-    const auto kernel = cache_rows_kernel<E4M3, BF16, D, NT>;
+    const auto kernel = cache_rows_kernel<E4M3, BF16, D, NT, PREFIX>;
     constexpr int kSmem = S::kWarps * S::kWarpBytes + 1024;
     CUtensorMap k_map, v_map;
     if (!cache_map(&k_map, p.cache, true) || !cache_map(&v_map, p.cache, false)) return cudaErrorNotSupported;
@@ -740,7 +765,8 @@ cudaError_t cache_rows_launch(const AttentionParams& p, bool e4m3, bool bf16, in
     const auto by_rows = [&](auto e, auto h, auto d) {
         constexpr bool E = decltype(e)::value, H = decltype(h)::value;
         constexpr int D = decltype(d)::value;
-        return few ? launch_rows<E, H, D, 1>(p, most_rows, stream) : launch_rows<E, H, D, 2>(p, most_rows, stream);
+        if (p.prefix_of) return few ? launch_rows<E, H, D, 1, true>(p, most_rows, stream) : launch_rows<E, H, D, 2, true>(p, most_rows, stream);
+        return few ? launch_rows<E, H, D, 1, false>(p, most_rows, stream) : launch_rows<E, H, D, 2, false>(p, most_rows, stream);
     };
     const auto by_dim = [&](auto e, auto h) {
         return p.cache.dim == 128 ? by_rows(e, h, std::integral_constant<int, 128>{}) : by_rows(e, h, std::integral_constant<int, 64>{});

@@ -9,8 +9,7 @@
 // (4.2 TB/s; 1000 instructions for 16 rows), and 25 us (5.6 TB/s) for the reader; one token 3 and 2 us.
 #include <algorithm>
 
-#include "cache.cuh"
-#include "common.cuh"
+#include "cache_bytes.cuh"
 #include "ptx.cuh"
 
 namespace i4mm {
@@ -19,89 +18,6 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kHeld = 8;                              // rows (two at head_dim 128, four at 64) that a warp of the writer holds at once
 constexpr uint32_t kAll = 0xFFFFFFFFu;
-
-template <bool BF16>
-__device__ __forceinline__ void unpack8(uint4 w, float (&f)[8]) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (BF16) {
-            f[2 * i] = __uint_as_float(u[i] << 16);
-            f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-        } else {
-            const float2 h = __half22float2(u32_as_h2(u[i]));
-            f[2 * i] = h.x;
-            f[2 * i + 1] = h.y;
-        }
-    }
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if (BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return h2_as_u32(__floats2half2_rn(a, b));
-}
-
-// the byte nearest to f, |f| within the type's range but for infinities; NaN -> 0
-template <bool E4M3>
-__device__ __forceinline__ uint32_t to_byte(float f) {
-    constexpr float kMost = E4M3 ? 448.f : 127.f;
-    f = f != f ? 0.f : fminf(fmaxf(f, -kMost), kMost);
-    if (E4M3) return (uint32_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3);
-    return (uint32_t)__float2int_rn(f) & 0xFFu;
-}
-template <bool E4M3>
-__device__ __forceinline__ float from_byte(uint32_t b) {
-    if (E4M3) return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
-    return (float)(int)(signed char)b;
-}
-
-// 8 values times `inverse` as bytes, all of them within the type's range: int8 in the low bits of 1.5 * 2^23 + q, whose addition rounds to
-// nearest even (the product with a power of two is exact)
-template <bool E4M3>
-__device__ __forceinline__ uint2 to_bytes(const float (&f)[8], float inverse) {
-    uint32_t r[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const float* const g = f + 4 * h;
-        if (E4M3) {
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(g[0] * inverse, g[1] * inverse), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(g[2] * inverse, g[3] * inverse), __NV_SATFINITE, __NV_E4M3);
-            r[h] = lo | hi << 16;
-        } else {
-            uint32_t b[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = __float_as_uint(fmaf(g[j], inverse, 12582912.f));
-            r[h] = prmt(prmt(b[0], b[1], 0x0040), prmt(b[2], b[3], 0x0040), 0x5410);
-        }
-    }
-    return make_uint2(r[0], r[1]);
-}
-// the same of 8 packed 16-bit values, some of them infinite or NaN
-template <bool E4M3, bool BF16>
-__device__ __noinline__ uint2 to_bytes_any(uint4 w, float inverse) {
-    float f[8];
-    unpack8<BF16>(w, f);
-    uint32_t r[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) r[j >> 2] |= to_byte<E4M3>(f[j] * inverse) << (8 * (j & 3));
-    return make_uint2(r[0], r[1]);
-}
-
-// The least power of two s with a <= most * s (0 for a = 0).  With a in [2^e, 2^(e+1)): most = 127 = 1.984 * 2^6 and 448 = 1.75 * 2^8, so
-// s is 2^(e-6) (2^(e-8)) or the next one.  Not below 2^-100, so that 1 / s is a finite number whatever the input.
-template <bool E4M3>
-__device__ __forceinline__ float scale_for(float a) {
-    if (a == 0.f) return 0.f;
-    constexpr int kTop = E4M3 ? 8 : 6;
-    constexpr float kMost = E4M3 ? 448.f : 127.f;
-    const int e = max((int)(__float_as_uint(a) >> 23) - 127 - kTop, -100);   // (a subnormal a lies below the limit anyhow)
-    const float s = __uint_as_float((uint32_t)(e + 127) << 23);
-    return a > kMost * s ? 2.f * s : s;
-}
 
 // A warp takes one head's keys or values (2 * head + which) of the runs that begin in a window of `window` tokens (window <= 16), of every
 // gridDim.y-th of them; neighbouring blocks take the heads of the same tokens, which lie side by side in memory.  A run: neighbouring tokens with ascending slots of one page; it ends with the page, so it has at most 128 tokens.
@@ -264,22 +180,6 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheView c, uint
     }
 }
 
-template <typename F, typename... Args>
-cudaError_t launch(F* kernel, dim3 grid, int threads, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)threads, 1, 1);
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    if (e == cudaSuccess) count_launch();
-    return e;
-}
-
 }  // namespace
 
 cudaError_t cache_write_launch(const CacheView& c, bool e4m3, const RowsView& k, const RowsView& v, bool bf16, int tokens, const int* slots,
@@ -290,7 +190,7 @@ cudaError_t cache_write_launch(const CacheView& c, bool e4m3, const RowsView& k,
     const dim3 grid((unsigned)blocks, window > 1 ? 2 : 1, 1);
     const auto kernel = e4m3 ? (bf16 ? cache_write_kernel<true, true> : cache_write_kernel<true, false>)
                              : (bf16 ? cache_write_kernel<false, true> : cache_write_kernel<false, false>);
-    return launch(kernel, grid, kWarps * 32, stream, c, k, v, tokens, slots, window);
+    return launch_overlapping(kernel, grid, kWarps * 32, stream, c, k, v, tokens, slots, window);
 }
 
 cudaError_t cache_read_launch(const CacheView& c, bool e4m3, void* k_out, void* v_out, bool bf16, int tokens, const int* slots,
@@ -299,7 +199,7 @@ cudaError_t cache_read_launch(const CacheView& c, bool e4m3, void* k_out, void* 
     const int threads = std::min(256, std::max(32, (2 * c.heads * (c.dim >> 3) / 4 + 31) / 32 * 32));
     const auto kernel = e4m3 ? (bf16 ? cache_read_kernel<true, true> : cache_read_kernel<true, false>)
                              : (bf16 ? cache_read_kernel<false, true> : cache_read_kernel<false, false>);
-    return launch(kernel, dim3((unsigned)tokens, 1, 1), threads, stream, c, (uint4*)k_out, (uint4*)v_out, slots);
+    return launch_overlapping(kernel, dim3((unsigned)tokens, 1, 1), threads, stream, c, (uint4*)k_out, (uint4*)v_out, slots);
 }
 
 }  // namespace i4mm

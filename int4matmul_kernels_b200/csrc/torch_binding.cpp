@@ -468,6 +468,114 @@ int rows_type(const Tensor& t, const c10::Device& dev, int64_t dim) {
 
 cudaStream_t current_stream(const c10::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
+// `count` views of `sizes` entries each, one behind the other, of flat; made without a trip through the dispatcher (seven of those take longer than
+// a small kernel)
+py::tuple views_of(const Tensor& flat, const int64_t* sizes, int count) {
+    py::tuple out(count);
+    int64_t at = 0;
+    for (int i = 0; i < count; ++i) {
+        auto impl = c10::make_intrusive<at::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
+        impl->set_storage_offset(at);
+        impl->set_sizes_contiguous({sizes[i]});
+        out[i] = py::cast(Tensor(std::move(impl)));
+        at += sizes[i];
+    }
+    return out;
+}
+
+// cache.angles: the table, or a status / -1
+py::object try_cache_angles(const py::object& positions_, const py::object& freqs_) {
+    Tensor positions, freqs;
+    if (!as_tensor(positions_, positions) || !as_tensor(freqs_, freqs)) return py::int_(-1);
+    try {
+        if (!positions.is_cuda()) return py::int_(-1);
+        const auto dev = positions.device();
+        if (c10::cuda::current_device() != dev.index() || !ints1(positions, dev) || freqs.device() != dev || freqs.scalar_type() != torch::kFloat || freqs.dim() != 1 ||
+            !freqs.is_contiguous())
+            return py::int_(-1);
+        Tensor out = at::empty({positions.size(0), freqs.size(0), 2}, freqs.options());
+        const cudaStream_t stream = current_stream(dev);
+        int status;
+        {
+            py::gil_scoped_release release;
+            status = i4mm_cache_angles(out.data_ptr(), positions.data_ptr(), freqs.data_ptr(), positions.size(0), freqs.size(0), (void*)stream);
+        }
+        if (status != I4MM_OK) return py::int_(status);
+        return py::cast(out);
+    } catch (const c10::Error&) {
+        return py::int_(-1);
+    }
+}
+
+// cache.share: its four outputs, or a status / -1
+py::object try_cache_share(const py::object& of_, const py::object& seq_, const py::object& cu_, const py::object& tokens_) {
+    Tensor of, seq, cu;
+    int64_t tokens = 0;
+    if (!as_tensor(of_, of) || !as_tensor(seq_, seq) || !as_tensor(cu_, cu) || !as_int(tokens_, tokens)) return py::int_(-1);
+    try {
+        if (!seq.is_cuda()) return py::int_(-1);
+        const auto dev = seq.device();
+        if (c10::cuda::current_device() != dev.index() || !ints1(of, dev) || !ints1(seq, dev) || !ints1(cu, dev) || tokens < 0 || tokens > (1 << 30)) return py::int_(-1);
+        const int64_t n = seq.size(0);
+        if (of.size(0) != n || cu.size(0) != n + 1) return py::int_(-1);
+        const int64_t sizes[4] = {n, n + 1, tokens, tokens};
+        const Tensor flat = at::empty({n + n + 1 + 2 * tokens}, at::TensorOptions().dtype(torch::kInt).device(dev));
+        int* const base = flat.data_ptr<int>();
+        const cudaStream_t stream = current_stream(dev);
+        int status;
+        {
+            py::gil_scoped_release release;
+            status = i4mm_cache_share(n, of.data_ptr(), seq.data_ptr(), cu.data_ptr(), tokens, base, base + n, base + 2 * n + 1, base + 2 * n + 1 + tokens, (void*)stream);
+        }
+        if (status != I4MM_OK) return py::int_(status);
+        return views_of(flat, sizes, 4);
+    } catch (const c10::Error&) {
+        return py::int_(-1);
+    }
+}
+
+// cache.append: the queries, or a status / -1
+py::object try_cache_append(const py::object& kc_, const py::object& vc_, const py::object& scales_, const py::object& q_, const py::object& k_, const py::object& v_,
+                            const py::object& slots_, const py::object& angles_, const py::object& qw_, const py::object& kw_, const py::object& eps_,
+                            const py::object& beside_) {
+    Tensor kc, vc, scales, q, k, v, slots, angles, qw, kw;
+    i4mm_cache c{};
+    if (!as_tensor(kc_, kc) || !as_tensor(vc_, vc) || !as_tensor(scales_, scales) || !as_tensor(q_, q) || !as_tensor(k_, k) || !as_tensor(v_, v) ||
+        !as_tensor(slots_, slots) || !as_optional_tensor(angles_, angles) || !as_optional_tensor(qw_, qw) || !as_optional_tensor(kw_, kw) || !PyFloat_Check(eps_.ptr()) ||
+        !PyBool_Check(beside_.ptr()))
+        return py::int_(-1);
+    try {
+        if (!cache_view(kc, vc, scales, c)) return py::int_(-1);
+        const auto dev = kc.device();
+        const int type = rows_type(k, dev, c.head_dim);
+        const int64_t tokens = k.size(0);
+        if (type < 0 || rows_type(v, dev, c.head_dim) != type || v.sizes() != k.sizes() || k.size(1) != c.heads || rows_type(q, dev, c.head_dim) != type ||
+            q.size(0) != tokens || !ints1(slots, dev) || slots.size(0) < tokens || c10::cuda::current_device() != dev.index())
+            return py::int_(-1);
+        if (angles.defined() && (angles.device() != dev || angles.scalar_type() != torch::kFloat || angles.dim() != 3 || angles.size(0) < tokens ||
+                                 angles.size(2) != 2 || !angles.is_contiguous()))
+            return py::int_(-1);
+        if (!angles.defined() && !qw.defined() && !kw.defined()) return py::int_(-1);
+        for (const Tensor* w : {&qw, &kw})
+            if (w->defined() && (w->device() != dev || w->scalar_type() != k.scalar_type() || w->dim() != 1 || w->size(0) != c.head_dim || !w->is_contiguous()))
+                return py::int_(-1);
+        Tensor out = at::empty({tokens, q.size(1), c.head_dim}, q.options());
+        const cudaStream_t stream = current_stream(dev);
+        int status;
+        {
+            py::gil_scoped_release release;
+            status = i4mm_cache_append(&c, out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), type, tokens, q.size(1), q.stride(0), q.stride(1), k.stride(0),
+                                       k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), angles.defined() ? angles.data_ptr() : nullptr,
+                                       angles.defined() ? angles.size(1) : 0, beside_.ptr() == Py_True, qw.defined() ? qw.data_ptr() : nullptr,
+                                       kw.defined() ? kw.data_ptr() : nullptr, (float)PyFloat_AS_DOUBLE(eps_.ptr()), (void*)stream);
+        }
+        if (status != I4MM_OK) return py::int_(status);
+        return py::cast(out);
+    } catch (const c10::Error&) {
+        return py::int_(-1);
+    }
+}
+
 // cache.plan: the seven outputs, or a status / -1
 py::object try_cache_plan(const py::object& seq_, const py::object& new_, const py::object& table_, const py::object& free_, const py::object& count_,
                           const py::object& page_, const py::object& tokens_) {
@@ -500,15 +608,7 @@ py::object try_cache_plan(const py::object& seq_, const py::object& new_, const 
                                      count.data_ptr(), page, tokens, base + at[0], base + at[1], base + at[2], base + at[3], base + at[4], base + at[5], (void*)stream);
         }
         if (status != I4MM_OK) return py::int_(status);
-        py::tuple out(7);
-        for (int i = 0; i < 7; ++i) {
-            // a view of `flat`, made without a trip through the dispatcher (seven of those take longer than the kernel)
-            auto impl = c10::make_intrusive<at::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
-            impl->set_storage_offset(at[i]);
-            impl->set_sizes_contiguous({sizes[i]});
-            out[i] = py::cast(Tensor(std::move(impl)));
-        }
-        return out;
+        return views_of(flat, sizes, 7);
     } catch (const c10::Error&) {
         return py::int_(-1);
     }
@@ -561,13 +661,18 @@ py::object try_cache_read(const py::object& kc_, const py::object& vc_, const py
 // cache.attention (`scale` None: 1 / sqrt(head_dim)): the output, or a status / -1
 py::object try_cache_attention(const py::object& q_, const py::object& kc_, const py::object& vc_, const py::object& scales_, const py::object& table_,
                                const py::object& seq_, const py::object& cu_, const py::object& longest_, const py::object& scale_, const py::object& window_,
-                               const py::dict& workspaces) {
-    Tensor q, kc, vc, scales, table, seq, cu;
+                               const py::object& shared_, const py::dict& workspaces) {
+    Tensor q, kc, vc, scales, table, seq, cu, of, starts, rows;
     int64_t longest = 0, window = 0, stride = 0;
     i4mm_cache c{};
     if (!as_tensor(q_, q) || !as_tensor(kc_, kc) || !as_tensor(vc_, vc) || !as_tensor(scales_, scales) || !as_tensor(table_, table) || !as_tensor(seq_, seq) ||
         !as_optional_tensor(cu_, cu) || !as_int(longest_, longest) || !as_int(window_, window) || !(scale_.is_none() || PyFloat_Check(scale_.ptr())))
         return py::int_(-1);
+    if (!shared_.is_none()) {
+        if (!PyTuple_Check(shared_.ptr()) || PyTuple_GET_SIZE(shared_.ptr()) != 4) return py::int_(-1);
+        const auto item = [&](int i) { return py::reinterpret_borrow<py::object>(PyTuple_GET_ITEM(shared_.ptr(), i)); };
+        if (!as_tensor(item(0), of) || !as_tensor(item(1), starts) || !as_tensor(item(2), rows)) return py::int_(-1);
+    }
     try {
         if (!cache_view(kc, vc, scales, c)) return py::int_(-1);
         const auto dev = kc.device();
@@ -576,17 +681,28 @@ py::object try_cache_attention(const py::object& q_, const py::object& kc_, cons
             window < 0 || c10::cuda::current_device() != dev.index())
             return py::int_(-1);
         if (cu.defined() ? !ints1(cu, dev) || cu.size(0) != seq.size(0) + 1 : q.size(0) < seq.size(0)) return py::int_(-1);
+        if (of.defined() && (!ints1(of, dev) || of.size(0) != seq.size(0) || !ints1(starts, dev) || starts.size(0) != seq.size(0) + 1 || !ints1(rows, dev) ||
+                             rows.size(0) < q.size(0)))
+            return py::int_(-1);
         const cudaStream_t stream = current_stream(dev);
         const Tensor ws = scratch(workspaces, dev, stream);
         if (!ws.defined()) return py::int_(-1);
         const float scale = scale_.is_none() ? (float)(1.0 / std::sqrt((double)c.head_dim)) : (float)PyFloat_AS_DOUBLE(scale_.ptr());
-        Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+        Tensor out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options()), room;
+        if (of.defined())
+            room = at::empty({(int64_t)i4mm_cache_shared_scratch_bytes(q.size(0), q.size(1), q.size(2))}, at::TensorOptions().dtype(torch::kByte).device(dev));
         int status;
         {
             py::gil_scoped_release release;
-            status = i4mm_cache_attention(&c, out.data_ptr(), q.data_ptr(), type, q.size(0), q.size(1), q.stride(0), q.stride(1), table.data_ptr(), table.size(1), stride,
-                                          seq.data_ptr(), cu.defined() ? cu.data_ptr() : nullptr, seq.size(0), longest, scale, window, ws.data_ptr(),
-                                          (size_t)ws.numel(), (void*)stream);
+            if (of.defined())
+                status = i4mm_cache_attention_shared(&c, out.data_ptr(), q.data_ptr(), type, q.size(0), q.size(1), q.stride(0), q.stride(1), table.data_ptr(),
+                                                     table.size(1), stride, seq.data_ptr(), cu.defined() ? cu.data_ptr() : nullptr, seq.size(0), longest, scale,
+                                                     window, of.data_ptr(), starts.data_ptr(), rows.data_ptr(), rows.size(0), room.data_ptr(),
+                                                     (size_t)room.numel(), ws.data_ptr(), (size_t)ws.numel(), (void*)stream);
+            else
+                status = i4mm_cache_attention(&c, out.data_ptr(), q.data_ptr(), type, q.size(0), q.size(1), q.stride(0), q.stride(1), table.data_ptr(), table.size(1),
+                                              stride, seq.data_ptr(), cu.defined() ? cu.data_ptr() : nullptr, seq.size(0), longest, scale, window, ws.data_ptr(),
+                                              (size_t)ws.numel(), (void*)stream);
         }
         if (status != I4MM_OK) return py::int_(status);
         return py::cast(out);
@@ -635,6 +751,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("_try_cache_plan", &try_cache_plan, "cache.plan for arguments that pass its checks: outputs, a status or -1");
     m.def("_try_cache_write", &try_cache_write, "cache.write for arguments that pass its checks: a status or -1");
     m.def("_try_cache_read", &try_cache_read, "cache.read for arguments that pass its checks: (k, v), a status or -1");
+    m.def("_try_cache_angles", &try_cache_angles, "cache.angles for arguments that pass its checks: the table, a status or -1");
+    m.def("_try_cache_share", &try_cache_share, "cache.share for arguments that pass its checks: outputs, a status or -1");
+    m.def("_try_cache_append", &try_cache_append, "cache.append for arguments that pass its checks: the queries, a status or -1");
     m.def("_try_cache_attention", &try_cache_attention, "cache.attention for arguments that pass its checks: output, a status or -1");
 
     m.def("weight_matrix_packing", &weight_matrix_packing, "int4_sparse_pack");
