@@ -48,7 +48,7 @@ struct AttentionParams {
     const int* seq_lens;
     const int* cu_lens;                               // or nullptr: one row for each request
     void* workspace;
-    size_t prompt_parts;                              // where in it the prompt kernel's parts lie
+    size_t prompt_parts, prefix_parts;                // where in it the prompt kernel's and the prefix kernel's parts lie
     long long table_stride;
     int table_width, requests, tokens, q_heads, group; // group = q_heads / cache.heads
     int window;                                       // 0: none

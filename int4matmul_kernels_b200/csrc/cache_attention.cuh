@@ -6,6 +6,7 @@
 #include "cache.cuh"
 #include "common.cuh"
 #include "ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace i4mm {
 
@@ -26,6 +27,10 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int 
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
                  ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
 // D[tmem] (+)= A[smem descriptor] * B[smem descriptor]; kind::f16; one thread issues
 __device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -45,6 +50,7 @@ constexpr size_t kRowsCounters = 0;                   // one per block
 constexpr size_t kPromptNext = 4096;                  // the next item to be worked on
 constexpr size_t kPromptCounters = 8192;              // two per part
 constexpr int kPromptParts = 320;
+constexpr size_t kPrefixCounters = 16384;             // two per block
 
 struct Request {
     int row0, rows;                                   // its packed rows
@@ -180,6 +186,20 @@ __device__ __forceinline__ Joint join_prefix(float m, float sum, float2 prefix) 
 // whether a row of request b at this position sees a prefix
 __device__ __forceinline__ bool sees_prefix(const AttentionParams& p, int b, int position) { return position >= 0 && p.prefix_of[b] >= 0; }
 
+// the cache's keys or values as (dim, token, head, page), read 16 tokens at a time in rows whose 16-byte chunks are swizzled
+inline bool cache_map(CUtensorMap* out, const CacheView& c, bool keys) {
+    const EncodeTiledFn encode = encode_tiled_fn();
+    if (!encode) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.dim, 1ull << c.page_shift, (cuuint64_t)c.heads, (cuuint64_t)c.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)(keys ? c.k_token : c.v_token), (cuuint64_t)(keys ? c.k_head : c.v_head), (cuuint64_t)(keys ? c.k_page : c.v_page)};
+    const cuuint32_t box[4] = {(cuuint32_t)c.dim, 16, 1, 1}, steps[4] = {1, 1, 1, 1};
+    return encode_with_context([&] {
+        return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, keys ? c.k : c.v, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      c.dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
+}
+
 // The two kernels.  Few rows: requests of more than most_rows rows are left to the other one; `few`: no request has more than 8.
 // Prompts: requests of fewer than least_rows rows are left to the other one; `alone`: it is not launched.
 // With p.prefix_of set, both add what p.prefix_total and p.prefix_sums say to each row that has a prefix.
@@ -189,5 +209,6 @@ cudaError_t cache_prompt_launch(const AttentionParams& p, bool e4m3, bool bf16, 
 cudaError_t cache_prefix_launch(const AttentionParams& p, bool e4m3, bool bf16, cudaStream_t stream);
 size_t cache_rows_workspace();                        // bytes behind the header
 size_t cache_prompt_workspace();                      // bytes behind those
+size_t cache_prefix_workspace();                      // and behind those
 
 }  // namespace i4mm

@@ -72,7 +72,7 @@ int view_of(const i4mm_cache* c, i4mm::CacheView& w) {
 
 thread_local int g_attention_kernels = 0;             // i4mm_last_attention_kernels
 
-size_t attention_workspace() { return i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace() + i4mm::cache_prompt_workspace(); }
+size_t attention_workspace() { return i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace() + i4mm::cache_prompt_workspace() + i4mm::cache_prefix_workspace(); }
 
 // Which kernel.  A request's rows are its new tokens times the query heads of a key head.  The few-row kernel takes 8 or 16 of them at a time
 // and reads the cache again (from the second-level cache) for the next ones, the prompt kernel works on 256 whatever they are: 16 requests of one
@@ -155,6 +155,7 @@ int attention(const i4mm_cache* cache, void* out, const void* q, int type, int64
     p.cu_lens = (const int*)cu_lens;
     p.workspace = workspace;
     p.prompt_parts = i4mm::kCacheHeaderBytes + i4mm::cache_rows_workspace();
+    p.prefix_parts = p.prompt_parts + i4mm::cache_prompt_workspace();
     p.table_stride = table_stride;
     p.table_width = (int)table_width;
     p.requests = (int)requests;

@@ -1,85 +1,849 @@
 // Attention of all rows that read a shared prefix over that prefix (the first half of i4mm_cache_attention_shared).
 //
-//   m = max_j s_j,  total = sum_j 2^(s_j - m),  sums = sum_j 2^(s_j - m) v_j,  s_j = log2(e) * scale * q . k_j, over the prefix's tokens that the row sees
-// Simplest form: a warp for a row and head, a token to a lane.
+//   x_j = log2(e) * scale * s_key * (q . k_j) + log2(s_value),  P_j = 2^(x_j - M)   (fp16), with a reference M, an x_j of the row,
+//   total = sum_j P_j / s_value,  sums = sum_j P_j v_j      over the prefix's tokens that the row sees, k_j and v_j the cache's bytes
+// M, total and sums of each row are what the kernel of its own tokens adds to its own.
+//
+// The rows of all readers of a place, times the query heads of a key head, are the rows of a tile, up to 128 of them.  With 16 to 128 rows for each byte,
+// DRAM bounds it up to about 64 rows (a tile of 128 tokens is 32 KB, 1400 cycles of an SM's share of DRAM) and the tensor cores and exponentials
+// above, so tokens are the 128 rows of both products and the readers their columns, as many as there are:
+//
+//   S^T = K Q^T      K: bytes -> fp16 -> tensor memory, a thread a token (no trip through shared memory, no transposition); Q: shared memory
+//   O^T = V^T P^T    V: bytes -> fp16 -> shared memory as they lie (dim fastest); P: shared memory, a thread a token
+// A thread of the softmax has one token, so a page's scales are its constants; it keeps its part of each row's total in a register, and nothing is summed
+// over threads until the end.  The largest score is looked for only where a weight would exceed 2^14: then sums follow to a new reference.
+//
+//   warps 0..3, 4..7   softmax of the first and of the second half of the rows
+//   warps 8..11        the rows' queries; bytes to operands
+//   warp 12            issues the products
+//   warp 13            deals out the work, fetches pages (a TMA copy for each 16 keys or values) into a ring of 7 half tiles
+//
+// The tiles of all segments (place, key head, 128 rows) in a row are dealt out in equal contiguous ranges to the blocks.  What a range cuts goes through the
+// workspace, and the block that comes last adds the parts in their order.  Nobody waits for another block.  Waits are bounded: a warp that gives up
+// sets the abort flag, which ends every other wait of the block, and the status word.
+#include <algorithm>
+#include <type_traits>
+
 #include "cache_attention.cuh"
-#include "cache_bytes.cuh"
 
 namespace i4mm {
 namespace {
 
+constexpr int kTokens = 128;                          // of a tile
+constexpr int kMostRows = 128;
+constexpr int kSoftmaxWarps = 8, kDecode0 = 8, kDecodeWarps = 4, kMma = 12, kCopy = 13, kThreads = 14 * 32;
+constexpr int kRing = 7;                              // half tiles: keys, values
+constexpr int kItems = 4, kScales = 4, kRawScales = 8;
+constexpr int kPieces = kTokens / 16;
+constexpr int kMinBlockTiles = 2;                     // fewer tiles than this are not cut further
+constexpr float kNone = -3e38f;                       // a reference below any score
+constexpr float kMostLog = 14.f;                      // fp16 holds 2^16
+constexpr uint32_t kNoPage = 0x7FC0DEADu;             // in the place of a scale: there is no such page
+constexpr uint32_t kMnStride = 16384;                 // 128 tokens of 64 columns
+
+template <int D>
+struct Layout {
+    static constexpr int kHalf = kTokens * D;                                 // bytes of a tile's keys or values
+    static constexpr int kV = 2 * kMnStride, kP = 2 * kMnStride, kQ = kMostRows * D * 2;
+    static constexpr int kV0 = 0, kP0 = kV0 + kV, kQ0 = kP0 + kP, kRing0 = kQ0 + kQ, kBytes = kRing0 + kRing * kHalf + 1024;
+    static constexpr int kPartFloats = kMostRows * D + 2 * kMostRows;         // sums [row][dim], references, totals
+};
+constexpr size_t kPartsBytes = (size_t)kMaxBlocks * 2 * Layout<128>::kPartFloats * 4;
+
+struct Item {
+    int valid, place, head, base, rows, n;            // base: first row of the tile; n: rows, rounded up to 16
+    int first;                                        // of the place's readers in the list
+    int lo, limit;                                    // tokens that may be seen
+    int tile0, tiles;
+    int first_block, last_block;                      // that have a part of its segment; one alone: the item is all of it
+};
+
+struct Barriers {
+    unsigned long long item_full[kItems], item_empty[kItems], q_full[kItems], full[kRing], empty[kRing], scale_full[kScales];
+    unsigned long long k_full[2], s_full[2], p_full[2], pv_done[2], v_full, drained;
+};
+
+// A whole warp waits; false (in all of its lanes) once the block gives up.
+__device__ __forceinline__ bool wait_on(unsigned long long* bar, uint32_t parity, volatile int* abort) {
+    const uint32_t at = ptx::smem_u32(bar);
+    for (uint32_t i = 0; i < ptx::kSpinLimit; ++i) {
+        if (__all_sync(kAll, ptx::mbar_try_wait(at, parity & 1))) return true;
+        if (__any_sync(kAll, *abort)) return false;
+    }
+    *abort = 1;
+    return false;
+}
+__device__ __forceinline__ void arrive(unsigned long long* bar) { ptx::mbar_arrive(ptx::smem_u32(bar)); }
+
+// ---- work ----------------------------------------------------------------------------------------------------------------------
+struct Place {
+    int first;                                        // of its readers in the list
+    long long rows;                                   // readers times query heads of a key head
+    int lo, limit, tiles;                             // tokens that any row sees; at least one tile, so that all rows are written
+    long long row_tiles;
+    int height;                                       // rows of a row tile: all of a place alike
+};
+__device__ __forceinline__ Place load_place(const AttentionParams& p, int b) {
+    Place r;
+    const int from = min(max(p.prefix_starts[b], 0), p.prefix_listed), to = min(max(p.prefix_starts[b + 1], 0), p.prefix_listed), seq = p.seq_lens[b];
+    r.first = from;
+    r.rows = (long long)max(to - from, 0) * p.group;
+    r.limit = max(min(seq, p.table_width << p.cache.page_shift), 0);
+    r.lo = p.window && seq >= p.window ? min(seq - p.window + 1, r.limit) : 0;
+    r.tiles = max((r.limit + kTokens - 1) / kTokens - r.lo / kTokens, 1);
+    r.row_tiles = (r.rows + kMostRows - 1) / kMostRows;
+    r.height = r.rows == 0 ? 0 : (int)((r.rows + 16 * r.row_tiles - 1) / (16 * r.row_tiles)) * 16;
+    return r;
+}
+__device__ __forceinline__ long long units_of(const AttentionParams& p, const Place& r) { return r.row_tiles * p.cache.heads * r.tiles; }
+
+// ---- two fp32 at a time ----
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 32 values of each lane -> lane l has the result over all lanes of value l
+template <int DISTANCE, typename F>
+__device__ __forceinline__ void reduce_step(float (&x)[32], F op) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < DISTANCE; ++i) {
+        const float send = lane & DISTANCE ? x[i] : x[i + DISTANCE], keep = lane & DISTANCE ? x[i + DISTANCE] : x[i];
+        x[i] = op(keep, __shfl_xor_sync(kAll, send, DISTANCE));
+    }
+}
+template <typename F>
+__device__ __forceinline__ float reduce32(float (&x)[32], F op) {
+    reduce_step<16>(x, op);
+    reduce_step<8>(x, op);
+    reduce_step<4>(x, op);
+    reduce_step<2>(x, op);
+    reduce_step<1>(x, op);
+    return x[0];
+}
+
+// address of 16 bytes (8 values) `unit` of `row` in Q: sub-tiles of 64 values, 128-byte rows, swizzled
+__device__ __forceinline__ uint32_t swizzled(uint32_t tile, int row, int unit) {
+    return tile + (unit >> 3) * (kMostRows * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
+}
+// address of 8 columns `unit` of `token` in V or P: blocks of 64 columns, 128-byte rows, swizzled
+__device__ __forceinline__ uint32_t swizzled_mn(uint32_t tile, int token, int unit) {
+    return tile + (unit >> 3) * kMnStride + token * 128 + (((unit & 7) ^ (token & 7)) << 4);
+}
+// Matrix descriptor of such an operand: its columns are the M or N of a product, its tokens the K.  8 tokens 1024 bytes apart, blocks of 64 columns kMnStride
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kMnStride >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+constexpr uint32_t kBothMn = (1u << 15) | (1u << 16); // of an instruction descriptor: A and B lie so
+
 template <bool E4M3, bool BF16, int D>
-__global__ void __launch_bounds__(256) cache_prefix_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const AttentionParams p, const __grid_constant__ CUtensorMap k_map,
+                                                                   const __grid_constant__ CUtensorMap v_map) {
+    using L = Layout<D>;
+    extern __shared__ uint8_t dynamic[];
+    __shared__ Barriers bars;
+    __shared__ Item items[kItems];
+    __shared__ float2 s_raw[kRawScales][kPieces];
+    __shared__ float4 s_scale[kScales][kPieces];      // key scale, log2 of the value scale, its inverse, whether there is such a page
+    __shared__ int s_row[kItems][kMostRows];          // packed row times query heads plus head; -1: none
+    __shared__ int s_low[kItems][kMostRows];          // the first token that the row sees
+    __shared__ float s_up[kItems][kMostRows];         // what its scores are multiplied with (bf16)
+    __shared__ int s_most_low[kItems];
+    __shared__ __align__(16) float s_minus_top[2][kMostRows / 2];             // the rows' references, their signs turned over
+    __shared__ __align__(16) float s_keep[2][kMostRows / 2];
+    __shared__ float s_warps[2][4][kMostRows / 2];
+    __shared__ volatile uint32_t s_need[2][2];
+    __shared__ volatile int s_abort, s_last[2];
+    __shared__ uint32_t tmem_smem;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t smem = (ptx::smem_u32(dynamic) + 1023u) & ~1023u;
+    const uint32_t q_tile = smem + L::kQ0, v_tile = smem + L::kV0, p_tile = smem + L::kP0, ring = smem + L::kRing0;
+    uint8_t* const header = static_cast<uint8_t*>(p.workspace);
+    const CacheView& cache = p.cache;
+
+    if (threadIdx.x == 0) {
+        const auto init = [](unsigned long long& b, uint32_t n) { ptx::mbar_init(ptx::smem_u32(&b), n); };
+        for (int i = 0; i < kItems; ++i) {
+            init(bars.item_full[i], 1);
+            init(bars.item_empty[i], kSoftmaxWarps + kDecodeWarps + 1);
+            init(bars.q_full[i], kDecodeWarps);
+        }
+        for (int i = 0; i < kRing; ++i) {
+            init(bars.full[i], 2 * kPieces);
+            init(bars.empty[i], kDecodeWarps);
+        }
+        for (int i = 0; i < kScales; ++i) init(bars.scale_full[i], 1);
+        for (int i = 0; i < 2; ++i) {
+            init(bars.k_full[i], kDecodeWarps);
+            init(bars.s_full[i], 1);
+            init(bars.p_full[i], kSoftmaxWarps);
+            init(bars.pv_done[i], 1);
+        }
+        init(bars.v_full, kDecodeWarps);
+        init(bars.drained, 1);
+        ptx::fence_mbar_init();
+        s_abort = 0;
+        for (int i = 0; i < 4; ++i) s_need[i >> 1][i & 1] = 0;
+    }
+    if (D == 64)                                      // the columns of V that there are not
+        for (int i = threadIdx.x; i < (int)kMnStride / 16; i += kThreads) ptx::sts128(v_tile + kMnStride + 16 * i, make_uint4(0, 0, 0, 0));
+    ptx::fence_proxy_async_smem();
+    if (warp == kMma) {
+        ptx::tmem_alloc(ptx::smem_u32(&tmem_smem), 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = tmem_smem;
+    const auto s_col = [&](uint32_t g) { return tmem + (g & 1) * 128; };
+    const uint32_t o_col = tmem + 256;
+    const auto k_col = [&](uint32_t g) { return tmem + 384 + (g & 1) * 64; };
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const CacheView& c = p.cache;
-    const int page_mask = (1 << c.page_shift) - 1;
-    const long long units = (long long)min(max(p.prefix_starts[p.requests], 0), p.prefix_listed) * p.q_heads;
-    for (long long u = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (long long)gridDim.x * 8) {
-        const int entry = (int)(u / p.q_heads), h = (int)(u - (long long)entry * p.q_heads), head = h / p.group, t = p.prefix_rows[entry];
-        if (t < 0 || t >= p.tokens) continue;
-        const auto owner = [&](const int* sums, int x) {
-            int lo = 0, hi = p.requests - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (sums[mid] <= x) lo = mid;
-                else hi = mid - 1;
-            }
-            return lo;
-        };
-        const int place = owner(p.prefix_starts, entry), b = p.cu_lens ? owner(p.cu_lens, t) : t;
-        const int length = min(p.seq_lens[place], p.table_width << c.page_shift);
-        const long long position = (long long)p.seq_lens[place] + p.seq_lens[b] - (p.cu_lens ? p.cu_lens[b + 1] : t + 1) + t;
-        const int lo = p.window ? (int)min(max(position - p.window + 1, 0ll), (long long)max(length, 0)) : 0;
-        const uint16_t* const q = static_cast<const uint16_t*>(p.q.p) + t * p.q.token + h * p.q.head;
-        float m = -INFINITY, total = 0.f, o[D / 32] = {};
-        for (int base = lo; base < length; base += 32) {
-            const int j = base + lane;
-            const int id = j < length ? p.table[place * p.table_stride + (j >> c.page_shift)] : -1;
-            const bool there = id >= 0 && id < c.pages;
-            float s = -INFINITY, v_scale = 0.f;
-            if (there) {
-                const uint8_t* const k = c.k + id * c.k_page + head * c.k_head + (j & page_mask) * c.k_token;
-                const float2 scales = c.scales[(long long)id * c.heads + head];
-                float dot = 0.f;
-                for (int d = 0; d < D; d += 8) {
-                    float f[8];
-                    unpack8<BF16>(*reinterpret_cast<const uint4*>(q + d), f);
-                    for (int i = 0; i < 8; ++i) dot = fmaf(f[i], from_byte<E4M3>(k[d + i]), dot);
-                }
-                s = dot * scales.x * (p.scale * kLog2e);
-                v_scale = scales.y;
-            }
-            float top = s;
-            for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(kAll, top, d));
-            const float next = fmaxf(m, top), from = next == -INFINITY ? 0.f : next, keep = m == -INFINITY ? 0.f : exp2f(m - next), e = exp2f(s - from);
-            m = next;
-            float sum = e;
-            for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(kAll, sum, d);
-            total = total * keep + sum;
-            for (int i = 0; i < D / 32; ++i) o[i] *= keep;
-            for (int l = 0; l < 32; ++l) {
-                const int at = __shfl_sync(kAll, there ? id : -1, l);
-                const float w = __shfl_sync(kAll, e * v_scale, l);
-                if (at < 0) continue;
-                const uint8_t* const v = c.v + at * c.v_page + head * c.v_head + ((base + l) & page_mask) * c.v_token + lane * (D / 32);
-                for (int i = 0; i < D / 32; ++i) o[i] = fmaf(w, from_byte<E4M3>(v[i]), o[i]);
-            }
+
+    // Named barriers among four warps.  One that gives up arrives once more as it leaves (s_abort is set by then), which lets the others through to see it.
+    const auto meet = [&](int id) -> bool {
+        ptx::named_bar_sync(id, 128);
+        return !__any_sync(kAll, s_abort);
+    };
+    const auto leave = [&](int id) { ptx::named_bar_arrive(id, 128); };
+    const auto done_with_item = [&](uint32_t n) {
+        __syncwarp();
+        if (lane == 0) arrive(&bars.item_empty[n % kItems]);
+    };
+    const auto next_item = [&](uint32_t n) { return wait_on(&bars.item_full[n % kItems], n / kItems, &s_abort); };
+    if (warp == kCopy) {
+        // the block's range
+        long long total = 0, at = 0, end = 0;
+        for (int b = lane; b < p.requests; b += 32) total += units_of(p, load_place(p, b));
+        total = warp_sum(total);
+        const int blocks = (int)min((long long)gridDim.x, (total + kMinBlockTiles - 1) / kMinBlockTiles);
+        if ((int)blockIdx.x < blocks) {
+            at = range_lo(total, blocks, blockIdx.x);
+            end = range_lo(total, blocks, blockIdx.x + 1);
         }
-        const long long row = (long long)t * p.q_heads + h;
-        if (lane == 0) p.prefix_total[row] = make_float2(m, total);
-        for (int i = 0; i < D / 32; ++i) p.prefix_sums[row * D + lane * (D / 32) + i] = o[i];
+        // the place that the range begins in
+        long long before = 0;
+        int b = 0;
+        Place r{};
+        const auto find_place = [&]() {               // from request b (a multiple of 32) on, `before` tiles before it
+            for (; b < p.requests; b += 32) {
+                const Place mine = b + lane < p.requests ? load_place(p, b + lane) : Place{};
+                const long long own = b + lane < p.requests ? units_of(p, mine) : 0, upto = warp_prefix(own);
+                const uint32_t here = __ballot_sync(kAll, before + upto > at);
+                if (here) {
+                    const int l = __ffs(here) - 1;
+                    before += __shfl_sync(kAll, upto - own, l);
+                    b += l;
+                    r = load_place(p, b);
+                    return;
+                }
+                before += __shfl_sync(kAll, upto, 31);
+            }
+        };
+        uint32_t n = 0, half = 0, g = 0;              // items, half tiles, tiles so far
+        bool ok = true;
+        int page = -1;
+        const int page_mask = (1 << cache.page_shift) - 1;
+        while (ok && at < end) {
+            if (n == 0 || at >= before + units_of(p, r)) {
+                // (the next place with rows: from the multiple of 32 at or below the current one, whose earlier tiles are counted again)
+                if (n > 0) {
+                    before += units_of(p, r);
+                    ++b;
+                    for (; b < p.requests && (b & 31); ++b) {
+                        r = load_place(p, b);
+                        if (r.rows > 0) break;
+                    }
+                    if (b < p.requests && !(b & 31)) find_place();
+                } else {
+                    find_place();
+                }
+                if (b >= p.requests) break;           // (not unless the lengths change under the kernel)
+            }
+            Item t;
+            {
+                const long long in = at - before, segment = div_nn(in, r.tiles), per_head = r.row_tiles;
+                const int tile = (int)(in - segment * r.tiles);
+                const long long head = div_nn(segment, per_head), row_tile = segment - head * per_head;
+                t.valid = 1;
+                t.place = b;
+                t.head = (int)head;
+                t.base = (int)(row_tile * r.height);
+                t.rows = (int)max(min((long long)r.height, r.rows - row_tile * r.height), 0ll);
+                t.n = max((t.rows + 15) & ~15, 16);
+                t.first = r.first;
+                t.lo = r.lo;
+                t.limit = r.limit;
+                t.tile0 = r.lo / kTokens + tile;
+                t.tiles = (int)min((long long)(r.tiles - tile), end - at);
+                const long long from = before + segment * r.tiles;
+                t.first_block = range_owner(total, blocks, from);
+                t.last_block = range_owner(total, blocks, from + r.tiles - 1);
+            }
+            ok = wait_on(&bars.item_empty[n % kItems], (n / kItems) ^ 1, &s_abort);
+            if (!ok) break;
+            if (lane == 0) {
+                items[n % kItems] = t;
+                arrive(&bars.item_full[n % kItems]);
+            }
+            __syncwarp();
+            ++n;
+            const int* const table = p.table + t.place * p.table_stride;
+            const auto find_page = [&](int j) {       // lane l: of tokens 16 * l of the tile
+                const int token = (t.tile0 + j) * kTokens + 16 * (lane & 7), i = token >> cache.page_shift;
+                page = -1;
+                if (token < t.limit && token + 16 > t.lo && i < p.table_width) page = table[i];
+            };
+            find_page(0);
+            for (int j = 0; j < t.tiles && ok; ++j, ++g) {
+                const int id = (unsigned int)page < (unsigned int)cache.pages ? page : -1;
+                if (j + 1 < t.tiles) find_page(j + 1);
+                const int place = ((t.tile0 + j) * kTokens + 16 * (lane & 7)) & page_mask;
+                for (int which = 0; which < 2; ++which, ++half) {
+                    const uint32_t slot = half % kRing, bar = ptx::smem_u32(&bars.full[slot]);
+                    ok = wait_on(&bars.empty[slot], (half / kRing) ^ 1, &s_abort);
+                    if (!ok) break;
+                    if (lane < kPieces) {
+                        if (id >= 0) {
+                            ptx::mbar_arrive_expect_tx(bar, 16 * D);
+                            ptx::tma_load_4d(ring + slot * L::kHalf + lane * 16 * D, which ? &v_map : &k_map, 0, place, t.head, id, bar);
+                        } else {
+                            ptx::mbar_arrive(bar);
+                        }
+                        if (which == 0 && id >= 0) {
+                            ptx::cp_async_8(ptx::smem_u32(&s_raw[g % kRawScales][lane]), cache.scales + (long long)id * cache.heads + t.head);
+                            ptx::cp_async_arrive(bar);
+                        } else {
+                            if (which == 0) s_raw[g % kRawScales][lane] = make_float2(__uint_as_float(kNoPage), 0.f);
+                            ptx::mbar_arrive(bar);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            at += t.tiles;
+        }
+        if (ok) ok = wait_on(&bars.item_empty[n % kItems], (n / kItems) ^ 1, &s_abort);
+        if (ok && lane == 0) {
+            items[n % kItems].valid = 0;
+            arrive(&bars.item_full[n % kItems]);
+        }
+        // A block that gives up waits, bounded again, for what is on its way to its ring: the shared memory is someone else's once it has ended.
+        if (!ok)
+            for (uint32_t h = half > kRing ? half - kRing : 0; h < half; ++h) (void)ptx::mbar_wait(ptx::smem_u32(&bars.full[h % kRing]), (h / kRing) & 1);
+    } else if (warp == kMma) {
+        // ---- products ----
+        uint32_t g = 0;
+        bool ok = true;
+        for (uint32_t n = 0; ok; ++n) {
+            ok = next_item(n);
+            if (!ok || !items[n % kItems].valid) break;
+            const int tiles = items[n % kItems].tiles, columns = items[n % kItems].n;
+            const uint32_t idesc = ptx::idesc_f16_m128(columns), idesc_mn = idesc | kBothMn, buffers = columns <= 64 ? 2 : 1;
+            ok = wait_on(&bars.q_full[n % kItems], n / kItems, &s_abort);
+            const auto score = [&](uint32_t i) {      // S_i = K_i Q^T; the weights of tile i - 2 are there by now, so its scores have been read
+                ok = ok && wait_on(&bars.k_full[i & 1], i >> 1, &s_abort);
+                if (!ok) return;
+                ptx::tc_fence_after_sync();
+                if (ptx::elect_one()) {
+                    const uint64_t b = ptx::smem_desc_sw128(q_tile);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        ptx::umma_f16_ts(s_col(i), k_col(i) + 8 * k, b + (uint64_t)((k >> 2) * (kMostRows * 128 >> 4) + (k & 3) * 2), idesc, k > 0);
+                    ptx::tc_commit(ptx::smem_u32(&bars.s_full[i & 1]));
+                }
+                __syncwarp();
+            };
+            score(g);
+            if (tiles > 1) score(g + 1);
+            for (int j = 0; j < tiles && ok; ++j) {
+                const uint32_t i = g + j;
+                ok = wait_on(&bars.v_full, i, &s_abort) && wait_on(&bars.p_full[i & 1], i >> 1, &s_abort);
+                if (!ok) break;
+                ptx::tc_fence_after_sync();
+                if (ptx::elect_one()) {
+                    const uint64_t a = smem_desc_mn(v_tile), b = smem_desc_mn(p_tile + (buffers == 2 ? (i & 1) * kMnStride : 0));
+#pragma unroll
+                    for (int k = 0; k < kTokens / 16; ++k) ptx::umma_f16_ss(o_col, a + (uint64_t)(k * 2048 >> 4), b + (uint64_t)(k * 2048 >> 4), idesc_mn, j > 0 || k > 0);
+                    ptx::tc_commit(ptx::smem_u32(&bars.pv_done[i & 1]));
+                }
+                __syncwarp();
+                if (j + 2 < tiles) score(i + 2);
+            }
+            g += tiles;
+            done_with_item(n);
+        }
+        // nothing of this block may be in flight when its tensor memory goes
+        if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars.drained));
+        __syncwarp();
+        for (uint32_t i = 0; i < ptx::kSpinLimit && !ptx::mbar_try_wait(ptx::smem_u32(&bars.drained), 0); ++i) {}
+    } else if (warp >= kDecode0) {
+        // ---- queries; bytes to operands ----
+        constexpr int kMeet = 3;
+        const int w = warp - kDecode0, tid = w * 32 + lane;
+        constexpr int kUnits = D / 8;                 // of 16 bytes in a query
+        uint32_t g = 0, half = 0;
+        bool ok = true;
+        for (uint32_t n = 0; ok; ++n) {
+            ok = next_item(n);
+            if (!ok || !items[n % kItems].valid) break;
+            const uint32_t slot = n % kItems;
+            const Item t = items[slot];
+            // whose rows they are
+            {
+                int id = -1, low = 0;
+                if (tid < t.rows) {
+                    const int in = t.base + tid, entry = t.first + in / p.group, token = entry < p.prefix_listed ? p.prefix_rows[entry] : -1;
+                    if (token >= 0 && token < p.tokens) {
+                        id = token * p.q_heads + t.head * p.group + in % p.group;
+                        if (p.window) {
+                            int b = token;
+                            if (p.cu_lens) {
+                                int hi = p.requests - 1;
+                                for (b = 0; b < hi;) {
+                                    const int mid = (b + hi + 1) >> 1;
+                                    if (p.cu_lens[mid] <= token) b = mid;
+                                    else hi = mid - 1;
+                                }
+                            }
+                            b = min(b, p.requests - 1);
+                            const long long position = (long long)p.seq_lens[t.place] + p.seq_lens[b] - (p.cu_lens ? p.cu_lens[b + 1] : b + 1) + token;
+                            low = (int)min(max(position - p.window + 1, 0ll), (long long)t.limit);
+                        }
+                    }
+                }
+                s_row[slot][tid] = id;
+                s_low[slot][tid] = low;
+                const int most = __reduce_max_sync(kAll, low);
+                if (p.window) {
+                    if (tid == 0) s_most_low[slot] = 0;
+                    if (!(ok = meet(kMeet))) break;
+                    if (lane == 0) atomicMax(&s_most_low[slot], most);
+                } else if (tid == 0) {
+                    s_most_low[slot] = 0;
+                }
+            }
+            if (!(ok = meet(kMeet))) break;
+            // (the scores of the item before are complete)
+            if (g > 0 && !(ok = wait_on(&bars.s_full[(g - 1) & 1], (g - 1) >> 1, &s_abort))) break;
+            constexpr int kAtOnce = 8, kRowsAtOnce = 32 / kUnits;             // of a warp
+            for (int r0 = w * kRowsAtOnce; r0 < t.n; r0 += kAtOnce * 4 * kRowsAtOnce) {
+                uint4 x[kAtOnce];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int r = r0 + i * 4 * kRowsAtOnce + lane / kUnits, id = r < t.n ? s_row[slot][r] : -1;
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (id >= 0) {
+                        const int token = id / p.q_heads, h = id - token * p.q_heads;
+                        x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q.p) + token * p.q.token + h * p.q.head + 8 * (lane % kUnits));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const int r = r0 + i * 4 * kRowsAtOnce + lane / kUnits;
+                    uint2 a = make_uint2(x[i].x, x[i].y), b = make_uint2(x[i].z, x[i].w);
+                    if (BF16) {
+                        float most = fmaxf(bf16_most(a), bf16_most(b)), up, down;
+#pragma unroll
+                        for (int d = kUnits / 2; d; d /= 2) most = fmaxf(most, __shfl_xor_sync(kAll, most, d));
+                        bf16_powers(most, up, down);
+                        a = bf16_scaled(a, down);
+                        b = bf16_scaled(b, down);
+                        if (lane % kUnits == 0 && r < t.n) s_up[slot][r] = up;
+                    }
+                    a = key_order<E4M3>(a);
+                    b = key_order<E4M3>(b);
+                    if (r < t.n) ptx::sts128(swizzled(q_tile, r, lane % kUnits), make_uint4(a.x, a.y, b.x, b.y));
+                }
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive(&bars.q_full[slot]);
+
+            for (int j = 0; j < t.tiles && ok; ++j, ++g) {
+                const int first = (t.tile0 + j) * kTokens;
+                // keys: a thread a token
+                {
+                    const uint32_t at = half % kRing, from = ring + at * L::kHalf;
+                    ok = wait_on(&bars.full[at], half / kRing, &s_abort);
+                    if (!ok) break;
+                    if (w == 0 && lane < kPieces) {
+                        const float2 both = s_raw[g % kRawScales][lane];
+                        const float value = fmaxf(both.y, kLeastScale);
+                        s_scale[g % kScales][lane] = __float_as_uint(both.x) == kNoPage ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                                                       : make_float4(both.x, log2f(value), 1.f / value, 1.f);
+                    }
+                    if (g >= 2) ok = wait_on(&bars.s_full[g & 1], (g >> 1) - 1, &s_abort);         // (the keys that lay there have been used)
+                    if (!ok) break;
+                    const uint32_t lanes = (uint32_t)(w * 32) << 16;
+#pragma unroll
+                    for (int c0 = 0; c0 < D / 16; c0 += 4) {
+                        uint32_t out[32];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t chunk = D == 128 ? tid * 128 + (((c0 + c) ^ (tid & 7)) << 4) : tid * 64 + (((c0 + c) ^ ((tid >> 1) & 3)) << 4);
+                            const uint4 x = ptx::lds128(from + chunk);
+                            decode4<E4M3>(x.x, out[8 * c], out[8 * c + 1]);
+                            decode4<E4M3>(x.y, out[8 * c + 2], out[8 * c + 3]);
+                            decode4<E4M3>(x.z, out[8 * c + 4], out[8 * c + 5]);
+                            decode4<E4M3>(x.w, out[8 * c + 6], out[8 * c + 7]);
+                        }
+                        ptx::tmem_st32(k_col(g) + lanes + 8 * c0, out);
+                    }
+                    ptx::tc_wait_st();
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        arrive(&bars.k_full[g & 1]);
+                        arrive(&bars.empty[at]);
+                        if (w == 0) arrive(&bars.scale_full[g % kScales]);
+                    }
+                    ++half;
+                }
+                // values: 8 tokens and 4 units of 16 at a time, in an order whose lanes meet in no bank
+                {
+                    const uint32_t at = half % kRing, from = ring + at * L::kHalf;
+                    ok = wait_on(&bars.full[at], half / kRing, &s_abort);
+                    if (ok && g >= 1) ok = wait_on(&bars.pv_done[(g - 1) & 1], (g - 1) >> 1, &s_abort);
+                    if (!ok) break;
+                    const int in8 = (lane >> 3) ^ (lane & 4 ? 5 : 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int token = w * 32 + 8 * i + in8;
+                        const bool seen = first + token >= t.lo && first + token < t.limit && __float_as_uint(s_raw[g % kRawScales][token >> 4].x) != kNoPage;
+#pragma unroll
+                        for (int c0 = 0; c0 < D / 16; c0 += 4) {
+                            const int c = c0 + (lane & 3);
+                            uint4 x = ptx::lds128(from + (D == 128 ? token * 128 + ((c ^ (token & 7)) << 4) : token * 64 + ((c ^ ((token >> 1) & 3)) << 4)));
+                            if (!seen) x = make_uint4(0, 0, 0, 0);    // (bytes of tokens that nobody sees may be anything, and 0 * NaN is NaN)
+                            uint4 a, b;
+                            decode4<E4M3>(x.x, a.x, a.y);
+                            decode4<E4M3>(x.y, a.z, a.w);
+                            decode4<E4M3>(x.z, b.x, b.y);
+                            decode4<E4M3>(x.w, b.z, b.w);
+                            ptx::sts128(swizzled_mn(v_tile, token, 2 * c), a);
+                            ptx::sts128(swizzled_mn(v_tile, token, 2 * c + 1), b);
+                        }
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        arrive(&bars.v_full);
+                        arrive(&bars.empty[at]);
+                    }
+                    ++half;
+                }
+            }
+            if (ok) done_with_item(n);
+        }
+        if (!ok) leave(kMeet);
+    } else {
+        // ---- softmax ----
+        const int h = warp >> 2, w = warp & 3, tid = w * 32 + lane, id_meet = 1 + h;
+        const uint32_t lanes = (uint32_t)(w * 32) << 16;
+        uint32_t g = 0, pass = 0;
+        bool ok = true;
+        const float factor = p.scale * kLog2e;
+        for (uint32_t n = 0; ok; ++n) {
+            ok = next_item(n);
+            if (!ok || !items[n % kItems].valid) break;
+            const uint32_t item_slot = n % kItems;
+            const Item& t = items[item_slot];
+            ok = wait_on(&bars.q_full[item_slot], n / kItems, &s_abort);
+            if (!ok) break;
+            const int columns = t.n / 2, row0 = h * columns, groups = columns / 8, tiles = t.tiles;
+            const uint32_t buffers = t.n <= 64 ? 2 : 1;
+            const int most_low = s_most_low[item_slot];
+            if (tid < kMostRows / 2) s_minus_top[h][tid] = -kNone;
+            float sums[kMostRows / 2];
+#pragma unroll
+            for (int i = 0; i < kMostRows / 2; ++i) sums[i] = 0.f;
+            if (!(ok = meet(id_meet))) break;
+            for (int j = 0; j < tiles; ++j) {
+                const uint32_t i = g + j;
+                ok = wait_on(&bars.scale_full[i % kScales], i / kScales, &s_abort) && wait_on(&bars.s_full[i & 1], i >> 1, &s_abort);
+                if (!ok) break;
+                ptx::tc_fence_after_sync();
+                const float4 sc = s_scale[i % kScales][tid >> 4];
+                const int first = (t.tile0 + j) * kTokens, token = first + tid;
+                const bool there = sc.w != 0.f && token >= t.lo && token < t.limit;
+                const bool whole = __all_sync(kAll, there) && first >= most_low;
+                const float a = factor * sc.x, b = sc.y, inverse = sc.z;
+                const uint32_t p_at = p_tile + (buffers == 2 ? (i & 1) * kMnStride : 0);
+                // exponents of 8 columns from `at` on, relative to the rows' references or not
+                const auto exponents = [&](uint32_t* x, int at, bool relative) {
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {
+                        float2 y = make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                        if (BF16) y = mul2(y, *reinterpret_cast<const float2*>(&s_up[item_slot][row0 + at + k]));
+                        float2 from = make_float2(b, b);
+                        if (relative) from = add2(from, *reinterpret_cast<const float2*>(&s_minus_top[h][at + k]));
+                        y = fma2(y, make_float2(a, a), from);
+                        if (!whole) {
+                            if (!there || token < s_low[item_slot][row0 + at + k]) y.x = -INFINITY;
+                            if (!there || token < s_low[item_slot][row0 + at + k + 1]) y.y = -INFINITY;
+                        }
+                        x[k] = __float_as_uint(y.x);
+                        x[k + 1] = __float_as_uint(y.y);
+                    }
+                };
+                // do any weights outgrow fp16?
+                float most = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (2 * c < groups) {
+                        uint32_t x[16];
+                        ptx::tmem_ld16(s_col(i) + lanes + row0 + 16 * c, x);
+                        ptx::tc_wait_ld();
+                        exponents(x, 16 * c, true);
+#pragma unroll
+                        for (int k = 0; k < 8; k += 2) most = max3(most, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                        if (2 * c + 1 < groups) {
+                            exponents(x + 8, 16 * c + 8, true);
+#pragma unroll
+                            for (int k = 8; k < 16; k += 2) most = max3(most, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                        }
+                    }
+                ++pass;
+                if (most > kMostLog) s_need[h][pass & 1] = pass;
+                if (!(ok = meet(id_meet))) break;
+                if (s_need[h][pass & 1] == pass) {
+                    // then the rows' references move to their largest so far, and what there is of sums follows
+                    if (j > 0) ok = wait_on(&bars.pv_done[(i - 1) & 1], (i - 1) >> 1, &s_abort);
+                    if (!ok) break;
+                    ptx::tc_fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        if (4 * c < groups) {
+                            uint32_t x[32];
+                            ptx::tmem_ld32(s_col(i) + lanes + row0 + 32 * c, x);
+                            ptx::tc_wait_ld();
+                            float y[32];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                if (4 * c + q < groups) exponents(x + 8 * q, 32 * c + 8 * q, false);
+#pragma unroll
+                                for (int k = 8 * q; k < 8 * q + 8; ++k) y[k] = 4 * c + q < groups ? __uint_as_float(x[k]) : -INFINITY;
+                            }
+                            s_warps[h][w][32 * c + lane] = reduce32(y, [](float u, float v) { return fmaxf(u, v); });
+                        }
+                    if (!(ok = meet(id_meet))) break;
+                    if (tid < columns) {
+                        const float old = -s_minus_top[h][tid];
+                        float top = old;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top = fmaxf(top, s_warps[h][k][tid]);
+                        s_minus_top[h][tid] = -top;
+                        s_keep[h][tid] = top == old ? 1.f : exp2_approx(old - top);
+                    }
+                    if (!(ok = meet(id_meet))) break;
+#pragma unroll
+                    for (int q = 0; q < kMostRows / 16; ++q)
+                        if (q < groups) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) sums[8 * q + k] *= s_keep[h][8 * q + k];
+                            if (j > 0) {
+                                uint32_t x[8];
+                                ptx::tmem_ld8(o_col + lanes + row0 + 8 * q, x);
+                                ptx::tc_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * s_keep[h][8 * q + k]);
+                                ptx::tmem_st8(o_col + lanes + row0 + 8 * q, x);
+                            }
+                        }
+                    ptx::tc_wait_st();
+                }
+                if (j >= (int)buffers) {                                      // (what lay in the weights' place has been used)
+                    const uint32_t used = i - buffers;
+                    ok = wait_on(&bars.pv_done[used & 1], used >> 1, &s_abort);
+                    if (!ok) break;
+                }
+                const auto weigh = [&](uint32_t* x, int at) {                 // 8 columns
+                    exponents(x, at, true);
+                    float e[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) e[k] = exp2_approx(__uint_as_float(x[k]));
+#pragma unroll
+                    for (int k = 0; k < 8; k += 2) {
+                        const float2 s2 = fma2(make_float2(e[k], e[k + 1]), make_float2(inverse, inverse), make_float2(sums[at + k], sums[at + k + 1]));
+                        sums[at + k] = s2.x;
+                        sums[at + k + 1] = s2.y;
+                    }
+                    ptx::sts128(swizzled_mn(p_at, tid, (row0 + at) / 8),
+                                make_uint4(h2_as_u32(__floats2half2_rn(e[0], e[1])), h2_as_u32(__floats2half2_rn(e[2], e[3])),
+                                           h2_as_u32(__floats2half2_rn(e[4], e[5])), h2_as_u32(__floats2half2_rn(e[6], e[7]))));
+                };
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (2 * c < groups) {
+                        uint32_t x[16];
+                        ptx::tmem_ld16(s_col(i) + lanes + row0 + 16 * c, x);
+                        ptx::tc_wait_ld();
+                        weigh(x, 16 * c);
+                        if (2 * c + 1 < groups) weigh(x + 8, 16 * c + 8);
+                    }
+                if (!ok) break;
+                ptx::tc_fence_before_sync();
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) arrive(&bars.p_full[i & 1]);
+            }
+            if (!ok) break;
+            g += tiles;
+            ok = wait_on(&bars.pv_done[(g - 1) & 1], (g - 1) >> 1, &s_abort);
+            if (!ok) break;
+            ptx::tc_fence_after_sync();
+            // totals: over the lanes, then over the warps
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float y[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k) y[k] = sums[32 * c + k];
+                s_warps[h][w][32 * c + lane] = reduce32(y, [](float u, float v) { return u + v; });
+            }
+            if (!(ok = meet(id_meet))) break;
+            const auto reference = [&](int r) { return s_minus_top[h][r] == -kNone ? -INFINITY : -s_minus_top[h][r]; };
+            const auto total_of = [&](int r) { return (s_warps[h][0][r] + s_warps[h][1][r]) + (s_warps[h][2][r] + s_warps[h][3][r]); };
+            // (int8: the products' rows are the dims in decode4's order)
+            const int dim = E4M3 ? tid : (tid & ~3) | ((tid & 1) << 1) | ((tid >> 1) & 1);
+            const bool real = tid < D;
+            if (t.first_block == t.last_block) {
+                if (tid < columns && s_row[item_slot][row0 + tid] >= 0) p.prefix_total[s_row[item_slot][row0 + tid]] = make_float2(reference(tid), total_of(tid));
+#pragma unroll 1
+                for (int c = 0; 4 * c < groups; ++c) {
+                    uint32_t x[32];
+                    ptx::tmem_ld32(o_col + lanes + row0 + 32 * c, x);
+                    ptx::tc_wait_ld();
+                    if (real)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            if (4 * c + k / 8 >= groups) break;
+                            const int id = s_row[item_slot][row0 + 32 * c + k];
+                            if (id >= 0) p.prefix_sums[(long long)id * D + dim] = __uint_as_float(x[k]);
+                        }
+                    __syncwarp();
+                }
+            } else {
+                // a part: the block's first item continues another block's, its last is continued; the one that comes last adds them up
+                const int a = t.first_block, z = t.last_block;
+                float* const parts = reinterpret_cast<float*>(header + p.prefix_parts);
+                const auto part_of = [&](int block) { return parts + ((size_t)block * 2 + (block == a ? 1 : 0)) * L::kPartFloats; };
+                float* const own = part_of(blockIdx.x);
+                if (tid < columns) {
+                    own[kMostRows * D + row0 + tid] = reference(tid);
+                    own[kMostRows * D + kMostRows + row0 + tid] = total_of(tid);
+                }
+#pragma unroll 1
+                for (int c = 0; 4 * c < groups; ++c) {
+                    uint32_t x[32];
+                    ptx::tmem_ld32(o_col + lanes + row0 + 32 * c, x);
+                    ptx::tc_wait_ld();
+                    if (real)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            if (4 * c + k / 8 >= groups) break;
+                            own[(row0 + 32 * c + k) * D + dim] = __uint_as_float(x[k]);
+                        }
+                    __syncwarp();
+                }
+                __threadfence();
+                if (!(ok = meet(id_meet))) break;
+                if (tid == 0) {
+                    unsigned int* const counter = reinterpret_cast<unsigned int*>(header + kPrefixCounters) + 2 * a + h;
+                    const bool last = atomicAdd(counter, 1u) == (unsigned int)(z - a);
+                    if (last) atomicExch(counter, 0u);                        // as the next launch expects it
+                    s_last[h] = last;
+                    __threadfence();
+                }
+                if (!(ok = meet(id_meet))) break;
+                if (s_last[h]) {
+                    __threadfence();
+                    for (int r = tid / D; r < columns; r += 128 / D) {
+                        const int row = row0 + r, id = s_row[item_slot][row], d = tid % D;
+                        if (id < 0) continue;
+                        float m = -INFINITY;
+#pragma unroll 4
+                        for (int b = a; b <= z; ++b) m = fmaxf(m, __ldcg(part_of(b) + kMostRows * D + row));
+                        const float from = m == -INFINITY ? 0.f : m;
+                        float all_total = 0.f, o = 0.f;
+#pragma unroll 4
+                        for (int b = a; b <= z; ++b) {
+                            const float* const part = part_of(b);
+                            const float take = exp2_approx(__ldcg(part + kMostRows * D + row) - from);
+                            all_total = fmaf(take, __ldcg(part + kMostRows * D + kMostRows + row), all_total);
+                            o = fmaf(take, __ldcg(part + row * D + d), o);
+                        }
+                        p.prefix_sums[(long long)id * D + d] = o;
+                        if (d == 0) p.prefix_total[id] = make_float2(m, all_total);
+                    }
+                }
+                if (!(ok = meet(id_meet))) break;                             // (s_last is free again)
+            }
+            // what was read of the sums is read before the next item's products overwrite them
+            ptx::tc_fence_before_sync();
+            done_with_item(n);
+        }
+        if (!ok) leave(id_meet);
     }
+
+    if (lane == 0 && s_abort) atomicExch(reinterpret_cast<int*>(header + kStatusOffset), 63);
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    if (warp == kMma) ptx::tmem_dealloc(tmem, 512);
+}
+
+template <bool E4M3, bool BF16, int D>
+cudaError_t launch_prefix(const AttentionParams& p, cudaStream_t stream) {
+    const auto kernel = cache_prefix_kernel<E4M3, BF16, D>;
+    constexpr int kSmem = Layout<D>::kBytes;
+    CUtensorMap k_map, v_map;
+    if (!cache_map(&k_map, p.cache, true) || !cache_map(&v_map, p.cache, false)) return cudaErrorNotSupported;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(kMaxBlocks, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, p, k_map, v_map);
+    if (e == cudaSuccess) count_launch();
+    return e;
 }
 
 }  // namespace
 
+size_t cache_prefix_workspace() { return kPartsBytes; }
+
 cudaError_t cache_prefix_launch(const AttentionParams& p, bool e4m3, bool bf16, cudaStream_t stream) {
     const auto by_dim = [&](auto e, auto h) {
         constexpr bool E = decltype(e)::value, H = decltype(h)::value;
-        const auto kernel = p.cache.dim == 128 ? cache_prefix_kernel<E, H, 128> : cache_prefix_kernel<E, H, 64>;
-        return launch_overlapping(kernel, dim3(148 * 8), 256, stream, p);
+        return p.cache.dim == 128 ? launch_prefix<E, H, 128>(p, stream) : launch_prefix<E, H, 64>(p, stream);
     };
     const auto by_type = [&](auto e) { return bf16 ? by_dim(e, std::true_type{}) : by_dim(e, std::false_type{}); };
     return e4m3 ? by_type(std::true_type{}) : by_type(std::false_type{});
