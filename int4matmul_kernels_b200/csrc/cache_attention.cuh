@@ -186,13 +186,13 @@ __device__ __forceinline__ Joint join_prefix(float m, float sum, float2 prefix) 
 // whether a row of request b at this position sees a prefix
 __device__ __forceinline__ bool sees_prefix(const AttentionParams& p, int b, int position) { return position >= 0 && p.prefix_of[b] >= 0; }
 
-// the cache's keys or values as (dim, token, head, page), read 16 tokens at a time in rows whose 16-byte chunks are swizzled
-inline bool cache_map(CUtensorMap* out, const CacheView& c, bool keys) {
+// the cache's keys or values as (dim, token, head, page), read `tokens` tokens at a time in rows whose 16-byte chunks are swizzled
+inline bool cache_map(CUtensorMap* out, const CacheView& c, bool keys, int tokens) {
     const EncodeTiledFn encode = encode_tiled_fn();
     if (!encode) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)c.dim, 1ull << c.page_shift, (cuuint64_t)c.heads, (cuuint64_t)c.pages};
     const cuuint64_t strides[3] = {(cuuint64_t)(keys ? c.k_token : c.v_token), (cuuint64_t)(keys ? c.k_head : c.v_head), (cuuint64_t)(keys ? c.k_page : c.v_page)};
-    const cuuint32_t box[4] = {(cuuint32_t)c.dim, 16, 1, 1}, steps[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {(cuuint32_t)c.dim, (cuuint32_t)tokens, 1, 1}, steps[4] = {1, 1, 1, 1};
     return encode_with_context([&] {
         return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, keys ? c.k : c.v, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       c.dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

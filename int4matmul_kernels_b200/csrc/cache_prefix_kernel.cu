@@ -16,7 +16,7 @@
 //   warps 0..3, 4..7   softmax of the first and of the second half of the rows
 //   warps 8..11        the rows' queries; bytes to operands
 //   warp 12            issues the products
-//   warp 13            deals out the work, fetches pages (a TMA copy for each 16 keys or values) into a ring of 7 half tiles
+//   warps 13, 14       fetch pages into rings, a TMA copy a page, keys and values; the first deals out the work
 //
 // The tiles of all segments (place, key head, 128 rows) in a row are dealt out in equal contiguous ranges to the blocks.  What a range cuts goes through the
 // workspace, and the block that comes last adds the parts in their order.  Nobody waits for another block.  Waits are bounded: a warp that gives up
@@ -31,10 +31,10 @@ namespace {
 
 constexpr int kTokens = 128;                          // of a tile
 constexpr int kMostRows = 128;
-constexpr int kSoftmaxWarps = 8, kDecode0 = 8, kDecodeWarps = 4, kMma = 12, kCopy = 13, kThreads = 14 * 32;
-constexpr int kRing = 7;                              // half tiles: keys, values
+constexpr int kSoftmaxWarps = 8, kDecode0 = 8, kDecodeWarps = 4, kMma = 12, kCopy = 13, kCopyValues = 14, kThreads = 15 * 32;
+constexpr int kKeys = 3, kValues = 4;                 // stages of the rings
 constexpr int kItems = 4, kScales = 4, kRawScales = 8;
-constexpr int kPieces = kTokens / 16;
+constexpr int kPieces = kTokens / 16;                 // pages of a tile, at most
 constexpr int kMinBlockTiles = 2;                     // fewer tiles than this are not cut further
 constexpr float kNone = -3e38f;                       // a reference below any score
 constexpr float kMostLog = 14.f;                      // fp16 holds 2^16
@@ -45,8 +45,9 @@ template <int D>
 struct Layout {
     static constexpr int kHalf = kTokens * D;                                 // bytes of a tile's keys or values
     static constexpr int kV = 2 * kMnStride, kP = 2 * kMnStride, kQ = kMostRows * D * 2;
-    static constexpr int kV0 = 0, kP0 = kV0 + kV, kQ0 = kP0 + kP, kRing0 = kQ0 + kQ, kBytes = kRing0 + kRing * kHalf + 1024;
-    static constexpr int kPartFloats = kMostRows * D + 2 * kMostRows;         // sums [row][dim], references, totals
+    static constexpr int kV0 = 0, kP0 = kV0 + kV, kQ0 = kP0 + kP, kKeys0 = kQ0 + kQ, kValues0 = kKeys0 + kKeys * kHalf,
+                         kBytes = kValues0 + kValues * kHalf + 1024;
+    static constexpr int kPartFloats = kMostRows * D + 2 * kMostRows;         // sums [row][dim], (reference, total) [row]
 };
 constexpr size_t kPartsBytes = (size_t)kMaxBlocks * 2 * Layout<128>::kPartFloats * 4;
 
@@ -59,7 +60,8 @@ struct Item {
 };
 
 struct Barriers {
-    unsigned long long item_full[kItems], item_empty[kItems], q_full[kItems], full[kRing], empty[kRing], scale_full[kScales];
+    unsigned long long item_full[kItems], item_empty[kItems], q_full[kItems], scale_full[kScales];
+    unsigned long long keys_full[kKeys], keys_empty[kKeys], values_full[kValues], values_empty[kValues];
     unsigned long long k_full[2], s_full[2], p_full[2], pv_done[2], v_full, drained;
 };
 
@@ -77,25 +79,24 @@ __device__ __forceinline__ void arrive(unsigned long long* bar) { ptx::mbar_arri
 
 // ---- work ----------------------------------------------------------------------------------------------------------------------
 struct Place {
-    int first;                                        // of its readers in the list
-    long long rows;                                   // readers times query heads of a key head
+    int first, rows;                                  // of its readers in the list; readers times query heads of a key head
     int lo, limit, tiles;                             // tokens that any row sees; at least one tile, so that all rows are written
-    long long row_tiles;
-    int height;                                       // rows of a row tile: all of a place alike
+    int row_tiles, height;                            // rows of a row tile: all of a place alike
 };
 __device__ __forceinline__ Place load_place(const AttentionParams& p, int b) {
     Place r;
     const int from = min(max(p.prefix_starts[b], 0), p.prefix_listed), to = min(max(p.prefix_starts[b + 1], 0), p.prefix_listed), seq = p.seq_lens[b];
     r.first = from;
-    r.rows = (long long)max(to - from, 0) * p.group;
+    r.rows = min(max(to - from, 0), p.tokens) * p.group;                      // (tokens * q_heads is below 2^31)
     r.limit = max(min(seq, p.table_width << p.cache.page_shift), 0);
     r.lo = p.window && seq >= p.window ? min(seq - p.window + 1, r.limit) : 0;
     r.tiles = max((r.limit + kTokens - 1) / kTokens - r.lo / kTokens, 1);
     r.row_tiles = (r.rows + kMostRows - 1) / kMostRows;
-    r.height = r.rows == 0 ? 0 : (int)((r.rows + 16 * r.row_tiles - 1) / (16 * r.row_tiles)) * 16;
+    r.height = (r.rows + 15) & ~15;
+    if (r.row_tiles > 1) r.height = (int)(((uint32_t)r.rows + 16u * r.row_tiles - 1) / (16u * r.row_tiles)) * 16;
     return r;
 }
-__device__ __forceinline__ long long units_of(const AttentionParams& p, const Place& r) { return r.row_tiles * p.cache.heads * r.tiles; }
+__device__ __forceinline__ long long units_of(const AttentionParams& p, const Place& r) { return (long long)(r.row_tiles * p.cache.heads) * r.tiles; }
 
 // ---- two fp32 at a time ----
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -122,32 +123,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // 32 values of each lane -> lane l has the result over all lanes of value l
 template <int DISTANCE, typename F>
-__device__ __forceinline__ void reduce_step(float (&x)[32], F op) {
+__device__ __forceinline__ void reduce_step(uint32_t (&x)[32], F op) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < DISTANCE; ++i) {
-        const float send = lane & DISTANCE ? x[i] : x[i + DISTANCE], keep = lane & DISTANCE ? x[i + DISTANCE] : x[i];
-        x[i] = op(keep, __shfl_xor_sync(kAll, send, DISTANCE));
+        const uint32_t send = lane & DISTANCE ? x[i] : x[i + DISTANCE], keep = lane & DISTANCE ? x[i + DISTANCE] : x[i];
+        x[i] = __float_as_uint(op(__uint_as_float(keep), __uint_as_float(__shfl_xor_sync(kAll, send, DISTANCE))));
     }
 }
 template <typename F>
-__device__ __forceinline__ float reduce32(float (&x)[32], F op) {
+__device__ __forceinline__ float reduce32(uint32_t (&x)[32], F op) {
     reduce_step<16>(x, op);
     reduce_step<8>(x, op);
     reduce_step<4>(x, op);
     reduce_step<2>(x, op);
     reduce_step<1>(x, op);
-    return x[0];
+    return __uint_as_float(x[0]);
 }
 
 // address of 16 bytes (8 values) `unit` of `row` in Q: sub-tiles of 64 values, 128-byte rows, swizzled
 __device__ __forceinline__ uint32_t swizzled(uint32_t tile, int row, int unit) {
     return tile + (unit >> 3) * (kMostRows * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
 }
-// address of 8 columns `unit` of `token` in V or P: blocks of 64 columns, 128-byte rows, swizzled
-__device__ __forceinline__ uint32_t swizzled_mn(uint32_t tile, int token, int unit) {
-    return tile + (unit >> 3) * kMnStride + token * 128 + (((unit & 7) ^ (token & 7)) << 4);
-}
+// V and P: blocks of 64 columns, a token's 128 bytes to a row, swizzled in the same way.
 // Matrix descriptor of such an operand: its columns are the M or N of a product, its tokens the K.  8 tokens 1024 bytes apart, blocks of 64 columns kMnStride
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kMnStride >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
@@ -164,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     __shared__ float2 s_raw[kRawScales][kPieces];
     __shared__ float4 s_scale[kScales][kPieces];      // key scale, log2 of the value scale, its inverse, whether there is such a page
     __shared__ int s_row[kItems][kMostRows];          // packed row times query heads plus head; -1: none
+    __shared__ long long s_query[kMostRows];          // where its query lies
     __shared__ int s_low[kItems][kMostRows];          // the first token that the row sees
     __shared__ float s_up[kItems][kMostRows];         // what its scores are multiplied with (bf16)
     __shared__ int s_most_low[kItems];
@@ -175,20 +174,25 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     __shared__ uint32_t tmem_smem;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem = (ptx::smem_u32(dynamic) + 1023u) & ~1023u;
-    const uint32_t q_tile = smem + L::kQ0, v_tile = smem + L::kV0, p_tile = smem + L::kP0, ring = smem + L::kRing0;
+    const uint32_t q_tile = smem + L::kQ0, v_tile = smem + L::kV0, p_tile = smem + L::kP0, keys_ring = smem + L::kKeys0, values_ring = smem + L::kValues0;
     uint8_t* const header = static_cast<uint8_t*>(p.workspace);
     const CacheView& cache = p.cache;
+    const int page_shift = cache.page_shift, pieces = kTokens >> page_shift;
 
     if (threadIdx.x == 0) {
         const auto init = [](unsigned long long& b, uint32_t n) { ptx::mbar_init(ptx::smem_u32(&b), n); };
         for (int i = 0; i < kItems; ++i) {
             init(bars.item_full[i], 1);
-            init(bars.item_empty[i], kSoftmaxWarps + kDecodeWarps + 1);
+            init(bars.item_empty[i], kSoftmaxWarps + kDecodeWarps + 2);
             init(bars.q_full[i], kDecodeWarps);
         }
-        for (int i = 0; i < kRing; ++i) {
-            init(bars.full[i], 2 * kPieces);
-            init(bars.empty[i], kDecodeWarps);
+        for (int i = 0; i < kKeys; ++i) {
+            init(bars.keys_full[i], 2 * pieces);      // each lane's bytes, and its scales
+            init(bars.keys_empty[i], kDecodeWarps);
+        }
+        for (int i = 0; i < kValues; ++i) {
+            init(bars.values_full[i], pieces);
+            init(bars.values_empty[i], kDecodeWarps);
         }
         for (int i = 0; i < kScales; ++i) init(bars.scale_full[i], 1);
         for (int i = 0; i < 2; ++i) {
@@ -231,9 +235,54 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
         if (lane == 0) arrive(&bars.item_empty[n % kItems]);
     };
     const auto next_item = [&](uint32_t n) { return wait_on(&bars.item_full[n % kItems], n / kItems, &s_abort); };
+    // Fetches an item's keys or values into a ring, a page to a lane; g: tiles before it.
+    uint32_t fetched = 0;
+    const auto copy = [&](const Item& t, uint32_t g, const CUtensorMap* map, uint32_t ring, unsigned long long* full, unsigned long long* empty, uint32_t stages,
+                          bool scales) -> bool {
+        const int* const table = p.table + t.place * p.table_stride;
+        int page = -1;
+        const auto find_page = [&](int j) {           // lane l: the tile's l-th
+            const int token = (t.tile0 + j) * kTokens + (lane << page_shift), i = token >> page_shift;
+            page = -1;
+            if (lane < pieces && token < t.limit && token + (1 << page_shift) > t.lo && i < p.table_width) page = table[i];
+        };
+        find_page(0);
+        for (int j = 0; j < t.tiles; ++j, ++g) {
+            const int id = (unsigned int)page < (unsigned int)cache.pages ? page : -1;
+            if (j + 1 < t.tiles) find_page(j + 1);
+            const uint32_t slot = g % stages, bar = ptx::smem_u32(&full[slot]);
+            if (!wait_on(&empty[slot], (g / stages) ^ 1, &s_abort)) return false;
+            if (lane < pieces) {
+                if (id >= 0) {
+                    ptx::mbar_arrive_expect_tx(bar, D << page_shift);
+                    ptx::tma_load_4d(ring + slot * L::kHalf + lane * (D << page_shift), map, 0, 0, t.head, id, bar);
+                } else {
+                    ptx::mbar_arrive(bar);
+                }
+                if (scales) {
+                    if (id >= 0) {
+                        ptx::cp_async_8(ptx::smem_u32(&s_raw[g % kRawScales][lane]), cache.scales + (long long)id * cache.heads + t.head);
+                        ptx::cp_async_arrive(bar);
+                    } else {
+                        s_raw[g % kRawScales][lane] = make_float2(__uint_as_float(kNoPage), 0.f);
+                        ptx::mbar_arrive(bar);
+                    }
+                }
+            }
+            __syncwarp();
+            fetched = g + 1;
+        }
+        return true;
+    };
+    // A block that gives up waits, bounded again, for what is on its way to its rings: the shared memory is someone else's once it has ended.
+    const auto landed = [&](unsigned long long* full, uint32_t stages) {
+        for (uint32_t i = fetched > stages ? fetched - stages : 0; i < fetched; ++i) (void)ptx::mbar_wait(ptx::smem_u32(&full[i % stages]), (i / stages) & 1);
+    };
+
     if (warp == kCopy) {
         // the block's range
         long long total = 0, at = 0, end = 0;
+#pragma unroll 4
         for (int b = lane; b < p.requests; b += 32) total += units_of(p, load_place(p, b));
         total = warp_sum(total);
         const int blocks = (int)min((long long)gridDim.x, (total + kMinBlockTiles - 1) / kMinBlockTiles);
@@ -260,10 +309,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 before += __shfl_sync(kAll, upto, 31);
             }
         };
-        uint32_t n = 0, half = 0, g = 0;              // items, half tiles, tiles so far
+        uint32_t n = 0, g = 0;                        // items, tiles so far
         bool ok = true;
-        int page = -1;
-        const int page_mask = (1 << cache.page_shift) - 1;
         while (ok && at < end) {
             if (n == 0 || at >= before + units_of(p, r)) {
                 // (the next place with rows: from the multiple of 32 at or below the current one, whose earlier tiles are counted again)
@@ -282,23 +329,26 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             }
             Item t;
             {
-                const long long in = at - before, segment = div_nn(in, r.tiles), per_head = r.row_tiles;
-                const int tile = (int)(in - segment * r.tiles);
-                const long long head = div_nn(segment, per_head), row_tile = segment - head * per_head;
+                const long long in = at - before;
+                const int segment = (int)div_nn(in, r.tiles), tile = (int)(in - (long long)segment * r.tiles);
+                const int head = segment / r.row_tiles, row_tile = segment - head * r.row_tiles;
                 t.valid = 1;
                 t.place = b;
-                t.head = (int)head;
-                t.base = (int)(row_tile * r.height);
-                t.rows = (int)max(min((long long)r.height, r.rows - row_tile * r.height), 0ll);
+                t.head = head;
+                t.base = row_tile * r.height;
+                t.rows = max(min(r.height, r.rows - t.base), 0);
                 t.n = max((t.rows + 15) & ~15, 16);
                 t.first = r.first;
                 t.lo = r.lo;
                 t.limit = r.limit;
                 t.tile0 = r.lo / kTokens + tile;
                 t.tiles = (int)min((long long)(r.tiles - tile), end - at);
-                const long long from = before + segment * r.tiles;
-                t.first_block = range_owner(total, blocks, from);
-                t.last_block = range_owner(total, blocks, from + r.tiles - 1);
+                t.first_block = t.last_block = (int)blockIdx.x;
+                if (t.tiles < r.tiles) {
+                    const long long from = at - tile;
+                    t.first_block = range_owner(total, blocks, from);
+                    t.last_block = range_owner(total, blocks, from + r.tiles - 1);
+                }
             }
             ok = wait_on(&bars.item_empty[n % kItems], (n / kItems) ^ 1, &s_abort);
             if (!ok) break;
@@ -308,39 +358,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             }
             __syncwarp();
             ++n;
-            const int* const table = p.table + t.place * p.table_stride;
-            const auto find_page = [&](int j) {       // lane l: of tokens 16 * l of the tile
-                const int token = (t.tile0 + j) * kTokens + 16 * (lane & 7), i = token >> cache.page_shift;
-                page = -1;
-                if (token < t.limit && token + 16 > t.lo && i < p.table_width) page = table[i];
-            };
-            find_page(0);
-            for (int j = 0; j < t.tiles && ok; ++j, ++g) {
-                const int id = (unsigned int)page < (unsigned int)cache.pages ? page : -1;
-                if (j + 1 < t.tiles) find_page(j + 1);
-                const int place = ((t.tile0 + j) * kTokens + 16 * (lane & 7)) & page_mask;
-                for (int which = 0; which < 2; ++which, ++half) {
-                    const uint32_t slot = half % kRing, bar = ptx::smem_u32(&bars.full[slot]);
-                    ok = wait_on(&bars.empty[slot], (half / kRing) ^ 1, &s_abort);
-                    if (!ok) break;
-                    if (lane < kPieces) {
-                        if (id >= 0) {
-                            ptx::mbar_arrive_expect_tx(bar, 16 * D);
-                            ptx::tma_load_4d(ring + slot * L::kHalf + lane * 16 * D, which ? &v_map : &k_map, 0, place, t.head, id, bar);
-                        } else {
-                            ptx::mbar_arrive(bar);
-                        }
-                        if (which == 0 && id >= 0) {
-                            ptx::cp_async_8(ptx::smem_u32(&s_raw[g % kRawScales][lane]), cache.scales + (long long)id * cache.heads + t.head);
-                            ptx::cp_async_arrive(bar);
-                        } else {
-                            if (which == 0) s_raw[g % kRawScales][lane] = make_float2(__uint_as_float(kNoPage), 0.f);
-                            ptx::mbar_arrive(bar);
-                        }
-                    }
-                    __syncwarp();
-                }
-            }
+            ok = copy(t, g, &k_map, keys_ring, bars.keys_full, bars.keys_empty, kKeys, true);
+            g += t.tiles;
             at += t.tiles;
         }
         if (ok) ok = wait_on(&bars.item_empty[n % kItems], (n / kItems) ^ 1, &s_abort);
@@ -348,9 +367,19 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             items[n % kItems].valid = 0;
             arrive(&bars.item_full[n % kItems]);
         }
-        // A block that gives up waits, bounded again, for what is on its way to its ring: the shared memory is someone else's once it has ended.
-        if (!ok)
-            for (uint32_t h = half > kRing ? half - kRing : 0; h < half; ++h) (void)ptx::mbar_wait(ptx::smem_u32(&bars.full[h % kRing]), (h / kRing) & 1);
+        if (!ok) landed(bars.keys_full, kKeys);
+    } else if (warp == kCopyValues) {
+        uint32_t g = 0;
+        bool ok = true;
+        for (uint32_t n = 0; ok; ++n) {
+            ok = next_item(n);
+            if (!ok || !items[n % kItems].valid) break;
+            const Item t = items[n % kItems];
+            ok = copy(t, g, &v_map, values_ring, bars.values_full, bars.values_empty, kValues, false);
+            g += t.tiles;
+            done_with_item(n);
+        }
+        if (!ok) landed(bars.values_full, kValues);
     } else if (warp == kMma) {
         // ---- products ----
         uint32_t g = 0;
@@ -402,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
         constexpr int kMeet = 3;
         const int w = warp - kDecode0, tid = w * 32 + lane;
         constexpr int kUnits = D / 8;                 // of 16 bytes in a query
-        uint32_t g = 0, half = 0;
+        uint32_t g = 0;
         bool ok = true;
         for (uint32_t n = 0; ok; ++n) {
             ok = next_item(n);
@@ -412,10 +441,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             // whose rows they are
             {
                 int id = -1, low = 0;
+                long long query = 0;
                 if (tid < t.rows) {
                     const int in = t.base + tid, entry = t.first + in / p.group, token = entry < p.prefix_listed ? p.prefix_rows[entry] : -1;
                     if (token >= 0 && token < p.tokens) {
-                        id = token * p.q_heads + t.head * p.group + in % p.group;
+                        const int h = t.head * p.group + in % p.group;
+                        id = token * p.q_heads + h;
+                        query = token * p.q.token + h * p.q.head;
                         if (p.window) {
                             int b = token;
                             if (p.cu_lens) {
@@ -433,6 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                     }
                 }
                 s_row[slot][tid] = id;
+                s_query[tid] = query;
                 s_low[slot][tid] = low;
                 const int most = __reduce_max_sync(kAll, low);
                 if (p.window) {
@@ -453,10 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 for (int i = 0; i < kAtOnce; ++i) {
                     const int r = r0 + i * 4 * kRowsAtOnce + lane / kUnits, id = r < t.n ? s_row[slot][r] : -1;
                     x[i] = make_uint4(0, 0, 0, 0);
-                    if (id >= 0) {
-                        const int token = id / p.q_heads, h = id - token * p.q_heads;
-                        x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q.p) + token * p.q.token + h * p.q.head + 8 * (lane % kUnits));
-                    }
+                    if (id >= 0) x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q.p) + s_query[r] + 8 * (lane % kUnits));
                 }
 #pragma unroll
                 for (int i = 0; i < kAtOnce; ++i) {
@@ -482,76 +512,81 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
 
             for (int j = 0; j < t.tiles && ok; ++j, ++g) {
                 const int first = (t.tile0 + j) * kTokens;
+                bool all;                             // whether all of the tile's tokens are there
                 // keys: a thread a token
                 {
-                    const uint32_t at = half % kRing, from = ring + at * L::kHalf;
-                    ok = wait_on(&bars.full[at], half / kRing, &s_abort);
+                    const uint32_t at = g % kKeys, from = keys_ring + at * L::kHalf + tid * D;
+                    ok = wait_on(&bars.keys_full[at], g / kKeys, &s_abort);
                     if (!ok) break;
-                    if (w == 0 && lane < kPieces) {
-                        const float2 both = s_raw[g % kRawScales][lane];
-                        const float value = fmaxf(both.y, kLeastScale);
-                        s_scale[g % kScales][lane] = __float_as_uint(both.x) == kNoPage ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                                                       : make_float4(both.x, log2f(value), 1.f / value, 1.f);
+                    const float2 raw = s_raw[g % kRawScales][lane & (pieces - 1)];
+                    const bool page = __float_as_uint(raw.x) != kNoPage;
+                    if (w == 0 && lane < pieces) {
+                        const float value = fmaxf(raw.y, kLeastScale);
+                        s_scale[g % kScales][lane] = page ? make_float4(raw.x, log2_approx(value), 1.f / value, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
                     }
+                    all = __all_sync(kAll, page) && first >= t.lo && first + kTokens <= t.limit;
+                    const bool seen = all || (first + tid >= t.lo && first + tid < t.limit && __float_as_uint(s_raw[g % kRawScales][tid >> page_shift].x) != kNoPage);
                     if (g >= 2) ok = wait_on(&bars.s_full[g & 1], (g >> 1) - 1, &s_abort);         // (the keys that lay there have been used)
                     if (!ok) break;
-                    const uint32_t lanes = (uint32_t)(w * 32) << 16;
+                    const uint32_t to = k_col(g) + ((uint32_t)(w * 32) << 16), swizzle = D == 128 ? (lane & 7) << 4 : ((lane >> 1) & 3) << 4;
 #pragma unroll
                     for (int c0 = 0; c0 < D / 16; c0 += 4) {
                         uint32_t out[32];
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            const uint32_t chunk = D == 128 ? tid * 128 + (((c0 + c) ^ (tid & 7)) << 4) : tid * 64 + (((c0 + c) ^ ((tid >> 1) & 3)) << 4);
-                            const uint4 x = ptx::lds128(from + chunk);
+                            const uint4 x = ptx::lds128(from + ((16 * (c0 + c)) ^ swizzle));
                             decode4<E4M3>(x.x, out[8 * c], out[8 * c + 1]);
                             decode4<E4M3>(x.y, out[8 * c + 2], out[8 * c + 3]);
                             decode4<E4M3>(x.z, out[8 * c + 4], out[8 * c + 5]);
                             decode4<E4M3>(x.w, out[8 * c + 6], out[8 * c + 7]);
                         }
-                        ptx::tmem_st32(k_col(g) + lanes + 8 * c0, out);
+                        if (!all) {                   // (bytes of tokens that nobody sees may be anything)
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) out[k] = seen ? out[k] : 0;
+                        }
+                        ptx::tmem_st32(to + 8 * c0, out);
                     }
                     ptx::tc_wait_st();
                     ptx::tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) {
                         arrive(&bars.k_full[g & 1]);
-                        arrive(&bars.empty[at]);
+                        arrive(&bars.keys_empty[at]);
                         if (w == 0) arrive(&bars.scale_full[g % kScales]);
                     }
-                    ++half;
                 }
                 // values: 8 tokens and 4 units of 16 at a time, in an order whose lanes meet in no bank
                 {
-                    const uint32_t at = half % kRing, from = ring + at * L::kHalf;
-                    ok = wait_on(&bars.full[at], half / kRing, &s_abort);
+                    const uint32_t at = g % kValues;
+                    ok = wait_on(&bars.values_full[at], g / kValues, &s_abort);
                     if (ok && g >= 1) ok = wait_on(&bars.pv_done[(g - 1) & 1], (g - 1) >> 1, &s_abort);
                     if (!ok) break;
-                    const int in8 = (lane >> 3) ^ (lane & 4 ? 5 : 0);
+                    const int in8 = (lane >> 3) ^ (lane & 4 ? 5 : 0), token0 = w * 32 + in8, unit = lane & 3;
+                    const uint32_t from = values_ring + at * L::kHalf + token0 * D + ((16 * unit) ^ (D == 128 ? in8 << 4 : ((in8 >> 1) & 3) << 4));
+                    const uint32_t to = v_tile + token0 * 128 + ((32 * unit) ^ (in8 << 4));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int token = w * 32 + 8 * i + in8;
-                        const bool seen = first + token >= t.lo && first + token < t.limit && __float_as_uint(s_raw[g % kRawScales][token >> 4].x) != kNoPage;
+                        const int token = token0 + 8 * i;
+                        const bool seen = all || (first + token >= t.lo && first + token < t.limit && __float_as_uint(s_raw[g % kRawScales][token >> page_shift].x) != kNoPage);
 #pragma unroll
-                        for (int c0 = 0; c0 < D / 16; c0 += 4) {
-                            const int c = c0 + (lane & 3);
-                            uint4 x = ptx::lds128(from + (D == 128 ? token * 128 + ((c ^ (token & 7)) << 4) : token * 64 + ((c ^ ((token >> 1) & 3)) << 4)));
-                            if (!seen) x = make_uint4(0, 0, 0, 0);    // (bytes of tokens that nobody sees may be anything, and 0 * NaN is NaN)
+                        for (int half = 0; half < D / 64; ++half) {
+                            uint4 x = ptx::lds128((from ^ (64 * half)) + i * 8 * D);
+                            if (!seen) x = make_uint4(0, 0, 0, 0);            // (and 0 * NaN is NaN)
                             uint4 a, b;
                             decode4<E4M3>(x.x, a.x, a.y);
                             decode4<E4M3>(x.y, a.z, a.w);
                             decode4<E4M3>(x.z, b.x, b.y);
                             decode4<E4M3>(x.w, b.z, b.w);
-                            ptx::sts128(swizzled_mn(v_tile, token, 2 * c), a);
-                            ptx::sts128(swizzled_mn(v_tile, token, 2 * c + 1), b);
+                            ptx::sts128(to + half * kMnStride + i * 1024, a);
+                            ptx::sts128((to ^ 16) + half * kMnStride + i * 1024, b);
                         }
                     }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
                         arrive(&bars.v_full);
-                        arrive(&bars.empty[at]);
+                        arrive(&bars.values_empty[at]);
                     }
-                    ++half;
                 }
             }
             if (ok) done_with_item(n);
@@ -574,7 +609,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             const int columns = t.n / 2, row0 = h * columns, groups = columns / 8, tiles = t.tiles;
             const uint32_t buffers = t.n <= 64 ? 2 : 1;
             const int most_low = s_most_low[item_slot];
-            if (tid < kMostRows / 2) s_minus_top[h][tid] = -kNone;
+            if (tid < kMostRows / 2) {
+                s_minus_top[h][tid] = tid < columns ? -kNone : -INFINITY;     // (columns that are another half's, or nobody's, have no weights)
+                s_keep[h][tid] = 1.f;
+            }
             float sums[kMostRows / 2];
 #pragma unroll
             for (int i = 0; i < kMostRows / 2; ++i) sums[i] = 0.f;
@@ -584,69 +622,106 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 ok = wait_on(&bars.scale_full[i % kScales], i / kScales, &s_abort) && wait_on(&bars.s_full[i & 1], i >> 1, &s_abort);
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
-                const float4 sc = s_scale[i % kScales][tid >> 4];
+                const float4 sc = s_scale[i % kScales][tid >> page_shift];
                 const int first = (t.tile0 + j) * kTokens, token = first + tid;
-                const bool there = sc.w != 0.f && token >= t.lo && token < t.limit;
-                const bool whole = __all_sync(kAll, there) && first >= most_low;
-                const float a = factor * sc.x, b = sc.y, inverse = sc.z;
-                const uint32_t p_at = p_tile + (buffers == 2 ? (i & 1) * kMnStride : 0);
-                // exponents of 8 columns from `at` on, relative to the rows' references or not
-                const auto exponents = [&](uint32_t* x, int at, bool relative) {
+                const bool there = sc.w != 0.f && token >= t.lo && token < t.limit, hide = first < most_low;
+                // (keys of tokens that are not there are 0)
+                const float a = there ? factor * sc.x : 0.f, b = there ? sc.y : -INFINITY, inverse = sc.z;
+                if (j >= (int)buffers) {                                      // (what lay in the weights' place has been used)
+                    const uint32_t used = i - buffers;
+                    ok = wait_on(&bars.pv_done[used & 1], used >> 1, &s_abort);
+                    if (!ok) break;
+                }
+                const uint32_t s_at = s_col(i) + lanes + row0;
+                const uint32_t p_at = p_tile + (buffers == 2 ? (i & 1) * kMnStride : 0) + tid * 128, unit0 = row0 / 8;
+                // exponents of N columns from `at` on, relative to the rows' references or not
+                const auto exponents = [&](auto& x, int at, bool relative) {
+                    constexpr int N = sizeof(x) / 4;
 #pragma unroll
-                    for (int k = 0; k < 8; k += 2) {
-                        float2 y = make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-                        if (BF16) y = mul2(y, *reinterpret_cast<const float2*>(&s_up[item_slot][row0 + at + k]));
-                        float2 from = make_float2(b, b);
-                        if (relative) from = add2(from, *reinterpret_cast<const float2*>(&s_minus_top[h][at + k]));
-                        y = fma2(y, make_float2(a, a), from);
-                        if (!whole) {
-                            if (!there || token < s_low[item_slot][row0 + at + k]) y.x = -INFINITY;
-                            if (!there || token < s_low[item_slot][row0 + at + k + 1]) y.y = -INFINITY;
+                    for (int k = 0; k < N; k += 4) {
+                        float4 from = make_float4(b, b, b, b);
+                        float2 a0 = make_float2(a, a), a1 = a0, f0 = make_float2(b, b), f1 = f0;
+                        if (BF16) {
+                            const float4 up = *reinterpret_cast<const float4*>(&s_up[item_slot][row0 + at + k]);
+                            a0 = mul2(a0, make_float2(up.x, up.y));
+                            a1 = mul2(a1, make_float2(up.z, up.w));
                         }
-                        x[k] = __float_as_uint(y.x);
-                        x[k + 1] = __float_as_uint(y.y);
+                        if (relative) {
+                            from = *reinterpret_cast<const float4*>(&s_minus_top[h][at + k]);
+                            f0 = add2(f0, make_float2(from.x, from.y));
+                            f1 = add2(f1, make_float2(from.z, from.w));
+                        }
+                        const float2 y0 = fma2(make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), a0, f0);
+                        const float2 y1 = fma2(make_float2(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3])), a1, f1);
+                        x[k] = __float_as_uint(y0.x);
+                        x[k + 1] = __float_as_uint(y0.y);
+                        x[k + 2] = __float_as_uint(y1.x);
+                        x[k + 3] = __float_as_uint(y1.y);
+                    }
+                    if (hide) {
+#pragma unroll
+                        for (int k = 0; k < N; ++k) x[k] = token < s_low[item_slot][row0 + at + k] ? 0xFF800000u : x[k];
                     }
                 };
-                // do any weights outgrow fp16?
-                float most = -INFINITY;
+                // 16 columns at a time; a warp that comes upon a weight that outgrows fp16 stops there.  Then the rows' references move, and all begin again;
+                // what is in the totals already is not added twice.
+                int added = 0;
+                bool again = false;
+                for (;;) {
+                    bool over = false;
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (2 * c < groups) {
-                        uint32_t x[16];
-                        ptx::tmem_ld16(s_col(i) + lanes + row0 + 16 * c, x);
-                        ptx::tc_wait_ld();
-                        exponents(x, 16 * c, true);
+                    for (int c = 0; c < kMostRows / 32; ++c)
+                        if (2 * c < groups && !over) {
+                            uint32_t x[16];
+                            ptx::tmem_ld16(s_at + 16 * c, x);
+                            ptx::tc_wait_ld();
+                            exponents(x, 16 * c, true);
+                            if (!again) {
+                                float most = -INFINITY;
 #pragma unroll
-                        for (int k = 0; k < 8; k += 2) most = max3(most, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
-                        if (2 * c + 1 < groups) {
-                            exponents(x + 8, 16 * c + 8, true);
+                                for (int k = 0; k < 16; k += 2) most = max3(most, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                                over = __any_sync(kAll, most > kMostLog);
+                            }
+                            if (!over) {
 #pragma unroll
-                            for (int k = 8; k < 16; k += 2) most = max3(most, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                                for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(exp2_approx(__uint_as_float(x[k])));
+                                if (c >= added) {
+                                    added = c + 1;
+#pragma unroll
+                                    for (int k = 0; k < 16; k += 2) {
+                                        const float2 s2 = fma2(make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), make_float2(inverse, inverse),
+                                                               make_float2(sums[16 * c + k], sums[16 * c + k + 1]));
+                                        sums[16 * c + k] = s2.x;
+                                        sums[16 * c + k + 1] = s2.y;
+                                    }
+                                }
+#pragma unroll
+                                for (int q = 0; q < 2; ++q) {
+                                    uint32_t y[4];
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k)
+                                        y[k] = h2_as_u32(__floats2half2_rn(__uint_as_float(x[8 * q + 2 * k]), __uint_as_float(x[8 * q + 2 * k + 1])));
+                                    const uint32_t unit = unit0 + 2 * c + q;
+                                    if (2 * c + q < groups) ptx::sts128(p_at + (unit >> 3) * kMnStride + (((unit ^ tid) & 7) << 4), make_uint4(y[0], y[1], y[2], y[3]));
+                                }
+                            }
                         }
-                    }
-                ++pass;
-                if (most > kMostLog) s_need[h][pass & 1] = pass;
-                if (!(ok = meet(id_meet))) break;
-                if (s_need[h][pass & 1] == pass) {
-                    // then the rows' references move to their largest so far, and what there is of sums follows
+                    if (again) break;
+                    ++pass;
+                    if (over) s_need[h][pass & 1] = pass;
+                    if (!(ok = meet(id_meet))) break;
+                    if (s_need[h][pass & 1] != pass) break;
                     if (j > 0) ok = wait_on(&bars.pv_done[(i - 1) & 1], (i - 1) >> 1, &s_abort);
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        if (4 * c < groups) {
-                            uint32_t x[32];
-                            ptx::tmem_ld32(s_col(i) + lanes + row0 + 32 * c, x);
-                            ptx::tc_wait_ld();
-                            float y[32];
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                if (4 * c + q < groups) exponents(x + 8 * q, 32 * c + 8 * q, false);
-#pragma unroll
-                                for (int k = 8 * q; k < 8 * q + 8; ++k) y[k] = 4 * c + q < groups ? __uint_as_float(x[k]) : -INFINITY;
-                            }
-                            s_warps[h][w][32 * c + lane] = reduce32(y, [](float u, float v) { return fmaxf(u, v); });
-                        }
+#pragma unroll 1
+                    for (int c = 0; 4 * c < groups; ++c) {
+                        uint32_t x[32];
+                        ptx::tmem_ld32(s_at + 32 * c, x);
+                        ptx::tc_wait_ld();
+                        exponents(x, 32 * c, false);
+                        s_warps[h][w][32 * c + lane] = reduce32(x, [](float u, float v) { return fmaxf(u, v); });
+                    }
                     if (!(ok = meet(id_meet))) break;
                     if (tid < columns) {
                         const float old = -s_minus_top[h][tid];
@@ -658,50 +733,21 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                     }
                     if (!(ok = meet(id_meet))) break;
 #pragma unroll
-                    for (int q = 0; q < kMostRows / 16; ++q)
-                        if (q < groups) {
+                    for (int k = 0; k < kMostRows / 2; ++k) sums[k] *= s_keep[h][k];
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int q = 0; q < groups; ++q) {
+                            uint32_t x[8];
+                            ptx::tmem_ld8(o_col + lanes + row0 + 8 * q, x);
+                            ptx::tc_wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) sums[8 * q + k] *= s_keep[h][8 * q + k];
-                            if (j > 0) {
-                                uint32_t x[8];
-                                ptx::tmem_ld8(o_col + lanes + row0 + 8 * q, x);
-                                ptx::tc_wait_ld();
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * s_keep[h][8 * q + k]);
-                                ptx::tmem_st8(o_col + lanes + row0 + 8 * q, x);
-                            }
+                            for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * s_keep[h][8 * q + k]);
+                            ptx::tmem_st8(o_col + lanes + row0 + 8 * q, x);
                         }
-                    ptx::tc_wait_st();
-                }
-                if (j >= (int)buffers) {                                      // (what lay in the weights' place has been used)
-                    const uint32_t used = i - buffers;
-                    ok = wait_on(&bars.pv_done[used & 1], used >> 1, &s_abort);
-                    if (!ok) break;
-                }
-                const auto weigh = [&](uint32_t* x, int at) {                 // 8 columns
-                    exponents(x, at, true);
-                    float e[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) e[k] = exp2_approx(__uint_as_float(x[k]));
-#pragma unroll
-                    for (int k = 0; k < 8; k += 2) {
-                        const float2 s2 = fma2(make_float2(e[k], e[k + 1]), make_float2(inverse, inverse), make_float2(sums[at + k], sums[at + k + 1]));
-                        sums[at + k] = s2.x;
-                        sums[at + k + 1] = s2.y;
+                        ptx::tc_wait_st();
                     }
-                    ptx::sts128(swizzled_mn(p_at, tid, (row0 + at) / 8),
-                                make_uint4(h2_as_u32(__floats2half2_rn(e[0], e[1])), h2_as_u32(__floats2half2_rn(e[2], e[3])),
-                                           h2_as_u32(__floats2half2_rn(e[4], e[5])), h2_as_u32(__floats2half2_rn(e[6], e[7]))));
-                };
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (2 * c < groups) {
-                        uint32_t x[16];
-                        ptx::tmem_ld16(s_col(i) + lanes + row0 + 16 * c, x);
-                        ptx::tc_wait_ld();
-                        weigh(x, 16 * c);
-                        if (2 * c + 1 < groups) weigh(x + 8, 16 * c + 8);
-                    }
+                    again = true;
+                }
                 if (!ok) break;
                 ptx::tc_fence_before_sync();
                 ptx::fence_proxy_async_smem();
@@ -716,9 +762,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             // totals: over the lanes, then over the warps
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float y[32];
+                if (4 * c >= groups) continue;
+                uint32_t y[32];
 #pragma unroll
-                for (int k = 0; k < 32; ++k) y[k] = sums[32 * c + k];
+                for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(sums[32 * c + k]);
                 s_warps[h][w][32 * c + lane] = reduce32(y, [](float u, float v) { return u + v; });
             }
             if (!(ok = meet(id_meet))) break;
@@ -749,10 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 float* const parts = reinterpret_cast<float*>(header + p.prefix_parts);
                 const auto part_of = [&](int block) { return parts + ((size_t)block * 2 + (block == a ? 1 : 0)) * L::kPartFloats; };
                 float* const own = part_of(blockIdx.x);
-                if (tid < columns) {
-                    own[kMostRows * D + row0 + tid] = reference(tid);
-                    own[kMostRows * D + kMostRows + row0 + tid] = total_of(tid);
-                }
+                if (tid < columns) *reinterpret_cast<float2*>(own + kMostRows * D + 2 * (row0 + tid)) = make_float2(reference(tid), total_of(tid));
 #pragma unroll 1
                 for (int c = 0; 4 * c < groups; ++c) {
                     uint32_t x[32];
@@ -778,23 +822,40 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 if (!(ok = meet(id_meet))) break;
                 if (s_last[h]) {
                     __threadfence();
-                    for (int r = tid / D; r < columns; r += 128 / D) {
-                        const int row = row0 + r, id = s_row[item_slot][row], d = tid % D;
+                    using Columns = std::conditional_t<D == 128, float4, float2>;             // of a lane
+                    for (int r = w; r < columns; r += 4) {
+                        const int row = row0 + r, id = s_row[item_slot][row];
                         if (id < 0) continue;
+                        const auto both = [&](int b) { return __ldcg(reinterpret_cast<const float2*>(part_of(b) + kMostRows * D + 2 * row)); };
                         float m = -INFINITY;
-#pragma unroll 4
-                        for (int b = a; b <= z; ++b) m = fmaxf(m, __ldcg(part_of(b) + kMostRows * D + row));
+                        for (int b = a + lane; b <= z; b += 32) m = fmaxf(m, both(b).x);
+#pragma unroll
+                        for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(kAll, m, d));
                         const float from = m == -INFINITY ? 0.f : m;
-                        float all_total = 0.f, o = 0.f;
+                        float all_total = 0.f;
+                        Columns o{};
+                        for (int b0 = a; b0 <= z; b0 += 32) {
+                            float2 mine = make_float2(-INFINITY, 0.f);
+                            if (b0 + lane <= z) mine = both(b0 + lane);
+                            const float take = exp2_approx(mine.x - from);
+                            all_total = fmaf(take, mine.y, all_total);
+                            const int count = min(32, z - b0 + 1);
 #pragma unroll 4
-                        for (int b = a; b <= z; ++b) {
-                            const float* const part = part_of(b);
-                            const float take = exp2_approx(__ldcg(part + kMostRows * D + row) - from);
-                            all_total = fmaf(take, __ldcg(part + kMostRows * D + kMostRows + row), all_total);
-                            o = fmaf(take, __ldcg(part + row * D + d), o);
+                            for (int i = 0; i < count; ++i) {
+                                const Columns x = __ldcg(reinterpret_cast<const Columns*>(part_of(b0 + i) + row * D) + lane);
+                                const float f = __shfl_sync(kAll, take, i);
+                                o.x = fmaf(f, x.x, o.x);
+                                o.y = fmaf(f, x.y, o.y);
+                                if constexpr (D == 128) {
+                                    o.z = fmaf(f, x.z, o.z);
+                                    o.w = fmaf(f, x.w, o.w);
+                                }
+                            }
                         }
-                        p.prefix_sums[(long long)id * D + d] = o;
-                        if (d == 0) p.prefix_total[id] = make_float2(m, all_total);
+#pragma unroll
+                        for (int d = 16; d; d /= 2) all_total += __shfl_xor_sync(kAll, all_total, d);
+                        reinterpret_cast<Columns*>(p.prefix_sums + (long long)id * D)[lane] = o;
+                        if (lane == 0) p.prefix_total[id] = make_float2(m, all_total);
                     }
                 }
                 if (!(ok = meet(id_meet))) break;                             // (s_last is free again)
@@ -818,7 +879,7 @@ cudaError_t launch_prefix(const AttentionParams& p, cudaStream_t stream) {
     const auto kernel = cache_prefix_kernel<E4M3, BF16, D>;
     constexpr int kSmem = Layout<D>::kBytes;
     CUtensorMap k_map, v_map;
-    if (!cache_map(&k_map, p.cache, true) || !cache_map(&v_map, p.cache, false)) return cudaErrorNotSupported;
+    if (!cache_map(&k_map, p.cache, true, 1 << p.cache.page_shift) || !cache_map(&v_map, p.cache, false, 1 << p.cache.page_shift)) return cudaErrorNotSupported;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

@@ -723,7 +723,7 @@ cudaError_t launch_rows(const AttentionParams& p, int most_rows, cudaStream_t st
     const auto kernel = cache_rows_kernel<E4M3, BF16, D, NT, PREFIX>;
     constexpr int kSmem = S::kWarps * S::kWarpBytes + 1024;
     CUtensorMap k_map, v_map;
-    if (!cache_map(&k_map, p.cache, true) || !cache_map(&v_map, p.cache, false)) return cudaErrorNotSupported;
+    if (!cache_map(&k_map, p.cache, true, 16) || !cache_map(&v_map, p.cache, false, 16)) return cudaErrorNotSupported;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
