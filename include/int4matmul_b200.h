@@ -324,7 +324,8 @@ int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int 
  * that must know which kernel they exercised. */
 #define I4MM_ATTENTION_FEW_ROWS 1
 #define I4MM_ATTENTION_PROMPT 2
-#define I4MM_ATTENTION_PREFIX 4
+#define I4MM_ATTENTION_PREFIX 4           /* prefixes that few rows read */
+#define I4MM_ATTENTION_MANY_READERS 8     /* prefixes that many rows read */
 int i4mm_last_attention_kernels(void);
 
 /*

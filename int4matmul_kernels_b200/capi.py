@@ -30,7 +30,7 @@ class Cache(ctypes.Structure):
 
 CACHE_INT8, CACHE_E4M3 = 0, 1
 TYPE_FP16, TYPE_BF16 = 0, 1
-ATTENTION_FEW_ROWS, ATTENTION_PROMPT, ATTENTION_PREFIX = 1, 2, 4    # i4mm_last_attention_kernels
+ATTENTION_FEW_ROWS, ATTENTION_PROMPT, ATTENTION_PREFIX, ATTENTION_MANY_READERS = 1, 2, 4, 8    # i4mm_last_attention_kernels
 
 # every symbol the header declares, with its ctypes signature
 _SIGNATURES = {

@@ -22,6 +22,7 @@ __device__ __forceinline__ void cp_async_8(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void prefetch_l1(const void* at) { asm volatile("prefetch.global.L1 [%0];" ::"l"(at)); }
 // 4-D tiled tensor-map copy, coordinates (x = innermost, y, z, w)
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int x, int y, int z, int w, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
@@ -50,7 +51,7 @@ constexpr size_t kRowsCounters = 0;                   // one per block
 constexpr size_t kPromptNext = 4096;                  // the next item to be worked on
 constexpr size_t kPromptCounters = 8192;              // two per part
 constexpr int kPromptParts = 320;
-constexpr size_t kPrefixCounters = 16384;             // two per block
+constexpr size_t kPrefixCounters = 16384;             // four per block
 
 struct Request {
     int row0, rows;                                   // its packed rows
@@ -183,6 +184,21 @@ __device__ __forceinline__ Joint join_prefix(float m, float sum, float2 prefix) 
     const float total = fmaf(sum, a, prefix.y * b), f = total > 0.f ? 1.f / total : total;      // (a NaN stays one)
     return {a * f, b * f};
 }
+// the position of packed row `token`, which reads the prefix at `place`, that prefix counted
+__device__ __forceinline__ int behind_prefix(const AttentionParams& p, int place, int token) {
+    int b = min(token, p.requests - 1);
+    if (p.cu_lens) {
+        int hi = p.requests - 1;
+#pragma unroll 1
+        for (b = 0; b < hi;) {
+            const int mid = (b + hi + 1) >> 1;
+            if (p.cu_lens[mid] <= token) b = mid;
+            else hi = mid - 1;
+        }
+    }
+    const long long position = (long long)p.seq_lens[place] + p.seq_lens[b] - (p.cu_lens ? p.cu_lens[b + 1] : b + 1) + token;
+    return (int)min(max(position, 0ll), 0x7FFFFFFEll);
+}
 // whether a row of request b at this position sees a prefix
 __device__ __forceinline__ bool sees_prefix(const AttentionParams& p, int b, int position) { return position >= 0 && p.prefix_of[b] >= 0; }
 
@@ -205,8 +221,10 @@ inline bool cache_map(CUtensorMap* out, const CacheView& c, bool keys, int token
 // With p.prefix_of set, both add what p.prefix_total and p.prefix_sums say to each row that has a prefix.
 cudaError_t cache_rows_launch(const AttentionParams& p, bool e4m3, bool bf16, int most_rows, bool few, cudaStream_t stream);
 cudaError_t cache_prompt_launch(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, bool alone, cudaStream_t stream);
-// Rows of all requests that share a prefix over that prefix, into p.prefix_total and p.prefix_sums.
-cudaError_t cache_prefix_launch(const AttentionParams& p, bool e4m3, bool bf16, cudaStream_t stream);
+// Rows of all requests that share a prefix over that prefix, into p.prefix_total and p.prefix_sums: of prefixes that up to most_rows rows of a key
+// head read, and of those that least_rows read or more.
+cudaError_t cache_prefix_launch(const AttentionParams& p, bool e4m3, bool bf16, int most_rows, cudaStream_t stream);
+cudaError_t cache_many_readers_launch(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, cudaStream_t stream);
 size_t cache_rows_workspace();                        // bytes behind the header
 size_t cache_prompt_workspace();                      // bytes behind those
 size_t cache_prefix_workspace();                      // and behind those

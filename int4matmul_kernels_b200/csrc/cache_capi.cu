@@ -104,6 +104,18 @@ cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t
     return e != cudaSuccess ? e : prompt(i4mm::kFewRows + 1, false);
 }
 
+// The rows that read prefixes over those.  Both kernels run where the step's rows are more than the first one takes.
+constexpr int kFewReaders = 128;                      // rows of a key head
+cudaError_t attend_prefixes(const i4mm::AttentionParams& p, bool e4m3, bool bf16, cudaStream_t stream) {
+    g_attention_kernels |= I4MM_ATTENTION_PREFIX;
+    cudaError_t e = i4mm::cache_prefix_launch(p, e4m3, bf16, kFewReaders, stream);
+    if (e == cudaSuccess && (int64_t)p.tokens * p.group > kFewReaders) {
+        g_attention_kernels |= I4MM_ATTENTION_MANY_READERS;
+        e = i4mm::cache_many_readers_launch(p, e4m3, bf16, kFewReaders + 1, stream);
+    }
+    return e;
+}
+
 // A step's shared prefixes, as i4mm_cache_share lays them out; prefix_of nullptr: none
 struct Prefixes {
     const void *prefix_of, *starts, *rows;
@@ -166,9 +178,8 @@ int attention(const i4mm_cache* cache, void* out, const void* q, int type, int64
     p.scale = scale;
     const bool e4m3 = cache->type == I4MM_CACHE_E4M3, bf16 = type == I4MM_TYPE_BF16;
     if (p.prefix_of && requests > 0) {
-        const cudaError_t e = i4mm::cache_prefix_launch(p, e4m3, bf16, (cudaStream_t)stream);
+        const cudaError_t e = attend_prefixes(p, e4m3, bf16, (cudaStream_t)stream);
         if (e != cudaSuccess) return finish(e);
-        g_attention_kernels |= I4MM_ATTENTION_PREFIX;
     }
     return finish(attend(p, e4m3, bf16, max_len, (cudaStream_t)stream));
 }

@@ -31,7 +31,9 @@ namespace {
 
 constexpr int kTokens = 128;                          // of a tile
 constexpr int kMostRows = 128;
-constexpr int kSoftmaxWarps = 8, kDecode0 = 8, kDecodeWarps = 4, kMma = 12, kCopy = 13, kCopyValues = 14, kThreads = 15 * 32;
+constexpr int kGroups = 4, kColumns = kMostRows / kGroups;                    // of softmax warps; columns of each
+constexpr int kSoftmaxWarps = 4 * kGroups, kDecode0 = kSoftmaxWarps, kDecodeWarps = 4, kMma = kDecode0 + 4, kCopy = kMma + 1, kCopyValues = kCopy + 1;
+constexpr int kThreads = 32 * (kCopyValues + 1);
 constexpr int kKeys = 3, kValues = 4;                 // stages of the rings
 constexpr int kItems = 4, kScales = 4, kRawScales = 8;
 constexpr int kPieces = kTokens / 16;                 // pages of a tile, at most
@@ -52,7 +54,7 @@ struct Layout {
 constexpr size_t kPartsBytes = (size_t)kMaxBlocks * 2 * Layout<128>::kPartFloats * 4;
 
 struct Item {
-    int valid, place, head, base, rows, n;            // base: first row of the tile; n: rows, rounded up to 16
+    int valid, place, head, base, rows, n;            // base: first row of the tile; n: rows, rounded up to 32
     int first;                                        // of the place's readers in the list
     int lo, limit;                                    // tokens that may be seen
     int tile0, tiles;
@@ -66,14 +68,18 @@ struct Barriers {
 };
 
 // A whole warp waits; false (in all of its lanes) once the block gives up.
-__device__ __forceinline__ bool wait_on(unsigned long long* bar, uint32_t parity, volatile int* abort) {
-    const uint32_t at = ptx::smem_u32(bar);
+__device__ __noinline__ bool wait_longer(uint32_t at, uint32_t parity, volatile int* abort) {
     for (uint32_t i = 0; i < ptx::kSpinLimit; ++i) {
-        if (__all_sync(kAll, ptx::mbar_try_wait(at, parity & 1))) return true;
+        if (__all_sync(kAll, ptx::mbar_try_wait(at, parity))) return true;
         if (__any_sync(kAll, *abort)) return false;
     }
     *abort = 1;
     return false;
+}
+__device__ __forceinline__ bool wait_on(unsigned long long* bar, uint32_t parity, volatile int* abort) {
+    const uint32_t at = ptx::smem_u32(bar);
+    if (__all_sync(kAll, ptx::mbar_try_wait(at, parity & 1))) return true;
+    return wait_longer(at, parity & 1, abort);
 }
 __device__ __forceinline__ void arrive(unsigned long long* bar) { ptx::mbar_arrive(ptx::smem_u32(bar)); }
 
@@ -83,17 +89,18 @@ struct Place {
     int lo, limit, tiles;                             // tokens that any row sees; at least one tile, so that all rows are written
     int row_tiles, height;                            // rows of a row tile: all of a place alike
 };
-__device__ __forceinline__ Place load_place(const AttentionParams& p, int b) {
+__device__ __forceinline__ Place load_place(const AttentionParams& p, int most_rows, int b) {
     Place r;
     const int from = min(max(p.prefix_starts[b], 0), p.prefix_listed), to = min(max(p.prefix_starts[b + 1], 0), p.prefix_listed), seq = p.seq_lens[b];
     r.first = from;
     r.rows = min(max(to - from, 0), p.tokens) * p.group;                      // (tokens * q_heads is below 2^31)
+    if (r.rows > most_rows) r.rows = 0;                                       // the other kernel's
     r.limit = max(min(seq, p.table_width << p.cache.page_shift), 0);
     r.lo = p.window && seq >= p.window ? min(seq - p.window + 1, r.limit) : 0;
     r.tiles = max((r.limit + kTokens - 1) / kTokens - r.lo / kTokens, 1);
     r.row_tiles = (r.rows + kMostRows - 1) / kMostRows;
-    r.height = (r.rows + 15) & ~15;
-    if (r.row_tiles > 1) r.height = (int)(((uint32_t)r.rows + 16u * r.row_tiles - 1) / (16u * r.row_tiles)) * 16;
+    r.height = (r.rows + 31) & ~31;
+    if (r.row_tiles > 1) r.height = (int)(((uint32_t)r.rows + 32u * r.row_tiles - 1) / (32u * r.row_tiles)) * 32;
     return r;
 }
 __device__ __forceinline__ long long units_of(const AttentionParams& p, const Place& r) { return (long long)(r.row_tiles * p.cache.heads) * r.tiles; }
@@ -153,7 +160,7 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr) {
 constexpr uint32_t kBothMn = (1u << 15) | (1u << 16); // of an instruction descriptor: A and B lie so
 
 template <bool E4M3, bool BF16, int D>
-__global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const AttentionParams p, const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const AttentionParams p, int most_rows, const __grid_constant__ CUtensorMap k_map,
                                                                    const __grid_constant__ CUtensorMap v_map) {
     using L = Layout<D>;
     extern __shared__ uint8_t dynamic[];
@@ -166,11 +173,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     __shared__ int s_low[kItems][kMostRows];          // the first token that the row sees
     __shared__ float s_up[kItems][kMostRows];         // what its scores are multiplied with (bf16)
     __shared__ int s_most_low[kItems];
-    __shared__ __align__(16) float s_minus_top[2][kMostRows / 2];             // the rows' references, their signs turned over
-    __shared__ __align__(16) float s_keep[2][kMostRows / 2];
-    __shared__ float s_warps[2][4][kMostRows / 2];
-    __shared__ volatile uint32_t s_need[2][2];
-    __shared__ volatile int s_abort, s_last[2];
+    __shared__ __align__(16) float s_minus_top[kGroups][kColumns];            // the rows' references, their signs turned over
+    __shared__ __align__(16) float s_keep[kGroups][kColumns];
+    __shared__ float s_warps[kGroups][4][kColumns];
+    __shared__ volatile uint32_t s_need[kGroups][2];
+    __shared__ volatile int s_abort, s_last[kGroups];
     __shared__ uint32_t tmem_smem;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem = (ptx::smem_u32(dynamic) + 1023u) & ~1023u;
@@ -181,20 +188,25 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
 
     if (threadIdx.x == 0) {
         const auto init = [](unsigned long long& b, uint32_t n) { ptx::mbar_init(ptx::smem_u32(&b), n); };
+#pragma unroll 1
         for (int i = 0; i < kItems; ++i) {
             init(bars.item_full[i], 1);
             init(bars.item_empty[i], kSoftmaxWarps + kDecodeWarps + 2);
             init(bars.q_full[i], kDecodeWarps);
         }
+#pragma unroll 1
         for (int i = 0; i < kKeys; ++i) {
             init(bars.keys_full[i], 2 * pieces);      // each lane's bytes, and its scales
             init(bars.keys_empty[i], kDecodeWarps);
         }
+#pragma unroll 1
         for (int i = 0; i < kValues; ++i) {
             init(bars.values_full[i], pieces);
             init(bars.values_empty[i], kDecodeWarps);
         }
+#pragma unroll 1
         for (int i = 0; i < kScales; ++i) init(bars.scale_full[i], 1);
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
             init(bars.k_full[i], kDecodeWarps);
             init(bars.s_full[i], 1);
@@ -205,9 +217,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
         init(bars.drained, 1);
         ptx::fence_mbar_init();
         s_abort = 0;
-        for (int i = 0; i < 4; ++i) s_need[i >> 1][i & 1] = 0;
+#pragma unroll 1
+        for (int i = 0; i < 2 * kGroups; ++i) s_need[i >> 1][i & 1] = 0;
     }
     if (D == 64)                                      // the columns of V that there are not
+#pragma unroll 1
         for (int i = threadIdx.x; i < (int)kMnStride / 16; i += kThreads) ptx::sts128(v_tile + kMnStride + 16 * i, make_uint4(0, 0, 0, 0));
     ptx::fence_proxy_async_smem();
     if (warp == kMma) {
@@ -247,6 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             if (lane < pieces && token < t.limit && token + (1 << page_shift) > t.lo && i < p.table_width) page = table[i];
         };
         find_page(0);
+#pragma unroll 1
         for (int j = 0; j < t.tiles; ++j, ++g) {
             const int id = (unsigned int)page < (unsigned int)cache.pages ? page : -1;
             if (j + 1 < t.tiles) find_page(j + 1);
@@ -276,34 +291,34 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     };
     // A block that gives up waits, bounded again, for what is on its way to its rings: the shared memory is someone else's once it has ended.
     const auto landed = [&](unsigned long long* full, uint32_t stages) {
+#pragma unroll 1
         for (uint32_t i = fetched > stages ? fetched - stages : 0; i < fetched; ++i) (void)ptx::mbar_wait(ptx::smem_u32(&full[i % stages]), (i / stages) & 1);
     };
 
     if (warp == kCopy) {
-        // the block's range
-        long long total = 0, at = 0, end = 0;
-#pragma unroll 4
-        for (int b = lane; b < p.requests; b += 32) total += units_of(p, load_place(p, b));
+        // the block's range: all have the same number of tiles, but for those at the end
+        long long total = 0;
+#pragma unroll 1
+        for (int b = lane; b < p.requests; b += 32) total += units_of(p, load_place(p, most_rows, b));
         total = warp_sum(total);
-        const int blocks = (int)min((long long)gridDim.x, (total + kMinBlockTiles - 1) / kMinBlockTiles);
-        if ((int)blockIdx.x < blocks) {
-            at = range_lo(total, blocks, blockIdx.x);
-            end = range_lo(total, blocks, blockIdx.x + 1);
-        }
+        const long long share = max(div_nn(total + gridDim.x - 1, gridDim.x), (long long)kMinBlockTiles);
+        long long at = blockIdx.x * share;
+        const long long end = min(at + share, total);
         // the place that the range begins in
         long long before = 0;
         int b = 0;
         Place r{};
         const auto find_place = [&]() {               // from request b (a multiple of 32) on, `before` tiles before it
+#pragma unroll 1
             for (; b < p.requests; b += 32) {
-                const Place mine = b + lane < p.requests ? load_place(p, b + lane) : Place{};
+                const Place mine = b + lane < p.requests ? load_place(p, most_rows, b + lane) : Place{};
                 const long long own = b + lane < p.requests ? units_of(p, mine) : 0, upto = warp_prefix(own);
                 const uint32_t here = __ballot_sync(kAll, before + upto > at);
                 if (here) {
                     const int l = __ffs(here) - 1;
                     before += __shfl_sync(kAll, upto - own, l);
                     b += l;
-                    r = load_place(p, b);
+                    r = load_place(p, most_rows, b);
                     return;
                 }
                 before += __shfl_sync(kAll, upto, 31);
@@ -311,14 +326,16 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
         };
         uint32_t n = 0, g = 0;                        // items, tiles so far
         bool ok = true;
+#pragma unroll 1
         while (ok && at < end) {
             if (n == 0 || at >= before + units_of(p, r)) {
                 // (the next place with rows: from the multiple of 32 at or below the current one, whose earlier tiles are counted again)
                 if (n > 0) {
                     before += units_of(p, r);
                     ++b;
+#pragma unroll 1
                     for (; b < p.requests && (b & 31); ++b) {
-                        r = load_place(p, b);
+                        r = load_place(p, most_rows, b);
                         if (r.rows > 0) break;
                     }
                     if (b < p.requests && !(b & 31)) find_place();
@@ -337,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 t.head = head;
                 t.base = row_tile * r.height;
                 t.rows = max(min(r.height, r.rows - t.base), 0);
-                t.n = max((t.rows + 15) & ~15, 16);
+                t.n = max((t.rows + 31) & ~31, 32);
                 t.first = r.first;
                 t.lo = r.lo;
                 t.limit = r.limit;
@@ -346,8 +363,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 t.first_block = t.last_block = (int)blockIdx.x;
                 if (t.tiles < r.tiles) {
                     const long long from = at - tile;
-                    t.first_block = range_owner(total, blocks, from);
-                    t.last_block = range_owner(total, blocks, from + r.tiles - 1);
+                    t.first_block = (int)div_nn(from, share);
+                    t.last_block = (int)div_nn(from + r.tiles - 1, share);
                 }
             }
             ok = wait_on(&bars.item_empty[n % kItems], (n / kItems) ^ 1, &s_abort);
@@ -371,6 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     } else if (warp == kCopyValues) {
         uint32_t g = 0;
         bool ok = true;
+#pragma unroll 1
         for (uint32_t n = 0; ok; ++n) {
             ok = next_item(n);
             if (!ok || !items[n % kItems].valid) break;
@@ -384,6 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
         // ---- products ----
         uint32_t g = 0;
         bool ok = true;
+#pragma unroll 1
         for (uint32_t n = 0; ok; ++n) {
             ok = next_item(n);
             if (!ok || !items[n % kItems].valid) break;
@@ -405,6 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             };
             score(g);
             if (tiles > 1) score(g + 1);
+#pragma unroll 1
             for (int j = 0; j < tiles && ok; ++j) {
                 const uint32_t i = g + j;
                 ok = wait_on(&bars.v_full, i, &s_abort) && wait_on(&bars.p_full[i & 1], i >> 1, &s_abort);
@@ -425,14 +445,16 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
         // nothing of this block may be in flight when its tensor memory goes
         if (ptx::elect_one()) ptx::tc_commit(ptx::smem_u32(&bars.drained));
         __syncwarp();
+#pragma unroll 1
         for (uint32_t i = 0; i < ptx::kSpinLimit && !ptx::mbar_try_wait(ptx::smem_u32(&bars.drained), 0); ++i) {}
     } else if (warp >= kDecode0) {
         // ---- queries; bytes to operands ----
-        constexpr int kMeet = 3;
+        constexpr int kMeet = kGroups + 1;
         const int w = warp - kDecode0, tid = w * 32 + lane;
         constexpr int kUnits = D / 8;                 // of 16 bytes in a query
         uint32_t g = 0;
         bool ok = true;
+#pragma unroll 1
         for (uint32_t n = 0; ok; ++n) {
             ok = next_item(n);
             if (!ok || !items[n % kItems].valid) break;
@@ -449,18 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                         id = token * p.q_heads + h;
                         query = token * p.q.token + h * p.q.head;
                         if (p.window) {
-                            int b = token;
-                            if (p.cu_lens) {
-                                int hi = p.requests - 1;
-                                for (b = 0; b < hi;) {
-                                    const int mid = (b + hi + 1) >> 1;
-                                    if (p.cu_lens[mid] <= token) b = mid;
-                                    else hi = mid - 1;
-                                }
-                            }
-                            b = min(b, p.requests - 1);
-                            const long long position = (long long)p.seq_lens[t.place] + p.seq_lens[b] - (p.cu_lens ? p.cu_lens[b + 1] : b + 1) + token;
-                            low = (int)min(max(position - p.window + 1, 0ll), (long long)t.limit);
+                            low = min(max(behind_prefix(p, t.place, token) - p.window + 1, 0), t.limit);
                         }
                     }
                 }
@@ -479,7 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             if (!(ok = meet(kMeet))) break;
             // (the scores of the item before are complete)
             if (g > 0 && !(ok = wait_on(&bars.s_full[(g - 1) & 1], (g - 1) >> 1, &s_abort))) break;
-            constexpr int kAtOnce = 8, kRowsAtOnce = 32 / kUnits;             // of a warp
+            constexpr int kAtOnce = 4, kRowsAtOnce = 32 / kUnits;             // of a warp
+#pragma unroll 1
             for (int r0 = w * kRowsAtOnce; r0 < t.n; r0 += kAtOnce * 4 * kRowsAtOnce) {
                 uint4 x[kAtOnce];
 #pragma unroll
@@ -510,95 +522,102 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             __syncwarp();
             if (lane == 0) arrive(&bars.q_full[slot]);
 
-            for (int j = 0; j < t.tiles && ok; ++j, ++g) {
+            const auto seen_at = [&](uint32_t g, int first, int token) {
+                return first + token >= t.lo && first + token < t.limit && __float_as_uint(s_raw[g % kRawScales][token >> page_shift].x) != kNoPage;
+            };
+            const auto all_there = [&](uint32_t g, int first) {
+                return __all_sync(kAll, __float_as_uint(s_raw[g % kRawScales][lane & (pieces - 1)].x) != kNoPage) && first >= t.lo && first + kTokens <= t.limit;
+            };
+            // keys: a thread a token
+            const auto keys = [&](int j) -> bool {
+                const uint32_t i = g + j, at = i % kKeys;
                 const int first = (t.tile0 + j) * kTokens;
-                bool all;                             // whether all of the tile's tokens are there
-                // keys: a thread a token
-                {
-                    const uint32_t at = g % kKeys, from = keys_ring + at * L::kHalf + tid * D;
-                    ok = wait_on(&bars.keys_full[at], g / kKeys, &s_abort);
-                    if (!ok) break;
-                    const float2 raw = s_raw[g % kRawScales][lane & (pieces - 1)];
-                    const bool page = __float_as_uint(raw.x) != kNoPage;
-                    if (w == 0 && lane < pieces) {
-                        const float value = fmaxf(raw.y, kLeastScale);
-                        s_scale[g % kScales][lane] = page ? make_float4(raw.x, log2_approx(value), 1.f / value, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (!wait_on(&bars.keys_full[at], i / kKeys, &s_abort)) return false;
+                if (w == 0 && lane < pieces) {
+                    const float2 raw = s_raw[i % kRawScales][lane];
+                    const float value = fmaxf(raw.y, kLeastScale);
+                    s_scale[i % kScales][lane] = __float_as_uint(raw.x) != kNoPage ? make_float4(raw.x, log2_approx(value), 1.f / value, 1.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                const bool all = all_there(i, first), seen = all || seen_at(i, first, tid);
+                if (i >= 2 && !wait_on(&bars.s_full[i & 1], (i >> 1) - 1, &s_abort)) return false;             // (the keys that lay there have been used)
+                const uint32_t from = keys_ring + at * L::kHalf + tid * D, to = k_col(i) + ((uint32_t)(w * 32) << 16);
+                const uint32_t swizzle = D == 128 ? (lane & 7) << 4 : ((lane >> 1) & 3) << 4;
+#pragma unroll 1
+                for (int c0 = 0; c0 < D / 16; c0 += 4) {
+                    uint32_t out[32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint4 x = ptx::lds128(from + ((16 * (c0 + c)) ^ swizzle));
+                        decode4<E4M3>(x.x, out[8 * c], out[8 * c + 1]);
+                        decode4<E4M3>(x.y, out[8 * c + 2], out[8 * c + 3]);
+                        decode4<E4M3>(x.z, out[8 * c + 4], out[8 * c + 5]);
+                        decode4<E4M3>(x.w, out[8 * c + 6], out[8 * c + 7]);
                     }
-                    all = __all_sync(kAll, page) && first >= t.lo && first + kTokens <= t.limit;
-                    const bool seen = all || (first + tid >= t.lo && first + tid < t.limit && __float_as_uint(s_raw[g % kRawScales][tid >> page_shift].x) != kNoPage);
-                    if (g >= 2) ok = wait_on(&bars.s_full[g & 1], (g >> 1) - 1, &s_abort);         // (the keys that lay there have been used)
-                    if (!ok) break;
-                    const uint32_t to = k_col(g) + ((uint32_t)(w * 32) << 16), swizzle = D == 128 ? (lane & 7) << 4 : ((lane >> 1) & 3) << 4;
+                    if (!all) {                       // (bytes of tokens that nobody sees may be anything)
 #pragma unroll
-                    for (int c0 = 0; c0 < D / 16; c0 += 4) {
-                        uint32_t out[32];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const uint4 x = ptx::lds128(from + ((16 * (c0 + c)) ^ swizzle));
-                            decode4<E4M3>(x.x, out[8 * c], out[8 * c + 1]);
-                            decode4<E4M3>(x.y, out[8 * c + 2], out[8 * c + 3]);
-                            decode4<E4M3>(x.z, out[8 * c + 4], out[8 * c + 5]);
-                            decode4<E4M3>(x.w, out[8 * c + 6], out[8 * c + 7]);
-                        }
-                        if (!all) {                   // (bytes of tokens that nobody sees may be anything)
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) out[k] = seen ? out[k] : 0;
-                        }
-                        ptx::tmem_st32(to + 8 * c0, out);
+                        for (int k = 0; k < 32; ++k) out[k] = seen ? out[k] : 0;
                     }
-                    ptx::tc_wait_st();
-                    ptx::tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) {
-                        arrive(&bars.k_full[g & 1]);
-                        arrive(&bars.keys_empty[at]);
-                        if (w == 0) arrive(&bars.scale_full[g % kScales]);
+                    ptx::tmem_st32(to + 8 * c0, out);
+                }
+                ptx::tc_wait_st();
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    arrive(&bars.k_full[i & 1]);
+                    arrive(&bars.keys_empty[at]);
+                    if (w == 0) arrive(&bars.scale_full[i % kScales]);
+                }
+                return true;
+            };
+            // values: 8 tokens and 4 units of 16 at a time, in an order whose lanes meet in no bank
+            const auto values = [&](int j) -> bool {
+                const uint32_t i = g + j, at = i % kValues;
+                const int first = (t.tile0 + j) * kTokens;
+                if (!wait_on(&bars.values_full[at], i / kValues, &s_abort)) return false;
+                if (i >= 1 && !wait_on(&bars.pv_done[(i - 1) & 1], (i - 1) >> 1, &s_abort)) return false;
+                const bool all = all_there(i, first);
+                const int in8 = (lane >> 3) ^ (lane & 4 ? 5 : 0), token0 = w * 32 + in8, unit = lane & 3;
+                const uint32_t from = values_ring + at * L::kHalf + token0 * D + ((16 * unit) ^ (D == 128 ? in8 << 4 : ((in8 >> 1) & 3) << 4));
+                const uint32_t to = v_tile + token0 * 128 + ((32 * unit) ^ (in8 << 4));
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    const bool seen = all || seen_at(i, first, token0 + 8 * q);
+#pragma unroll
+                    for (int half = 0; half < D / 64; ++half) {
+                        uint4 x = ptx::lds128((from ^ (64 * half)) + q * 8 * D);
+                        if (!seen) x = make_uint4(0, 0, 0, 0);                // (0 * NaN is NaN)
+                        uint4 a, b;
+                        decode4<E4M3>(x.x, a.x, a.y);
+                        decode4<E4M3>(x.y, a.z, a.w);
+                        decode4<E4M3>(x.z, b.x, b.y);
+                        decode4<E4M3>(x.w, b.z, b.w);
+                        ptx::sts128(to + half * kMnStride + q * 1024, a);
+                        ptx::sts128((to ^ 16) + half * kMnStride + q * 1024, b);
                     }
                 }
-                // values: 8 tokens and 4 units of 16 at a time, in an order whose lanes meet in no bank
-                {
-                    const uint32_t at = g % kValues;
-                    ok = wait_on(&bars.values_full[at], g / kValues, &s_abort);
-                    if (ok && g >= 1) ok = wait_on(&bars.pv_done[(g - 1) & 1], (g - 1) >> 1, &s_abort);
-                    if (!ok) break;
-                    const int in8 = (lane >> 3) ^ (lane & 4 ? 5 : 0), token0 = w * 32 + in8, unit = lane & 3;
-                    const uint32_t from = values_ring + at * L::kHalf + token0 * D + ((16 * unit) ^ (D == 128 ? in8 << 4 : ((in8 >> 1) & 3) << 4));
-                    const uint32_t to = v_tile + token0 * 128 + ((32 * unit) ^ (in8 << 4));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int token = token0 + 8 * i;
-                        const bool seen = all || (first + token >= t.lo && first + token < t.limit && __float_as_uint(s_raw[g % kRawScales][token >> page_shift].x) != kNoPage);
-#pragma unroll
-                        for (int half = 0; half < D / 64; ++half) {
-                            uint4 x = ptx::lds128((from ^ (64 * half)) + i * 8 * D);
-                            if (!seen) x = make_uint4(0, 0, 0, 0);            // (and 0 * NaN is NaN)
-                            uint4 a, b;
-                            decode4<E4M3>(x.x, a.x, a.y);
-                            decode4<E4M3>(x.y, a.z, a.w);
-                            decode4<E4M3>(x.z, b.x, b.y);
-                            decode4<E4M3>(x.w, b.z, b.w);
-                            ptx::sts128(to + half * kMnStride + i * 1024, a);
-                            ptx::sts128((to ^ 16) + half * kMnStride + i * 1024, b);
-                        }
-                    }
-                    ptx::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        arrive(&bars.v_full);
-                        arrive(&bars.values_empty[at]);
-                    }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    arrive(&bars.v_full);
+                    arrive(&bars.values_empty[at]);
                 }
-            }
+                return true;
+            };
+            // (the next tile's keys come first, so that its scores do not wait for this one's products)
+#pragma unroll 1
+            for (int j = 0; j <= t.tiles && ok; ++j) ok = (j == t.tiles || keys(j)) && (j == 0 || values(j - 1));
+            g += t.tiles;
             if (ok) done_with_item(n);
         }
         if (!ok) leave(kMeet);
     } else {
         // ---- softmax ----
-        const int h = warp >> 2, w = warp & 3, tid = w * 32 + lane, id_meet = 1 + h;
+        const int h = warp >> 2, w = warp & 3, tid = w * 32 + lane, id_meet = 1 + h;      // h: the group
         const uint32_t lanes = (uint32_t)(w * 32) << 16;
         uint32_t g = 0, pass = 0;
         bool ok = true;
         const float factor = p.scale * kLog2e;
+#pragma unroll 1
         for (uint32_t n = 0; ok; ++n) {
             ok = next_item(n);
             if (!ok || !items[n % kItems].valid) break;
@@ -606,17 +625,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             const Item& t = items[item_slot];
             ok = wait_on(&bars.q_full[item_slot], n / kItems, &s_abort);
             if (!ok) break;
-            const int columns = t.n / 2, row0 = h * columns, groups = columns / 8, tiles = t.tiles;
+            const int columns = t.n / kGroups, row0 = h * columns, groups = columns / 8, tiles = t.tiles;       // groups of 8
             const uint32_t buffers = t.n <= 64 ? 2 : 1;
             const int most_low = s_most_low[item_slot];
-            if (tid < kMostRows / 2) {
+            if (tid < kColumns) {
                 s_minus_top[h][tid] = tid < columns ? -kNone : -INFINITY;     // (columns that are another half's, or nobody's, have no weights)
                 s_keep[h][tid] = 1.f;
             }
-            float sums[kMostRows / 2];
+            float sums[kColumns];
 #pragma unroll
-            for (int i = 0; i < kMostRows / 2; ++i) sums[i] = 0.f;
+            for (int i = 0; i < kColumns; ++i) sums[i] = 0.f;
             if (!(ok = meet(id_meet))) break;
+#pragma unroll 1
             for (int j = 0; j < tiles; ++j) {
                 const uint32_t i = g + j;
                 ok = wait_on(&bars.scale_full[i % kScales], i / kScales, &s_abort) && wait_on(&bars.s_full[i & 1], i >> 1, &s_abort);
@@ -667,10 +687,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 // what is in the totals already is not added twice.
                 int added = 0;
                 bool again = false;
+#pragma unroll 1
                 for (;;) {
                     bool over = false;
 #pragma unroll
-                    for (int c = 0; c < kMostRows / 32; ++c)
+                    for (int c = 0; c < kColumns / 16; ++c)
                         if (2 * c < groups && !over) {
                             uint32_t x[16];
                             ptx::tmem_ld16(s_at + 16 * c, x);
@@ -714,13 +735,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                     if (j > 0) ok = wait_on(&bars.pv_done[(i - 1) & 1], (i - 1) >> 1, &s_abort);
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
-#pragma unroll 1
-                    for (int c = 0; 4 * c < groups; ++c) {
-                        uint32_t x[32];
-                        ptx::tmem_ld32(s_at + 32 * c, x);
+                    {
+                        uint32_t x[kColumns];
+                        ptx::tmem_ld32(s_at, x);
                         ptx::tc_wait_ld();
-                        exponents(x, 32 * c, false);
-                        s_warps[h][w][32 * c + lane] = reduce32(x, [](float u, float v) { return fmaxf(u, v); });
+                        exponents(x, 0, false);
+                        s_warps[h][w][lane] = reduce32(x, [](float u, float v) { return fmaxf(u, v); });
                     }
                     if (!(ok = meet(id_meet))) break;
                     if (tid < columns) {
@@ -733,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                     }
                     if (!(ok = meet(id_meet))) break;
 #pragma unroll
-                    for (int k = 0; k < kMostRows / 2; ++k) sums[k] *= s_keep[h][k];
+                    for (int k = 0; k < kColumns; ++k) sums[k] *= s_keep[h][k];
                     if (j > 0) {
 #pragma unroll 1
                         for (int q = 0; q < groups; ++q) {
@@ -760,13 +780,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             if (!ok) break;
             ptx::tc_fence_after_sync();
             // totals: over the lanes, then over the warps
+            {
+                uint32_t x[kColumns];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if (4 * c >= groups) continue;
-                uint32_t y[32];
-#pragma unroll
-                for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(sums[32 * c + k]);
-                s_warps[h][w][32 * c + lane] = reduce32(y, [](float u, float v) { return u + v; });
+                for (int k = 0; k < kColumns; ++k) x[k] = __float_as_uint(sums[k]);
+                s_warps[h][w][lane] = reduce32(x, [](float u, float v) { return u + v; });
             }
             if (!(ok = meet(id_meet))) break;
             const auto reference = [&](int r) { return s_minus_top[h][r] == -kNone ? -INFINITY : -s_minus_top[h][r]; };
@@ -774,46 +792,37 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             // (int8: the products' rows are the dims in decode4's order)
             const int dim = E4M3 ? tid : (tid & ~3) | ((tid & 1) << 1) | ((tid >> 1) & 1);
             const bool real = tid < D;
-            if (t.first_block == t.last_block) {
-                if (tid < columns && s_row[item_slot][row0 + tid] >= 0) p.prefix_total[s_row[item_slot][row0 + tid]] = make_float2(reference(tid), total_of(tid));
+            // a part: the block's first item continues another block's, its last is continued; the one that comes last adds them up
+            const bool whole = t.first_block == t.last_block;
+            const int a = t.first_block, z = t.last_block;
+            float* const parts = reinterpret_cast<float*>(header + p.prefix_parts);
+            const auto part_of = [&](int block) { return parts + ((size_t)block * 2 + (block == a ? 1 : 0)) * L::kPartFloats; };
+            float* const own = part_of(blockIdx.x);
+            if (tid < columns) {
+                const float2 both = make_float2(reference(tid), total_of(tid));
+                const int id = s_row[item_slot][row0 + tid];
+                if (!whole) *reinterpret_cast<float2*>(own + kMostRows * D + 2 * (row0 + tid)) = both;
+                else if (id >= 0) p.prefix_total[id] = both;
+            }
 #pragma unroll 1
-                for (int c = 0; 4 * c < groups; ++c) {
-                    uint32_t x[32];
-                    ptx::tmem_ld32(o_col + lanes + row0 + 32 * c, x);
-                    ptx::tc_wait_ld();
-                    if (real)
+            for (int q = 0; q < groups; ++q) {
+                uint32_t x[8];
+                ptx::tmem_ld8(o_col + lanes + row0 + 8 * q, x);
+                ptx::tc_wait_ld();
+                if (real)
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            if (4 * c + k / 8 >= groups) break;
-                            const int id = s_row[item_slot][row0 + 32 * c + k];
-                            if (id >= 0) p.prefix_sums[(long long)id * D + dim] = __uint_as_float(x[k]);
-                        }
-                    __syncwarp();
-                }
-            } else {
-                // a part: the block's first item continues another block's, its last is continued; the one that comes last adds them up
-                const int a = t.first_block, z = t.last_block;
-                float* const parts = reinterpret_cast<float*>(header + p.prefix_parts);
-                const auto part_of = [&](int block) { return parts + ((size_t)block * 2 + (block == a ? 1 : 0)) * L::kPartFloats; };
-                float* const own = part_of(blockIdx.x);
-                if (tid < columns) *reinterpret_cast<float2*>(own + kMostRows * D + 2 * (row0 + tid)) = make_float2(reference(tid), total_of(tid));
-#pragma unroll 1
-                for (int c = 0; 4 * c < groups; ++c) {
-                    uint32_t x[32];
-                    ptx::tmem_ld32(o_col + lanes + row0 + 32 * c, x);
-                    ptx::tc_wait_ld();
-                    if (real)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            if (4 * c + k / 8 >= groups) break;
-                            own[(row0 + 32 * c + k) * D + dim] = __uint_as_float(x[k]);
-                        }
-                    __syncwarp();
-                }
+                    for (int k = 0; k < 8; ++k) {
+                        const int row = row0 + 8 * q + k, id = s_row[item_slot][row];
+                        float* const to = whole ? p.prefix_sums + (long long)id * D : own + row * D;
+                        if (id >= 0) to[dim] = __uint_as_float(x[k]);
+                    }
+                __syncwarp();
+            }
+            if (!whole) {
                 __threadfence();
                 if (!(ok = meet(id_meet))) break;
                 if (tid == 0) {
-                    unsigned int* const counter = reinterpret_cast<unsigned int*>(header + kPrefixCounters) + 2 * a + h;
+                    unsigned int* const counter = reinterpret_cast<unsigned int*>(header + kPrefixCounters) + kGroups * a + h;
                     const bool last = atomicAdd(counter, 1u) == (unsigned int)(z - a);
                     if (last) atomicExch(counter, 0u);                        // as the next launch expects it
                     s_last[h] = last;
@@ -823,17 +832,20 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 if (s_last[h]) {
                     __threadfence();
                     using Columns = std::conditional_t<D == 128, float4, float2>;             // of a lane
+#pragma unroll 1
                     for (int r = w; r < columns; r += 4) {
                         const int row = row0 + r, id = s_row[item_slot][row];
                         if (id < 0) continue;
                         const auto both = [&](int b) { return __ldcg(reinterpret_cast<const float2*>(part_of(b) + kMostRows * D + 2 * row)); };
                         float m = -INFINITY;
+#pragma unroll 1
                         for (int b = a + lane; b <= z; b += 32) m = fmaxf(m, both(b).x);
 #pragma unroll
                         for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor_sync(kAll, m, d));
                         const float from = m == -INFINITY ? 0.f : m;
                         float all_total = 0.f;
                         Columns o{};
+#pragma unroll 1
                         for (int b0 = a; b0 <= z; b0 += 32) {
                             float2 mine = make_float2(-INFINITY, 0.f);
                             if (b0 + lane <= z) mine = both(b0 + lane);
@@ -875,7 +887,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
 }
 
 template <bool E4M3, bool BF16, int D>
-cudaError_t launch_prefix(const AttentionParams& p, cudaStream_t stream) {
+cudaError_t launch_prefix(const AttentionParams& p, int most_rows, cudaStream_t stream) {
     const auto kernel = cache_prefix_kernel<E4M3, BF16, D>;
     constexpr int kSmem = Layout<D>::kBytes;
     CUtensorMap k_map, v_map;
@@ -892,7 +904,7 @@ cudaError_t launch_prefix(const AttentionParams& p, cudaStream_t stream) {
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, p, k_map, v_map);
+    e = cudaLaunchKernelEx(&cfg, kernel, p, most_rows, k_map, v_map);
     if (e == cudaSuccess) count_launch();
     return e;
 }
@@ -901,10 +913,10 @@ cudaError_t launch_prefix(const AttentionParams& p, cudaStream_t stream) {
 
 size_t cache_prefix_workspace() { return kPartsBytes; }
 
-cudaError_t cache_prefix_launch(const AttentionParams& p, bool e4m3, bool bf16, cudaStream_t stream) {
+cudaError_t cache_prefix_launch(const AttentionParams& p, bool e4m3, bool bf16, int most_rows, cudaStream_t stream) {
     const auto by_dim = [&](auto e, auto h) {
         constexpr bool E = decltype(e)::value, H = decltype(h)::value;
-        return p.cache.dim == 128 ? launch_prefix<E, H, 128>(p, stream) : launch_prefix<E, H, 64>(p, stream);
+        return p.cache.dim == 128 ? launch_prefix<E, H, 128>(p, most_rows, stream) : launch_prefix<E, H, 64>(p, most_rows, stream);
     };
     const auto by_type = [&](auto e) { return bf16 ? by_dim(e, std::true_type{}) : by_dim(e, std::false_type{}); };
     return e4m3 ? by_type(std::true_type{}) : by_type(std::false_type{});

@@ -82,6 +82,25 @@ __device__ __forceinline__ bool wait_on(unsigned long long* bar, uint32_t parity
 }
 __device__ __forceinline__ void arrive(unsigned long long* bar) { ptx::mbar_arrive(ptx::smem_u32(bar)); }
 
+// What a launch is for: rows over their own tokens; the same, and what a shared prefix came to is added at the end; or all rows that read a prefix,
+// over that prefix, whose sums and totals are kept for that.
+enum Kind { kOwn, kJoining, kPrefixes };
+
+// The segments' owner: a request, or a place and its readers (row0: their first in the list of readers).  All of a prefix is seen by every reader, but
+// for what a window hides.
+template <int KIND>
+__device__ __forceinline__ Request load_owner(const AttentionParams& p, int b) {
+    if (KIND != kPrefixes) return load_request(p, b);
+    Request r;
+    const int from = min(max(p.prefix_starts[b], 0), p.prefix_listed), to = min(max(p.prefix_starts[b + 1], 0), p.prefix_listed), seq = p.seq_lens[b];
+    r.row0 = from;
+    r.rows = min(max(to - from, 0), p.tokens);
+    r.limit = max(min(seq, p.table_width << p.cache.page_shift), 0);
+    r.position = r.limit;
+    r.lo = p.window && seq >= p.window ? min(seq - p.window + 1, r.limit) : 0;
+    return r;
+}
+
 // ---- items ---------------------------------------------------------------------------------------------------------------------
 // A segment is a key head and a tile of 256 rows of a request.  Segments are items of their own, or cut along the tokens into parts:
 //   * long ones, so that none has more than its share of the GPU's work;
@@ -120,11 +139,12 @@ __device__ __forceinline__ long long parts_of(const Cut& c) {             // of 
 }
 
 // How all segments are cut, and the number of items.  Parts must find room in the workspace.
+template <int KIND>
 __device__ __forceinline__ Split choose_split(const AttentionParams& p, int least_rows, int blocks, long long* items) {
     const int lane = threadIdx.x & 31;
     long long tiles = 0, segments = 0;
     for (int b = lane; b < p.requests; b += 32) {
-        const Request r = load_request(p, b);
+        const Request r = load_owner<KIND>(p, b);
         const long long n = (long long)row_tiles_of(p, r, least_rows) * p.cache.heads;
         segments += n;
         tiles += n * tiles_of(r);
@@ -142,7 +162,7 @@ __device__ __forceinline__ Split choose_split(const AttentionParams& p, int leas
             Cut c{};
             c.parts = c.last_parts = 1;
             Request r{};
-            if (base + lane < p.requests) r = load_request(p, base + lane);
+            if (base + lane < p.requests) r = load_owner<KIND>(p, base + lane);
             const long long own = base + lane < p.requests ? (long long)row_tiles_of(p, r, least_rows) * p.cache.heads : 0, upto = warp_prefix(own);
             if (base + lane < p.requests) c = cut_of(p, r, least_rows, s, before + upto - own);
             before += __shfl_sync(kAll, upto, 31);
@@ -160,6 +180,7 @@ __device__ __forceinline__ Split choose_split(const AttentionParams& p, int leas
 }
 
 // Item `index` in the order of requests, from each one's last rows to its first (they see the most).  The whole warp calls.
+template <int KIND>
 __device__ __forceinline__ void find_item(const AttentionParams& p, int least_rows, const Split& split, long long index, Item* out) {
     const int lane = threadIdx.x & 31;
     long long before = 0, parts_before = 0, segments_before = 0;
@@ -167,7 +188,7 @@ __device__ __forceinline__ void find_item(const AttentionParams& p, int least_ro
         Request r{};
         Cut c{};
         c.parts = c.last_parts = 1;
-        if (base + lane < p.requests) r = load_request(p, base + lane);
+        if (base + lane < p.requests) r = load_owner<KIND>(p, base + lane);
         const long long segments = base + lane < p.requests ? (long long)row_tiles_of(p, r, least_rows) * p.cache.heads : 0, upto = warp_prefix(segments);
         if (base + lane < p.requests) c = cut_of(p, r, least_rows, split, segments_before + upto - segments);
         segments_before += __shfl_sync(kAll, upto, 31);
@@ -205,7 +226,7 @@ __device__ __forceinline__ void find_item(const AttentionParams& p, int least_ro
             t.part = n_parts > 1 ? (int)(first_part + in - which) : -1;
             // the tokens that the rows of A and of B see, in tiles
             const int first = t.base / p.group;
-            t.lo = p.window && r.position + first >= p.window ? min(r.position + first - p.window + 1, r.limit) : r.lo;
+            t.lo = KIND != kPrefixes && p.window && r.position + first >= p.window ? min(r.position + first - p.window + 1, r.limit) : r.lo;
             int end[2] = {0, 0};
             for (int h = 0; h < 2; ++h) {
                 t.rows[h] = min(max(t.all_rows - t.base - h * kHalf, 0), kHalf);
@@ -250,8 +271,7 @@ __device__ __forceinline__ uint32_t swizzled(uint32_t tile, int rows, int row, i
     return tile + (unit >> 3) * (rows * 128) + row * 128 + (((unit & 7) ^ (row & 7)) << 4);
 }
 
-// PREFIX: a request's rows may have seen a shared prefix before its own tokens; what that came to is added at the end.
-template <bool E4M3, bool BF16, int D, bool PREFIX>
+template <bool E4M3, bool BF16, int D, int KIND>
 __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const AttentionParams p, int least_rows, int alone) {
     using L = Layout<D>;
     extern __shared__ uint8_t dynamic[];
@@ -319,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
 
     if (warp == kSchedule) {
         long long count = 0;
-        const Split split = choose_split(p, least_rows, gridDim.x, &count);
+        const Split split = choose_split<KIND>(p, least_rows, gridDim.x, &count);
         unsigned int* const next = reinterpret_cast<unsigned int*>(header + kPromptNext);
         for (uint32_t n = 0;; ++n) {
             if (!wait_on(&bars.item_empty[n & 1], ((n >> 1) & 1) ^ 1, &s_abort)) break;
@@ -331,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                 i = (long long)gridDim.x + __shfl_sync(kAll, taken, 0);
             }
             const bool more = i < count;
-            if (more) find_item(p, least_rows, split, i, &items[n & 1]);
+            if (more) find_item<KIND>(p, least_rows, split, i, &items[n & 1]);
             else if (lane == 0) items[n & 1].valid = 0;
             __syncwarp();
             if (lane == 0) {
@@ -562,9 +582,22 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
             const Item& t = items[n & 1];
             const int tiles = t.tiles[h], most = max(t.tiles[0], t.tiles[1]);
             const int mine = t.base + h * kHalf + row;                        // the row
-            const bool real = row < t.rows[h];
-            const int token = mine / p.group, head = t.head * p.group + mine - token * p.group;
-            const int position = real ? t.position + token : -1;
+            bool real = row < t.rows[h];
+            int token = mine / p.group;
+            const int head = t.head * p.group + mine - token * p.group;
+            int position = real ? t.position + token : -1;
+            if constexpr (KIND == kPrefixes) {        // the row that the list names, at its place behind the prefix
+                const int entry = t.row0 + token;
+                token = real && entry < p.prefix_listed ? p.prefix_rows[entry] : -1;
+                real = token >= 0 && token < p.tokens;
+                position = real ? t.position : -1;
+                if (real && p.window) position = behind_prefix(p, t.b, token);
+                token -= t.row0;
+            }
+            float2 prefix = make_float2(-INFINITY, 0.f);
+            if constexpr (KIND == kJoining) {         // (asked for long before it is used)
+                if (real && sees_prefix(p, t.b, position)) prefix = p.prefix_total[(long long)(t.row0 + token) * p.q_heads + head];
+            }
             float factor = p.scale * kLog2e;
             if (tiles > 0) {
                 // q -> shared memory; a negative scale goes into q, so that larger scores are larger weights
@@ -610,10 +643,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                 s_phase ^= 1;
                 ptx::tc_fence_after_sync();
                 const bool all_real = __all_sync(kAll, real);
-                const bool whole = all_real && first + kTokens - 1 <= first_position && first + kTokens <= t.limit && first >= t.lo &&
+                const bool whole = all_real && (KIND == kPrefixes || first + kTokens - 1 <= first_position) && first + kTokens <= t.limit && first >= t.lo &&
                                    (!p.window || first > last_position - p.window);
                 // tokens below `from` and at `to` and beyond are hidden from this row (relative to the tile)
-                const int from = max(p.window ? position - p.window + 1 : 0, t.lo) - first, to = min(position + 1, t.limit) - first;
+                const int from = max(p.window ? position - p.window + 1 : 0, t.lo) - first, to = (KIND == kPrefixes ? (real ? t.limit : 0) : min(position + 1, t.limit)) - first;
                 // Half a tile of tokens at a time: x = a * score + b of each 16 (a is not 0: hidden scores are -infinity), weights 2^x.  They are
                 // taken relative to a reference that is no maximum any more once scores exceed it, which does no harm until the half's
                 // weights add up to more than kMostWeight; then the reference moves, sums follow it, and the half is taken again.
@@ -733,12 +766,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                 uint16_t* const out = static_cast<uint16_t*>(p.out) + to;
                 // what the sums are multiplied with, once there are all of the row's own; the same of its prefix's
                 const auto joint = [&](float m, float sum) {
-                    if constexpr (PREFIX) {
-                        if (real && sees_prefix(p, t.b, position)) return join_prefix(m, sum, __ldcg(p.prefix_total + (long long)(t.row0 + token) * p.q_heads + head));
-                    }
+                    if constexpr (KIND == kJoining) return join_prefix(m, sum, prefix);
                     return Joint{sum > 0.f ? 1.f / sum : sum, 0.f};                           // (a NaN stays one)
                 };
-                const auto prefix4 = [&](int at) { return __ldcg(reinterpret_cast<const float4*>(p.prefix_sums + to + at)); };
+                float* const kept = KIND == kPrefixes ? p.prefix_sums + to : nullptr;
+                const auto prefix4 = [&](int at) { return *reinterpret_cast<const float4*>(p.prefix_sums + to + at); };
                 if (t.part < 0) {
                     const Joint both = joint(top, sum);
                     const float f = both.own;
@@ -749,7 +781,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                             ptx::tmem_ld32(o_at + 32 * c, x);
                             ptx::tc_wait_ld();
                         }
-                        if (PREFIX && both.prefix != 0.f) {
+                        if constexpr (KIND == kPrefixes) {
+                            if (real)
+#pragma unroll
+                                for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(kept + 32 * c + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                        } else if (KIND == kJoining && both.prefix != 0.f) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 8) {
                                 const float4 a = prefix4(32 * c + i), b = prefix4(32 * c + i + 4);
@@ -770,7 +806,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                                 *reinterpret_cast<uint4*>(out + 32 * c + i) = make_uint4(y[0], y[1], y[2], y[3]);
                             }
                         }
-                        if (PREFIX) __syncwarp();
+                        if (KIND != kOwn) __syncwarp();
+                    }
+                    if constexpr (KIND == kPrefixes) {
+                        if (real) p.prefix_total[(long long)(t.row0 + token) * p.q_heads + head] = make_float2(top, sum);
                     }
                 } else {
                     float* const parts = reinterpret_cast<float*>(header + p.prompt_parts) + (size_t)h * L::kPartFloats;
@@ -812,11 +851,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                         for (int i = 0; i < t.parts; ++i)
                             total += exp2_approx(__ldcg(part_at(i) + kHalf * D + row) - from) * __ldcg(part_at(i) + kHalf * D + kHalf + row);
                         const Joint both = joint(m, total);
-                        const float f = both.own;
+                        const float f = KIND == kPrefixes ? 1.f : both.own;
+                        if constexpr (KIND == kPrefixes) p.prefix_total[(long long)(t.row0 + token) * p.q_heads + head] = make_float2(m, total);
 #pragma unroll 1
                         for (int c = 0; c < D; c += 32) {
                             float y[32] = {};
-                            if constexpr (PREFIX) {
+                            if constexpr (KIND == kJoining) {
                                 if (both.prefix != 0.f)
 #pragma unroll
                                     for (int k = 0; k < 8; ++k) {
@@ -838,6 +878,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                                     y[4 * k + 2] += take * x.z;
                                     y[4 * k + 3] += take * x.w;
                                 }
+                            }
+                            if constexpr (KIND == kPrefixes) {
+#pragma unroll
+                                for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(kept + c + k) = make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                                continue;
                             }
 #pragma unroll
                             for (int k = 0; k < 32; k += 8)
@@ -862,9 +907,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
     if (warp == kMma) ptx::tmem_dealloc(tmem, 512);
 }
 
-template <bool E4M3, bool BF16, int D, bool PREFIX>
+template <bool E4M3, bool BF16, int D, int KIND>
 cudaError_t launch_prompt(const AttentionParams& p, int least_rows, bool alone, cudaStream_t stream) {
-    const auto kernel = cache_prompt_kernel<E4M3, BF16, D, PREFIX>;
+    const auto kernel = cache_prompt_kernel<E4M3, BF16, D, KIND>;
     constexpr int kSmem = Layout<D>::kBytes;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
@@ -883,18 +928,26 @@ cudaError_t launch_prompt(const AttentionParams& p, int least_rows, bool alone, 
     return e;
 }
 
+template <int KIND>
+cudaError_t by_types(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, bool alone, cudaStream_t stream) {
+    const auto by_dim = [&](auto e, auto h) {
+        constexpr bool E = decltype(e)::value, H = decltype(h)::value;
+        return p.cache.dim == 128 ? launch_prompt<E, H, 128, KIND>(p, least_rows, alone, stream) : launch_prompt<E, H, 64, KIND>(p, least_rows, alone, stream);
+    };
+    const auto by_type = [&](auto e) { return bf16 ? by_dim(e, std::true_type{}) : by_dim(e, std::false_type{}); };
+    return e4m3 ? by_type(std::true_type{}) : by_type(std::false_type{});
+}
+
 }  // namespace
 
 size_t cache_prompt_workspace() { return (size_t)kPromptParts * 2 * Layout<128>::kPartFloats * 4; }
 
 cudaError_t cache_prompt_launch(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, bool alone, cudaStream_t stream) {
-    const auto by_dim = [&](auto e, auto h) {
-        constexpr bool E = decltype(e)::value, H = decltype(h)::value;
-        if (p.prefix_of) return p.cache.dim == 128 ? launch_prompt<E, H, 128, true>(p, least_rows, alone, stream) : launch_prompt<E, H, 64, true>(p, least_rows, alone, stream);
-        return p.cache.dim == 128 ? launch_prompt<E, H, 128, false>(p, least_rows, alone, stream) : launch_prompt<E, H, 64, false>(p, least_rows, alone, stream);
-    };
-    const auto by_type = [&](auto e) { return bf16 ? by_dim(e, std::true_type{}) : by_dim(e, std::false_type{}); };
-    return e4m3 ? by_type(std::true_type{}) : by_type(std::false_type{});
+    return p.prefix_of ? by_types<kJoining>(p, e4m3, bf16, least_rows, alone, stream) : by_types<kOwn>(p, e4m3, bf16, least_rows, alone, stream);
+}
+
+cudaError_t cache_many_readers_launch(const AttentionParams& p, bool e4m3, bool bf16, int least_rows, cudaStream_t stream) {
+    return by_types<kPrefixes>(p, e4m3, bf16, least_rows, false, stream);
 }
 
 }  // namespace i4mm

@@ -64,10 +64,13 @@ constexpr size_t kBlockPartsBytes = (size_t)kMaxBlocks * 2 * Shape<128, 2>::kPar
 // a request and its tiles of tokens: at least one if there are rows (rows that see nothing are written too)
 struct Few : Request {
     int tiles;
+    int joins;                                        // whether its rows see a prefix
 };
+template <bool PREFIX>
 __device__ __forceinline__ Few load_few(const AttentionParams& p, int most_rows, int b) {
     Few r;
     static_cast<Request&>(r) = load_request(p, b);
+    r.joins = PREFIX && p.prefix_of[b] >= 0;
     if ((long long)r.rows * p.group > most_rows) r.rows = 0;    // the other kernel's
     r.tiles = max((r.limit + kTile - 1) / kTile - r.lo / kTile, 1);
     return r;
@@ -116,6 +119,7 @@ __device__ __forceinline__ void store4(void* out, long long at, float a, float b
 struct Piece {
     long long from, to;                               // from < 0: none
     int b, segment, rows;                             // rows of its row tile
+    int row0, position, joins, head, base;            // with prefixes: the request's, and where its row tile lies
 };
 
 // PREFIX: a request's rows may have seen a shared prefix before its own tokens; what that came to is added at the end.
@@ -154,11 +158,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
     Few mine{};
     long long own = 0;
     if (lane < p.requests) {
-        mine = load_few(p, most_rows, lane);
+        mine = load_few<PREFIX>(p, most_rows, lane);
         own = units_of<S::kRows>(p, mine);
     }
     long long total = own;
-    for (int b = lane + 32; b < p.requests; b += 32) total += units_of<S::kRows>(p, load_few(p, most_rows, b));
+    for (int b = lane + 32; b < p.requests; b += 32) total += units_of<S::kRows>(p, load_few<PREFIX>(p, most_rows, b));
     const long long own_upto = warp_prefix(own);
     total = warp_sum(total);
     const long long blocks = min((long long)gridDim.x, (total + kMinBlockTiles - 1) / kMinBlockTiles);
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                 before += __shfl_sync(kAll, upto, 31);
                 b += 32;
                 if (b >= p.requests) break;           // (not unless the lengths change under the kernel)
-                here_own = b + lane < p.requests ? units_of<S::kRows>(p, load_few(p, most_rows, b + lane)) : 0;
+                here_own = b + lane < p.requests ? units_of<S::kRows>(p, load_few<PREFIX>(p, most_rows, b + lane)) : 0;
                 upto = warp_prefix(here_own);
             }
             b = min(b, p.requests - 1);
@@ -202,8 +206,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                 r.lo = __shfl_sync(kAll, mine.lo, b);
                 r.limit = __shfl_sync(kAll, mine.limit, b);
                 r.tiles = __shfl_sync(kAll, mine.tiles, b);
+                if constexpr (PREFIX) r.joins = __shfl_sync(kAll, mine.joins, b);
             } else {
-                r = load_few(p, most_rows, b);
+                r = load_few<PREFIX>(p, most_rows, b);
             }
             segment = (int)((u0 - before) / r.tiles);
             tile = (int)(u0 - before - (long long)segment * r.tiles);
@@ -267,7 +272,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                     Few next;
                     do {
                         ++c.b;
-                        if (c.b < p.requests) next = load_few(p, most_rows, c.b);
+                        if (c.b < p.requests) next = load_few<PREFIX>(p, most_rows, c.b);
                     } while (c.b < p.requests && next.rows == 0);
                     if (c.b < p.requests) enter_request(next);
                     else c.left = 0;                  // (as above)
@@ -347,6 +352,22 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                     for (int i = 0; i < 4; ++i) o[n][j][i] = 0.f;
             }
 
+            // What the rows' prefixes came to is asked for now: the last tile would otherwise wait for it, and the warp's copies with it.
+            float2 prefix[NT][2];
+            if constexpr (PREFIX) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = base + 8 * n + 2 * t + i, token = row / p.group, h = head * p.group + row - token * p.group;
+                        prefix[n][i] = make_float2(-INFINITY, 0.f);
+                        if (r.joins && position[n][i] >= 0) {
+                            const long long at = (long long)(r.row0 + token) * p.q_heads + h;
+                            prefix[n][i] = *(p.prefix_total + at);
+                            if (tiles_here == r.tiles) ptx::prefetch_l1(p.prefix_sums + at * D + (D / 8) * g);
+                        }
+                    }
+            }
             // tiles that begin in [whole_from, whole_to] are seen whole by all rows of the tile of rows
             const int whole_from = p.window ? max(r.position + r.rows - p.window, r.lo) : r.lo;
             const int whole_to = base + S::kRows <= all_rows ? min(r.position + 1, r.limit) - kTile : -1;
@@ -530,11 +551,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                         const int token = row / p.group, h = head * p.group + row - token * p.group;
                         const long long to = ((long long)(r.row0 + token) * p.q_heads + h) * D + (D / 8) * g;
                         if constexpr (PREFIX) {
-                            if (sees_prefix(p, b, r.position + token)) {
-                                const Joint f = join_prefix(m[n][i], sum[n][i], __ldcg(p.prefix_total + (long long)(r.row0 + token) * p.q_heads + h));
+                            if (prefix[n][i].y != 0.f) {
+                                const Joint f = join_prefix(m[n][i], sum[n][i], prefix[n][i]);
 #pragma unroll
                                 for (int j = 0; j < kWords; ++j) {
-                                    const float4 x = __ldcg(reinterpret_cast<const float4*>(p.prefix_sums + to + 4 * j));
+                                    const float4 x = *reinterpret_cast<const float4*>(p.prefix_sums + to + 4 * j);
                                     store4<BF16>(p.out, to + 4 * j, fmaf(o[n][2 * j][i], f.own, x.x * f.prefix), fmaf(o[n][2 * j][2 + i], f.own, x.y * f.prefix),
                                                  fmaf(o[n][2 * j + 1][i], f.own, x.z * f.prefix), fmaf(o[n][2 * j + 1][2 + i], f.own, x.w * f.prefix));
                                 }
@@ -568,7 +589,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                     }
                 if (lane == 0) {
                     const long long from = at - tiles_here - tile;
-                    (last ? s_tail : s_head)[warp] = Piece{from, from + r.tiles, b, segment, min(S::kRows, all_rows - base)};
+                    (last ? s_tail : s_head)[warp] = Piece{from, from + r.tiles, b, segment, min(S::kRows, all_rows - base), r.row0, r.position, r.joins, head, base};
                 }
             }
             // the next segment
@@ -577,7 +598,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                 segment = 0;
                 do {
                     ++b;
-                    if (b < p.requests) r = load_few(p, most_rows, b);
+                    if (b < p.requests) r = load_few<PREFIX>(p, most_rows, b);
                 } while (b < p.requests && r.rows == 0);
                 if (b >= p.requests) break;           // (as above)
             }
@@ -618,29 +639,54 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
             a.o[3] = a.o[3] * keep + x.w * take;
         }
     };
-    const auto finish = [&](const Joined& a, const Piece& piece, int row) {
-        const Request r = load_request(p, piece.b);
-        const int count = row_tiles<S::kRows>(p, r), head = piece.segment / count, in = (piece.segment - head * count) * S::kRows + row;
-        const int token = in / p.group, h = head * p.group + in - token * p.group;
-        const long long to = ((long long)(r.row0 + token) * p.q_heads + h) * D + kMine * lane;
+    // where a row's result goes and, with prefixes, what its prefix came to (asked for before the row's own parts are added up)
+    struct Place {
+        long long to;
+        float2 total;
+        float sums[kMine];
+    };
+    const auto place_of = [&](const Piece& piece, int row) {
+        Place x;
+        int row0, head, in;
         if constexpr (PREFIX) {
-            if (sees_prefix(p, piece.b, r.position + token)) {
-                const Joint f = join_prefix(a.m, a.sum, __ldcg(p.prefix_total + (long long)(r.row0 + token) * p.q_heads + h));
-                const float* const x = p.prefix_sums + to;
-                float y[kMine];
+            row0 = piece.row0;
+            head = piece.head;
+            in = piece.base + row;
+        } else {
+            const Request r = load_request(p, piece.b);
+            const int count = row_tiles<S::kRows>(p, r);
+            row0 = r.row0;
+            head = piece.segment / count;
+            in = (piece.segment - head * count) * S::kRows + row;
+        }
+        const int token = in / p.group, h = head * p.group + in - token * p.group;
+        const long long at = (long long)(row0 + token) * p.q_heads + h;
+        x.to = at * D + kMine * lane;
+        if constexpr (PREFIX) {
+            x.total = make_float2(-INFINITY, 0.f);
 #pragma unroll
-                for (int i = 0; i < kMine; ++i) y[i] = fmaf(a.o[i], f.own, __ldcg(x + i) * f.prefix);
-                if constexpr (kMine == 4) store4<BF16>(p.out, to, y[0], y[1], y[2], y[3]);
-                else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + to) = pack_out<BF16>(y[0], y[1]);
-                return;
+            for (int i = 0; i < kMine; ++i) x.sums[i] = 0.f;
+            if (piece.joins && piece.position + token >= 0) {
+                x.total = p.prefix_total[at];
+                using Columns = std::conditional_t<kMine == 4, float4, float2>;
+                *reinterpret_cast<Columns*>(x.sums) = *reinterpret_cast<const Columns*>(p.prefix_sums + x.to);
             }
         }
-        const float f = a.sum > 0.f ? 1.f / a.sum : a.sum;
-        if constexpr (kMine == 4) {
-            store4<BF16>(p.out, to, a.o[0] * f, a.o[1] * f, a.o[2] * f, a.o[3] * f);
+        return x;
+    };
+    const auto finish = [&](const Joined& a, const Place& x) {
+        float y[kMine];
+        if constexpr (PREFIX) {
+            const Joint f = join_prefix(a.m, a.sum, x.total);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) y[i] = fmaf(a.o[i], f.own, x.sums[i] * f.prefix);
         } else {
-            *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + to) = pack_out<BF16>(a.o[0] * f, a.o[1] * f);
+            const float f = a.sum > 0.f ? 1.f / a.sum : a.sum;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) y[i] = a.o[i] * f;
         }
+        if constexpr (kMine == 4) store4<BF16>(p.out, x.to, y[0], y[1], y[2], y[3]);
+        else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + x.to) = pack_out<BF16>(y[0], y[1]);
     };
     float* const block_parts = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + kCacheHeaderBytes + kWarpPartsBytes);
     const auto ring_part = [&](int w) { return reinterpret_cast<const float*>(ring + w * S::kWarpBytes); };
@@ -655,6 +701,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         const bool inside = piece.from >= c0 && piece.to <= c1;
         for (int row = 0; row < piece.rows; ++row) {
             if (item++ % S::kWarps != warp) continue;
+            Place place;
+            if (PREFIX && inside) place = place_of(piece, row);
             Joined a{-INFINITY, 0.f, {}};
             add(a, l < 0 ? workspace_part(0) : ring_part(l), row, true);
             for (int w = l + 1; l >= 0 && w < S::kWarps; ++w) {
@@ -666,7 +714,8 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                 add(a, ring_part(w), row, true);
             }
             if (inside) {
-                finish(a, piece, row);
+                if (!PREFIX) place = place_of(piece, row);
+                finish(a, place);
             } else {
                 float* const to = block_parts + ((size_t)blockIdx.x * 2 + (piece.from >= c0 ? 1 : 0)) * S::kPartFloats;
 #pragma unroll
@@ -710,9 +759,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         if (!s_last[i]) continue;
         const int a = range_owner(total, blocks, cut[i].from), z = range_owner(total, blocks, cut[i].to - 1);
         for (int row = warp; row < cut[i].rows; row += S::kWarps) {
+            Place place;
+            if (PREFIX) place = place_of(cut[i], row);
             Joined j{-INFINITY, 0.f, {}};
             for (int c = a; c <= z; ++c) add(j, block_parts + ((size_t)c * 2 + (c == a ? 1 : 0)) * S::kPartFloats, row, false);
-            finish(j, cut[i], row);
+            if (!PREFIX) place = place_of(cut[i], row);
+            finish(j, place);
         }
     }
 }
