@@ -20,15 +20,30 @@ constexpr uint32_t kAll = 0xFFFFFFFFu;
 
 enum Turn { kStraight, kHalves, kPairs };             // no rotation; pairs (i, i + F); pairs (2 i, 2 i + 1)
 
+constexpr int kStaged = 32;                           // tokens whose angles a block keeps in shared memory
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+
 // What a lane does to its 8 values of a row; the lanes of a row call together.
 template <bool BF16, int TURN>
 struct Turned {
-    float weight[8];
-    bool norm, turns, second;                         // second: the lane has the b of its pairs (kHalves)
+    static constexpr int kTable = TURN == kHalves ? 4 : TURN == kPairs ? 2 : 1;         // 16 bytes of angles of a lane: two pairs each
+    float2 weight[4];
+    bool norm, turns;
     int partner, lanes;                               // the lane with the other halves; lanes of a row
+    float sign;                                       // of the other value's part (kHalves)
     float eps, per;                                   // 1 / head_dim
-    const float2* angles;                             // the lane's first pair of token 0
-    long long stride;                                 // pairs of a token
+    int first;                                        // the lane's first pair
 
     __device__ __forceinline__ Turned(const AppendParams& p, const void* w, int lane) {
         lanes = p.cache.dim >> 3;
@@ -37,61 +52,82 @@ struct Turned {
         eps = p.eps;
         per = 1.f / (float)p.cache.dim;
         turns = TURN != kStraight && col < 2 * pairs;
-        second = TURN == kHalves && col >= pairs;
+        const bool second = TURN == kHalves && col >= pairs;
         partner = !turns ? lane : second ? lane - (pairs >> 3) : lane + (pairs >> 3);
-        stride = pairs;
-        angles = p.angles + (!turns ? 0 : TURN == kPairs ? col / 2 : second ? col - pairs : col);
+        sign = second ? 1.f : -1.f;
+        first = !turns ? 0 : TURN == kPairs ? col / 2 : second ? col - pairs : col;
         if (norm) {
-            unpack8<BF16>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + col), weight);
+            float f[8];
+            unpack8<BF16>(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + col), f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) weight[i] = make_float2(f[2 * i], f[2 * i + 1]);
+        }
+    }
+    // A token's angles, (cos, cos, sin, sin) of two pairs at a time: from shared memory, where the i-th 16 bytes of all lanes lie side by side, or
+    // from the table
+    __device__ __forceinline__ void angles(float4 (&t)[kTable], const float4* staged, int token, int pairs) const {
+        if (TURN == kStraight) return;
+        const int per_lane = 2 * kTable, across = pairs / per_lane;
+#pragma unroll
+        for (int i = 0; i < kTable; ++i) t[i] = staged[(token * kTable + i) * across + first / per_lane];
+    }
+    __device__ __forceinline__ void angles(float4 (&t)[kTable], const float2* table, long long token, int pairs) const {
+        if (TURN == kStraight) return;
+        const float4* const from = reinterpret_cast<const float4*>(table + token * pairs + first);
+#pragma unroll
+        for (int i = 0; i < kTable; ++i) {
+            const float4 x = __ldg(from + i);
+            t[i] = make_float4(x.x, x.z, x.y, x.w);
         }
     }
 
-    __device__ __forceinline__ uint4 operator()(uint4 w, long long token) const {
-        float4 table[4];
-        if (turns) {
-            const float4* const from = reinterpret_cast<const float4*>(angles + token * stride);
+    __device__ __forceinline__ uint4 operator()(uint4 w, const float4 (&t)[kTable]) const {
+        float g[8];
+        unpack8<BF16>(w, g);
+        float2 f[4];
 #pragma unroll
-            for (int i = 0; i < (TURN == kPairs ? 2 : 4); ++i) table[i] = __ldg(from + i);
-        }
-        float f[8];
-        unpack8<BF16>(w, f);
+        for (int i = 0; i < 4; ++i) f[i] = make_float2(g[2 * i], g[2 * i + 1]);
         if (norm) {
-            float sum = 0.f;
+            float2 squares = mul2(f[0], f[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
-            for (int d = lanes >> 1; d; d >>= 1) sum += __shfl_xor_sync(kAll, sum, d);
+            for (int i = 1; i < 4; ++i) squares = fma2(f[i], f[i], squares);
+            float sum = squares.x + squares.y;
+            sum += __shfl_xor_sync(kAll, sum, 4);
+            sum += __shfl_xor_sync(kAll, sum, 2);
+            sum += __shfl_xor_sync(kAll, sum, 1);
+            if (lanes == 16) sum += __shfl_xor_sync(kAll, sum, 8);
             const float r = rsqrtf(fmaf(sum, per, eps));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] *= r * weight[i];
+            for (int i = 0; i < 4; ++i) f[i] = mul2(f[i], mul2(weight[i], make_float2(r, r)));
         }
-        if (TURN == kHalves) {
-            float other[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) other[i] = __shfl_sync(kAll, f[i], partner);
-            if (turns) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float c = i & 1 ? table[i / 2].z : table[i / 2].x, s = i & 1 ? table[i / 2].w : table[i / 2].y;
-                    f[i] = fmaf(f[i], c, other[i] * (second ? s : -s));
-                }
-            }
-        } else if (TURN == kPairs && turns) {
+        if constexpr (TURN == kHalves) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float c = i & 1 ? table[i / 2].z : table[i / 2].x, s = i & 1 ? table[i / 2].w : table[i / 2].y, a = f[2 * i], b = f[2 * i + 1];
-                f[2 * i] = fmaf(a, c, -b * s);
-                f[2 * i + 1] = fmaf(b, c, a * s);
+                const float2 other = make_float2(__shfl_sync(kAll, f[i].x, partner), __shfl_sync(kAll, f[i].y, partner));
+                const float2 y = fma2(f[i], make_float2(t[i].x, t[i].y), mul2(mul2(other, make_float2(sign, sign)), make_float2(t[i].z, t[i].w)));
+                if (turns) f[i] = y;
+            }
+        } else if constexpr (TURN == kPairs) {
+            if (turns) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float c = i & 1 ? t[i / 2].y : t[i / 2].x, s = i & 1 ? t[i / 2].w : t[i / 2].z;
+                    f[i] = make_float2(fmaf(f[i].x, c, -f[i].y * s), fmaf(f[i].y, c, f[i].x * s));
+                }
             }
         }
-        return make_uint4(pack2<BF16>(f[0], f[1]), pack2<BF16>(f[2], f[3]), pack2<BF16>(f[4], f[5]), pack2<BF16>(f[6], f[7]));
+        return make_uint4(pack2<BF16>(f[0].x, f[0].y), pack2<BF16>(f[1].x, f[1].y), pack2<BF16>(f[2].x, f[2].y), pack2<BF16>(f[3].x, f[3].y));
     }
 };
 
 // Units of the tokens of a window (at most 16): the heads' keys, then their values, then the queries' heads.  A block takes a window and every
 // `groups`-th eight units, a warp one at a time.  Keys and values go by runs: neighbouring tokens with ascending slots of one page, of which those
-// that begin in the window are the window's, every gridDim.y-th of them to a block; queries are cut into gridDim.y parts.
-template <bool E4M3, bool BF16, int TURN>
+// that begin in the window are the window's.  STAGED: the angles of the window's tokens, and of those that its runs may go on to, are brought to
+// shared memory once for all heads.
+template <bool E4M3, bool BF16, int TURN, bool STAGED>
 __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const AppendParams p, int window, int groups) {
+    using T = Turned<BF16, TURN>;
+    __shared__ float4 s_angles[STAGED && TURN != kStraight ? kStaged * 32 : 1];
     const int lane = threadIdx.x & 31;
     const int block = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - block * groups), units = 2 * p.cache.heads + p.q_heads;
     const CacheView& c = p.cache;
@@ -103,6 +139,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
     // lane i: the slot of token t0 - 1 + i, and whether it goes on with the run of the one before
     const int t = t0 - 1 + lane;
     const int slot = t >= 0 && t < tokens ? p.slots[t] : -1;
+    if constexpr (STAGED && TURN != kStraight) {
+        const int two = p.pairs / 2, across = p.pairs / (2 * T::kTable), all = min(kStaged, tokens - t0) * two;
+        const float4* const from = reinterpret_cast<const float4*>(p.angles + (long long)t0 * p.pairs);
+        for (int i = threadIdx.x; i < all; i += kWarps * 32) {
+            const float4 x = __ldg(from + i);
+            const int token = i / two, j = i - token * two;
+            s_angles[(token * T::kTable + j % T::kTable) * across + j / T::kTable] = make_float4(x.x, x.z, x.y, x.w);
+        }
+        __syncthreads();
+    }
     const int before = __shfl_up_sync(kAll, slot, 1);
     const bool goes_on = lane > 0 && before >= 0 && slot == before + 1 && (slot & (page - 1)) != 0;
     const bool begins = lane > 0 && lane <= window && slot >= 0 && (slot >> c.page_shift) < c.pages && !goes_on;
@@ -112,12 +158,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
         uint4 w[kHeld];
         if (unit >= 2 * c.heads) {
             // ---- queries ----
-            const int head = unit - 2 * c.heads, n = min(window, tokens - t0), part = (n + (int)gridDim.y - 1) / (int)gridDim.y;
-            const Turned<BF16, TURN> turned(p, p.q_weight, lane);
+            const int head = unit - 2 * c.heads, end = min(window, tokens - t0);
+            const T turned(p, p.q_weight, lane);
             const uint16_t* const from = static_cast<const uint16_t*>(p.q.p) + head * p.q.head + col;
             uint16_t* const to = static_cast<uint16_t*>(p.q_out) + head * c.dim + col;
-            const int end = min(n, part * ((int)blockIdx.y + 1));
-            for (int i0 = part * (int)blockIdx.y; i0 < end; i0 += chunk) {
+#pragma unroll 1
+            for (int i0 = 0; i0 < end; i0 += chunk) {
 #pragma unroll
                 for (int i = 0; i < kHeld; ++i) {
                     const int r = i0 + i * rows_per_step + row;
@@ -126,9 +172,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
                 }
 #pragma unroll
                 for (int i = 0; i < kHeld; ++i) {
-                    if (i0 + i * rows_per_step >= end) break;
-                    const int r = i0 + i * rows_per_step + row;
-                    const uint4 y = turned(w[i], t0 + min(r, end - 1));
+                    if (!STAGED && i0 + i * rows_per_step >= end) break;
+                    const int r = i0 + i * rows_per_step + row, at = min(r, end - 1);
+                    float4 table[T::kTable];
+                    if constexpr (STAGED) turned.angles(table, s_angles, at, p.pairs);
+                    else turned.angles(table, p.angles, (long long)t0 + at, p.pairs);
+                    const uint4 y = turned(w[i], table);
                     if (r < end) *reinterpret_cast<uint4*>(to + (long long)(t0 + r) * p.q_heads * c.dim) = y;
                 }
             }
@@ -136,12 +185,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
         }
         // ---- keys and values ----
         const int which = unit >= c.heads, head = which ? unit - c.heads : unit;
-        const Turned<BF16, TURN> turned(p, which ? nullptr : p.k_weight, lane);
+        const T turned(p, which ? nullptr : p.k_weight, lane);
         const uint16_t* const x = (const uint16_t*)(which ? p.v.p : p.k.p) + head * (which ? p.v.head : p.k.head) + col;
         const long long x_token = which ? p.v.token : p.k.token;
-        int turn = 0;
+#pragma unroll 1
         for (uint32_t starts = all_starts; starts; starts &= starts - 1) {
-            if (turn++ % (int)gridDim.y != (int)blockIdx.y) continue;
             const int from = __ffs(starts) - 1, run = t0 - 1 + from;
             const int first_slot = __shfl_sync(kAll, slot, from);
             const int id = first_slot >> c.page_shift, place = first_slot & (page - 1);
@@ -167,11 +215,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
                     w[i] = make_uint4(0, 0, 0, 0);
                     if (r < n) w[i] = *reinterpret_cast<const uint4*>(rows + r * x_token);
                 }
-                if (which == 0 && (TURN != kStraight || turned.norm)) {
+                if (which == 0) {
+                    // (rows beyond the run are 0 and stay so)
+                    const bool near = STAGED && run + n <= t0 + kStaged;
 #pragma unroll
                     for (int i = 0; i < kHeld; ++i) {
-                        if (i0 + i * rows_per_step >= n) break;
-                        w[i] = turned(w[i], run + min(i0 + i * rows_per_step + row, n - 1));       // (rows beyond the run are 0 and stay so)
+                        if (!STAGED && i0 + i * rows_per_step >= n) break;
+                        const int token = run + min(i0 + i * rows_per_step + row, n - 1);
+                        float4 table[T::kTable];
+                        if (near) turned.angles(table, s_angles, token - t0, p.pairs);
+                        else turned.angles(table, p.angles, (long long)token, p.pairs);
+                        w[i] = turned(w[i], table);
                     }
                 }
             };
@@ -243,18 +297,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
 
 }  // namespace
 
+// Up to 1024 tokens each has blocks of its own, so that a few tokens are spread over the GPU: a warp a unit; more of them go by sixteen.
 cudaError_t cache_append_launch(const AppendParams& p, bool e4m3, bool bf16, bool pairs_beside, cudaStream_t stream) {
-    const int window = p.tokens > 1024 ? 16 : 1, units = 2 * p.cache.heads + p.q_heads;
-    const int groups = (units + kWarps - 1) / kWarps;
+    const bool staged = p.tokens > 1024;
+    const int window = staged ? 16 : 1, units = 2 * p.cache.heads + p.q_heads, most = (units + kWarps - 1) / kWarps;
+    const int groups = staged ? std::max(1, most / 4) : most;
     const long long blocks = (long long)((p.tokens + window - 1) / window) * groups;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    const dim3 grid((unsigned)blocks, window > 1 ? 2 : 1, 1);
-    const auto go = [&](auto e, auto h, auto t) {
-        return launch_overlapping(cache_append_kernel<decltype(e)::value, decltype(h)::value, decltype(t)::value>, grid, kWarps * 32, stream, p, window, groups);
+    const auto go = [&](auto e, auto h, auto t, auto s) {
+        return launch_overlapping(cache_append_kernel<decltype(e)::value, decltype(h)::value, decltype(t)::value, decltype(s)::value>, dim3((unsigned)blocks),
+                                  kWarps * 32, stream, p, window, groups);
     };
+    const auto by_size = [&](auto e, auto h, auto t) { return staged ? go(e, h, t, std::true_type{}) : go(e, h, t, std::false_type{}); };
     const auto by_turn = [&](auto e, auto h) {
-        if (p.pairs == 0) return go(e, h, std::integral_constant<int, kStraight>{});
-        return pairs_beside ? go(e, h, std::integral_constant<int, kPairs>{}) : go(e, h, std::integral_constant<int, kHalves>{});
+        if (p.pairs == 0) return by_size(e, h, std::integral_constant<int, kStraight>{});
+        return pairs_beside ? by_size(e, h, std::integral_constant<int, kPairs>{}) : by_size(e, h, std::integral_constant<int, kHalves>{});
     };
     const auto by_type = [&](auto e) { return bf16 ? by_turn(e, std::true_type{}) : by_turn(e, std::false_type{}); };
     return e4m3 ? by_type(std::true_type{}) : by_type(std::false_type{});

@@ -46,25 +46,28 @@ __global__ void __launch_bounds__(kShareThreads) cache_share_kernel(const ShareP
     extern __shared__ int shared[];
     __shared__ int warp_sums[kShareThreads / 32];
     const int n = p.requests, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int *s_starts = shared, *s_offset = shared + n + 1, *s_of = shared + 2 * n + 1;
+    int *s_starts = shared, *s_offset = shared + n + 1, *s_cu = shared + 2 * n + 1;
+    short* const s_of = reinterpret_cast<short*>(shared + 3 * n + 2);         // (there are 16384 places at most)
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    const auto prefix_of = [&](int b) {
-        const int of = p.prefix_of[b];
-        return of >= 0 && of < n && of != b && p.seq_lens[b] > 0 && p.seq_lens[of] > 0 ? of : -1;
-    };
     // first row that counts, and their number
-    const auto rows_of = [&](int b, int& from) {
-        const long long lo = p.cu_lens[b], hi = p.cu_lens[b + 1], skip = max(hi - lo - max(p.seq_lens[b], 0), 0ll);
+    const auto rows_of = [&](int seq, int cu, int next, int& from) {
+        const long long lo = cu, hi = next, skip = max(hi - lo - max(seq, 0), 0ll);
         from = (int)min(max(lo + skip, 0ll), (long long)p.max_tokens);
         return (int)max(min(hi, (long long)p.max_tokens) - from, 0ll);
     };
     for (int b = threadIdx.x; b <= n; b += kShareThreads) s_starts[b] = 0;
     __syncthreads();
-    for (int b = threadIdx.x; b < n; b += kShareThreads) {
-        const int of = prefix_of(b);
-        int from, count = rows_of(b, from);
-        s_of[b] = of;
+    for (int b = threadIdx.x; b <= n; b += kShareThreads) {
+        const int cu = p.cu_lens[b];
+        s_cu[b] = cu;
+        if (b == n) break;
+        const int seq = p.seq_lens[b], next = p.cu_lens[b + 1];
+        int of = p.prefix_of[b];
+        if (of < 0 || of >= n || of == b || seq <= 0 || p.seq_lens[of] <= 0) of = -1;
+        int from;
+        const int count = rows_of(seq, cu, next, from);
+        s_of[b] = (short)of;
         s_offset[b] = count;
         if (of >= 0 && count > 0) atomicAdd(&s_starts[of], count);
     }
@@ -97,14 +100,10 @@ __global__ void __launch_bounds__(kShareThreads) cache_share_kernel(const ShareP
         for (int base = 0; base < n; base += 32) {
             const int b = base + lane, of = b < n ? s_of[b] : -1, count = b < n ? s_offset[b] : 0;
             const uint32_t peers = __match_any_sync(kAll, of);
+            // counts of the peers in lower lanes, bit by bit
+            const uint32_t lower = peers & ((1u << lane) - 1), bits = __reduce_or_sync(kAll, (uint32_t)count);
             int before = 0;
-            if (__any_sync(kAll, of >= 0 && (peers & (peers - 1)) != 0)) {
-#pragma unroll
-                for (int d = 0; d < 31; ++d) {
-                    const int o = __shfl_sync(kAll, count, d);
-                    if (d < lane && (peers >> d & 1)) before += o;
-                }
-            }
+            for (int i = 0; bits >> i; ++i) before += __popc(__ballot_sync(kAll, count >> i & 1) & lower) << i;
             const int at = of >= 0 ? s_starts[of] : 0;
             __syncwarp();
             if (of >= 0 && 31 - __clz(peers) == lane) s_starts[of] = at + before + count;
@@ -117,17 +116,17 @@ __global__ void __launch_bounds__(kShareThreads) cache_share_kernel(const ShareP
     for (int t = first; t < p.max_tokens; t += step) {
         if (t >= listed) p.rows[t] = -1;
         int position = -1;
-        if (n > 0 && t < p.cu_lens[n] && t >= p.cu_lens[0]) {
+        if (n > 0 && t < s_cu[n] && t >= s_cu[0]) {
             int lo = 0, hi = n - 1;                   // the b with cu_lens[b] <= t < cu_lens[b + 1]
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
-                if (p.cu_lens[mid] <= t) lo = mid;
+                if (s_cu[mid] <= t) lo = mid;
                 else hi = mid - 1;
             }
-            const int of = s_of[lo];
+            const int of = s_of[lo], seq = p.seq_lens[lo];
             int from;
-            const int count = rows_of(lo, from);
-            const long long pos = (long long)p.seq_lens[lo] - p.cu_lens[lo + 1] + t;
+            const int count = rows_of(seq, s_cu[lo], s_cu[lo + 1], from);
+            const long long pos = (long long)seq - s_cu[lo + 1] + t;
             if (t >= from && t < from + count && pos >= 0) {
                 position = (int)min(pos + (of >= 0 ? p.seq_lens[of] : 0), 0x7FFFFFFFll);
                 const long long at = (long long)s_offset[lo] + (t - from);
@@ -147,7 +146,7 @@ cudaError_t cache_angles_launch(void* out, const int* positions, const float* fr
 }
 
 cudaError_t cache_share_launch(const ShareParams& p, cudaStream_t stream) {
-    const size_t smem = (3 * (size_t)p.requests + 1) * sizeof(int);
+    const size_t smem = (3 * (size_t)p.requests + 2) * sizeof(int) + (size_t)p.requests * sizeof(short);
     if (smem > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(cache_share_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
