@@ -20,6 +20,8 @@ constexpr uint32_t kAll = 0xFFFFFFFFu;
 
 enum Turn { kStraight, kHalves, kPairs };             // no rotation; pairs (i, i + F); pairs (2 i, 2 i + 1)
 
+constexpr int kWindow = 16;                           // tokens whose runs a block looks at
+constexpr int kMostStaging = 8;                       // blocks of a window, each of which would bring its angles to shared memory
 constexpr int kStaged = 32;                           // tokens whose angles a block keeps in shared memory
 
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -32,6 +34,35 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
         "l"(*reinterpret_cast<unsigned long long*>(&c)));
     return *reinterpret_cast<float2*>(&d);
+}
+
+// 8 bytes of a page whose scale grows
+template <bool E4M3>
+__device__ __forceinline__ void requantise(uint8_t* at, float ratio) {
+    const uint2 b = *reinterpret_cast<const uint2*>(at);
+    const uint32_t u[2] = {b.x, b.y};
+    uint32_t r[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j >> 2] |= to_byte<E4M3>(from_byte<E4M3>(u[j >> 2] >> (8 * (j & 3)) & 0xFFu) * ratio) << (8 * (j & 3));
+    *reinterpret_cast<uint2*>(at) = make_uint2(r[0], r[1]);
+}
+template <bool E4M3, bool BF16>
+__device__ __forceinline__ uint2 to_bytes_of(uint4 w, float inverse, bool finite) {
+    if (!finite) return to_bytes_any<E4M3, BF16>(w, inverse);
+    if (!BF16 && normal_half(inverse)) return half_to_bytes<E4M3>(w, h2_as_u32(__float2half2_rn(inverse)));
+    float f[8];
+    unpack8<BF16>(w, f);
+    return to_bytes<E4M3>(f, inverse);
+}
+
+// the largest finite magnitude among 8 values
+template <bool BF16>
+__device__ __noinline__ float largest_finite(uint4 w) {
+    float f[8], a = 0.f;
+    unpack8<BF16>(w, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a = fabsf(f[j]) <= 3.4e38f ? fmaxf(a, fabsf(f[j])) : a;
+    return a;
 }
 
 // What a lane does to its 8 values of a row; the lanes of a row call together.
@@ -120,20 +151,23 @@ struct Turned {
     }
 };
 
-// Units of the tokens of a window (at most 16): the heads' keys, then their values, then the queries' heads.  A block takes a window and every
-// `groups`-th eight units, a warp one at a time.  Keys and values go by runs: neighbouring tokens with ascending slots of one page, of which those
-// that begin in the window are the window's.  STAGED: the angles of the window's tokens, and of those that its runs may go on to, are brought to
-// shared memory once for all heads.
+// A block's share of a window of 16 tokens, a warp a unit at a time:
+//   * runs of several neighbouring tokens with ascending slots of one page, those that begin in the window: a head's keys or values, as
+//     the writer takes them (a prompt's tokens);
+//   * tokens that are runs of their own (a decoding step's): rows of `steps` times as many heads' keys or values as the warp has at once, each with its
+//     own page and scale;
+//   * the window's queries, as many rows of all tokens and heads.
+// STAGED: the angles of the window's tokens, and of those that its runs may go on to, are brought to shared memory once for all heads.
 template <bool E4M3, bool BF16, int TURN, bool STAGED>
-__global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const AppendParams p, int window, int groups) {
+__global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const AppendParams p, int groups, int steps) {
     using T = Turned<BF16, TURN>;
     __shared__ float4 s_angles[STAGED && TURN != kStraight ? kStaged * 32 : 1];
     const int lane = threadIdx.x & 31;
-    const int block = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - block * groups), units = 2 * p.cache.heads + p.q_heads;
+    const int block = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - block * groups);
     const CacheView& c = p.cache;
     const int page = 1 << c.page_shift, lanes_per_row = c.dim >> 3, rows_per_step = 32 / lanes_per_row;
     const int row = lane / lanes_per_row, col = (lane % lanes_per_row) * 8, chunk = kHeld * rows_per_step;
-    const int t0 = block * window, tokens = p.tokens;
+    const int t0 = block * kWindow, tokens = p.tokens;
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     // lane i: the slot of token t0 - 1 + i, and whether it goes on with the run of the one before
@@ -151,54 +185,39 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
     }
     const int before = __shfl_up_sync(kAll, slot, 1);
     const bool goes_on = lane > 0 && before >= 0 && slot == before + 1 && (slot & (page - 1)) != 0;
-    const bool begins = lane > 0 && lane <= window && slot >= 0 && (slot >> c.page_shift) < c.pages && !goes_on;
-    const uint32_t on = __ballot_sync(kAll, goes_on), all_starts = __ballot_sync(kAll, begins);
+    const bool begins = lane > 0 && lane <= kWindow && slot >= 0 && (slot >> c.page_shift) < c.pages && !goes_on;
+    const uint32_t on = __ballot_sync(kAll, goes_on), starts = __ballot_sync(kAll, begins), singles = starts & ~(on >> 1), runs = starts & ~singles;
+    const int rows = steps * rows_per_step, per_token = (c.heads + rows - 1) / rows, here = min(kWindow, tokens - t0);
+    const int stride = groups * kWarps;
+    int unit = group * kWarps + (threadIdx.x >> 5);   // the warp's next one, counted from the first of the kind that is being worked on
+    // the place of the n-th bit of a mask
+    const auto nth_of = [](uint32_t mask, int n) {
+        for (; n > 0; --n) mask &= mask - 1;
+        return __ffs(mask) - 1;
+    };
+    uint4 w[kHeld];
+    T turned(p, p.k_weight, lane);
 
-    for (int unit = group * kWarps + (threadIdx.x >> 5); unit < units; unit += groups * kWarps) {
-        uint4 w[kHeld];
-        if (unit >= 2 * c.heads) {
-            // ---- queries ----
-            const int head = unit - 2 * c.heads, end = min(window, tokens - t0);
-            const T turned(p, p.q_weight, lane);
-            const uint16_t* const from = static_cast<const uint16_t*>(p.q.p) + head * p.q.head + col;
-            uint16_t* const to = static_cast<uint16_t*>(p.q_out) + head * c.dim + col;
+    // ---- runs of a head's keys, then of its values ----
 #pragma unroll 1
-            for (int i0 = 0; i0 < end; i0 += chunk) {
-#pragma unroll
-                for (int i = 0; i < kHeld; ++i) {
-                    const int r = i0 + i * rows_per_step + row;
-                    w[i] = make_uint4(0, 0, 0, 0);
-                    if (r < end) w[i] = *reinterpret_cast<const uint4*>(from + (long long)(t0 + r) * p.q.token);
-                }
-#pragma unroll
-                for (int i = 0; i < kHeld; ++i) {
-                    if (!STAGED && i0 + i * rows_per_step >= end) break;
-                    const int r = i0 + i * rows_per_step + row, at = min(r, end - 1);
-                    float4 table[T::kTable];
-                    if constexpr (STAGED) turned.angles(table, s_angles, at, p.pairs);
-                    else turned.angles(table, p.angles, (long long)t0 + at, p.pairs);
-                    const uint4 y = turned(w[i], table);
-                    if (r < end) *reinterpret_cast<uint4*>(to + (long long)(t0 + r) * p.q_heads * c.dim) = y;
-                }
-            }
-            continue;
-        }
-        // ---- keys and values ----
-        const int which = unit >= c.heads, head = which ? unit - c.heads : unit;
-        const T turned(p, which ? nullptr : p.k_weight, lane);
-        const uint16_t* const x = (const uint16_t*)(which ? p.v.p : p.k.p) + head * (which ? p.v.head : p.k.head) + col;
-        const long long x_token = which ? p.v.token : p.k.token;
+    for (int which = 0; which < 2; ++which) {
+        const RowsView view = which ? p.v : p.k;
+        const long long page_stride = which ? c.v_page : c.k_page, head_stride = which ? c.v_head : c.k_head, token_stride = which ? c.v_token : c.k_token;
+        const int count = __popc(runs) * c.heads;
 #pragma unroll 1
-        for (uint32_t starts = all_starts; starts; starts &= starts - 1) {
-            const int from = __ffs(starts) - 1, run = t0 - 1 + from;
-            const int first_slot = __shfl_sync(kAll, slot, from);
-            const int id = first_slot >> c.page_shift, place = first_slot & (page - 1);
+        for (; unit < count; unit += stride) {
+            int head = unit, nth = 0;
+            for (; head >= c.heads; head -= c.heads) ++nth;
+            const int from = nth_of(runs, nth), run = t0 - 1 + from, first_slot = __shfl_sync(kAll, slot, from);
+            const int id = first_slot >> c.page_shift, at = first_slot & (page - 1);
+            float* const scale = reinterpret_cast<float*>(c.scales + (long long)id * c.heads + head) + which;
+            const float old = at ? *scale : 0.f;
             // its length: up to the first lane that does not go on; beyond the 32 lanes it is looked for
-            const uint32_t stop = ~on & (from == 31 ? 0u : ~0u << (from + 1));
+            const uint32_t stop = ~on & (~0u << (from + 1));
             int n = stop ? __ffs(stop) - 1 - from : 32 - from;
-            while (!stop && n < page - place) {
+            while (!stop && n < page - at) {
                 const int i = n + lane;
-                const bool more = i < page - place && run + i < tokens && p.slots[run + i] == first_slot + i;
+                const bool more = i < page - at && run + i < tokens && p.slots[run + i] == first_slot + i;
                 const uint32_t end = __ballot_sync(kAll, !more);
                 if (end) {
                     n += __ffs(end) - 1;
@@ -207,30 +226,31 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
                 n += 32;
             }
             // the lane's part of kHeld rows at a time; a run that fits (a page of 16 tokens does) is read once
-            const uint16_t* const rows = x + (long long)run * x_token;
+            const uint16_t* const first = static_cast<const uint16_t*>(view.p) + head * view.head + (run + row) * view.token + col;
+            const long long step = rows_per_step * view.token;
+            const bool near = STAGED && run + n <= t0 + kStaged;
             const auto fetch = [&](int i0) {
+                const uint16_t* x = first + i0 * view.token;
+                const int left = n - i0 - row;        // of the lane's rows: those with i * rows_per_step < left
 #pragma unroll
-                for (int i = 0; i < kHeld; ++i) {
-                    const int r = i0 + i * rows_per_step + row;
+                for (int i = 0; i < kHeld; ++i, x += step) {
                     w[i] = make_uint4(0, 0, 0, 0);
-                    if (r < n) w[i] = *reinterpret_cast<const uint4*>(rows + r * x_token);
+                    if (i * rows_per_step < left) w[i] = *reinterpret_cast<const uint4*>(x);
                 }
-                if (which == 0) {
-                    // (rows beyond the run are 0 and stay so)
-                    const bool near = STAGED && run + n <= t0 + kStaged;
+                if (which) return;
 #pragma unroll
-                    for (int i = 0; i < kHeld; ++i) {
-                        if (!STAGED && i0 + i * rows_per_step >= n) break;
-                        const int token = run + min(i0 + i * rows_per_step + row, n - 1);
-                        float4 table[T::kTable];
-                        if (near) turned.angles(table, s_angles, token - t0, p.pairs);
-                        else turned.angles(table, p.angles, (long long)token, p.pairs);
-                        w[i] = turned(w[i], table);
-                    }
+                for (int i = 0; i < kHeld; ++i) {     // (rows beyond the run are not used)
+                    if (i0 + i * rows_per_step >= n) break;
+                    const int token = run + min(i0 + i * rows_per_step + row, n - 1);
+                    float4 table[T::kTable];
+                    if (near) turned.angles(table, s_angles, token - t0, p.pairs);
+                    else turned.angles(table, p.angles, (long long)token, p.pairs);
+                    const uint4 y = turned(w[i], table);
+                    if (i * rows_per_step < left) w[i] = y;
                 }
             };
-            // magnitudes of either 16-bit type are ordered as their bits are, infinities and NaN on top
             uint32_t most = 0;
+#pragma unroll 1
             for (int i0 = 0; i0 < n; i0 += chunk) {
                 fetch(i0);
 #pragma unroll
@@ -242,71 +262,163 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
             float a = BF16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half((unsigned short)most));
             if (!finite) {                                                   // the largest of the others
                 a = 0.f;
+#pragma unroll 1
                 for (int i0 = 0; i0 < n; i0 += chunk) {
                     if (n > chunk) fetch(i0);
 #pragma unroll
-                    for (int i = 0; i < kHeld; ++i) {
-                        float f[8];
-                        unpack8<BF16>(w[i], f);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) a = fabsf(f[j]) <= 3.4e38f ? fmaxf(a, fabsf(f[j])) : a;
-                    }
+                    for (int i = 0; i < kHeld; ++i) a = fmaxf(a, largest_finite<BF16>(w[i]));
                 }
 #pragma unroll
                 for (int d = 16; d; d /= 2) a = fmaxf(a, __shfl_xor_sync(kAll, a, d));
             }
-            float* const scale = reinterpret_cast<float*>(c.scales + (long long)id * c.heads + head) + which;
-            const float old = place ? *scale : 0.f;
             const float s = fmaxf(old, scale_for<E4M3>(a));
-            uint8_t* const held = (which ? c.v : c.k) + id * (which ? c.v_page : c.k_page) + head * (which ? c.v_head : c.k_head);
-            const long long held_token = which ? c.v_token : c.k_token;
-            if (s > old && place > 0) {
+            uint8_t* const held = (which ? c.v : c.k) + id * page_stride + head * head_stride + col;
+            if (s > old && at > 0) {
                 const float ratio = old / s;          // (0 where the scale was: bytes of infinities beside zeros go on standing for 0)
-                for (int i = row; i < place; i += rows_per_step) {
-                    uint2* const at = reinterpret_cast<uint2*>(held + i * held_token + col);
-                    const uint2 b = *at;
-                    uint32_t u[2] = {b.x, b.y}, r[2] = {0, 0};
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) r[j >> 2] |= to_byte<E4M3>(from_byte<E4M3>(u[j >> 2] >> (8 * (j & 3)) & 0xFFu) * ratio) << (8 * (j & 3));
-                    *at = make_uint2(r[0], r[1]);
-                }
+#pragma unroll 1
+                for (int i = row; i < at; i += rows_per_step) requantise<E4M3>(held + i * token_stride, ratio);
             }
             const float inverse = s > 0.f ? 1.f / s : 1.f;
+            const uint32_t inverse2 = h2_as_u32(__float2half2_rn(inverse));
+            const bool by_halves = !BF16 && finite && normal_half(inverse);
+            const long long bytes_step = rows_per_step * token_stride;
+#pragma unroll 1
             for (int i0 = 0; i0 < n; i0 += chunk) {
                 if (n > chunk) fetch(i0);
+                const int left = n - i0 - row;
+                uint8_t* to = held + (at + i0 + row) * token_stride;
+                if (by_halves) {
 #pragma unroll
-                for (int i = 0; i < kHeld; ++i) {
-                    if (i0 + i * rows_per_step >= n) break;
-                    const int r = i0 + i * rows_per_step + row;
-                    uint2 q;
-                    if (finite) {
-                        float f[8];
-                        unpack8<BF16>(w[i], f);
-                        q = to_bytes<E4M3>(f, inverse);
-                    } else {
-                        q = to_bytes_any<E4M3, BF16>(w[i], inverse);
-                    }
-                    if (r < n) *reinterpret_cast<uint2*>(held + (place + r) * held_token + col) = q;
+                    for (int i = 0; i < kHeld; ++i, to += bytes_step)
+                        if (i * rows_per_step < left) *reinterpret_cast<uint2*>(to) = half_to_bytes<E4M3>(w[i], inverse2);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i, to += bytes_step)
+                        if (i * rows_per_step < left) *reinterpret_cast<uint2*>(to) = to_bytes_of<E4M3, BF16>(w[i], inverse, finite);
                 }
             }
             __syncwarp();
             if (lane == 0) *scale = s;
+        }
+        unit -= count;
+    }
+
+    // ---- keys, then values, of single tokens: rows are heads, each with its own scale ----
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        const RowsView view = which ? p.v : p.k;
+        const int count = __popc(singles) * per_token;
+#pragma unroll 1
+        for (; unit < count; unit += stride) {
+            int part = unit, nth = 0;
+            for (; part >= per_token; part -= per_token) ++nth;
+            const int from = nth_of(singles, nth), token = t0 - 1 + from, from_slot = __shfl_sync(kAll, slot, from);
+            const int id = from_slot >> c.page_shift, at = from_slot & (page - 1), first = part * rows + row;
+            const uint16_t* const x = static_cast<const uint16_t*>(view.p) + token * view.token + col;
+            uint8_t* const held0 = (which ? c.v + id * c.v_page : c.k + id * c.k_page) + col;
+            const long long held_token = which ? c.v_token : c.k_token, held_head = which ? c.v_head : c.k_head;
+            float* const scales = reinterpret_cast<float*>(c.scales + (long long)id * c.heads) + which;
+            float olds[kHeld];
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (i >= steps) break;
+                const int head = first + i * rows_per_step;
+                w[i] = make_uint4(0, 0, 0, 0);
+                olds[i] = 0.f;
+                if (head < c.heads) {
+                    w[i] = *reinterpret_cast<const uint4*>(x + head * view.head);
+                    if (at) olds[i] = scales[2 * head];
+                }
+            }
+            float4 table[T::kTable];
+            if (!which) {
+                if constexpr (STAGED) turned.angles(table, s_angles, token - t0, p.pairs);
+                else turned.angles(table, p.angles, (long long)token, p.pairs);
+            }
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                if (i >= steps) break;
+                const int head = first + i * rows_per_step;
+                const bool real = head < c.heads;
+                if (!which) w[i] = turned(w[i], table);
+                uint32_t most = __vmaxu2(__vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu));
+                most = max(most & 0xFFFFu, most >> 16);
+                const bool finite = most < (BF16 ? 0x7F80u : 0x7C00u);        // (the lane's; what is not is left out of the row's largest)
+                float a = BF16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half((unsigned short)most));
+                if (!finite) a = largest_finite<BF16>(w[i]);
+                for (int d = lanes_per_row >> 1; d; d >>= 1) a = fmaxf(a, __shfl_xor_sync(kAll, a, d));
+                const float old = olds[i], s = fmaxf(old, scale_for<E4M3>(a));
+                uint8_t* const held = held0 + head * held_head;
+                if (real && s > old && at > 0) {
+                    const float ratio = old / s;
+#pragma unroll 1
+                    for (int j = 0; j < at; ++j) requantise<E4M3>(held + j * held_token, ratio);
+                }
+                const uint2 q = to_bytes_of<E4M3, BF16>(w[i], s > 0.f ? 1.f / s : 1.f, finite);
+                if (real) {
+                    *reinterpret_cast<uint2*>(held + at * held_token) = q;
+                    if (col == 0) scales[2 * head] = s;
+                }
+            }
+        }
+        unit -= count;
+    }
+
+    // ---- queries: rows of the window in the order of tokens and heads ----
+    const int end = here * p.q_heads, count = (end + rows - 1) / rows;
+    if (unit >= count) return;
+    turned = T(p, p.q_weight, lane);
+#pragma unroll 1
+    for (; unit < count; unit += stride) {
+        const int first = unit * rows + row, token0 = first / p.q_heads, head0 = first - token0 * p.q_heads;
+        const uint16_t* const q = static_cast<const uint16_t*>(p.q.p) + t0 * p.q.token + col;
+        const int left = end - first;                 // of the lane's rows: those with i * rows_per_step < left
+        int token = token0, head = head0;
+        const auto next = [&]() {
+            for (head += rows_per_step; head >= p.q_heads; head -= p.q_heads) ++token;
+        };
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            if (i >= steps) break;
+            if (i * rows_per_step < left) w[i] = *reinterpret_cast<const uint4*>(q + token * p.q.token + head * p.q.head);
+            next();
+        }
+        token = token0;
+        head = head0;
+        uint16_t* to = static_cast<uint16_t*>(p.q_out) + ((long long)t0 * p.q_heads + first) * c.dim + col;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i, to += rows_per_step * c.dim) {
+            if (i >= steps) break;
+            const bool real = i * rows_per_step < left;
+            const int at = real ? token : 0;
+            float4 table[T::kTable];
+            if constexpr (STAGED) turned.angles(table, s_angles, at, p.pairs);
+            else turned.angles(table, p.angles, (long long)t0 + at, p.pairs);
+            const uint4 y = turned(w[i], table);
+            if (real) *reinterpret_cast<uint4*>(to) = y;
+            next();
         }
     }
 }
 
 }  // namespace
 
-// Up to 1024 tokens each has blocks of its own, so that a few tokens are spread over the GPU: a warp a unit; more of them go by sixteen.
+// Blocks enough for the GPU, a window to several of them, and no more rows to a warp than leave it full: a few tokens are spread over all of it.
 cudaError_t cache_append_launch(const AppendParams& p, bool e4m3, bool bf16, bool pairs_beside, cudaStream_t stream) {
-    const bool staged = p.tokens > 1024;
-    const int window = staged ? 16 : 1, units = 2 * p.cache.heads + p.q_heads, most = (units + kWarps - 1) / kWarps;
-    const int groups = staged ? std::max(1, most / 4) : most;
-    const long long blocks = (long long)((p.tokens + window - 1) / window) * groups;
+    constexpr int kBlocks = 148 * 4;
+    const int windows = (p.tokens + kWindow - 1) / kWindow, here = std::min(p.tokens, kWindow), rows_per_step = 256 / p.cache.dim;
+    const long long all_steps = (long long)p.tokens * (p.q_heads + 2 * p.cache.heads) / rows_per_step;
+    const int steps = (int)std::min<long long>(kHeld, all_steps / (kBlocks * kWarps / 2) + 1), rows = steps * rows_per_step;
+    // (units of a window at most: tokens that are runs of their own, or runs of two)
+    const long long singles = (long long)here * 2 * ((p.cache.heads + rows - 1) / rows), runs = (long long)(here + 1) / 2 * 2 * p.cache.heads;
+    const long long units = std::max(singles, runs) + ((long long)here * p.q_heads + rows - 1) / rows;
+    const int groups = (int)std::max<long long>(1, std::min<long long>((units + kWarps - 1) / kWarps, (kBlocks + windows - 1) / windows));
+    const long long blocks = (long long)windows * groups;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    const bool staged = groups <= kMostStaging;
     const auto go = [&](auto e, auto h, auto t, auto s) {
         return launch_overlapping(cache_append_kernel<decltype(e)::value, decltype(h)::value, decltype(t)::value, decltype(s)::value>, dim3((unsigned)blocks),
-                                  kWarps * 32, stream, p, window, groups);
+                                  kWarps * 32, stream, p, groups, steps);
     };
     const auto by_size = [&](auto e, auto h, auto t) { return staged ? go(e, h, t, std::true_type{}) : go(e, h, t, std::false_type{}); };
     const auto by_turn = [&](auto e, auto h) {

@@ -80,6 +80,27 @@ __device__ __noinline__ uint2 to_bytes_any(uint4 w, float inverse) {
     return make_uint2(r[0], r[1]);
 }
 
+// The same bytes of 8 packed fp16 values that are all finite, two at a time, where `inverse` is a normal fp16 number.  int8: 1536 + x * inverse is rounded
+// once, to whole numbers, and its low byte is q.  e4m3: the product is exact down to 2^-14, and what is below that is 0 either way.
+template <bool E4M3>
+__device__ __forceinline__ uint2 half_to_bytes(uint4 w, uint32_t inverse2) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (E4M3) {
+            unsigned short two;
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(two) : "r"(hmul2_u(u[i], inverse2)));
+            r[i] = two;
+        } else {
+            r[i] = hfma2_u(u[i], inverse2, 0x66006600u);
+        }
+    }
+    if (E4M3) return make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+    return make_uint2(prmt(r[0], r[1], 0x6420), prmt(r[2], r[3], 0x6420));
+}
+__device__ __forceinline__ bool normal_half(float power) { return power >= 6.103515625e-5f && power <= 32768.f; }
+
 // The least power of two s with a <= most * s (0 for a = 0).  With a in [2^e, 2^(e+1)): most = 127 = 1.984 * 2^6 and 448 = 1.75 * 2^8, so
 // s is 2^(e-6) (2^(e-8)) or the next one.  Not below 2^-100, so that 1 / s is a finite number whatever the input.
 template <bool E4M3>
