@@ -21,7 +21,8 @@ constexpr uint32_t kAll = 0xFFFFFFFFu;
 enum Turn { kStraight, kHalves, kPairs };             // no rotation; pairs (i, i + F); pairs (2 i, 2 i + 1)
 
 constexpr int kWindow = 16;                           // tokens whose runs a block looks at
-constexpr int kMostStaging = 8;                       // blocks of a window, each of which would bring its angles to shared memory
+constexpr int kMostGroups = 8;                        // more blocks of a window than these would each bring its angles to shared memory
+constexpr int kManyWarps = 8;
 constexpr int kStaged = 32;                           // tokens whose angles a block keeps in shared memory
 
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -37,6 +38,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 
 // 8 bytes of a page whose scale grows
+// 1 / s; the writers' scales are powers of two, whose exponents turn over
+__device__ __forceinline__ float inverse_of(float s) {
+    const uint32_t bits = __float_as_uint(s);
+    if (bits == 0) return 1.f;
+    return (bits & 0x7FFFFFu) || bits >= 0x7F000000u ? 1.f / s : __uint_as_float(0x7F000000u - bits);
+}
 template <bool E4M3>
 __device__ __forceinline__ void requantise(uint8_t* at, float ratio) {
     const uint2 b = *reinterpret_cast<const uint2*>(at);
@@ -151,173 +158,78 @@ struct Turned {
     }
 };
 
-// A block's share of a window of 16 tokens, a warp a unit at a time:
-//   * runs of several neighbouring tokens with ascending slots of one page, those that begin in the window: a head's keys or values, as
-//     the writer takes them (a prompt's tokens);
-//   * tokens that are runs of their own (a decoding step's): rows of `steps` times as many heads' keys or values as the warp has at once, each with its
-//     own page and scale;
-//   * the window's queries, as many rows of all tokens and heads.
-// STAGED: the angles of the window's tokens, and of those that its runs may go on to, are brought to shared memory once for all heads.
-template <bool E4M3, bool BF16, int TURN, bool STAGED>
-__global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const AppendParams p, int groups, int steps) {
-    using T = Turned<BF16, TURN>;
-    __shared__ float4 s_angles[STAGED && TURN != kStraight ? kStaged * 32 : 1];
-    const int lane = threadIdx.x & 31;
-    const int block = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - block * groups);
-    const CacheView& c = p.cache;
-    const int page = 1 << c.page_shift, lanes_per_row = c.dim >> 3, rows_per_step = 32 / lanes_per_row;
-    const int row = lane / lanes_per_row, col = (lane % lanes_per_row) * 8, chunk = kHeld * rows_per_step;
-    const int t0 = block * kWindow, tokens = p.tokens;
-    ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
-    // lane i: the slot of token t0 - 1 + i, and whether it goes on with the run of the one before
-    const int t = t0 - 1 + lane;
-    const int slot = t >= 0 && t < tokens ? p.slots[t] : -1;
-    if constexpr (STAGED && TURN != kStraight) {
-        const int two = p.pairs / 2, across = p.pairs / (2 * T::kTable), all = min(kStaged, tokens - t0) * two;
-        const float4* const from = reinterpret_cast<const float4*>(p.angles + (long long)t0 * p.pairs);
-        for (int i = threadIdx.x; i < all; i += kWarps * 32) {
-            const float4 x = __ldg(from + i);
-            const int token = i / two, j = i - token * two;
-            s_angles[(token * T::kTable + j % T::kTable) * across + j / T::kTable] = make_float4(x.x, x.z, x.y, x.w);
-        }
-        __syncthreads();
+// A block's view of its window: neighbouring tokens with ascending slots of one page are a run, the window's if it begins there.
+struct Window {
+    int t0, slot;                                     // lane i: the slot of token t0 - 1 + i
+    uint32_t on, singles, runs;                       // lanes that go on with a run; where runs of one token and of several begin
+    __device__ __forceinline__ Window(const AppendParams& p, int first) {
+        const int lane = threadIdx.x & 31, t = first - 1 + lane, page = 1 << p.cache.page_shift;
+        t0 = first;
+        slot = t >= 0 && t < p.tokens ? p.slots[t] : -1;
+        const int before = __shfl_up_sync(kAll, slot, 1);
+        const bool goes_on = lane > 0 && before >= 0 && slot == before + 1 && (slot & (page - 1)) != 0;
+        const bool begins = lane > 0 && lane <= kWindow && slot >= 0 && (slot >> p.cache.page_shift) < p.cache.pages && !goes_on;
+        on = __ballot_sync(kAll, goes_on);
+        const uint32_t starts = __ballot_sync(kAll, begins);
+        singles = starts & ~(on >> 1);
+        runs = starts & ~singles;
     }
-    const int before = __shfl_up_sync(kAll, slot, 1);
-    const bool goes_on = lane > 0 && before >= 0 && slot == before + 1 && (slot & (page - 1)) != 0;
-    const bool begins = lane > 0 && lane <= kWindow && slot >= 0 && (slot >> c.page_shift) < c.pages && !goes_on;
-    const uint32_t on = __ballot_sync(kAll, goes_on), starts = __ballot_sync(kAll, begins), singles = starts & ~(on >> 1), runs = starts & ~singles;
-    const int rows = steps * rows_per_step, per_token = (c.heads + rows - 1) / rows, here = min(kWindow, tokens - t0);
-    const int stride = groups * kWarps;
-    int unit = group * kWarps + (threadIdx.x >> 5);   // the warp's next one, counted from the first of the kind that is being worked on
     // the place of the n-th bit of a mask
-    const auto nth_of = [](uint32_t mask, int n) {
+    __device__ __forceinline__ static int nth_of(uint32_t mask, int n) {
         for (; n > 0; --n) mask &= mask - 1;
         return __ffs(mask) - 1;
-    };
-    uint4 w[kHeld];
-    T turned(p, p.k_weight, lane);
-
-    // ---- runs of a head's keys, then of its values ----
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
-        const RowsView view = which ? p.v : p.k;
-        const long long page_stride = which ? c.v_page : c.k_page, head_stride = which ? c.v_head : c.k_head, token_stride = which ? c.v_token : c.k_token;
-        const int count = __popc(runs) * c.heads;
-#pragma unroll 1
-        for (; unit < count; unit += stride) {
-            int head = unit, nth = 0;
-            for (; head >= c.heads; head -= c.heads) ++nth;
-            const int from = nth_of(runs, nth), run = t0 - 1 + from, first_slot = __shfl_sync(kAll, slot, from);
-            const int id = first_slot >> c.page_shift, at = first_slot & (page - 1);
-            float* const scale = reinterpret_cast<float*>(c.scales + (long long)id * c.heads + head) + which;
-            const float old = at ? *scale : 0.f;
-            // its length: up to the first lane that does not go on; beyond the 32 lanes it is looked for
-            const uint32_t stop = ~on & (~0u << (from + 1));
-            int n = stop ? __ffs(stop) - 1 - from : 32 - from;
-            while (!stop && n < page - at) {
-                const int i = n + lane;
-                const bool more = i < page - at && run + i < tokens && p.slots[run + i] == first_slot + i;
-                const uint32_t end = __ballot_sync(kAll, !more);
-                if (end) {
-                    n += __ffs(end) - 1;
-                    break;
-                }
-                n += 32;
-            }
-            // the lane's part of kHeld rows at a time; a run that fits (a page of 16 tokens does) is read once
-            const uint16_t* const first = static_cast<const uint16_t*>(view.p) + head * view.head + (run + row) * view.token + col;
-            const long long step = rows_per_step * view.token;
-            const bool near = STAGED && run + n <= t0 + kStaged;
-            const auto fetch = [&](int i0) {
-                const uint16_t* x = first + i0 * view.token;
-                const int left = n - i0 - row;        // of the lane's rows: those with i * rows_per_step < left
-#pragma unroll
-                for (int i = 0; i < kHeld; ++i, x += step) {
-                    w[i] = make_uint4(0, 0, 0, 0);
-                    if (i * rows_per_step < left) w[i] = *reinterpret_cast<const uint4*>(x);
-                }
-                if (which) return;
-#pragma unroll
-                for (int i = 0; i < kHeld; ++i) {     // (rows beyond the run are not used)
-                    if (i0 + i * rows_per_step >= n) break;
-                    const int token = run + min(i0 + i * rows_per_step + row, n - 1);
-                    float4 table[T::kTable];
-                    if (near) turned.angles(table, s_angles, token - t0, p.pairs);
-                    else turned.angles(table, p.angles, (long long)token, p.pairs);
-                    const uint4 y = turned(w[i], table);
-                    if (i * rows_per_step < left) w[i] = y;
-                }
-            };
-            uint32_t most = 0;
-#pragma unroll 1
-            for (int i0 = 0; i0 < n; i0 += chunk) {
-                fetch(i0);
-#pragma unroll
-                for (int i = 0; i < kHeld; ++i)
-                    most = __vmaxu2(most, __vmaxu2(__vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu)));
-            }
-            most = __reduce_max_sync(kAll, max(most & 0xFFFFu, most >> 16));
-            const bool finite = most < (BF16 ? 0x7F80u : 0x7C00u);
-            float a = BF16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half((unsigned short)most));
-            if (!finite) {                                                   // the largest of the others
-                a = 0.f;
-#pragma unroll 1
-                for (int i0 = 0; i0 < n; i0 += chunk) {
-                    if (n > chunk) fetch(i0);
-#pragma unroll
-                    for (int i = 0; i < kHeld; ++i) a = fmaxf(a, largest_finite<BF16>(w[i]));
-                }
-#pragma unroll
-                for (int d = 16; d; d /= 2) a = fmaxf(a, __shfl_xor_sync(kAll, a, d));
-            }
-            const float s = fmaxf(old, scale_for<E4M3>(a));
-            uint8_t* const held = (which ? c.v : c.k) + id * page_stride + head * head_stride + col;
-            if (s > old && at > 0) {
-                const float ratio = old / s;          // (0 where the scale was: bytes of infinities beside zeros go on standing for 0)
-#pragma unroll 1
-                for (int i = row; i < at; i += rows_per_step) requantise<E4M3>(held + i * token_stride, ratio);
-            }
-            const float inverse = s > 0.f ? 1.f / s : 1.f;
-            const uint32_t inverse2 = h2_as_u32(__float2half2_rn(inverse));
-            const bool by_halves = !BF16 && finite && normal_half(inverse);
-            const long long bytes_step = rows_per_step * token_stride;
-#pragma unroll 1
-            for (int i0 = 0; i0 < n; i0 += chunk) {
-                if (n > chunk) fetch(i0);
-                const int left = n - i0 - row;
-                uint8_t* to = held + (at + i0 + row) * token_stride;
-                if (by_halves) {
-#pragma unroll
-                    for (int i = 0; i < kHeld; ++i, to += bytes_step)
-                        if (i * rows_per_step < left) *reinterpret_cast<uint2*>(to) = half_to_bytes<E4M3>(w[i], inverse2);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kHeld; ++i, to += bytes_step)
-                        if (i * rows_per_step < left) *reinterpret_cast<uint2*>(to) = to_bytes_of<E4M3, BF16>(w[i], inverse, finite);
-                }
-            }
-            __syncwarp();
-            if (lane == 0) *scale = s;
-        }
-        unit -= count;
     }
+    // tokens of the run that begins at lane `from`: up to the first lane that does not go on; beyond the 32 lanes it is looked for
+    __device__ __forceinline__ int length(const AppendParams& p, int from, int first_slot) const {
+        const int lane = threadIdx.x & 31, page = 1 << p.cache.page_shift, left = page - (first_slot & (page - 1)), run = t0 - 1 + from;
+        const uint32_t stop = ~on & (~0u << (from + 1));
+        int n = stop ? __ffs(stop) - 1 - from : 32 - from;
+#pragma unroll 1
+        while (!stop && n < left) {
+            const int i = n + lane;
+            const bool more = i < left && run + i < p.tokens && p.slots[run + i] == first_slot + i;
+            const uint32_t end = __ballot_sync(kAll, !more);
+            if (end) {
+                n += __ffs(end) - 1;
+                break;
+            }
+            n += 32;
+        }
+        return n;
+    }
+};
 
-    // ---- keys, then values, of single tokens: rows are heads, each with its own scale ----
+__device__ __forceinline__ uint32_t largest_bits(uint32_t most, uint4 w) {                    // of magnitudes, two 16-bit values at a time
+    return __vmaxu2(most, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+}
+template <bool BF16>
+__device__ __forceinline__ float from_bits(uint32_t most) {
+    return BF16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half((unsigned short)most));
+}
+
+// Keys, then values, of tokens that are runs of their own: a warp takes `rows` heads of a token, each with its own scale.  `unit`: the warp's next one of
+// units that all warps take in turns, counted from the first of these; it is moved on behind them.
+template <bool E4M3, bool BF16, int TURN>
+__device__ __forceinline__ void append_singles(const AppendParams& p, const Window& window, const Turned<BF16, TURN>& turned, int steps, int stride, int& unit) {
+    using T = Turned<BF16, TURN>;
+    const CacheView& c = p.cache;
+    const int lane = threadIdx.x & 31, page = 1 << c.page_shift, lanes_per_row = c.dim >> 3, rows_per_step = 32 / lanes_per_row;
+    const int row = lane / lanes_per_row, col = (lane % lanes_per_row) * 8, rows = steps * rows_per_step, per_token = (c.heads + rows - 1) / rows;
 #pragma unroll 1
     for (int which = 0; which < 2; ++which) {
         const RowsView view = which ? p.v : p.k;
-        const int count = __popc(singles) * per_token;
+        const int count = __popc(window.singles) * per_token;
 #pragma unroll 1
         for (; unit < count; unit += stride) {
             int part = unit, nth = 0;
             for (; part >= per_token; part -= per_token) ++nth;
-            const int from = nth_of(singles, nth), token = t0 - 1 + from, from_slot = __shfl_sync(kAll, slot, from);
+            const int from = Window::nth_of(window.singles, nth), token = window.t0 - 1 + from, from_slot = __shfl_sync(kAll, window.slot, from);
             const int id = from_slot >> c.page_shift, at = from_slot & (page - 1), first = part * rows + row;
             const uint16_t* const x = static_cast<const uint16_t*>(view.p) + token * view.token + col;
             uint8_t* const held0 = (which ? c.v + id * c.v_page : c.k + id * c.k_page) + col;
             const long long held_token = which ? c.v_token : c.k_token, held_head = which ? c.v_head : c.k_head;
             float* const scales = reinterpret_cast<float*>(c.scales + (long long)id * c.heads) + which;
+            uint4 w[kHeld];
             float olds[kHeld];
 #pragma unroll
             for (int i = 0; i < kHeld; ++i) {
@@ -331,30 +243,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
                 }
             }
             float4 table[T::kTable];
-            if (!which) {
-                if constexpr (STAGED) turned.angles(table, s_angles, token - t0, p.pairs);
-                else turned.angles(table, p.angles, (long long)token, p.pairs);
-            }
+            if (!which) turned.angles(table, p.angles, (long long)token, p.pairs);
 #pragma unroll
             for (int i = 0; i < kHeld; ++i) {
                 if (i >= steps) break;
                 const int head = first + i * rows_per_step;
                 const bool real = head < c.heads;
                 if (!which) w[i] = turned(w[i], table);
-                uint32_t most = __vmaxu2(__vmaxu2(w[i].x & 0x7FFF7FFFu, w[i].y & 0x7FFF7FFFu), __vmaxu2(w[i].z & 0x7FFF7FFFu, w[i].w & 0x7FFF7FFFu));
+                uint32_t most = largest_bits(0, w[i]);
                 most = max(most & 0xFFFFu, most >> 16);
                 const bool finite = most < (BF16 ? 0x7F80u : 0x7C00u);        // (the lane's; what is not is left out of the row's largest)
-                float a = BF16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half((unsigned short)most));
+                float a = from_bits<BF16>(most);
                 if (!finite) a = largest_finite<BF16>(w[i]);
                 for (int d = lanes_per_row >> 1; d; d >>= 1) a = fmaxf(a, __shfl_xor_sync(kAll, a, d));
                 const float old = olds[i], s = fmaxf(old, scale_for<E4M3>(a));
                 uint8_t* const held = held0 + head * held_head;
                 if (real && s > old && at > 0) {
-                    const float ratio = old / s;
+                    const float ratio = old / s;      // (0 where the scale was: bytes of infinities beside zeros go on standing for 0)
 #pragma unroll 1
                     for (int j = 0; j < at; ++j) requantise<E4M3>(held + j * held_token, ratio);
                 }
-                const uint2 q = to_bytes_of<E4M3, BF16>(w[i], s > 0.f ? 1.f / s : 1.f, finite);
+                const uint2 q = to_bytes_of<E4M3, BF16>(w[i], inverse_of(s), finite);
                 if (real) {
                     *reinterpret_cast<uint2*>(held + at * held_token) = q;
                     if (col == 0) scales[2 * head] = s;
@@ -363,11 +272,114 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
         }
         unit -= count;
     }
+}
+
+// Few tokens: a block's share of a window of 16, a warp a unit at a time.  Runs of a head's keys or values as the writer takes them, single tokens by
+// heads, and the window's queries in the order of tokens and heads: `steps` times as many rows as the warp has at once.
+template <bool E4M3, bool BF16, int TURN>
+__global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const AppendParams p, int groups, int steps) {
+    using T = Turned<BF16, TURN>;
+    const int lane = threadIdx.x & 31;
+    const int block = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - block * groups);
+    const CacheView& c = p.cache;
+    const int page = 1 << c.page_shift, lanes_per_row = c.dim >> 3, rows_per_step = 32 / lanes_per_row;
+    const int row = lane / lanes_per_row, col = (lane % lanes_per_row) * 8, chunk = kHeld * rows_per_step, t0 = block * kWindow;
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const Window window(p, t0);
+    const int rows = steps * rows_per_step, here = min(kWindow, p.tokens - t0), stride = groups * kWarps;
+    int unit = group * kWarps + (threadIdx.x >> 5);   // the warp's next one, counted from the first of the kind that is being worked on
+    uint4 w[kHeld];
+    const int others = 2 * (__popc(window.runs) * c.heads + __popc(window.singles) * ((c.heads + rows - 1) / rows));
+
+    // ---- runs of a head's keys, then of its values; single tokens ----
+    if (unit < others) {
+        const T turned(p, p.k_weight, lane);
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+            const RowsView view = which ? p.v : p.k;
+            const long long page_stride = which ? c.v_page : c.k_page, head_stride = which ? c.v_head : c.k_head, token_stride = which ? c.v_token : c.k_token;
+            const int count = __popc(window.runs) * c.heads;
+#pragma unroll 1
+            for (; unit < count; unit += stride) {
+                int head = unit, nth = 0;
+                for (; head >= c.heads; head -= c.heads) ++nth;
+                const int from = Window::nth_of(window.runs, nth), run = t0 - 1 + from, first_slot = __shfl_sync(kAll, window.slot, from);
+                const int id = first_slot >> c.page_shift, at = first_slot & (page - 1), n = window.length(p, from, first_slot);
+                float* const scale = reinterpret_cast<float*>(c.scales + (long long)id * c.heads + head) + which;
+                const float old = at ? *scale : 0.f;
+                // the lane's part of kHeld rows at a time; a run that fits (a page of 16 tokens does) is read once
+                const uint16_t* const first = static_cast<const uint16_t*>(view.p) + head * view.head + (run + row) * view.token + col;
+                const auto fetch = [&](int i0) {
+                    const uint16_t* x = first + i0 * view.token;
+                    const int left = n - i0 - row;        // of the lane's rows: those with i * rows_per_step < left
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i, x += rows_per_step * view.token) {
+                        w[i] = make_uint4(0, 0, 0, 0);
+                        if (i * rows_per_step < left) w[i] = *reinterpret_cast<const uint4*>(x);
+                    }
+                    if (which) return;
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i) {     // (rows beyond the run are not used)
+                        if (i0 + i * rows_per_step >= n) break;
+                        float4 table[T::kTable];
+                        turned.angles(table, p.angles, (long long)run + min(i0 + i * rows_per_step + row, n - 1), p.pairs);
+                        const uint4 y = turned(w[i], table);
+                        if (i * rows_per_step < left) w[i] = y;
+                    }
+                };
+                uint32_t most = 0;
+#pragma unroll 1
+                for (int i0 = 0; i0 < n; i0 += chunk) {
+                    fetch(i0);
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i) most = largest_bits(most, w[i]);
+                }
+                most = __reduce_max_sync(kAll, max(most & 0xFFFFu, most >> 16));
+                const bool finite = most < (BF16 ? 0x7F80u : 0x7C00u);
+                float a = from_bits<BF16>(most);
+                if (!finite) {                                                   // the largest of the others
+                    a = 0.f;
+#pragma unroll 1
+                    for (int i0 = 0; i0 < n; i0 += chunk) {
+                        if (n > chunk) fetch(i0);
+#pragma unroll
+                        for (int i = 0; i < kHeld; ++i) a = fmaxf(a, largest_finite<BF16>(w[i]));
+                    }
+#pragma unroll
+                    for (int d = 16; d; d /= 2) a = fmaxf(a, __shfl_xor_sync(kAll, a, d));
+                }
+                const float s = fmaxf(old, scale_for<E4M3>(a));
+                uint8_t* const held = (which ? c.v : c.k) + id * page_stride + head * head_stride + col;
+                if (s > old && at > 0) {
+                    const float ratio = old / s;
+#pragma unroll 1
+                    for (int i = row; i < at; i += rows_per_step) requantise<E4M3>(held + i * token_stride, ratio);
+                }
+                const float inverse = inverse_of(s);
+#pragma unroll 1
+                for (int i0 = 0; i0 < n; i0 += chunk) {
+                    if (n > chunk) fetch(i0);
+                    const int left = n - i0 - row;
+                    uint8_t* to = held + (at + i0 + row) * token_stride;
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i, to += rows_per_step * token_stride)
+                        if (i * rows_per_step < left) *reinterpret_cast<uint2*>(to) = to_bytes_of<E4M3, BF16>(w[i], inverse, finite);
+                }
+                __syncwarp();
+                if (lane == 0) *scale = s;
+            }
+            unit -= count;
+        }
+        append_singles<E4M3, BF16, TURN>(p, window, turned, steps, stride, unit);
+    } else {
+        unit -= others;
+    }
 
     // ---- queries: rows of the window in the order of tokens and heads ----
     const int end = here * p.q_heads, count = (end + rows - 1) / rows;
     if (unit >= count) return;
-    turned = T(p, p.q_weight, lane);
+    const T turned(p, p.q_weight, lane);
 #pragma unroll 1
     for (; unit < count; unit += stride) {
         const int first = unit * rows + row, token0 = first / p.q_heads, head0 = first - token0 * p.q_heads;
@@ -390,15 +402,224 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_append_kernel(const Appe
         for (int i = 0; i < kHeld; ++i, to += rows_per_step * c.dim) {
             if (i >= steps) break;
             const bool real = i * rows_per_step < left;
-            const int at = real ? token : 0;
             float4 table[T::kTable];
-            if constexpr (STAGED) turned.angles(table, s_angles, at, p.pairs);
-            else turned.angles(table, p.angles, (long long)t0 + at, p.pairs);
+            turned.angles(table, p.angles, (long long)t0 + (real ? token : 0), p.pairs);
             const uint4 y = turned(w[i], table);
             if (real) *reinterpret_cast<uint4*>(to) = y;
             next();
         }
     }
+}
+
+// Many tokens: the window's angles are brought to shared memory once for all heads, and a unit's rows (a head's run of keys or values, or a head's
+// queries of the window) while the one before is worked on, each lane its own part of them, so that no registers hold them and no lane waits for another.
+template <bool E4M3, bool BF16, int TURN>
+__global__ void __launch_bounds__(kManyWarps * 32, 2) cache_append_many_kernel(const AppendParams p, int groups) {
+    using T = Turned<BF16, TURN>;
+    extern __shared__ uint4 s_rows[];                 // [warp][2][kHeld][lane], then the angles
+    float4* const s_angles = reinterpret_cast<float4*>(s_rows + kManyWarps * 2 * kHeld * 32);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int block = (int)(blockIdx.x / groups), group = (int)(blockIdx.x - block * groups);
+    const CacheView& c = p.cache;
+    const int page = 1 << c.page_shift, lanes_per_row = c.dim >> 3, rows_per_step = 32 / lanes_per_row;
+    const int row = lane / lanes_per_row, col = (lane % lanes_per_row) * 8, chunk = kHeld * rows_per_step, t0 = block * kWindow;
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const Window window(p, t0);
+    const int here = min(kWindow, p.tokens - t0), stride = groups * kManyWarps, run_units = __popc(window.runs) * c.heads, units = 2 * run_units + p.q_heads;
+    uint4* const mine = s_rows + warp * 2 * kHeld * 32 + lane;
+
+    struct Unit {
+        int kind, n;                                  // 0 keys, 1 values, 2 queries; rows
+        int head, run, id, at;                        // run: the first token
+        float old;
+        const uint16_t* x;                            // the lane's first row
+        long long token;                              // stride
+    };
+    const auto describe = [&](int unit) {
+        Unit u;
+        u.kind = unit < run_units ? 0 : unit < 2 * run_units ? 1 : 2;
+        u.head = unit - u.kind * run_units;
+        u.run = t0;
+        u.n = here;
+        u.old = 0.f;
+        u.id = u.at = 0;
+        if (u.kind < 2) {
+            int nth = 0;
+            for (; u.head >= c.heads; u.head -= c.heads) ++nth;
+            const int from = Window::nth_of(window.runs, nth), first_slot = __shfl_sync(kAll, window.slot, from);
+            u.run = t0 - 1 + from;
+            u.id = first_slot >> c.page_shift;
+            u.at = first_slot & (page - 1);
+            u.n = window.length(p, from, first_slot);
+            if (u.at) u.old = *(reinterpret_cast<const float*>(c.scales + (long long)u.id * c.heads + u.head) + u.kind);
+        }
+        const RowsView& view = u.kind == 0 ? p.k : u.kind == 1 ? p.v : p.q;
+        u.token = view.token;
+        u.x = static_cast<const uint16_t*>(view.p) + u.head * view.head + (u.run + row) * u.token + col;
+        return u;
+    };
+    const auto ask = [&](const Unit& u, int i0, uint4* to) {
+        const uint16_t* x = u.x + i0 * u.token;
+        const int left = u.n - i0 - row;              // of the lane's rows: those with i * rows_per_step < left
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i, x += rows_per_step * u.token)
+            if (i * rows_per_step < left) ptx::cp_async_16(ptx::smem_u32(to + 32 * i), x, 16);
+    };
+
+    int unit = group * kManyWarps + warp, buffer = 0;
+    Unit now{};
+    if (unit < units) {
+        now = describe(unit);
+        ask(now, 0, mine);
+    }
+    ptx::cp_async_commit();
+    if constexpr (TURN != kStraight) {
+        const int two = p.pairs / 2, across = p.pairs / (2 * T::kTable), all = min(kStaged, p.tokens - t0) * two;
+        const float4* const from = reinterpret_cast<const float4*>(p.angles + (long long)t0 * p.pairs);
+        for (int i = threadIdx.x; i < all; i += kManyWarps * 32) {
+            const float4 x = __ldg(from + i);
+            const int token = i / two, j = i - token * two;
+            s_angles[(token * T::kTable + j % T::kTable) * across + j / T::kTable] = make_float4(x.x, x.z, x.y, x.w);
+        }
+        __syncthreads();
+    }
+    T turned(p, now.kind == 2 ? p.q_weight : p.k_weight, lane);
+    bool of_queries = now.kind == 2;
+
+#pragma unroll 1
+    for (; unit < units; unit += stride) {
+        Unit next{};
+        uint4* const rows = mine + buffer * kHeld * 32;
+        buffer ^= 1;
+        if (unit + stride < units) {
+            next = describe(unit + stride);
+            ask(next, 0, mine + buffer * kHeld * 32);
+        }
+        ptx::cp_async_commit();
+        ptx::cp_async_wait_group<1>();
+        const int n = now.n;
+        if (now.kind == 2) {
+            if (!of_queries) turned = T(p, p.q_weight, lane);
+            of_queries = true;
+            uint16_t* to = static_cast<uint16_t*>(p.q_out) + ((long long)(t0 + row) * p.q_heads + now.head) * c.dim + col;
+#pragma unroll 2
+            for (int i = 0; i < kHeld; ++i, to += (long long)rows_per_step * p.q_heads * c.dim) {
+                if (i * rows_per_step >= n) break;
+                const int r = i * rows_per_step + row;
+                float4 table[T::kTable];
+                turned.angles(table, s_angles, min(r, n - 1), p.pairs);
+                const uint4 y = turned(rows[32 * i], table);
+                if (r < n) *reinterpret_cast<uint4*>(to) = y;
+            }
+            now = next;
+            continue;
+        }
+        const bool near = now.run + n <= t0 + kStaged;
+        uint32_t most = 0;
+        // a run that does not fit in the lane's places is read again, and its keys are treated again, for the second pass
+        const auto again = [&](int i0) {
+            ask(now, i0, rows);
+            ptx::cp_async_commit();
+            ptx::cp_async_wait_group<0>();
+        };
+        const auto treat = [&](int i0) {
+            if (now.kind) return;
+#pragma unroll 2
+            for (int i = 0; i < kHeld; ++i) {
+                const int r = i0 + i * rows_per_step + row, token = now.run + min(r, n - 1);
+                if (i0 + i * rows_per_step >= n) break;
+                float4 table[T::kTable];
+                if (near) turned.angles(table, s_angles, token - t0, p.pairs);
+                else turned.angles(table, p.angles, (long long)token, p.pairs);
+                rows[32 * i] = turned(rows[32 * i], table);
+            }
+        };
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += chunk) {
+            if (i0 > 0) again(i0);
+            treat(i0);
+            const int left = n - i0 - row;
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (i * rows_per_step < left) most = largest_bits(most, rows[32 * i]);
+        }
+        most = __reduce_max_sync(kAll, max(most & 0xFFFFu, most >> 16));
+        const bool finite = most < (BF16 ? 0x7F80u : 0x7C00u);
+        float a = from_bits<BF16>(most);
+        if (!finite) {                                                       // the largest of the others
+            a = 0.f;
+#pragma unroll 1
+            for (int i0 = 0; i0 < n; i0 += chunk) {
+                if (n > chunk) {
+                    again(i0);
+                    treat(i0);
+                }
+                const int left = n - i0 - row;
+#pragma unroll 1
+                for (int i = 0; i * rows_per_step < left && i < kHeld; ++i) a = fmaxf(a, largest_finite<BF16>(rows[32 * i]));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int d = 16; d; d /= 2) a = fmaxf(a, __shfl_xor_sync(kAll, a, d));
+        }
+        const float old = now.old, s = fmaxf(old, scale_for<E4M3>(a));
+        const long long token_stride = now.kind ? c.v_token : c.k_token;
+        uint8_t* const held = (now.kind ? c.v + now.id * c.v_page + now.head * c.v_head : c.k + now.id * c.k_page + now.head * c.k_head) + col;
+        if (s > old && now.at > 0) {
+            const float ratio = old / s;              // (0 where the scale was: bytes of infinities beside zeros go on standing for 0)
+#pragma unroll 1
+            for (int i = row; i < now.at; i += rows_per_step) requantise<E4M3>(held + i * token_stride, ratio);
+        }
+        const float inverse = inverse_of(s);
+        const uint32_t inverse2 = h2_as_u32(__float2half2_rn(inverse));
+        const bool by_halves = !BF16 && finite && normal_half(inverse);
+#pragma unroll 1
+        for (int i0 = 0; i0 < n; i0 += chunk) {
+            if (n > chunk) {
+                again(i0);
+                treat(i0);
+            }
+            const int left = n - i0 - row;
+            uint8_t* to = held + (now.at + i0 + row) * token_stride;
+            if (by_halves) {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i, to += rows_per_step * token_stride)
+                    if (i * rows_per_step < left) *reinterpret_cast<uint2*>(to) = half_to_bytes<E4M3>(rows[32 * i], inverse2);
+            } else {
+#pragma unroll 2
+                for (int i = 0; i < kHeld; ++i, to += rows_per_step * token_stride)
+                    if (i * rows_per_step < left) *reinterpret_cast<uint2*>(to) = to_bytes_of<E4M3, BF16>(rows[32 * i], inverse, finite);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) *(reinterpret_cast<float*>(c.scales + (long long)now.id * c.heads + now.head) + now.kind) = s;
+        now = next;
+    }
+    ptx::cp_async_wait_group<0>();
+    if (window.singles == 0) return;
+    unit -= units;
+    append_singles<E4M3, BF16, TURN>(p, window, T(p, p.k_weight, lane), kHeld, stride, unit);
+}
+
+template <typename F>
+cudaError_t launch_many(F* kernel, long long blocks, cudaStream_t stream, const AppendParams& p, int groups) {
+    constexpr int kSmem = (kManyWarps * 2 * kHeld + kStaged) * 32 * 16;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kManyWarps * 32);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, p, groups);
+    if (e == cudaSuccess) count_launch();
+    return e;
 }
 
 }  // namespace
@@ -415,12 +636,12 @@ cudaError_t cache_append_launch(const AppendParams& p, bool e4m3, bool bf16, boo
     const int groups = (int)std::max<long long>(1, std::min<long long>((units + kWarps - 1) / kWarps, (kBlocks + windows - 1) / windows));
     const long long blocks = (long long)windows * groups;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    const bool staged = groups <= kMostStaging;
-    const auto go = [&](auto e, auto h, auto t, auto s) {
-        return launch_overlapping(cache_append_kernel<decltype(e)::value, decltype(h)::value, decltype(t)::value, decltype(s)::value>, dim3((unsigned)blocks),
-                                  kWarps * 32, stream, p, groups, steps);
+    const auto by_size = [&](auto e, auto h, auto t) {
+        constexpr bool E = decltype(e)::value, H = decltype(h)::value;
+        constexpr int turn = decltype(t)::value;
+        if (groups > kMostGroups) return launch_overlapping(cache_append_kernel<E, H, turn>, dim3((unsigned)blocks), kWarps * 32, stream, p, groups, steps);
+        return launch_many(cache_append_many_kernel<E, H, turn>, blocks, stream, p, groups);
     };
-    const auto by_size = [&](auto e, auto h, auto t) { return staged ? go(e, h, t, std::true_type{}) : go(e, h, t, std::false_type{}); };
     const auto by_turn = [&](auto e, auto h) {
         if (p.pairs == 0) return by_size(e, h, std::integral_constant<int, kStraight>{});
         return pairs_beside ? by_size(e, h, std::integral_constant<int, kPairs>{}) : by_size(e, h, std::integral_constant<int, kHalves>{});
