@@ -367,7 +367,8 @@ int i4mm_cache_share(int64_t requests, const void* prefix_of, const void* seq_le
  * are read once for all rows that share it, not once for each.
  *   prefix_of, prefix_starts, prefix_rows (listed >= tokens entries)   i4mm_cache_share's effective, starts and rows of the same step
  *   scratch   i4mm_cache_shared_scratch_bytes(tokens, q_heads, head_dim) bytes, 16-byte aligned, of any contents, this call's alone
- * The prefix's sums are fp32 too, its weights rounded to fp16; everything else is as above.
+ * heads * (table_width * page_size / 128 + 2) * (tokens * (q_heads / heads) / 128 + the smaller of requests and tokens) has to be below 2^31
+ * (I4MM_ERR_TOO_LARGE otherwise).  The prefix's sums are fp32 too, its weights rounded to fp16; everything else is as above.
  */
 size_t i4mm_cache_shared_scratch_bytes(int64_t tokens, int64_t q_heads, int64_t head_dim);
 int i4mm_cache_attention_shared(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,

@@ -106,6 +106,12 @@ cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t
 
 // The rows that read prefixes over those.  Both kernels run where the step's rows are more than the first one takes.
 constexpr int kFewReaders = 128;                      // rows of a key head
+// The prefix kernel counts tiles of 128 tokens and 128 rows in 32 bits: what the host knows of their number has to fit.
+bool countable(const i4mm::AttentionParams& p) {
+    const int64_t span = ((int64_t)p.table_width << p.cache.page_shift) / 128 + 2, rows = (int64_t)p.tokens * p.group / 128 + std::min<int64_t>(p.requests, p.tokens);
+    return span <= kMost / p.cache.heads && rows <= kMost / (span * p.cache.heads);
+}
+
 cudaError_t attend_prefixes(const i4mm::AttentionParams& p, bool e4m3, bool bf16, cudaStream_t stream) {
     g_attention_kernels |= I4MM_ATTENTION_PREFIX;
     cudaError_t e = i4mm::cache_prefix_launch(p, e4m3, bf16, kFewReaders, stream);
@@ -178,6 +184,7 @@ int attention(const i4mm_cache* cache, void* out, const void* q, int type, int64
     p.scale = scale;
     const bool e4m3 = cache->type == I4MM_CACHE_E4M3, bf16 = type == I4MM_TYPE_BF16;
     if (p.prefix_of && requests > 0) {
+        if (!countable(p)) return I4MM_ERR_TOO_LARGE;
         const cudaError_t e = attend_prefixes(p, e4m3, bf16, (cudaStream_t)stream);
         if (e != cudaSuccess) return finish(e);
     }

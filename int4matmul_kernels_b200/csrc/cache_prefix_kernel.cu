@@ -103,7 +103,8 @@ __device__ __forceinline__ Place load_place(const AttentionParams& p, int most_r
     if (r.row_tiles > 1) r.height = (int)(((uint32_t)r.rows + 32u * r.row_tiles - 1) / (32u * r.row_tiles)) * 32;
     return r;
 }
-__device__ __forceinline__ long long units_of(const AttentionParams& p, const Place& r) { return (long long)(r.row_tiles * p.cache.heads) * r.tiles; }
+// (the host has made sure that all of them together are below 2^31)
+__device__ __forceinline__ uint32_t units_of(const AttentionParams& p, const Place& r) { return (uint32_t)(r.row_tiles * p.cache.heads) * (uint32_t)r.tiles; }
 
 // ---- two fp32 at a time ----
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -296,29 +297,49 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     };
 
     if (warp == kCopy) {
-        // the block's range: all have the same number of tiles, but for those at the end
-        long long total = 0;
+        // the block's range: all have the same number of tiles, but for those at the end.  The first 32 places stay in the lanes' registers.
+        Place mine{};
+        uint32_t own = 0;
+        if (lane < p.requests) {
+            mine = load_place(p, most_rows, lane);
+            own = units_of(p, mine);
+        }
+        uint32_t total = own;
 #pragma unroll 1
-        for (int b = lane; b < p.requests; b += 32) total += units_of(p, load_place(p, most_rows, b));
-        total = warp_sum(total);
-        const long long share = max(div_nn(total + gridDim.x - 1, gridDim.x), (long long)kMinBlockTiles);
-        long long at = blockIdx.x * share;
-        const long long end = min(at + share, total);
+        for (int b = lane + 32; b < p.requests; b += 32) total += units_of(p, load_place(p, most_rows, b));
+        total = __reduce_add_sync(kAll, total);
+        const uint32_t share = max((total + gridDim.x - 1) / gridDim.x, (uint32_t)kMinBlockTiles);
+        uint32_t at = min(blockIdx.x * share, total);
+        const uint32_t end = min(at + share, total);
         // the place that the range begins in
-        long long before = 0;
+        uint32_t before = 0;
         int b = 0;
         Place r{};
         const auto find_place = [&]() {               // from request b (a multiple of 32) on, `before` tiles before it
 #pragma unroll 1
             for (; b < p.requests; b += 32) {
-                const Place mine = b + lane < p.requests ? load_place(p, most_rows, b + lane) : Place{};
-                const long long own = b + lane < p.requests ? units_of(p, mine) : 0, upto = warp_prefix(own);
+                if (b > 0) {
+                    mine = b + lane < p.requests ? load_place(p, most_rows, b + lane) : Place{};
+                    own = b + lane < p.requests ? units_of(p, mine) : 0;
+                }
+                uint32_t upto = own;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const uint32_t o = __shfl_up_sync(kAll, upto, d);
+                    if (lane >= d) upto += o;
+                }
                 const uint32_t here = __ballot_sync(kAll, before + upto > at);
                 if (here) {
                     const int l = __ffs(here) - 1;
                     before += __shfl_sync(kAll, upto - own, l);
                     b += l;
-                    r = load_place(p, most_rows, b);
+                    r.first = __shfl_sync(kAll, mine.first, l);
+                    r.rows = __shfl_sync(kAll, mine.rows, l);
+                    r.lo = __shfl_sync(kAll, mine.lo, l);
+                    r.limit = __shfl_sync(kAll, mine.limit, l);
+                    r.tiles = __shfl_sync(kAll, mine.tiles, l);
+                    r.row_tiles = __shfl_sync(kAll, mine.row_tiles, l);
+                    r.height = __shfl_sync(kAll, mine.height, l);
                     return;
                 }
                 before += __shfl_sync(kAll, upto, 31);
@@ -346,8 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             }
             Item t;
             {
-                const long long in = at - before;
-                const int segment = (int)div_nn(in, r.tiles), tile = (int)(in - (long long)segment * r.tiles);
+                const uint32_t in = at - before;
+                const int segment = (int)(in / (uint32_t)r.tiles), tile = (int)(in - (uint32_t)segment * r.tiles);
                 const int head = segment / r.row_tiles, row_tile = segment - head * r.row_tiles;
                 t.valid = 1;
                 t.place = b;
@@ -359,12 +380,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 t.lo = r.lo;
                 t.limit = r.limit;
                 t.tile0 = r.lo / kTokens + tile;
-                t.tiles = (int)min((long long)(r.tiles - tile), end - at);
+                t.tiles = (int)min((uint32_t)(r.tiles - tile), end - at);
                 t.first_block = t.last_block = (int)blockIdx.x;
                 if (t.tiles < r.tiles) {
-                    const long long from = at - tile;
-                    t.first_block = (int)div_nn(from, share);
-                    t.last_block = (int)div_nn(from + r.tiles - 1, share);
+                    const uint32_t from = at - tile;
+                    t.first_block = (int)(from / share);
+                    t.last_block = (int)((from + r.tiles - 1) / share);
                 }
             }
             ok = wait_on(&bars.item_empty[n % kItems], (n / kItems) ^ 1, &s_abort);
@@ -689,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 bool again = false;
 #pragma unroll 1
                 for (;;) {
-                    bool over = false;
+                    bool over = j == 0 && !again;     // (the rows have no reference yet: to that at once)
 #pragma unroll
                     for (int c = 0; c < kColumns / 16; ++c)
                         if (2 * c < groups && !over) {
@@ -728,10 +749,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                             }
                         }
                     if (again) break;
-                    ++pass;
-                    if (over) s_need[h][pass & 1] = pass;
-                    if (!(ok = meet(id_meet))) break;
-                    if (s_need[h][pass & 1] != pass) break;
+                    if (j > 0) {
+                        ++pass;
+                        if (over) s_need[h][pass & 1] = pass;
+                        if (!(ok = meet(id_meet))) break;
+                        if (s_need[h][pass & 1] != pass) break;
+                    }
                     if (j > 0) ok = wait_on(&bars.pv_done[(i - 1) & 1], (i - 1) >> 1, &s_abort);
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
@@ -752,9 +775,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                         s_keep[h][tid] = top == old ? 1.f : exp2_approx(old - top);
                     }
                     if (!(ok = meet(id_meet))) break;
-#pragma unroll
-                    for (int k = 0; k < kColumns; ++k) sums[k] *= s_keep[h][k];
                     if (j > 0) {
+#pragma unroll
+                        for (int k = 0; k < kColumns; ++k) sums[k] *= s_keep[h][k];
 #pragma unroll 1
                         for (int q = 0; q < groups; ++q) {
                             uint32_t x[8];

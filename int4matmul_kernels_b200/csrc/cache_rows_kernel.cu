@@ -143,8 +143,18 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         ptx::fence_mbar_init();
     }
     __syncwarp();
-    ptx::grid_dependency_wait();
-    ptx::grid_launch_dependents();
+    // With prefixes, the kernel before this one is that of the prefixes, which let this one begin once it knew all before it complete: the rows' own
+    // tokens are worked on beside it, and it is waited for when what it writes is needed.  (No thread leaves before that: this kernel must not be
+    // complete before that one is.)
+    bool waited = false;
+    const auto await_prefixes = [&]() {
+        if (!waited) {
+            ptx::grid_dependency_wait();
+            ptx::grid_launch_dependents();
+        }
+        waited = true;
+    };
+    if (!PREFIX) await_prefixes();
 
     // rows of no request
     {
@@ -166,7 +176,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
     const long long own_upto = warp_prefix(own);
     total = warp_sum(total);
     const long long blocks = min((long long)gridDim.x, (total + kMinBlockTiles - 1) / kMinBlockTiles);
-    if (blockIdx.x >= blocks) return;
+    if (blockIdx.x >= blocks) {
+        await_prefixes();
+        return;
+    }
     const long long c0 = range_lo(total, blocks, blockIdx.x), c1 = range_lo(total, blocks, blockIdx.x + 1);
     const long long warps = min((long long)S::kWarps, (c1 - c0 + kMinWarpTiles - 1) / kMinWarpTiles);
     const long long u0 = warp < warps ? c0 + range_lo(c1 - c0, warps, warp) : c1, u1 = warp < warps ? c0 + range_lo(c1 - c0, warps, warp + 1) : c1;
@@ -352,9 +365,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                     for (int i = 0; i < 4; ++i) o[n][j][i] = 0.f;
             }
 
-            // What the rows' prefixes came to is asked for now: the last tile would otherwise wait for it, and the warp's copies with it.
+            // What the rows' prefixes came to is asked for now, if it is there: the last tile would otherwise wait for it, and the warp's copies with it.
             float2 prefix[NT][2];
-            if constexpr (PREFIX) {
+            const auto ask_prefixes = [&]() {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -363,11 +376,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                         prefix[n][i] = make_float2(-INFINITY, 0.f);
                         if (r.joins && position[n][i] >= 0) {
                             const long long at = (long long)(r.row0 + token) * p.q_heads + h;
-                            prefix[n][i] = *(p.prefix_total + at);
-                            if (tiles_here == r.tiles) ptx::prefetch_l1(p.prefix_sums + at * D + (D / 8) * g);
+                            prefix[n][i] = p.prefix_total[at];
+                            ptx::prefetch_l1(p.prefix_sums + at * D + (D / 8) * g);
                         }
                     }
-            }
+            };
+            const bool joins_here = PREFIX && tiles_here == r.tiles, asked = waited;
+            if (joins_here && asked) ask_prefixes();
             // tiles that begin in [whole_from, whole_to] are seen whole by all rows of the tile of rows
             const int whole_from = p.window ? max(r.position + r.rows - p.window, r.lo) : r.lo;
             const int whole_to = base + S::kRows <= all_rows ? min(r.position + 1, r.limit) - kTile : -1;
@@ -541,6 +556,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) sum[n][i] += __shfl_xor_sync(kAll, sum[n][i], d);
 
+            if (joins_here && !asked) {
+                await_prefixes();
+                ask_prefixes();
+            }
             if (tiles_here == r.tiles) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -615,6 +634,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
         }
     }
     __syncthreads();
+    await_prefixes();
 
     // ---- parts of one segment are added up, a row by a warp ----
     constexpr int kMine = D / 32;                     // columns of a lane
