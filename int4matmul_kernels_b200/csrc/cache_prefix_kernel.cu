@@ -30,11 +30,11 @@ namespace i4mm {
 namespace {
 
 constexpr int kTokens = 128;                          // of a tile
-constexpr int kMostRows = 128;
-constexpr int kGroups = 4, kColumns = kMostRows / kGroups;                    // of softmax warps; columns of each
-constexpr int kSoftmaxWarps = 4 * kGroups, kDecode0 = kSoftmaxWarps, kDecodeWarps = 4, kMma = kDecode0 + 4, kCopy = kMma + 1, kCopyValues = kCopy + 1;
+constexpr int kMostRows = 64;
+constexpr int kHalves = 2, kColumns = kMostRows / kHalves;                   // of a tile's rows; columns of each
+constexpr int kSoftmaxWarps = 4 * 2 * kHalves, kDecode0 = kSoftmaxWarps, kDecodeWarps = 4, kMma = kDecode0 + 4, kCopy = kMma + 1, kCopyValues = kCopy + 1;
 constexpr int kThreads = 32 * (kCopyValues + 1);
-constexpr int kKeys = 3, kValues = 4;                 // stages of the rings
+constexpr int kStages = 3;                            // of either ring
 constexpr int kItems = 4, kScales = 4, kRawScales = 8;
 constexpr int kPieces = kTokens / 16;                 // pages of a tile, at most
 constexpr int kMinBlockTiles = 2;                     // fewer tiles than this are not cut further
@@ -46,15 +46,15 @@ constexpr uint32_t kMnStride = 16384;                 // 128 tokens of 64 column
 template <int D>
 struct Layout {
     static constexpr int kHalf = kTokens * D;                                 // bytes of a tile's keys or values
-    static constexpr int kV = 2 * kMnStride, kP = 2 * kMnStride, kQ = kMostRows * D * 2;
-    static constexpr int kV0 = 0, kP0 = kV0 + kV, kQ0 = kP0 + kP, kKeys0 = kQ0 + kQ, kValues0 = kKeys0 + kKeys * kHalf,
-                         kBytes = kValues0 + kValues * kHalf + 1024;
+    static constexpr int kV = 2 * kMnStride, kP = kMnStride, kQ = kMostRows * D * 2;         // V and P: one of two
+    static constexpr int kV0 = 0, kP0 = kV0 + 2 * kV, kQ0 = kP0 + 2 * kP, kKeys0 = kQ0 + kQ, kValues0 = kKeys0 + kStages * kHalf,
+                         kBytes = kValues0 + kStages * kHalf + 1024;
     static constexpr int kPartFloats = kMostRows * D + 2 * kMostRows;         // sums [row][dim], (reference, total) [row]
 };
 constexpr size_t kPartsBytes = (size_t)kMaxBlocks * 2 * Layout<128>::kPartFloats * 4;
 
 struct Item {
-    int valid, place, head, base, rows, n;            // base: first row of the tile; n: rows, rounded up to 32
+    int valid, place, head, base, rows, n;            // base: first row of the tile; n: rows, rounded up to 16
     int first;                                        // of the place's readers in the list
     int lo, limit;                                    // tokens that may be seen
     int tile0, tiles;
@@ -63,8 +63,8 @@ struct Item {
 
 struct Barriers {
     unsigned long long item_full[kItems], item_empty[kItems], q_full[kItems], scale_full[kScales];
-    unsigned long long keys_full[kKeys], keys_empty[kKeys], values_full[kValues], values_empty[kValues];
-    unsigned long long k_full[2], s_full[2], p_full[2], pv_done[2], v_full, drained;
+    unsigned long long keys_full[kStages], keys_empty[kStages], values_full[kStages], values_empty[kStages];
+    unsigned long long k_full[2], s_full[2], p_full[2], v_full[2], pv_done[2], drained;
 };
 
 // A whole warp waits; false (in all of its lanes) once the block gives up.
@@ -99,8 +99,8 @@ __device__ __forceinline__ Place load_place(const AttentionParams& p, int most_r
     r.lo = p.window && seq >= p.window ? min(seq - p.window + 1, r.limit) : 0;
     r.tiles = max((r.limit + kTokens - 1) / kTokens - r.lo / kTokens, 1);
     r.row_tiles = (r.rows + kMostRows - 1) / kMostRows;
-    r.height = (r.rows + 31) & ~31;
-    if (r.row_tiles > 1) r.height = (int)(((uint32_t)r.rows + 32u * r.row_tiles - 1) / (32u * r.row_tiles)) * 32;
+    r.height = (r.rows + 15) & ~15;
+    if (r.row_tiles > 1) r.height = (int)(((uint32_t)r.rows + 16u * r.row_tiles - 1) / (16u * r.row_tiles)) * 16;
     return r;
 }
 // (the host has made sure that all of them together are below 2^31)
@@ -174,11 +174,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     __shared__ int s_low[kItems][kMostRows];          // the first token that the row sees
     __shared__ float s_up[kItems][kMostRows];         // what its scores are multiplied with (bf16)
     __shared__ int s_most_low[kItems];
-    __shared__ __align__(16) float s_minus_top[kGroups][kColumns];            // the rows' references, their signs turned over
-    __shared__ __align__(16) float s_keep[kGroups][kColumns];
-    __shared__ float s_warps[kGroups][4][kColumns];
-    __shared__ volatile uint32_t s_need[kGroups][2];
-    __shared__ volatile int s_abort, s_last[kGroups];
+    // (by set and half)
+    __shared__ __align__(16) float s_minus_top[2 * kHalves][kColumns];        // the rows' references, their signs turned over
+    __shared__ __align__(16) float s_keep[2 * kHalves][kColumns];
+    __shared__ float s_warps[2 * kHalves][4][kColumns];
+    __shared__ volatile uint32_t s_need[2 * kHalves][2];
+    __shared__ float2 s_take[kMostRows];              // of a row, what either set's sums are multiplied with
+    __shared__ volatile int s_abort, s_last[kHalves];
     __shared__ uint32_t tmem_smem;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t smem = (ptx::smem_u32(dynamic) + 1023u) & ~1023u;
@@ -196,12 +198,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             init(bars.q_full[i], kDecodeWarps);
         }
 #pragma unroll 1
-        for (int i = 0; i < kKeys; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             init(bars.keys_full[i], 2 * pieces);      // each lane's bytes, and its scales
             init(bars.keys_empty[i], kDecodeWarps);
         }
 #pragma unroll 1
-        for (int i = 0; i < kValues; ++i) {
+        for (int i = 0; i < kStages; ++i) {
             init(bars.values_full[i], pieces);
             init(bars.values_empty[i], kDecodeWarps);
         }
@@ -211,19 +213,22 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
         for (int i = 0; i < 2; ++i) {
             init(bars.k_full[i], kDecodeWarps);
             init(bars.s_full[i], 1);
-            init(bars.p_full[i], kSoftmaxWarps);
+            init(bars.p_full[i], kSoftmaxWarps / 2);
             init(bars.pv_done[i], 1);
+            init(bars.v_full[i], kDecodeWarps);
         }
-        init(bars.v_full, kDecodeWarps);
         init(bars.drained, 1);
         ptx::fence_mbar_init();
         s_abort = 0;
 #pragma unroll 1
-        for (int i = 0; i < 2 * kGroups; ++i) s_need[i >> 1][i & 1] = 0;
+        for (int i = 0; i < 4 * kHalves; ++i) s_need[i >> 1][i & 1] = 0;
     }
     if (D == 64)                                      // the columns of V that there are not
 #pragma unroll 1
-        for (int i = threadIdx.x; i < (int)kMnStride / 16; i += kThreads) ptx::sts128(v_tile + kMnStride + 16 * i, make_uint4(0, 0, 0, 0));
+        for (int i = threadIdx.x; i < (int)kMnStride / 16; i += kThreads) {
+            ptx::sts128(v_tile + kMnStride + 16 * i, make_uint4(0, 0, 0, 0));
+            ptx::sts128(v_tile + L::kV + kMnStride + 16 * i, make_uint4(0, 0, 0, 0));
+        }
     ptx::fence_proxy_async_smem();
     if (warp == kMma) {
         ptx::tmem_alloc(ptx::smem_u32(&tmem_smem), 512);
@@ -233,18 +238,17 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     __syncthreads();
     ptx::tc_fence_after_sync();
     const uint32_t tmem = tmem_smem;
-    const auto s_col = [&](uint32_t g) { return tmem + (g & 1) * 128; };
-    const uint32_t o_col = tmem + 256;
-    const auto k_col = [&](uint32_t g) { return tmem + 384 + (g & 1) * 64; };
+    const auto s_col = [&](uint32_t g) { return tmem + (g & 1) * kMostRows; };
+    const auto o_col = [&](uint32_t g) { return tmem + (2 + (g & 1)) * kMostRows; };
+    const auto k_col = [&](uint32_t g) { return tmem + 4 * kMostRows + (g & 1) * 64; };
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
 
     // Named barriers among four warps.  One that gives up arrives once more as it leaves (s_abort is set by then), which lets the others through to see it.
-    const auto meet = [&](int id) -> bool {
-        ptx::named_bar_sync(id, 128);
+    const auto meet = [&](int id, int threads) -> bool {
+        ptx::named_bar_sync(id, threads);
         return !__any_sync(kAll, s_abort);
     };
-    const auto leave = [&](int id) { ptx::named_bar_arrive(id, 128); };
     const auto done_with_item = [&](uint32_t n) {
         __syncwarp();
         if (lane == 0) arrive(&bars.item_empty[n % kItems]);
@@ -375,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 t.head = head;
                 t.base = row_tile * r.height;
                 t.rows = max(min(r.height, r.rows - t.base), 0);
-                t.n = max((t.rows + 31) & ~31, 32);
+                t.n = max((t.rows + 15) & ~15, 16);
                 t.first = r.first;
                 t.lo = r.lo;
                 t.limit = r.limit;
@@ -396,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             }
             __syncwarp();
             ++n;
-            ok = copy(t, g, &k_map, keys_ring, bars.keys_full, bars.keys_empty, kKeys, true);
+            ok = copy(t, g, &k_map, keys_ring, bars.keys_full, bars.keys_empty, kStages, true);
             g += t.tiles;
             at += t.tiles;
         }
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             items[n % kItems].valid = 0;
             arrive(&bars.item_full[n % kItems]);
         }
-        if (!ok) landed(bars.keys_full, kKeys);
+        if (!ok) landed(bars.keys_full, kStages);
     } else if (warp == kCopyValues) {
         uint32_t g = 0;
         bool ok = true;
@@ -414,11 +418,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             ok = next_item(n);
             if (!ok || !items[n % kItems].valid) break;
             const Item t = items[n % kItems];
-            ok = copy(t, g, &v_map, values_ring, bars.values_full, bars.values_empty, kValues, false);
+            ok = copy(t, g, &v_map, values_ring, bars.values_full, bars.values_empty, kStages, false);
             g += t.tiles;
             done_with_item(n);
         }
-        if (!ok) landed(bars.values_full, kValues);
+        if (!ok) landed(bars.values_full, kStages);
     } else if (warp == kMma) {
         // ---- products ----
         uint32_t g = 0;
@@ -428,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             ok = next_item(n);
             if (!ok || !items[n % kItems].valid) break;
             const int tiles = items[n % kItems].tiles, columns = items[n % kItems].n;
-            const uint32_t idesc = ptx::idesc_f16_m128(columns), idesc_mn = idesc | kBothMn, buffers = columns <= 64 ? 2 : 1;
+            const uint32_t idesc = ptx::idesc_f16_m128(columns), idesc_mn = idesc | kBothMn;
             ok = wait_on(&bars.q_full[n % kItems], n / kItems, &s_abort);
             const auto score = [&](uint32_t i) {      // S_i = K_i Q^T; the weights of tile i - 2 are there by now, so its scores have been read
                 ok = ok && wait_on(&bars.k_full[i & 1], i >> 1, &s_abort);
@@ -448,13 +452,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
 #pragma unroll 1
             for (int j = 0; j < tiles && ok; ++j) {
                 const uint32_t i = g + j;
-                ok = wait_on(&bars.v_full, i, &s_abort) && wait_on(&bars.p_full[i & 1], i >> 1, &s_abort);
+                ok = wait_on(&bars.v_full[i & 1], i >> 1, &s_abort) && wait_on(&bars.p_full[i & 1], i >> 1, &s_abort);
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
                 if (ptx::elect_one()) {
-                    const uint64_t a = smem_desc_mn(v_tile), b = smem_desc_mn(p_tile + (buffers == 2 ? (i & 1) * kMnStride : 0));
+                    const uint64_t a = smem_desc_mn(v_tile + (i & 1) * L::kV), b = smem_desc_mn(p_tile + (i & 1) * L::kP);
 #pragma unroll
-                    for (int k = 0; k < kTokens / 16; ++k) ptx::umma_f16_ss(o_col, a + (uint64_t)(k * 2048 >> 4), b + (uint64_t)(k * 2048 >> 4), idesc_mn, j > 0 || k > 0);
+                    for (int k = 0; k < kTokens / 16; ++k) ptx::umma_f16_ss(o_col(i), a + (uint64_t)(k * 2048 >> 4), b + (uint64_t)(k * 2048 >> 4), idesc_mn, j > 1 || k > 0);
                     ptx::tc_commit(ptx::smem_u32(&bars.pv_done[i & 1]));
                 }
                 __syncwarp();
@@ -470,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
         for (uint32_t i = 0; i < ptx::kSpinLimit && !ptx::mbar_try_wait(ptx::smem_u32(&bars.drained), 0); ++i) {}
     } else if (warp >= kDecode0) {
         // ---- queries; bytes to operands ----
-        constexpr int kMeet = kGroups + 1;
+        constexpr int kMeet = 7;
         const int w = warp - kDecode0, tid = w * 32 + lane;
         constexpr int kUnits = D / 8;                 // of 16 bytes in a query
         uint32_t g = 0;
@@ -496,19 +500,21 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                         }
                     }
                 }
-                s_row[slot][tid] = id;
-                s_query[tid] = query;
-                s_low[slot][tid] = low;
+                if (tid < kMostRows) {
+                    s_row[slot][tid] = id;
+                    s_query[tid] = query;
+                    s_low[slot][tid] = low;
+                }
                 const int most = __reduce_max_sync(kAll, low);
                 if (p.window) {
                     if (tid == 0) s_most_low[slot] = 0;
-                    if (!(ok = meet(kMeet))) break;
+                    if (!(ok = meet(kMeet, 128))) break;
                     if (lane == 0) atomicMax(&s_most_low[slot], most);
                 } else if (tid == 0) {
                     s_most_low[slot] = 0;
                 }
             }
-            if (!(ok = meet(kMeet))) break;
+            if (!(ok = meet(kMeet, 128))) break;
             // (the scores of the item before are complete)
             if (g > 0 && !(ok = wait_on(&bars.s_full[(g - 1) & 1], (g - 1) >> 1, &s_abort))) break;
             constexpr int kAtOnce = 4, kRowsAtOnce = 32 / kUnits;             // of a warp
@@ -551,9 +557,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             };
             // keys: a thread a token
             const auto keys = [&](int j) -> bool {
-                const uint32_t i = g + j, at = i % kKeys;
+                const uint32_t i = g + j, at = i % kStages;
                 const int first = (t.tile0 + j) * kTokens;
-                if (!wait_on(&bars.keys_full[at], i / kKeys, &s_abort)) return false;
+                if (!wait_on(&bars.keys_full[at], i / kStages, &s_abort)) return false;
                 if (w == 0 && lane < pieces) {
                     const float2 raw = s_raw[i % kRawScales][lane];
                     const float value = fmaxf(raw.y, kLeastScale);
@@ -592,14 +598,14 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             };
             // values: 8 tokens and 4 units of 16 at a time, in an order whose lanes meet in no bank
             const auto values = [&](int j) -> bool {
-                const uint32_t i = g + j, at = i % kValues;
+                const uint32_t i = g + j, at = i % kStages;
                 const int first = (t.tile0 + j) * kTokens;
-                if (!wait_on(&bars.values_full[at], i / kValues, &s_abort)) return false;
-                if (i >= 1 && !wait_on(&bars.pv_done[(i - 1) & 1], (i - 1) >> 1, &s_abort)) return false;
+                if (!wait_on(&bars.values_full[at], i / kStages, &s_abort)) return false;
+                if (i >= 2 && !wait_on(&bars.pv_done[i & 1], (i >> 1) - 1, &s_abort)) return false;              // (the values that lay there have been used)
                 const bool all = all_there(i, first);
                 const int in8 = (lane >> 3) ^ (lane & 4 ? 5 : 0), token0 = w * 32 + in8, unit = lane & 3;
                 const uint32_t from = values_ring + at * L::kHalf + token0 * D + ((16 * unit) ^ (D == 128 ? in8 << 4 : ((in8 >> 1) & 3) << 4));
-                const uint32_t to = v_tile + token0 * 128 + ((32 * unit) ^ (in8 << 4));
+                const uint32_t to = v_tile + (i & 1) * L::kV + token0 * 128 + ((32 * unit) ^ (in8 << 4));
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {
                     const bool seen = all || seen_at(i, first, token0 + 8 * q);
@@ -619,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    arrive(&bars.v_full);
+                    arrive(&bars.v_full[i & 1]);
                     arrive(&bars.values_empty[at]);
                 }
                 return true;
@@ -630,10 +636,12 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             g += t.tiles;
             if (ok) done_with_item(n);
         }
-        if (!ok) leave(kMeet);
+        if (!ok) ptx::named_bar_arrive(kMeet, 128);
     } else {
         // ---- softmax ----
-        const int h = warp >> 2, w = warp & 3, tid = w * 32 + lane, id_meet = 1 + h;      // h: the group
+        // A set of eight warps has every other tile, with references, totals and sums of its own, so that one set's chain of steps runs beside the other's.
+        const int set = warp >> 3, h = (warp >> 2) & 1, me = warp >> 2, w = warp & 3, tid = w * 32 + lane;
+        const int id_set = 1 + me, id_half = 5 + h;   // named barriers: of four warps, and of both sets' for a half
         const uint32_t lanes = (uint32_t)(w * 32) << 16;
         uint32_t g = 0, pass = 0;
         bool ok = true;
@@ -646,21 +654,20 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             const Item& t = items[item_slot];
             ok = wait_on(&bars.q_full[item_slot], n / kItems, &s_abort);
             if (!ok) break;
-            const int columns = t.n / kGroups, row0 = h * columns, groups = columns / 8, tiles = t.tiles;       // groups of 8
-            const uint32_t buffers = t.n <= 64 ? 2 : 1;
+            const int columns = t.n / kHalves, row0 = h * columns, groups = columns / 8, tiles = t.tiles;       // groups of 8
             const int most_low = s_most_low[item_slot];
-            if (tid < kColumns) {
-                s_minus_top[h][tid] = tid < columns ? -kNone : -INFINITY;     // (columns that are another half's, or nobody's, have no weights)
-                s_keep[h][tid] = 1.f;
-            }
+            if (tid < kColumns) s_minus_top[me][tid] = tid < columns ? -kNone : -INFINITY;   // (columns that are the other half's, or nobody's, have no weights)
             float sums[kColumns];
 #pragma unroll
             for (int i = 0; i < kColumns; ++i) sums[i] = 0.f;
-            if (!(ok = meet(id_meet))) break;
+            if (!(ok = meet(id_set, 128))) break;
+            const int j0 = (set ^ g) & 1;
 #pragma unroll 1
-            for (int j = 0; j < tiles; ++j) {
+            for (int j = j0; j < tiles; j += 2) {
                 const uint32_t i = g + j;
-                ok = wait_on(&bars.scale_full[i % kScales], i / kScales, &s_abort) && wait_on(&bars.s_full[i & 1], i >> 1, &s_abort);
+                ok = wait_on(&bars.scale_full[i % kScales], i / kScales, &s_abort) && wait_on(&bars.s_full[set], i >> 1, &s_abort);
+                // (what lay in the weights' place has been used, and is in the sums)
+                if (ok && j >= 2) ok = wait_on(&bars.pv_done[set], (i >> 1) - 1, &s_abort);
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
                 const float4 sc = s_scale[i % kScales][tid >> page_shift];
@@ -668,13 +675,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 const bool there = sc.w != 0.f && token >= t.lo && token < t.limit, hide = first < most_low;
                 // (keys of tokens that are not there are 0)
                 const float a = there ? factor * sc.x : 0.f, b = there ? sc.y : -INFINITY, inverse = sc.z;
-                if (j >= (int)buffers) {                                      // (what lay in the weights' place has been used)
-                    const uint32_t used = i - buffers;
-                    ok = wait_on(&bars.pv_done[used & 1], used >> 1, &s_abort);
-                    if (!ok) break;
-                }
                 const uint32_t s_at = s_col(i) + lanes + row0;
-                const uint32_t p_at = p_tile + (buffers == 2 ? (i & 1) * kMnStride : 0) + tid * 128, unit0 = row0 / 8;
+                const uint32_t p_at = p_tile + set * L::kP + tid * 128, unit0 = row0 / 8;
                 // exponents of N columns from `at` on, relative to the rows' references or not
                 const auto exponents = [&](auto& x, int at, bool relative) {
                     constexpr int N = sizeof(x) / 4;
@@ -688,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                             a1 = mul2(a1, make_float2(up.z, up.w));
                         }
                         if (relative) {
-                            from = *reinterpret_cast<const float4*>(&s_minus_top[h][at + k]);
+                            from = *reinterpret_cast<const float4*>(&s_minus_top[me][at + k]);
                             f0 = add2(f0, make_float2(from.x, from.y));
                             f1 = add2(f1, make_float2(from.z, from.w));
                         }
@@ -710,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 bool again = false;
 #pragma unroll 1
                 for (;;) {
-                    bool over = j == 0 && !again;     // (the rows have no reference yet: to that at once)
+                    bool over = j < 2 && !again;     // (the rows have no reference yet: to that at once)
 #pragma unroll
                     for (int c = 0; c < kColumns / 16; ++c)
                         if (2 * c < groups && !over) {
@@ -744,48 +746,45 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                                     for (int k = 0; k < 4; ++k)
                                         y[k] = h2_as_u32(__floats2half2_rn(__uint_as_float(x[8 * q + 2 * k]), __uint_as_float(x[8 * q + 2 * k + 1])));
                                     const uint32_t unit = unit0 + 2 * c + q;
-                                    if (2 * c + q < groups) ptx::sts128(p_at + (unit >> 3) * kMnStride + (((unit ^ tid) & 7) << 4), make_uint4(y[0], y[1], y[2], y[3]));
+                                    if (2 * c + q < groups) ptx::sts128(p_at + ((unit ^ (tid & 7)) << 4), make_uint4(y[0], y[1], y[2], y[3]));
                                 }
                             }
                         }
                     if (again) break;
-                    if (j > 0) {
+                    if (j >= 2) {
                         ++pass;
-                        if (over) s_need[h][pass & 1] = pass;
-                        if (!(ok = meet(id_meet))) break;
-                        if (s_need[h][pass & 1] != pass) break;
+                        if (over) s_need[me][pass & 1] = pass;
+                        if (!(ok = meet(id_set, 128))) break;
+                        if (s_need[me][pass & 1] != pass) break;
                     }
-                    if (j > 0) ok = wait_on(&bars.pv_done[(i - 1) & 1], (i - 1) >> 1, &s_abort);
-                    if (!ok) break;
-                    ptx::tc_fence_after_sync();
                     {
                         uint32_t x[kColumns];
                         ptx::tmem_ld32(s_at, x);
                         ptx::tc_wait_ld();
                         exponents(x, 0, false);
-                        s_warps[h][w][lane] = reduce32(x, [](float u, float v) { return fmaxf(u, v); });
+                        s_warps[me][w][lane] = reduce32(x, [](float u, float v) { return fmaxf(u, v); });
                     }
-                    if (!(ok = meet(id_meet))) break;
+                    if (!(ok = meet(id_set, 128))) break;
                     if (tid < columns) {
-                        const float old = -s_minus_top[h][tid];
+                        const float old = -s_minus_top[me][tid];
                         float top = old;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) top = fmaxf(top, s_warps[h][k][tid]);
-                        s_minus_top[h][tid] = -top;
-                        s_keep[h][tid] = top == old ? 1.f : exp2_approx(old - top);
+                        for (int k = 0; k < 4; ++k) top = fmaxf(top, s_warps[me][k][tid]);
+                        s_minus_top[me][tid] = -top;
+                        s_keep[me][tid] = top == old ? 1.f : exp2_approx(old - top);
                     }
-                    if (!(ok = meet(id_meet))) break;
-                    if (j > 0) {
+                    if (!(ok = meet(id_set, 128))) break;
+                    if (j >= 2) {
 #pragma unroll
-                        for (int k = 0; k < kColumns; ++k) sums[k] *= s_keep[h][k];
+                        for (int k = 0; k < kColumns; ++k) sums[k] *= s_keep[me][k];
 #pragma unroll 1
                         for (int q = 0; q < groups; ++q) {
                             uint32_t x[8];
-                            ptx::tmem_ld8(o_col + lanes + row0 + 8 * q, x);
+                            ptx::tmem_ld8(o_col(set) + lanes + row0 + 8 * q, x);
                             ptx::tc_wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * s_keep[h][8 * q + k]);
-                            ptx::tmem_st8(o_col + lanes + row0 + 8 * q, x);
+                            for (int k = 0; k < 8; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * s_keep[me][8 * q + k]);
+                            ptx::tmem_st8(o_col(set) + lanes + row0 + 8 * q, x);
                         }
                         ptx::tc_wait_st();
                     }
@@ -795,68 +794,83 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 ptx::tc_fence_before_sync();
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) arrive(&bars.p_full[i & 1]);
+                if (lane == 0) arrive(&bars.p_full[set]);
             }
             if (!ok) break;
             g += tiles;
-            ok = wait_on(&bars.pv_done[(g - 1) & 1], (g - 1) >> 1, &s_abort);
+            for (uint32_t i = tiles > 1 ? g - 2 : g - 1; i != g && ok; ++i) ok = wait_on(&bars.pv_done[i & 1], i >> 1, &s_abort);
             if (!ok) break;
             ptx::tc_fence_after_sync();
-            // totals: over the lanes, then over the warps
+            // totals: over the lanes, then over the warps, then of both sets
             {
                 uint32_t x[kColumns];
 #pragma unroll
                 for (int k = 0; k < kColumns; ++k) x[k] = __float_as_uint(sums[k]);
-                s_warps[h][w][lane] = reduce32(x, [](float u, float v) { return u + v; });
+                s_warps[me][w][lane] = reduce32(x, [](float u, float v) { return u + v; });
             }
-            if (!(ok = meet(id_meet))) break;
-            const auto reference = [&](int r) { return s_minus_top[h][r] == -kNone ? -INFINITY : -s_minus_top[h][r]; };
-            const auto total_of = [&](int r) { return (s_warps[h][0][r] + s_warps[h][1][r]) + (s_warps[h][2][r] + s_warps[h][3][r]); };
-            // (int8: the products' rows are the dims in decode4's order)
-            const int dim = E4M3 ? tid : (tid & ~3) | ((tid & 1) << 1) | ((tid >> 1) & 1);
-            const bool real = tid < D;
+            if (!(ok = meet(id_half, 256))) break;
             // a part: the block's first item continues another block's, its last is continued; the one that comes last adds them up
             const bool whole = t.first_block == t.last_block;
             const int a = t.first_block, z = t.last_block;
             float* const parts = reinterpret_cast<float*>(header + p.prefix_parts);
             const auto part_of = [&](int block) { return parts + ((size_t)block * 2 + (block == a ? 1 : 0)) * L::kPartFloats; };
             float* const own = part_of(blockIdx.x);
-            if (tid < columns) {
-                const float2 both = make_float2(reference(tid), total_of(tid));
+            if (set == 0 && tid < columns) {
+                float top[2], total[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int of = 2 * k + h;
+                    const float minus = s_minus_top[of][tid];
+                    top[k] = minus == -kNone ? -INFINITY : -minus;
+                    total[k] = (s_warps[of][0][tid] + s_warps[of][1][tid]) + (s_warps[of][2][tid] + s_warps[of][3][tid]);
+                }
+                const float most = fmaxf(top[0], top[1]), from = most == -INFINITY ? 0.f : most;
+                const float2 take = make_float2(exp2_approx(top[0] - from), exp2_approx(top[1] - from));
+                const float2 both = make_float2(most, total[0] * take.x + total[1] * take.y);
                 const int id = s_row[item_slot][row0 + tid];
+                s_take[row0 + tid] = take;
                 if (!whole) *reinterpret_cast<float2*>(own + kMostRows * D + 2 * (row0 + tid)) = both;
                 else if (id >= 0) p.prefix_total[id] = both;
             }
+            if (!(ok = meet(id_half, 256))) break;
+            // (int8: the products' rows are the dims in decode4's order)
+            const int dim = E4M3 ? tid : (tid & ~3) | ((tid & 1) << 1) | ((tid >> 1) & 1);
+            const bool real = tid < D;
 #pragma unroll 1
-            for (int q = 0; q < groups; ++q) {
-                uint32_t x[8];
-                ptx::tmem_ld8(o_col + lanes + row0 + 8 * q, x);
+            for (int q = set; q < groups; q += 2) {   // (a set that had no tile has no sums)
+                uint32_t x[8], y[8];
+                ptx::tmem_ld8(o_col(g - 1) + lanes + row0 + 8 * q, x);
+                ptx::tmem_ld8(o_col(tiles > 1 ? g : g - 1) + lanes + row0 + 8 * q, y);
                 ptx::tc_wait_ld();
                 if (real)
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int row = row0 + 8 * q + k, id = s_row[item_slot][row];
+                        const float2 take = s_take[row];
+                        const float last = (g - 1) & 1 ? take.y : take.x, other = (g - 1) & 1 ? take.x : take.y;
                         float* const to = whole ? p.prefix_sums + (long long)id * D : own + row * D;
-                        if (id >= 0) to[dim] = __uint_as_float(x[k]);
+                        float sum = __uint_as_float(x[k]) * last;
+                        if (tiles > 1) sum = fmaf(__uint_as_float(y[k]), other, sum);
+                        if (id >= 0) to[dim] = sum;
                     }
                 __syncwarp();
             }
             if (!whole) {
                 __threadfence();
-                if (!(ok = meet(id_meet))) break;
-                if (tid == 0) {
-                    unsigned int* const counter = reinterpret_cast<unsigned int*>(header + kPrefixCounters) + kGroups * a + h;
+                if (!(ok = meet(id_half, 256))) break;
+                if (set == 0 && tid == 0) {
+                    unsigned int* const counter = reinterpret_cast<unsigned int*>(header + kPrefixCounters) + kHalves * a + h;
                     const bool last = atomicAdd(counter, 1u) == (unsigned int)(z - a);
                     if (last) atomicExch(counter, 0u);                        // as the next launch expects it
                     s_last[h] = last;
                     __threadfence();
                 }
-                if (!(ok = meet(id_meet))) break;
+                if (!(ok = meet(id_half, 256))) break;
                 if (s_last[h]) {
                     __threadfence();
                     using Columns = std::conditional_t<D == 128, float4, float2>;             // of a lane
 #pragma unroll 1
-                    for (int r = w; r < columns; r += 4) {
+                    for (int r = 4 * set + w; r < columns; r += 8) {
                         const int row = row0 + r, id = s_row[item_slot][row];
                         if (id < 0) continue;
                         const auto both = [&](int b) { return __ldcg(reinterpret_cast<const float2*>(part_of(b) + kMostRows * D + 2 * row)); };
@@ -893,13 +907,16 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                         if (lane == 0) p.prefix_total[id] = make_float2(m, all_total);
                     }
                 }
-                if (!(ok = meet(id_meet))) break;                             // (s_last is free again)
             }
-            // what was read of the sums is read before the next item's products overwrite them
+            // what was read of the sums is read before the next item's products overwrite them, whichever set it was of
             ptx::tc_fence_before_sync();
+            if (!(ok = meet(id_half, 256))) break;
             done_with_item(n);
         }
-        if (!ok) leave(id_meet);
+        if (!ok) {
+            ptx::named_bar_arrive(id_set, 128);
+            ptx::named_bar_arrive(id_half, 256);
+        }
     }
 
     if (lane == 0 && s_abort) atomicExch(reinterpret_cast<int*>(header + kStatusOffset), 63);
