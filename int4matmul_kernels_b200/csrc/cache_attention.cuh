@@ -3,6 +3,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "cache.cuh"
 #include "common.cuh"
 #include "ptx.cuh"
@@ -51,7 +53,8 @@ constexpr size_t kRowsCounters = 0;                   // one per block
 constexpr size_t kPromptNext = 4096;                  // the next item to be worked on
 constexpr size_t kPromptCounters = 8192;              // two per part
 constexpr int kPromptParts = 320;
-constexpr size_t kPrefixCounters = 16384;             // four per block
+constexpr size_t kPrefixCounters = 16384;             // two per block
+constexpr int kPrefixRows = 64;                       // rows of a tile of the prefix kernel
 
 struct Request {
     int row0, rows;                                   // its packed rows
@@ -184,6 +187,66 @@ __device__ __forceinline__ Joint join_prefix(float m, float sum, float2 prefix) 
     const float total = fmaf(sum, a, prefix.y * b), f = total > 0.f ? 1.f / total : total;      // (a NaN stays one)
     return {a * f, b * f};
 }
+// ---- what a row's prefix came to: joined, or in parts -----------------------------------------------------------------------------
+// The prefix kernel leaves a row's (m, total) and sums.  Where many blocks had a part of the prefix each, `total` is negative and m's bits name
+// them: blocks a .. a + count - 1, and the row's place in their tiles.  Whoever reads the row adds them up: all SMs do that at once, where a block that
+// joined 18 parts of 64 rows read 0.6 MB alone (8 us).  A few parts are better joined there (64 requests of 300 tokens of their own behind 4000
+// of 40 heads, 4 parts: 130 us, and 175 where each row's reader looks for them at the end of its tokens).
+__device__ __forceinline__ float2 in_parts(int a, int count, int row) { return make_float2(__int_as_float(a | count << 8 | row << 16), -1.f); }
+struct PrefixParts {
+    const float* base;
+    int a, count, row, dim;
+    __device__ __forceinline__ PrefixParts(const AttentionParams& p, float2 told) {
+        const int bits = __float_as_int(told.x);
+        a = bits & 0xFF;
+        count = bits >> 8 & 0xFF;
+        row = bits >> 16 & 0xFF;
+        dim = p.cache.dim;
+        base = reinterpret_cast<const float*>(static_cast<const uint8_t*>(p.workspace) + p.prefix_parts);
+    }
+    // a block's two places: of a segment that it goes on with, and of one that begins with it
+    __device__ __forceinline__ const float* part(int i) const { return base + (size_t)(2 * (a + i) + (i == 0 ? 1 : 0)) * (kPrefixRows * dim + 2 * kPrefixRows); }
+    __device__ __forceinline__ const float* sums(int i) const { return part(i) + row * dim; }
+    __device__ __forceinline__ float2 total(int i) const { return __ldcg(reinterpret_cast<const float2*>(part(i) + kPrefixRows * dim + 2 * row)); }
+    __device__ __forceinline__ float most() const {
+        float m = -INFINITY;
+#pragma unroll 8
+        for (int i = 0; i < count; ++i) m = fmaxf(m, total(i).x);
+        return m;
+    }
+};
+// N of the row's sums, from column `col` on, and its (m, total)
+template <int N>
+__device__ __forceinline__ float2 prefix_sums(const AttentionParams& p, float2 told, long long at, int col, float (&sums)[N]) {
+    static_assert(N % 2 == 0, "two at a time at least");
+    using Some = std::conditional_t<N % 4 == 0, float4, float2>;
+    constexpr int kSome = sizeof(Some) / 4;
+    if (!(told.y < 0.f)) {
+#pragma unroll
+        for (int k = 0; k < N; k += kSome) *reinterpret_cast<Some*>(sums + k) = *reinterpret_cast<const Some*>(p.prefix_sums + at * p.cache.dim + col + k);
+        return told;
+    }
+    const PrefixParts parts(p, told);
+    const float m = parts.most(), from = m == -INFINITY ? 0.f : m;
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) sums[k] = 0.f;
+#pragma unroll 2
+    for (int i = 0; i < parts.count; ++i) {
+        const float2 of = parts.total(i);
+        const float take = exp2_approx(of.x - from);
+        total = fmaf(take, of.y, total);
+#pragma unroll
+        for (int k = 0; k < N; k += kSome) {
+            float x[kSome];
+            *reinterpret_cast<Some*>(x) = __ldcg(reinterpret_cast<const Some*>(parts.sums(i) + col + k));
+#pragma unroll
+            for (int e = 0; e < kSome; ++e) sums[k + e] = fmaf(take, x[e], sums[k + e]);
+        }
+    }
+    return make_float2(m, total);
+}
+
 // the position of packed row `token`, which reads the prefix at `place`, that prefix counted
 __device__ __forceinline__ int behind_prefix(const AttentionParams& p, int place, int token) {
     int b = min(token, p.requests - 1);

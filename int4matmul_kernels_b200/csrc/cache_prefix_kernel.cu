@@ -30,14 +30,15 @@ namespace i4mm {
 namespace {
 
 constexpr int kTokens = 128;                          // of a tile
-constexpr int kMostRows = 64;
+constexpr int kMostRows = kPrefixRows;
 constexpr int kHalves = 2, kColumns = kMostRows / kHalves;                   // of a tile's rows; columns of each
 constexpr int kSoftmaxWarps = 4 * 2 * kHalves, kDecode0 = kSoftmaxWarps, kDecodeWarps = 4, kMma = kDecode0 + 4, kCopy = kMma + 1, kCopyValues = kCopy + 1;
 constexpr int kThreads = 32 * (kCopyValues + 1);
 constexpr int kStages = 3;                            // of either ring
 constexpr int kItems = 4, kScales = 4, kRawScales = 8;
 constexpr int kPieces = kTokens / 16;                 // pages of a tile, at most
-constexpr int kMinBlockTiles = 2;                     // fewer tiles than this are not cut further
+constexpr int kJoined = 6;                            // parts of a segment that one block adds up
+constexpr int kMinBlockTiles = 4;                     // fewer tiles than this are not cut further
 constexpr float kNone = -3e38f;                       // a reference below any score
 constexpr float kMostLog = 14.f;                      // fp16 holds 2^16
 constexpr uint32_t kNoPage = 0x7FC0DEADu;             // in the place of a scale: there is no such page
@@ -569,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 if (i >= 2 && !wait_on(&bars.s_full[i & 1], (i >> 1) - 1, &s_abort)) return false;             // (the keys that lay there have been used)
                 const uint32_t from = keys_ring + at * L::kHalf + tid * D, to = k_col(i) + ((uint32_t)(w * 32) << 16);
                 const uint32_t swizzle = D == 128 ? (lane & 7) << 4 : ((lane >> 1) & 3) << 4;
-#pragma unroll 1
+#pragma unroll
                 for (int c0 = 0; c0 < D / 16; c0 += 4) {
                     uint32_t out[32];
 #pragma unroll
@@ -606,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 const int in8 = (lane >> 3) ^ (lane & 4 ? 5 : 0), token0 = w * 32 + in8, unit = lane & 3;
                 const uint32_t from = values_ring + at * L::kHalf + token0 * D + ((16 * unit) ^ (D == 128 ? in8 << 4 : ((in8 >> 1) & 3) << 4));
                 const uint32_t to = v_tile + (i & 1) * L::kV + token0 * 128 + ((32 * unit) ^ (in8 << 4));
-#pragma unroll 1
+#pragma unroll 2
                 for (int q = 0; q < 4; ++q) {
                     const bool seen = all || seen_at(i, first, token0 + 8 * q);
 #pragma unroll
@@ -809,9 +810,10 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 s_warps[me][w][lane] = reduce32(x, [](float u, float v) { return u + v; });
             }
             if (!(ok = meet(id_half, 256))) break;
-            // a part: the block's first item continues another block's, its last is continued; the one that comes last adds them up
-            const bool whole = t.first_block == t.last_block;
+            // A part: the block's first item continues another block's, its last is continued.  Few parts are added up by the block that comes last; more of
+            // them would take it longer than they take those who read the rows.
             const int a = t.first_block, z = t.last_block;
+            const bool whole = a == z, joins = !whole && z - a < kJoined;
             float* const parts = reinterpret_cast<float*>(header + p.prefix_parts);
             const auto part_of = [&](int block) { return parts + ((size_t)block * 2 + (block == a ? 1 : 0)) * L::kPartFloats; };
             float* const own = part_of(blockIdx.x);
@@ -830,7 +832,8 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 const int id = s_row[item_slot][row0 + tid];
                 s_take[row0 + tid] = take;
                 if (!whole) *reinterpret_cast<float2*>(own + kMostRows * D + 2 * (row0 + tid)) = both;
-                else if (id >= 0) p.prefix_total[id] = both;
+                if (id >= 0 && whole) p.prefix_total[id] = both;
+                if (id >= 0 && !whole && !joins && (int)blockIdx.x == a) p.prefix_total[id] = in_parts(a, z - a + 1, row0 + tid);
             }
             if (!(ok = meet(id_half, 256))) break;
             // (int8: the products' rows are the dims in decode4's order)
@@ -855,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                     }
                 __syncwarp();
             }
-            if (!whole) {
+            if (joins) {
                 __threadfence();
                 if (!(ok = meet(id_half, 256))) break;
                 if (set == 0 && tid == 0) {

@@ -766,7 +766,18 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
                 uint16_t* const out = static_cast<uint16_t*>(p.out) + to;
                 // what the sums are multiplied with, once there are all of the row's own; the same of its prefix's
                 const auto joint = [&](float m, float sum) {
-                    if constexpr (KIND == kJoining) return join_prefix(m, sum, prefix);
+                    if constexpr (KIND == kJoining) {
+                        if (prefix.y < 0.f) {         // parts: joined where their sums would lie, for this thread alone
+                            const float2 told = prefix;
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 4) {
+                                alignas(16) float x[4];
+                                prefix = prefix_sums(p, told, 0, c, x);
+                                *reinterpret_cast<float4*>(p.prefix_sums + to + c) = make_float4(x[0], x[1], x[2], x[3]);
+                            }
+                        }
+                        return join_prefix(m, sum, prefix);
+                    }
                     return Joint{sum > 0.f ? 1.f / sum : sum, 0.f};                           // (a NaN stays one)
                 };
                 float* const kept = KIND == kPrefixes ? p.prefix_sums + to : nullptr;

@@ -571,13 +571,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
                         const long long to = ((long long)(r.row0 + token) * p.q_heads + h) * D + (D / 8) * g;
                         if constexpr (PREFIX) {
                             if (prefix[n][i].y != 0.f) {
-                                const Joint f = join_prefix(m[n][i], sum[n][i], prefix[n][i]);
+                                alignas(16) float x[D / 8];
+                                const long long at = (long long)(r.row0 + token) * p.q_heads + h;
+                                const Joint f = join_prefix(m[n][i], sum[n][i], prefix_sums(p, prefix[n][i], at, (D / 8) * g, x));
 #pragma unroll
-                                for (int j = 0; j < kWords; ++j) {
-                                    const float4 x = *reinterpret_cast<const float4*>(p.prefix_sums + to + 4 * j);
-                                    store4<BF16>(p.out, to + 4 * j, fmaf(o[n][2 * j][i], f.own, x.x * f.prefix), fmaf(o[n][2 * j][2 + i], f.own, x.y * f.prefix),
-                                                 fmaf(o[n][2 * j + 1][i], f.own, x.z * f.prefix), fmaf(o[n][2 * j + 1][2 + i], f.own, x.w * f.prefix));
-                                }
+                                for (int j = 0; j < kWords; ++j)
+                                    store4<BF16>(p.out, to + 4 * j, fmaf(o[n][2 * j][i], f.own, x[4 * j] * f.prefix), fmaf(o[n][2 * j][2 + i], f.own, x[4 * j + 1] * f.prefix),
+                                                 fmaf(o[n][2 * j + 1][i], f.own, x[4 * j + 2] * f.prefix), fmaf(o[n][2 * j + 1][2 + i], f.own, x[4 * j + 3] * f.prefix));
                                 continue;
                             }
                         }
@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
     struct Place {
         long long to;
         float2 total;
-        float sums[kMine];
+        alignas(16) float sums[kMine];
     };
     const auto place_of = [&](const Piece& piece, int row) {
         Place x;
@@ -687,9 +687,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kThreads, 1) cache_rows_kernel(c
 #pragma unroll
             for (int i = 0; i < kMine; ++i) x.sums[i] = 0.f;
             if (piece.joins && piece.position + token >= 0) {
-                x.total = p.prefix_total[at];
-                using Columns = std::conditional_t<kMine == 4, float4, float2>;
-                *reinterpret_cast<Columns*>(x.sums) = *reinterpret_cast<const Columns*>(p.prefix_sums + x.to);
+                x.total = prefix_sums(p, p.prefix_total[at], at, kMine * lane, x.sums);
             }
         }
         return x;
