@@ -21,7 +21,7 @@ constexpr uint32_t kAll = 0xFFFFFFFFu;
 enum Turn { kStraight, kHalves, kPairs };             // no rotation; pairs (i, i + F); pairs (2 i, 2 i + 1)
 
 constexpr int kWindow = 16;                           // tokens whose runs a block looks at
-constexpr int kMostGroups = 8;                        // more blocks of a window than these would each bring its angles to shared memory
+constexpr int kMostGroups = 16;                       // more blocks of a window than these would each bring its angles to shared memory (cache_append_launch)
 constexpr int kManyWarps = 8;
 constexpr int kStaged = 32;                           // tokens whose angles a block keeps in shared memory
 
@@ -37,13 +37,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return *reinterpret_cast<float2*>(&d);
 }
 
-// 8 bytes of a page whose scale grows
 // 1 / s; the writers' scales are powers of two, whose exponents turn over
 __device__ __forceinline__ float inverse_of(float s) {
     const uint32_t bits = __float_as_uint(s);
     if (bits == 0) return 1.f;
     return (bits & 0x7FFFFFu) || bits >= 0x7F000000u ? 1.f / s : __uint_as_float(0x7F000000u - bits);
 }
+// 8 bytes of a page whose scale grows
 template <bool E4M3>
 __device__ __forceinline__ void requantise(uint8_t* at, float ratio) {
     const uint2 b = *reinterpret_cast<const uint2*>(at);
@@ -625,6 +625,9 @@ cudaError_t launch_many(F* kernel, long long blocks, cudaStream_t stream, const 
 }  // namespace
 
 // Blocks enough for the GPU, a window to several of them, and no more rows to a warp than leave it full: a few tokens are spread over all of it.
+// The second kernel where that gives a window 16 blocks or fewer (577 tokens and more): with more of them what it brings to shared memory is used too
+// little.  First / second, dim 128, us: a prompt of 250 tokens, 40 on 40 heads 11.4 / 11.1, 600 18.3 / 15.7, 800 25.4 / 20.7, 1100 with 32 on 8 heads
+// 16.7 / 14.0; single tokens, 32 on 8 heads: 250 8.5 / 12.0, 400 11.3 / 14.0, 600 16.1 / 16.1, 1000 20.5 / 18.9.
 cudaError_t cache_append_launch(const AppendParams& p, bool e4m3, bool bf16, bool pairs_beside, cudaStream_t stream) {
     constexpr int kBlocks = 148 * 4;
     const int windows = (p.tokens + kWindow - 1) / kWindow, here = std::min(p.tokens, kWindow), rows_per_step = 256 / p.cache.dim;
@@ -635,11 +638,10 @@ cudaError_t cache_append_launch(const AppendParams& p, bool e4m3, bool bf16, boo
     const long long units = std::max(singles, runs) + ((long long)here * p.q_heads + rows - 1) / rows;
     const int groups = (int)std::max<long long>(1, std::min<long long>((units + kWarps - 1) / kWarps, (kBlocks + windows - 1) / windows));
     const long long blocks = (long long)windows * groups;
-    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const auto by_size = [&](auto e, auto h, auto t) {
         constexpr bool E = decltype(e)::value, H = decltype(h)::value;
         constexpr int turn = decltype(t)::value;
-        if (groups > kMostGroups) return launch_overlapping(cache_append_kernel<E, H, turn>, dim3((unsigned)blocks), kWarps * 32, stream, p, groups, steps);
+        if ((kBlocks + windows - 1) / windows > kMostGroups) return launch_overlapping(cache_append_kernel<E, H, turn>, dim3((unsigned)blocks), kWarps * 32, stream, p, groups, steps);
         return launch_many(cache_append_many_kernel<E, H, turn>, blocks, stream, p, groups);
     };
     const auto by_turn = [&](auto e, auto h) {

@@ -84,6 +84,35 @@ def test_token_counts(tokens):
     check([7], [tokens], 4, 2, 128, 32, INT8, BF16, 64, False, True, tokens)
 
 
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("dim,pairs,interleaved,norm,kind,dtype", [(128, 64, False, True, INT8, FP16), (128, 32, True, True, E4M3, BF16), (64, 32, False, True, E4M3, FP16),
+                                                                   (64, 8, True, False, INT8, BF16), (128, 0, False, True, INT8, FP16), (64, 0, False, True, E4M3, BF16)])
+def test_many_tokens(dim, pairs, interleaved, norm, kind, dtype, page):
+    """Prompts that begin anywhere in a page, single tokens and drafts between them, padding behind."""
+    held = [0, 5, 127, 200, 31, 16, 15, 3, 0, 64, 90, 1]
+    new = [900, 1, 333, 1, 2, 1, 1, 5, 17, 700, 129, 40]
+    check(held, new, 7, 3, dim, page, kind, dtype, pairs, interleaved, norm, page + dim, pad=21)
+
+
+@pytest.mark.parametrize("tokens", [60, 1500])
+@pytest.mark.parametrize("kind,dtype", [(INT8, FP16), (E4M3, BF16)])
+def test_infinities_among_many_tokens(kind, dtype, tokens):
+    """Held as a write of the same keys and values holds them, with few tokens and with many, in runs and alone."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    slots, pages = slots_of([3, 0, 40, 9, 7], [tokens, 1, 1, 50, 1], 32, 2)
+    n = len(slots)
+    q, k, v = torch.randn((3, n, 4, 128), device="cuda", generator=gen).to(dtype).unbind(0)
+    for x in (k, v):
+        for i, token in enumerate((0, 5, 17, 40, tokens - 1, tokens, tokens + 1, tokens + 9, n - 1)):
+            x[token, i % 4, (31 * i) % 128] = (float("inf"), float("-inf"), float("nan"))[i % 3]
+    table = cache.angles(torch.arange(n, dtype=torch.int32, device="cuda"), torch.ones(64, device="cuda"))
+    a, b, spare = (empty_cache(pages, 4, 32, 128, kind, 3) for _ in range(3))
+    cache.append(*a, q, k, v, ints(slots), table)
+    turned_k = cache.append(*spare, k, k, v, ints(slots), table)
+    cache.write(*b, turned_k, v, ints(slots))
+    assert same_bytes(a[0], b[0]) and same_bytes(a[1], b[1]) and torch.equal(a[2], b[2])
+
+
 @pytest.mark.parametrize("size", [0.0, 1e-4, 1.0, 300.0])
 def test_sizes(size):
     for norm in (True, False):
