@@ -105,10 +105,11 @@ cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t
 }
 
 // The rows that read prefixes over those.  Both kernels run where the step's rows are more than the first one takes.
-constexpr int kFewReaders = 128;                      // rows of a key head
-// The prefix kernel counts tiles of 128 tokens and 128 rows in 32 bits: what the host knows of their number has to fit.
+constexpr int kFewReaders = 256;                      // rows of a key head
+// The prefix kernel counts tiles of 128 tokens and kPrefixRows rows in 32 bits: what the host knows of their number has to fit.
 bool countable(const i4mm::AttentionParams& p) {
-    const int64_t span = ((int64_t)p.table_width << p.cache.page_shift) / 128 + 2, rows = (int64_t)p.tokens * p.group / 128 + std::min<int64_t>(p.requests, p.tokens);
+    const int64_t span = ((int64_t)p.table_width << p.cache.page_shift) / 128 + 2;
+    const int64_t rows = (int64_t)p.tokens * p.group / i4mm::kPrefixRows + std::min<int64_t>(p.requests, p.tokens);
     return span <= kMost / p.cache.heads && rows <= kMost / (span * p.cache.heads);
 }
 
@@ -160,7 +161,7 @@ int attention(const i4mm_cache* cache, void* out, const void* q, int type, int64
         if (!shared.starts || !shared.rows || !shared.scratch) return I4MM_ERR_NULL;
         if (!aligned(shared.prefix_of, 4) || !aligned(shared.starts, 4) || !aligned(shared.rows, 4) || !aligned(shared.scratch, 16)) return I4MM_ERR_ALIGN;
         if (shared.scratch_bytes < shared_scratch(tokens, q_heads, cache->head_dim)) return I4MM_ERR_WORKSPACE;
-        p.prefix_of = (const int*)shared.prefix_of;
+        p.prefix_of = requests > 0 ? (const int*)shared.prefix_of : nullptr;  // (nobody reads in a step of no requests)
         p.prefix_starts = (const int*)shared.starts;
         p.prefix_rows = (const int*)shared.rows;
         p.prefix_listed = (int)shared.listed;
@@ -183,7 +184,7 @@ int attention(const i4mm_cache* cache, void* out, const void* q, int type, int64
     p.window = (int)window;
     p.scale = scale;
     const bool e4m3 = cache->type == I4MM_CACHE_E4M3, bf16 = type == I4MM_TYPE_BF16;
-    if (p.prefix_of && requests > 0) {
+    if (p.prefix_of) {
         if (!countable(p)) return I4MM_ERR_TOO_LARGE;
         const cudaError_t e = attend_prefixes(p, e4m3, bf16, (cudaStream_t)stream);
         if (e != cudaSuccess) return finish(e);
@@ -282,7 +283,7 @@ int i4mm_cache_attention_shared(const i4mm_cache* cache, void* out, const void* 
                                 int64_t table_stride, const void* seq_lens, const void* cu_lens, int64_t requests, int64_t max_len, float scale,
                                 int64_t window, const void* prefix_of, const void* prefix_starts, const void* prefix_rows, int64_t listed,
                                 void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, void* stream) {
-    if (tokens > 0 && !prefix_of) {
+    if (tokens > 0 && requests > 0 && !prefix_of) {
         g_attention_kernels = 0;
         return I4MM_ERR_NULL;
     }

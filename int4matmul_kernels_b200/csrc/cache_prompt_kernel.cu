@@ -320,7 +320,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
     const uint32_t tmem = tmem_smem;
     const auto s_col = [&](int h) { return tmem + h * 128; };
     const auto o_col = [&](int h) { return tmem + 256 + h * 128; };
-    ptx::grid_dependency_wait();
+    // (kPrefixes: the kernel before is that of places with few readers, which let this one begin once it knew all before it complete.  They write different
+    // rows and share nothing else, so it is only waited for before a block leaves: this kernel must not be complete before that one is.)
+    if (KIND != kPrefixes) ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
 
     if (alone) {                                      // rows of no request
@@ -911,6 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prompt_kernel(const Attenti
         }
     }
 
+    if (KIND == kPrefixes) ptx::grid_dependency_wait();
     if (lane == 0 && s_abort) atomicExch(status, 61);
     ptx::tc_fence_before_sync();
     __syncthreads();

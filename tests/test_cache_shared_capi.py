@@ -69,3 +69,15 @@ def test_attention(built_library):
         assert attend(**bad) == capi.ERR_ALIGN, bad
     assert attend(size=enough - 1) == capi.ERR_WORKSPACE and attend(ws=None) == capi.ERR_WORKSPACE and attend(ws_size=8) == capi.ERR_WORKSPACE
     assert lib.i4mm_last_attention_kernels() == 0
+
+
+def test_attention_counts_in_32_bits(built_library):
+    """A table and rows of which there could be more than 2^31 tiles are refused; half of that is not what is wrong."""
+    lib, wide = built_library, ((1 << 31) - 1 - 127) // 16
+
+    def attend(tokens, size):
+        return lib.i4mm_cache_attention_shared(cache(), 16, 16, 0, tokens, 2, 256, 128, 16, wide, wide, 16, 16, 1, 1, 1.0, 0, 16, 16, 16, tokens, 16, size, 16, 1 << 30, None)
+    # 2 key heads, 2^24 + 1 tiles of 128 tokens: 63 tiles of 64 rows are counted, 64 are not
+    tokens = 64 * 63
+    assert attend(tokens, lib.i4mm_cache_shared_scratch_bytes(tokens, 2, 128)) == capi.ERR_TOO_LARGE
+    assert attend(tokens, 16) == capi.ERR_WORKSPACE and lib.i4mm_last_attention_kernels() == 0

@@ -159,6 +159,45 @@ def test_equal_to_requests_that_hold_everything():
     assert (got.float() - other.float()).abs().max() < 2e-3 * other.float().abs().max()
 
 
+@pytest.mark.parametrize("window", [0, 90, 20000])
+@pytest.mark.parametrize("held,dtype,dim", [(INT8, BF16, 128), (E4M3, FP16, 64)])
+def test_parts_of_a_prefix_under_rows_of_chunks(held, dtype, dim, window):
+    """One head of a long prefix: all blocks have a part, and rows of a chunk, of drafts and of single tokens add them up."""
+    seqs, lens, of = [30000, 130, 1, 50, 6], [0, 101, 1, 4, 1], [-1, 0, 0, 0, 0]
+    k, v, scales, table, gen = make(seqs, 1, 64, dim, held, window)
+    check(queries(gen, sum(lens), 2, dim, dtype), k, v, scales, table, seqs, lens, of, window=window)
+
+
+@pytest.mark.parametrize("readers", [255, 256, 257])
+def test_rows_that_both_kernels_take(readers):
+    """Places on both sides of what the kernel of few readers takes, in one call, and more places than a warp keeps in registers."""
+    prefixes = [300, 70] + [20 + i for i in range(40)]
+    of = [-1] * 42 + [0] * readers + [1] * 40 + [2 + i for i in range(40)]
+    own = [1 + i % 5 for i in range(readers + 80)]
+    k, v, scales, table, gen = make(prefixes + own, 2, 16, 64, INT8, readers)
+    check(queries(gen, len(own), 2, 64, FP16), k, v, scales, table, prefixes + own, [0] * 42 + [1] * len(own), of)
+
+
+def test_which_kernels_run():
+    seqs, lens = [100] + [3] * 257, [0] + [1] * 257
+    k, v, scales, table, gen = make(seqs, 1, 16, 64, INT8, 1)
+    for readers, many in ((1, False), (256, False), (257, True)):
+        seq, cu = ints(seqs[:readers + 1]), ints(sums(lens[:readers + 1]))
+        shared = cache.share(ints([-1] + [0] * readers), seq, cu, readers)
+        cache.attention(queries(gen, readers, 1, 64, FP16), k, v, scales, table[:readers + 1], seq, cu, 1, shared=shared)
+        ran = capi.load().i4mm_last_attention_kernels()
+        assert ran & capi.ATTENTION_PREFIX and ran & capi.ATTENTION_FEW_ROWS and bool(ran & capi.ATTENTION_MANY_READERS) == many
+
+
+def test_no_requests():
+    k, v, scales, table, gen = make([20], 2, 16, 64, INT8, 1)
+    q = queries(gen, 3, 2, 64, FP16)
+    shared = cache.share(ints([]), ints([]), ints([0]), 3)
+    assert shared.rows.tolist() == [-1] * 3 and shared.positions.tolist() == [-1] * 3
+    got = cache.attention(q, k, v, scales, table[:0], ints([]), ints([0]), 1, shared=shared)
+    assert (got == 0).all() and not capi.load().i4mm_last_attention_kernels() & capi.ATTENTION_PREFIX
+
+
 def test_nobody_shares():
     """Tables without a reader: a call without them, but for the order of fp32 operations, which may differ from one compiled kernel to the other.  So
     both results are fp16 roundings of numbers that are 2^-17 of the summands apart at most, and so one step (2^-10) apart at most, and that."""
