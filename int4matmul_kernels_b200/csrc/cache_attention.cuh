@@ -54,6 +54,10 @@ constexpr size_t kPromptNext = 4096;                  // the next item to be wor
 constexpr size_t kPromptCounters = 8192;              // two per part
 constexpr int kPromptParts = 320;
 constexpr size_t kPrefixCounters = 16384;             // two per block
+// Tiles' worth of a block's time that it takes to begin a segment of the prefix kernel, where there are enough of them that many blocks begin a second one
+// (an eighth of the blocks).  0 / 3 / 6, us: 64 rows, 40 heads, 4000 tokens 128.6 / 124.1 / 125.0, 16 rows 39.0 / 36.5 / 38.0, 5 prefixes of 48 rows, 8 heads
+// of 64 41.4 / 37.6 / 39.2; 16 rows of 8 heads, 4000 tokens, with and without 26.5 / 23.4.
+constexpr int kPrefixBegin = 3;
 constexpr int kPrefixRows = 64;                       // rows of a tile of the prefix kernel
 
 struct Request {

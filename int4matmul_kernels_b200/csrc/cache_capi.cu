@@ -104,11 +104,14 @@ cudaError_t attend(const i4mm::AttentionParams& p, bool e4m3, bool bf16, int64_t
     return e != cudaSuccess ? e : prompt(i4mm::kFewRows + 1, false);
 }
 
-// The rows that read prefixes over those.  Both kernels run where the step's rows are more than the first one takes.
-constexpr int kFewReaders = 256;                      // rows of a key head
+// The rows that read prefixes over those.  Up to kFewReaders rows of a key head are the prefix kernel's, in tiles of 64 rows, each of which decodes the bytes
+// anew; more are the prompt kernel's, which works on 256 whatever they are and fetches bytes for all of them.  Both run where the step's rows are more than
+// the first one takes.  First / second, us with own tokens: 160 rows, 40 heads, 4000 tokens 98 / 147, 240 132 / 168; 8 heads, 16000 tokens: 192 rows 67 / 94, 256 75 / 92,
+// 384 94 / 95, 512 122 / 97; 8 heads, 500 tokens: 256 rows 27 / 40, 400 27 / 47; 3 prefixes of 270 rows, dim 64 54 / 48.
+constexpr int kFewReaders = 256;
 // The prefix kernel counts tiles of 128 tokens and kPrefixRows rows in 32 bits: what the host knows of their number has to fit.
 bool countable(const i4mm::AttentionParams& p) {
-    const int64_t span = ((int64_t)p.table_width << p.cache.page_shift) / 128 + 2;
+    const int64_t span = ((int64_t)p.table_width << p.cache.page_shift) / 128 + 2 + i4mm::kPrefixBegin;
     const int64_t rows = (int64_t)p.tokens * p.group / i4mm::kPrefixRows + std::min<int64_t>(p.requests, p.tokens);
     return span <= kMost / p.cache.heads && rows <= kMost / (span * p.cache.heads);
 }

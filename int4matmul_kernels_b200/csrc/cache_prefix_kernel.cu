@@ -4,23 +4,29 @@
 //   total = sum_j P_j / s_value,  sums = sum_j P_j v_j      over the prefix's tokens that the row sees, k_j and v_j the cache's bytes
 // M, total and sums of each row are what the kernel of its own tokens adds to its own.
 //
-// The rows of all readers of a place, times the query heads of a key head, are the rows of a tile, up to 128 of them.  With 16 to 128 rows for each byte,
-// DRAM bounds it up to about 64 rows (a tile of 128 tokens is 32 KB, 1400 cycles of an SM's share of DRAM) and the tensor cores and exponentials
-// above, so tokens are the 128 rows of both products and the readers their columns, as many as there are:
+// The rows of all readers of a place, times the query heads of a key head, are the rows of tiles of up to 64.  With 4 to 64 rows for each byte, DRAM would
+// bound it (a tile of 128 tokens is 32 KB at head_dim 128, 1400 cycles of an SM's share), and many columns are what the tensor cores do not have to be
+// given, so tokens are the 128 rows of both products and the readers their columns, as many as there are:
 //
 //   S^T = K Q^T      K: bytes -> fp16 -> tensor memory, a thread a token (no trip through shared memory, no transposition); Q: shared memory
 //   O^T = V^T P^T    V: bytes -> fp16 -> shared memory as they lie (dim fastest); P: shared memory, a thread a token
 // A thread of the softmax has one token, so a page's scales are its constants; it keeps its part of each row's total in a register, and nothing is summed
 // over threads until the end.  The largest score is looked for only where a weight would exceed 2^14: then sums follow to a new reference.
 //
-//   warps 0..3, 4..7   softmax of the first and of the second half of the rows
-//   warps 8..11        the rows' queries; bytes to operands
-//   warp 12            issues the products
-//   warps 13, 14       fetch pages into rings, a TMA copy a page, keys and values; the first deals out the work
+//   warps 0..15        softmax: two sets, which take tiles in turns, of four warps (32 tokens each) for either half of the rows
+//   warps 16..19       the rows' queries; bytes to operands
+//   warp 20            issues the products
+//   warps 21, 22       fetch pages into rings, a TMA copy a page, keys and values; the first deals out the work
 //
-// The tiles of all segments (place, key head, 128 rows) in a row are dealt out in equal contiguous ranges to the blocks.  What a range cuts goes through the
-// workspace, and the block that comes last adds the parts in their order.  Nobody waits for another block.  Waits are bounded: a warp that gives up
-// sets the abort flag, which ends every other wait of the block, and the status word.
+// The tiles of all segments (place, key head, up to 64 rows) in a row are dealt out in equal contiguous ranges to the blocks.  What a range cuts goes through
+// the workspace: few parts are added up by the block that comes last, many by those who read the rows (kJoined).  Nobody waits for another block.  Waits
+// are bounded: a warp that gives up sets the abort flag, which ends every other wait of the block, and the status word.
+//
+// What bounds it: the steps of a tile one after the other.  A set takes 6200 cycles for one of its tiles (64 rows, head_dim 64): scores 450, weights 3700, the
+// product with the values 800; the decoding warps are busy for 2600 of the 3100 a tile (at head_dim 128 as long as the softmax).  A block's first scores
+// come after 12000 cycles (loads that depend on one another, code that is not there yet), and a further segment costs 6000 to 20000.  Issue slots are
+// filled to 42 %, the tensor cores to 8.  One set of softmax warps instead of two: 64 readers with 40 heads, 4000 tokens 151 us
+// with the kernel of own tokens, for 132.
 #include <algorithm>
 #include <type_traits>
 
@@ -37,8 +43,10 @@ constexpr int kThreads = 32 * (kCopyValues + 1);
 constexpr int kStages = 3;                            // of either ring
 constexpr int kItems = 4, kScales = 4, kRawScales = 8;
 constexpr int kPieces = kTokens / 16;                 // pages of a tile, at most
-constexpr int kJoined = 6;                            // parts of a segment that one block adds up
-constexpr int kMinBlockTiles = 4;                     // fewer tiles than this are not cut further
+// Parts of a segment that one block adds up; 3 / 6 / 10, us with the kernel of own tokens: 64 rows over 4000 tokens, 40 heads (4 parts) 176 / 128 / 128, 8 rows of
+// 8 heads (8 parts) 26.8 / 26.9 / 30.0, 16 over 16000 49.4 / 49.5 / 53.8
+constexpr int kJoined = 6;
+constexpr int kMinBlockTiles = 4;                     // fewer tiles than this are not cut further, nor twice as many of whole segments
 constexpr float kNone = -3e38f;                       // a reference below any score
 constexpr float kMostLog = 14.f;                      // fp16 holds 2^16
 constexpr uint32_t kNoPage = 0x7FC0DEADu;             // in the place of a scale: there is no such page
@@ -104,8 +112,8 @@ __device__ __forceinline__ Place load_place(const AttentionParams& p, int most_r
     if (r.row_tiles > 1) r.height = (int)(((uint32_t)r.rows + 16u * r.row_tiles - 1) / (16u * r.row_tiles)) * 16;
     return r;
 }
-// (the host has made sure that all of them together are below 2^31)
-__device__ __forceinline__ uint32_t units_of(const AttentionParams& p, const Place& r) { return (uint32_t)(r.row_tiles * p.cache.heads) * (uint32_t)r.tiles; }
+// (the host has made sure that all of these together are below 2^31)
+__device__ __forceinline__ uint32_t segments_of(const AttentionParams& p, const Place& r) { return (uint32_t)(r.row_tiles * p.cache.heads); }
 
 // ---- two fp32 at a time ----
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -304,17 +312,28 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     if (warp == kCopy) {
         // the block's range: all have the same number of tiles, but for those at the end.  The first 32 places stay in the lanes' registers.
         Place mine{};
-        uint32_t own = 0;
+        uint32_t segments = 0, all_tiles = 0, longest = 0;
         if (lane < p.requests) {
             mine = load_place(p, most_rows, lane);
-            own = units_of(p, mine);
+            segments = segments_of(p, mine);
+            all_tiles = segments * mine.tiles;
+            longest = segments ? mine.tiles : 0;
         }
-        uint32_t total = own;
 #pragma unroll 1
-        for (int b = lane + 32; b < p.requests; b += 32) total += units_of(p, load_place(p, most_rows, b));
-        total = __reduce_add_sync(kAll, total);
-        const uint32_t share = max((total + gridDim.x - 1) / gridDim.x, (uint32_t)kMinBlockTiles);
-        uint32_t at = min(blockIdx.x * share, total);
+        for (int b = lane + 32; b < p.requests; b += 32) {
+            const Place r = load_place(p, most_rows, b);
+            segments += segments_of(p, r);
+            all_tiles += segments_of(p, r) * r.tiles;
+            if (r.row_tiles) longest = max(longest, (uint32_t)r.tiles);
+        }
+        segments = __reduce_add_sync(kAll, segments);
+        all_tiles = __reduce_add_sync(kAll, all_tiles);
+        longest = __reduce_max_sync(kAll, longest);
+        const uint32_t begin = segments * 8 < gridDim.x ? 0 : kPrefixBegin, total = all_tiles + segments * begin;
+        const uint32_t least = (longest <= 2 * kMinBlockTiles ? longest : kMinBlockTiles) + begin;
+        const auto units_of = [&](const Place& r) { return segments_of(p, r) * (r.tiles + begin); };
+        const uint32_t share = max((total + gridDim.x - 1) / gridDim.x, max(least, 1u));
+        uint32_t own = units_of(mine), at = min(blockIdx.x * share, total);
         const uint32_t end = min(at + share, total);
         // the place that the range begins in
         uint32_t before = 0;
@@ -325,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             for (; b < p.requests; b += 32) {
                 if (b > 0) {
                     mine = b + lane < p.requests ? load_place(p, most_rows, b + lane) : Place{};
-                    own = b + lane < p.requests ? units_of(p, mine) : 0;
+                    own = units_of(mine);
                 }
                 uint32_t upto = own;
 #pragma unroll
@@ -351,13 +370,13 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             }
         };
         uint32_t n = 0, g = 0;                        // items, tiles so far
-        bool ok = true;
+        bool ok = true, placed = false;
 #pragma unroll 1
         while (ok && at < end) {
-            if (n == 0 || at >= before + units_of(p, r)) {
+            if (!placed || at >= before + units_of(r)) {
                 // (the next place with rows: from the multiple of 32 at or below the current one, whose earlier tiles are counted again)
-                if (n > 0) {
-                    before += units_of(p, r);
+                if (placed) {
+                    before += units_of(r);
                     ++b;
 #pragma unroll 1
                     for (; b < p.requests && (b & 31); ++b) {
@@ -369,12 +388,15 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                     find_place();
                 }
                 if (b >= p.requests) break;           // (not unless the lengths change under the kernel)
+                placed = true;
             }
             Item t;
             {
-                const uint32_t in = at - before;
-                const int segment = (int)(in / (uint32_t)r.tiles), tile = (int)(in - (uint32_t)segment * r.tiles);
-                const int head = segment / r.row_tiles, row_tile = segment - head * r.row_tiles;
+                const uint32_t length = r.tiles + begin, segment = (at - before) / length, from = before + segment * length, stop = min(from + length, end);
+                const int tile = max((int)(at - from - begin), 0), tiles = (int)(stop - from - begin) - tile;
+                at = stop;
+                if (tiles <= 0) continue;             // (what it costs to begin is this block's, the tiles are the next one's)
+                const int head = (int)segment / r.row_tiles, row_tile = (int)segment - head * r.row_tiles;
                 t.valid = 1;
                 t.place = b;
                 t.head = head;
@@ -385,12 +407,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 t.lo = r.lo;
                 t.limit = r.limit;
                 t.tile0 = r.lo / kTokens + tile;
-                t.tiles = (int)min((uint32_t)(r.tiles - tile), end - at);
+                t.tiles = tiles;
                 t.first_block = t.last_block = (int)blockIdx.x;
                 if (t.tiles < r.tiles) {
-                    const uint32_t from = at - tile;
-                    t.first_block = (int)(from / share);
-                    t.last_block = (int)((from + r.tiles - 1) / share);
+                    t.first_block = (int)((from + begin) / share);
+                    t.last_block = (int)((from + length - 1) / share);
                 }
             }
             ok = wait_on(&bars.item_empty[n % kItems], (n / kItems) ^ 1, &s_abort);
@@ -403,7 +424,6 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
             ++n;
             ok = copy(t, g, &k_map, keys_ring, bars.keys_full, bars.keys_empty, kStages, true);
             g += t.tiles;
-            at += t.tiles;
         }
         if (ok) ok = wait_on(&bars.item_empty[n % kItems], (n / kItems) ^ 1, &s_abort);
         if (ok && lane == 0) {
