@@ -312,7 +312,7 @@ int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type,
  *   max_len                   the most rows of a request, for the choice of a kernel (a wrong one costs time, nothing else)
  * Sums and softmax statistics are fp32.  Which kernel runs goes by sizes that the host has (rows, max_len, the table's width, window), and the two
  * round differently: the one for few rows multiplies the values by weights of about 22 bits, the one for prompts by weights rounded to fp16
- * (2^-11 of each; against 64 bits 2.6e-4 to 2.8e-4 of an fp16 output's norm, where rounding the output alone makes 2.1e-4).  The same call gives the same bits.  `workspace` (about 55 MB): i4mm_cache_attention_workspace_bytes() bytes, zero-filled before the first use
+ * (2^-11 of each; against 64 bits 2.6e-4 to 2.8e-4 of an fp16 output's norm, where rounding the output alone makes 2.1e-4).  The same call gives the same bits.  `workspace` (about 65 MB): i4mm_cache_attention_workspace_bytes() bytes, zero-filled before the first use
  * and after i4mm_device_status has reported I4MM_ERR_TIMEOUT for it, shared by calls of one stream only.
  */
 size_t i4mm_cache_attention_workspace_bytes(void);
@@ -367,8 +367,9 @@ int i4mm_cache_share(int64_t requests, const void* prefix_of, const void* seq_le
  * are read once for all rows that share it, not once for each.
  *   prefix_of, prefix_starts, prefix_rows (listed >= tokens entries)   i4mm_cache_share's effective, starts and rows of the same step
  *   scratch   i4mm_cache_shared_scratch_bytes(tokens, q_heads, head_dim) bytes, 16-byte aligned, of any contents, this call's alone
- * heads * (table_width * page_size / 128 + 2) * (tokens * (q_heads / heads) / 128 + the smaller of requests and tokens) has to be below 2^31
- * (I4MM_ERR_TOO_LARGE otherwise).  The prefix's sums are fp32 too, its weights rounded to fp16; everything else is as above.
+ * heads * (table_width * page_size / 128 + 5) * (tokens * (q_heads / heads) / 64 + the smaller of requests and tokens) has to be below 2^31
+ * (I4MM_ERR_TOO_LARGE otherwise).  In a step of no requests the tables are not looked at.  The prefix's sums are fp32 too, its weights rounded to fp16;
+ * everything else is as above.
  */
 size_t i4mm_cache_shared_scratch_bytes(int64_t tokens, int64_t q_heads, int64_t head_dim);
 int i4mm_cache_attention_shared(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,
