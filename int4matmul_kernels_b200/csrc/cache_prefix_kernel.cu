@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     __shared__ float2 s_raw[kRawScales][kPieces];
     __shared__ float4 s_scale[kScales][kPieces];      // key scale, log2 of the value scale, its inverse, whether there is such a page
     __shared__ int s_row[kItems][kMostRows];          // packed row times query heads plus head; -1: none
-    __shared__ long long s_query[kMostRows];          // where its query lies
+    __shared__ long long s_query[kItems][kMostRows];  // where its query lies (a warp may write the next item's while another one reads this one's)
     __shared__ int s_low[kItems][kMostRows];          // the first token that the row sees
     __shared__ float s_up[kItems][kMostRows];         // what its scores are multiplied with (bf16)
     __shared__ int s_most_low[kItems];
@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 }
                 if (tid < kMostRows) {
                     s_row[slot][tid] = id;
-                    s_query[tid] = query;
+                    s_query[slot][tid] = query;
                     s_low[slot][tid] = low;
                 }
                 const int most = __reduce_max_sync(kAll, low);
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
                 for (int i = 0; i < kAtOnce; ++i) {
                     const int r = r0 + i * 4 * kRowsAtOnce + lane / kUnits, id = r < t.n ? s_row[slot][r] : -1;
                     x[i] = make_uint4(0, 0, 0, 0);
-                    if (id >= 0) x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q.p) + s_query[r] + 8 * (lane % kUnits));
+                    if (id >= 0) x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q.p) + s_query[slot][r] + 8 * (lane % kUnits));
                 }
 #pragma unroll
                 for (int i = 0; i < kAtOnce; ++i) {
