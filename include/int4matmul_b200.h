@@ -366,7 +366,9 @@ int i4mm_cache_share(int64_t requests, const void* prefix_of, const void* seq_le
  * (p >= 0) sees tokens j of the prefix and j' <= p of its own; with window > 0 those with j > L + p - window and j' > p - window.  The prefix's pages
  * are read once for all rows that share it, not once for each.
  *   prefix_of, prefix_starts, prefix_rows (listed >= tokens entries)   i4mm_cache_share's effective, starts and rows of the same step
- *   scratch   i4mm_cache_shared_scratch_bytes(tokens, q_heads, head_dim) bytes, 16-byte aligned, of any contents, this call's alone
+ *   scratch   i4mm_cache_shared_scratch_bytes(tokens, q_heads, head_dim) bytes, 16-byte aligned, of any contents, this call's alone.  What it held
+ *             counts for rows whose request names a prefix and which no list names (lists of another step): their results are void, but nothing
+ *             beyond the arrays is read for them
  * heads * (table_width * page_size / 128 + 5) * (tokens * (q_heads / heads) / 64 + the smaller of requests and tokens) has to be below 2^31
  * (I4MM_ERR_TOO_LARGE otherwise).  In a step of no requests the tables are not looked at.  The prefix's sums are fp32 too, its weights rounded to fp16;
  * everything else is as above.

@@ -205,6 +205,8 @@ struct PrefixParts {
         a = bits & 0xFF;
         count = bits >> 8 & 0xFF;
         row = bits >> 16 & 0xFF;
+        // A row that no list names, or whose prefix kernel gave up, has in this place whatever the caller's scratch holds: what names no parts is no prefix.
+        if (bits >> 24 || a + count > kMaxBlocks || row >= kPrefixRows) count = 0;
         dim = p.cache.dim;
         base = reinterpret_cast<const float*>(static_cast<const uint8_t*>(p.workspace) + p.prefix_parts);
     }
