@@ -313,7 +313,8 @@ int i4mm_cache_read(const i4mm_cache* cache, void* k_out, void* v_out, int type,
  * Sums and softmax statistics are fp32.  Which kernel runs goes by sizes that the host has (rows, max_len, the table's width, window), and the two
  * round differently: the one for few rows multiplies the values by weights of about 22 bits, the one for prompts by weights rounded to fp16
  * (2^-11 of each; against 64 bits 2.6e-4 to 2.8e-4 of an fp16 output's norm, where rounding the output alone makes 2.1e-4).  The same call gives the same bits.  `workspace` (about 65 MB): i4mm_cache_attention_workspace_bytes() bytes, zero-filled before the first use
- * and after i4mm_device_status has reported I4MM_ERR_TIMEOUT for it, shared by calls of one stream only.
+ * and after i4mm_device_status has reported I4MM_ERR_TIMEOUT for it, shared by calls of one stream only
+ * (made by any number of host threads: calls with one workspace launch their kernels one call after the other).
  */
 size_t i4mm_cache_attention_workspace_bytes(void);
 int i4mm_cache_attention(const i4mm_cache* cache, void* out, const void* q, int type, int64_t tokens, int64_t q_heads,

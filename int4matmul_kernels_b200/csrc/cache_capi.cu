@@ -2,6 +2,7 @@
 #include "../../include/int4matmul_b200.h"
 
 #include <algorithm>
+#include <mutex>
 
 #include "cache_attention.cuh"
 #include "common.cuh"
@@ -126,6 +127,13 @@ cudaError_t attend_prefixes(const i4mm::AttentionParams& p, bool e4m3, bool bf16
     return e;
 }
 
+// A call of shared prefixes launches kernels of which the later ones begin beside the one before and read what an earlier one left in the workspace, so nothing
+// else that uses the workspace may come between them in the stream: calls with one workspace launch one after the other, whatever host threads make them.
+std::mutex& launch_lock(const void* workspace) {
+    static std::mutex locks[16];
+    return locks[(reinterpret_cast<uintptr_t>(workspace) >> 21) % 16];
+}
+
 // A step's shared prefixes, as i4mm_cache_share lays them out; prefix_of nullptr: none
 struct Prefixes {
     const void *prefix_of, *starts, *rows;
@@ -187,8 +195,9 @@ int attention(const i4mm_cache* cache, void* out, const void* q, int type, int64
     p.window = (int)window;
     p.scale = scale;
     const bool e4m3 = cache->type == I4MM_CACHE_E4M3, bf16 = type == I4MM_TYPE_BF16;
+    if (p.prefix_of && !countable(p)) return I4MM_ERR_TOO_LARGE;
+    const std::lock_guard<std::mutex> alone(launch_lock(workspace));
     if (p.prefix_of) {
-        if (!countable(p)) return I4MM_ERR_TOO_LARGE;
         const cudaError_t e = attend_prefixes(p, e4m3, bf16, (cudaStream_t)stream);
         if (e != cudaSuccess) return finish(e);
     }
