@@ -244,7 +244,7 @@ __device__ __forceinline__ float2 prefix_sums(const AttentionParams& p, float2 t
         total = fmaf(take, of.y, total);
 #pragma unroll
         for (int k = 0; k < N; k += kSome) {
-            float x[kSome];
+            alignas(16) float x[kSome];
             *reinterpret_cast<Some*>(x) = __ldcg(reinterpret_cast<const Some*>(parts.sums(i) + col + k));
 #pragma unroll
             for (int e = 0; e < kSome; ++e) sums[k + e] = fmaf(take, x[e], sums[k + e]);

@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_prefix_kernel(const Attenti
     __shared__ int s_row[kItems][kMostRows];          // packed row times query heads plus head; -1: none
     __shared__ long long s_query[kItems][kMostRows];  // where its query lies (a warp may write the next item's while another one reads this one's)
     __shared__ int s_low[kItems][kMostRows];          // the first token that the row sees
-    __shared__ float s_up[kItems][kMostRows];         // what its scores are multiplied with (bf16)
+    __shared__ __align__(16) float s_up[kItems][kMostRows];                   // what its scores are multiplied with (bf16; read four at a time)
     __shared__ int s_most_low[kItems];
     // (by set and half)
     __shared__ __align__(16) float s_minus_top[2 * kHalves][kColumns];        // the rows' references, their signs turned over
