@@ -332,7 +332,8 @@ int i4mm_last_attention_kernels(void);
 /*
  * angles[t, i] = (cos, sin) of positions[t] * freqs[i], fp32 (tokens, pairs, 2) contiguous; (1, 0) where the position is negative (padding).
  *   positions int32 (tokens), freqs fp32 (pairs), pairs a multiple of 8 up to 128; angles 16-byte, freqs 8-byte aligned.
- * The products and their reduction by whole turns are fp64, so that far positions are as exact as near ones.
+ * The products and their reduction by whole turns are fp64: the angle is off by at most 9.4e-8 (its rounding to fp32 after that) and 2^-51 of itself,
+ * 1.5e-7 for 2^27 radians and 1.1e-6 for 2^31.
  */
 int i4mm_cache_angles(void* angles, const void* positions, const void* freqs, int64_t tokens, int64_t pairs, void* stream);
 
@@ -342,7 +343,8 @@ int i4mm_cache_angles(void* angles, const void* positions, const void* freqs, in
  *   (a, b) -> (a cos - b sin, b cos + a sin)   of the first 2 * pairs values, a and b being values i and i + pairs, or with pairs_beside 2 i and 2 i + 1;
  *                                              cos, sin = angles[t, i] (fp32 (tokens, pairs, 2), 16-byte aligned); pairs a multiple of 8, 0: no rotation
  * in fp32, rounded once to the activations' type.  q_out (tokens, q_heads, head_dim) contiguous gets the queries of all tokens; the keys, and
- * the values as they are, go into the cache as i4mm_cache_write's do, to the byte.  q_out is none of the inputs; q_heads is free here.
+ * the values as they are, go into the cache as i4mm_cache_write's do, to the byte.  q_out is none of the inputs; q_heads is free here.  With neither
+ * weights nor pairs it is a write that also copies the queries.
  */
 int i4mm_cache_append(const i4mm_cache* cache, void* q_out, const void* q, const void* k, const void* v, int type, int64_t tokens, int64_t q_heads,
                       int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
@@ -353,7 +355,8 @@ int i4mm_cache_append(const i4mm_cache* cache, void* q_out, const void* q, const
  * Shared prefixes: requests that begin alike hold what they share once.  A prefix is a place of the batch like any request (its tokens are
  * written, and its pages given back, as theirs are); a request names it and holds only what comes after it.
  *   prefix_of (requests)      the place whose tokens come before the request's own.  None: negative, no place of the batch, the request itself, a
- *                             place without tokens; a prefix's own prefix is not looked at.
+ *                             place without tokens; a prefix's own prefix is not looked at.  Positions behind a place count its tokens: where keys
+ *                             are rotated it must not grow any more.
  *   seq_lens, cu_lens         as for i4mm_cache_attention, after the step
  * Outputs: effective (requests): prefix_of, -1 for none; starts (requests + 1), rows (max_tokens): the packed rows that read place p are
  * rows[starts[p]] .. rows[starts[p + 1] - 1], ascending, -1 behind the last of all; positions (max_tokens): of the packed rows, the prefix counted
@@ -365,9 +368,10 @@ int i4mm_cache_share(int64_t requests, const void* prefix_of, const void* seq_le
 /*
  * i4mm_cache_attention of rows that see their request's prefix before its own tokens: with L tokens in the prefix, a row at position p of its request
  * (p >= 0) sees tokens j of the prefix and j' <= p of its own; with window > 0 those with j > L + p - window and j' > p - window.  The prefix's pages
- * are read once for all rows that share it, not once for each.
+ * are fetched and decoded once for every 64 rows of a key head (readers times q_heads / heads), once for every 256 where there are more than 256.
  *   prefix_of, prefix_starts, prefix_rows (listed >= tokens entries)   i4mm_cache_share's effective, starts and rows of the same step
- *   scratch   i4mm_cache_shared_scratch_bytes(tokens, q_heads, head_dim) bytes, 16-byte aligned, of any contents, this call's alone.  What it held
+ *   scratch   i4mm_cache_shared_scratch_bytes(tokens, q_heads, head_dim) bytes (4 a value of q and 8 a row and head, whichever rows have a prefix),
+ *             16-byte aligned, of any contents, this call's alone.  What it held
  *             counts for rows whose request names a prefix and which no list names (lists of another step): their results are void, but nothing
  *             beyond the arrays is read for them
  * heads * (table_width * page_size / 128 + 5) * (tokens * (q_heads / heads) / 64 + the smaller of requests and tokens) has to be below 2^31

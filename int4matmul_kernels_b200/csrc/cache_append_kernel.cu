@@ -6,7 +6,11 @@
 // in fp32, rounded once to the activations' type; queries are stored so, keys go on to the cache as cache_write_kernel.cu says, and so do values,
 // which are not changed.  So the bytes are those of a write of the rotated keys.
 // What bounds it: with few tokens the chain of launch, slots, rows and old scales (1 token, 40 heads 4.0 us, 150 tokens, 32 on 8 heads 5.3; a write alone 2.3 and
-// 3.6); with many, issue slots (3 prompts, 4500 tokens, 40 heads 71 us where 16-bit rows in and out and bytes out are 36, a write alone 31).
+// 3.6).  These are of steps in which no scale grows.  Where one does, a warp holds the page's earlier rows in the new scale one after the other, a load and a store
+// each (append_singles; the writer takes two at a time), and the launch takes as long as the longest of these: 150 requests that decode on with normal values, pages of 64,
+// grow 14 (int8, fp16) or 34 (e4m3, bf16) of 2400 scales a step, and take 29 or 26 us by events around the call, where the same without growth takes 10 (a write 14 to
+// 16, and 7).
+// With many tokens, issue slots (3 prompts, 4500 tokens, 40 heads 71 us where 16-bit rows in and out and bytes out are 36, a write alone 31).
 #include <algorithm>
 
 #include "cache_bytes.cuh"

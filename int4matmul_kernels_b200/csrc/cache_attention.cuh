@@ -1,4 +1,4 @@
-// What the two attention kernels of the paged 8-bit cache share: a request as they see it, the decoding of bytes, the workspace.
+// What the attention kernels of the paged 8-bit cache share: a request as they see it, the decoding of bytes, the workspace.
 #pragma once
 
 #include <cuda.h>
@@ -285,7 +285,7 @@ inline bool cache_map(CUtensorMap* out, const CacheView& c, bool keys, int token
     });
 }
 
-// The two kernels.  Few rows: requests of more than most_rows rows are left to the other one; `few`: no request has more than 8.
+// The two kernels of requests' own tokens.  Few rows: requests of more than most_rows rows are left to the other one; `few`: no request has more than 8.
 // Prompts: requests of fewer than least_rows rows are left to the other one; `alone`: it is not launched.
 // With p.prefix_of set, both add what p.prefix_total and p.prefix_sums say to each row that has a prefix.
 cudaError_t cache_rows_launch(const AttentionParams& p, bool e4m3, bool bf16, int most_rows, bool few, cudaStream_t stream);

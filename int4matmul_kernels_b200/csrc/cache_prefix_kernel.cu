@@ -2,11 +2,13 @@
 //
 //   x_j = log2(e) * scale * s_key * (q . k_j) + log2(s_value),  P_j = 2^(x_j - M)   (fp16), with a reference M, an x_j of the row,
 //   total = sum_j P_j / s_value,  sums = sum_j P_j v_j      over the prefix's tokens that the row sees, k_j and v_j the cache's bytes
-// M, total and sums of each row are what the kernel of its own tokens adds to its own.
+// M, total and sums of each row are what the kernel of its own tokens adds to its own.  Weights are rounded to fp16 for the product, as the prompt kernel's are
+// (2^-11 of each, and they are rounded apart from one another): against 64 bits an fp16 output is off by 2.5e-4 to 2.9e-4 of its norm, by 2.1e-4 where it alone
+// is rounded.  Carrying the rounding errors, as the few-row kernel does, would double the weights' shared memory and the second product.
 //
-// The rows of all readers of a place, times the query heads of a key head, are the rows of tiles of up to 64.  With 4 to 64 rows for each byte, DRAM would
-// bound it (a tile of 128 tokens is 32 KB at head_dim 128, 1400 cycles of an SM's share), and many columns are what the tensor cores do not have to be
-// given, so tokens are the 128 rows of both products and the readers their columns, as many as there are:
+// The rows of all readers of a place, times the query heads of a key head, are the rows of tiles of up to 64.  With so few rows for each byte the floor is DRAM's (a
+// tile of 128 tokens is 32 KB at head_dim 128, 1400 cycles of an SM's share; what bounds the kernel instead stands below), and many columns are what the
+// tensor cores do not have to be given, so tokens are the 128 rows of both products and the readers their columns, as many as there are:
 //
 //   S^T = K Q^T      K: bytes -> fp16 -> tensor memory, a thread a token (no trip through shared memory, no transposition); Q: shared memory
 //   O^T = V^T P^T    V: bytes -> fp16 -> shared memory as they lie (dim fastest); P: shared memory, a thread a token

@@ -12,8 +12,9 @@ constexpr uint32_t kAll = 0xFFFFFFFFu;
 
 // (cos, sin) of position * freq.  The product of two fp32-sized numbers in fp64 is exact up to positions of 2^29, and so good to 2^-52 above; whole
 // turns are taken off in fp64, which leaves the fp32 functions an argument of at most one turn: positions of a million are as good as those
-// below ten.  Two angles a thread, 16 bytes a store.  What bounds it: the stores (8 bytes an angle), a few fp64 instructions and the fp32 functions': 36000
-// tokens of 64 pairs 7.3 us (18.4 MB, 2.5 TB/s), 64 tokens 1.6.
+// below ten, and from 2^28 radians on the fp64 roundings show (2^-51 of the angle).  Two angles a thread, 16 bytes a store.  What bounds it: instructions. Each
+// 16 bytes cost a 64-bit division, a load and conversion of the position, conversions of two frequencies, fp64 products and the fp32 functions: 36000
+// tokens of 64 pairs 7.3 us (18.4 MB, 2.5 TB/s; the stores alone would be 2.8), 64 tokens 1.6.
 __global__ void __launch_bounds__(256) cache_angles_kernel(float4* out, const int* positions, const float* freqs, long long twos, int per_token) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
@@ -40,7 +41,7 @@ __global__ void __launch_bounds__(256) cache_angles_kernel(float4* out, const in
 //   offset(b) = starts(of(b)) + sum of rows(b') over the b' < b with of(b') = of(b)
 // and row i of b is entry offset(b) + i of the list.  Every block takes the sums itself (they are a few loads per thread) and keeps its own part
 // of the rows.  The sums over equal prefixes are taken in order by one warp, 32 requests at a time, so that the list's order is always the same.
-// What bounds it: the launch and that chain (4 requests 3.0 us, 500 requests 8.5).
+// What bounds it: the launch, and a chain of loads, sums, that one warp's pass and a search for each token (4 requests 3.0 us, 500 requests 8.5).
 constexpr int kShareThreads = 512;
 
 __global__ void __launch_bounds__(kShareThreads) cache_share_kernel(const ShareParams p) {
